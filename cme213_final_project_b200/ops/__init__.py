@@ -60,7 +60,8 @@ _PROTOTYPES = {
 # Entry points that the compiled wrappers call.
 _WRAPPED = ("cme_last_error", "cme_cross_entropy", "cme_attention_fwd", "cme_attention_bwd", "cme_attention_path",
             "cme_attention_gemm_ws_bytes", "cme_layernorm_fwd", "cme_layernorm_bwd_blocks", "cme_layernorm_bwd",
-            "cme_bias_act_residual", "cme_colsum_splits", "cme_dact_colsum", "cme_embedding_fwd", "cme_embedding_bwd")
+            "cme_bias_act_residual", "cme_colsum_splits", "cme_dact_colsum", "cme_embedding_fwd", "cme_embedding_bwd",
+            "cme_paged_append", "cme_paged_attention_ws_bytes", "cme_paged_attention", "cme_next_token")
 _CTYPES = {"v": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "u": ctypes.c_uint}
 
 
@@ -404,6 +405,56 @@ def attention_bwd(q, k, v, out, lse, dout, B: int, H: int, T: int, layout: str =
     acc, sem = (None, None) if scratch is None else scratch
     return _native().attention_bwd(q, k, v, out, lse, dout, B, H, T, layout == "flat", int(causal), _BACKENDS[backend], int(dq_mode),
                                    acc, sem)
+
+
+# --------------------------------------------------------------------------------------------------
+# Generation: a paged cache of keys and values, attention over it, the next token
+# --------------------------------------------------------------------------------------------------
+_PAGED_BACKENDS = {"auto": 0, "single": 1, "rows": 2, "tc": 3}
+
+
+def cache_append(k, v, cache_k, cache_v, pages, offsets, lengths) -> None:
+    """Write new tokens' keys and values (``[tokens, kv_heads, head_dim]``, any strides of multiples of 16 bytes) into a paged cache.
+
+    ``cache_k``, ``cache_v``: ``[pages, kv_heads, slots, head_dim]``, any strides of multiples of 16 bytes, slots a multiple of 8;
+    head sizes 32, 64 and 128, bf16 or fp32.  ``pages`` (int32 ``[seqs, columns]``): position p of a sequence lies in slot
+    ``p % slots`` of page ``pages[seq, p // slots]``; an entry outside the cache (-1) is a page that is not there.  ``offsets``
+    (int32 ``[seqs + 1]``, from 0 to the number of tokens): the tokens of a sequence.  ``lengths`` (int32 ``[seqs]``): tokens of
+    a sequence with the new ones, which come last.  A token without a place (page not there, position beyond the table) is dropped.
+    A page belongs to one sequence at a time as far as new tokens go; pages that are only read may be shared."""
+    _native().cache_append(k, v, cache_k, cache_v, pages, offsets, lengths)
+
+
+def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Optional[float] = None, max_len: Optional[int] = None,
+                    backend: str = "auto", splits: int = 0):
+    """Causal attention of new tokens, ``q`` = ``[tokens, heads, head_dim]``, over a paged cache that holds their keys too (see
+    :func:`cache_append` for the cache and the tables).  ``heads`` is a multiple of the cache's heads, which as many query heads
+    in a row share.  Returns ``(out, lse)``: ``[tokens, heads, head_dim]`` and the log-sum-exp of the scaled scores, fp32
+    ``[tokens, heads]``.  Keys on pages that are not there do not take part; a row without any key gets zeros and ``-inf``.
+    What the cache holds beyond a sequence's length may be anything, within it the values have to be finite.
+
+    ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_len``: no length is larger (default: what the table
+    holds); the number of parts that the keys are divided into goes by it.  ``backend``: ``auto`` | ``single`` (few rows) | ``rows`` |
+    ``tc`` (tcgen05: bf16, head sizes 64 and 128); ``splits``: parts of the keys, 0 = by the rule, negative = joined
+    through scratch memory in any case."""
+    return _native().paged_attention(q, cache_k, cache_v, pages, offsets, lengths, scale, max_len, _PAGED_BACKENDS[backend], splits)
+
+
+def next_token(logits, *, history=None, lengths=None, prompts=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+               bias_values=None, temperature=None, allowed=None, noise=None, processed: bool = False):
+    """From ``logits`` (``[rows, vocab]``, bf16 or fp32) to each row's next token.  Returns ``(token, logprob, processed)``: int32
+    and fp32 ``[rows]``, and the processed logits in the type of ``logits`` (``None`` unless ``processed``).
+
+    In 32 bits and in this order: tokens of the row's ``history`` (int32 ``[rows, columns]``, the first ``lengths[row]`` of
+    them; others than tokens are skipped) get ``x / r`` where x > 0, else ``x * r``, r = ``repetition``; those at ``prompts[row]``
+    or later in it (generated, c times; all without ``prompts``) ``x - c * frequency - presence``; tokens of ``bias_ids`` (int32 ``[rows, k]``, others skipped, the last
+    one counts if a token comes twice) ``+ bias_values``; all ``x / temperature`` where that is above 0; tokens whose bit of
+    ``allowed`` (int32 ``[rows or 1, ceil(vocab / 32)]``, the lowest bit first) is not set ``-inf``.  The token is
+    the largest x, or x + ``noise`` (fp32 ``[rows, vocab]``; Gumbel noise makes it a sample of the softmax) where the
+    temperature is above 0, the lowest index of equals, -1 if all are ``-inf``; ``logprob`` is its x minus the
+    log-sum-exp of the row (``-inf`` without a token).  ``repetition``, ``presence``, ``frequency``, ``temperature``: fp32 ``[rows]``."""
+    return _native().next_token(logits, history, lengths, prompts, repetition, presence, frequency, bias_ids, bias_values, temperature,
+                                allowed, noise, processed)
 
 
 def launch_count() -> int:

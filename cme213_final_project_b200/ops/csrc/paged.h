@@ -1,0 +1,91 @@
+// Paged cache of keys and values: what its kernels share.
+#pragma once
+#include "common.h"
+#include "paged_desc.h"
+
+#include <cuda.h>
+
+// The kernel and the division of the keys that a call takes.
+struct PagedPlan {
+    int kernel;          // PAGED_*
+    int row_tile;        // rows (tokens x query heads of one key head) of a CTA
+    int tiles;           // row tiles of all sequences at the most
+    int splits;          // parts that the keys of a row tile are divided into
+    int cluster;         // non-zero: the parts are one cluster's CTAs, which join them through shared memory
+    int split_keys;      // keys of a part otherwise (multiple of the key tile); the parts are joined through `ws`
+};
+enum PagedKernel : int { PAGED_SINGLE = 0, PAGED_ROWS = 1, PAGED_TC = 2 };
+
+int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long long page_stride, long long head_stride,
+                   long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle);
+int paged_attention_mma(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
+int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
+int paged_join(const CmePaged* a, int splits, cudaStream_t st);      // the parts in a->ws to a->o and a->lse
+// Keys of the tiles that the kernels walk in.
+int paged_mma_key_tile(int dtype, int head_dim);
+constexpr int PAGED_TC_KEYS = 64;
+
+// Division by a page size that the host knows, for 0 <= x < 2^31: x / d = (x * m) >> s with m = ceil(2^s / d) and s = 31 + ceil(log2 d)
+// (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994).
+struct PagedDiv {
+    unsigned long long m;
+    int s, d;
+    __host__ __device__ int div(int x) const { return (int)(((unsigned long long)(unsigned)x * m) >> s); }
+};
+inline PagedDiv paged_div(int d) {
+    PagedDiv p;
+    int lg = 0;
+    while ((1ll << lg) < d) ++lg;
+    p.d = d;
+    p.s = 31 + lg;
+    p.m = ((1ull << p.s) + d - 1) / d;
+    return p;
+}
+
+#ifdef __CUDACC__
+
+// What a CTA works on: rows [first, first + rows) of a sequence's tokens x group, for one key head.
+struct PagedTile {
+    int seq, first, rows;        // rows == 0: the tile does not exist
+    int token0, n, length;       // the sequence's first row of q, its new tokens, its tokens
+};
+
+// Finds row tile `tile`, counting ceil(new tokens x group / row_tile) tiles per sequence.  Whole warps call it; every warp gets
+// the answer.  offsets and lengths that make no sense cannot lead outside of the buffers: they are cut to them.
+__device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile, int group, int row_tile) {
+    const int lane = threadIdx.x & 31;
+    PagedTile t{0, 0, 0, 0, 0, 0};
+    int base = 0;
+    for (int b0 = 0; b0 < a.seqs; b0 += 32) {
+        const int b = b0 + lane;
+        int lo = 0, hi = 0, len = 0;
+        if (b < a.seqs) { lo = a.offsets[b]; hi = a.offsets[b + 1]; len = a.lengths[b]; }
+        lo = max(0, min(lo, a.rows));
+        hi = max(lo, min(hi, a.rows));
+        const int n = hi - lo;
+        const int own = (int)(((long long)n * group + row_tile - 1) / row_tile);
+        int upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned found = __ballot_sync(0xffffffffu, tile < base + upto);
+        if (found) {
+            const int src = __ffs(found) - 1;
+            const int first = (tile - base - __shfl_sync(0xffffffffu, upto - own, src)) * row_tile;
+            t.seq = b0 + src;
+            t.token0 = __shfl_sync(0xffffffffu, lo, src);
+            t.n = __shfl_sync(0xffffffffu, n, src);
+            const long long most = (long long)a.width * a.page;
+            t.length = (int)min((long long)max(0, min(__shfl_sync(0xffffffffu, len, src), a.max_len)), most);
+            t.first = first;
+            t.rows = (int)min((long long)row_tile, (long long)t.n * group - first);
+            return t;
+        }
+        base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return t;
+}
+
+#endif  // __CUDACC__

@@ -1,0 +1,229 @@
+// A paged cache of keys and values: what goes into it, and the host side of the attention that reads it.
+#include "paged.h"
+
+#include <algorithm>
+#include <mutex>
+
+namespace {
+
+// ------------------------------------------------------------------------------------------------------
+// Append
+// ------------------------------------------------------------------------------------------------------
+// Token i of a sequence's n new ones goes to position length - n + i.  A copy, so bytes bound it (read once, written once); one warp per
+// token, whose loads are on their way before it looks up where they go: offsets -> length -> page is a chain of three.
+constexpr int APPEND_WARPS = 4;
+constexpr int APPEND_UNROLL = 4;           // 16-byte pieces per lane of keys, and as many of values, at a time
+
+template <bool WIDE>                       // whether a token has more pieces than one round of a warp takes
+__global__ void __launch_bounds__(APPEND_WARPS * 32) paged_append_kernel(const CmePaged a, PagedDiv page_div, int elem, int head_log) {
+    pdl_wait();
+    const int token = blockIdx.x * APPEND_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (token >= a.rows) return;
+    const int pieces = a.kv_heads << head_log;             // of 16 bytes, keys
+    const char* k = static_cast<const char*>(a.q) + token * a.q_token * elem;
+    const char* v = static_cast<const char*>(a.nv) + token * a.v_token * elem;
+    uint4 kr[APPEND_UNROLL], vr[APPEND_UNROLL];
+    auto load = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < APPEND_UNROLL; ++u) {
+            const int c = c0 + u * 32 + lane, h = c >> head_log, d = (c - (h << head_log)) * 16;
+            if (c < pieces) {
+                kr[u] = *reinterpret_cast<const uint4*>(k + h * a.q_head * elem + d);
+                vr[u] = *reinterpret_cast<const uint4*>(v + h * a.v_head * elem + d);
+            }
+        }
+    };
+    load(0);
+    // the sequence whose rows hold the token: the last b with offsets[b] <= token, a 32nd of the range at a time
+    int lo = 0, n = a.seqs;                                // it lies in [lo, lo + n)
+    while (n > 1) {
+        const int step = (n + 31) >> 5, b = lo + lane * step;
+        const unsigned le = __ballot_sync(0xffffffffu, lane * step < n && a.offsets[b] <= token);
+        const int last = le ? 31 - __clz(le) : 0;
+        n = min(step, n - last * step);
+        lo += last * step;
+    }
+    const int first = a.offsets[lo], next = a.offsets[lo + 1];
+    const int length = a.lengths[lo];
+    if (token < first || token >= next || next > a.rows) return;
+    const long long pos = (long long)length - next + token;
+    if (pos < 0 || pos >= min((long long)a.width * a.page, (long long)a.max_len)) return;
+    const int col = page_div.div((int)pos), slot = (int)pos - col * a.page;
+    const int page = a.pages[lo * a.pages_ld + col];
+    if (page < 0 || page >= a.num_pages) return;
+    char* dk = static_cast<char*>(a.k) + (page * a.k_page_stride + slot * a.k_slot_stride) * elem;
+    char* dv = static_cast<char*>(a.v) + (page * a.v_page_stride + slot * a.v_slot_stride) * elem;
+    for (int c0 = 0; c0 < pieces; c0 += APPEND_UNROLL * 32) {
+        if (WIDE && c0) load(c0);
+#pragma unroll
+        for (int u = 0; u < APPEND_UNROLL; ++u) {
+            const int c = c0 + u * 32 + lane, h = c >> head_log, d = (c - (h << head_log)) * 16;
+            if (c < pieces) {
+                *reinterpret_cast<uint4*>(dk + h * a.k_head_stride * elem + d) = kr[u];
+                *reinterpret_cast<uint4*>(dv + h * a.v_head_stride * elem + d) = vr[u];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Checks, and the choice of a kernel
+// ------------------------------------------------------------------------------------------------------
+int check_cache(const CmePaged* a, const char* what) {
+    CME_REQUIRE(a->dtype == CME_F32 || a->dtype == CME_BF16, CME_ERR_UNSUPPORTED, "%s: unsupported dtype", what);
+    CME_REQUIRE(a->head_dim == 32 || a->head_dim == 64 || a->head_dim == 128, CME_ERR_SHAPE, "%s: head size %d is not 32, 64 or 128",
+                what, a->head_dim);
+    CME_REQUIRE(a->page >= 8 && a->page % 8 == 0, CME_ERR_SHAPE, "%s: pages of %d slots (a multiple of 8 is needed)", what, a->page);
+    CME_REQUIRE(a->seqs >= 0 && a->rows >= 0 && a->kv_heads > 0 && a->kv_heads <= 65535 && a->width >= 0 && a->num_pages >= 0 &&
+                a->max_len >= 0, CME_ERR_SHAPE, "%s: bad sizes", what);
+    const int per16 = a->dtype == CME_F32 ? 4 : 8;
+    auto ok = [&](const void* p, long long s0, long long s1, long long s2) {
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % per16 == 0 && s1 % per16 == 0 && s2 % per16 == 0;
+    };
+    CME_REQUIRE(ok(a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride) && ok(a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride),
+                CME_ERR_SHAPE, "%s: the cache has to start, and its strides have to be, at multiples of 16 bytes", what);
+    CME_REQUIRE(ok(a->q, a->q_token, a->q_head, 0) && ok(a->nv, a->v_token, a->v_head, 0), CME_ERR_SHAPE,
+                "%s: new rows have to start, and their strides have to be, at multiples of 16 bytes", what);
+    return CME_OK;
+}
+
+constexpr int MAX_SPLITS = 128;
+
+// backend: 0 by the rule, 1 + PagedKernel otherwise.  splits: 0 by the rule; k parts (in a cluster where the kernel has that form), -k
+// parts through scratch.
+int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* plan) {
+    const int group = a->heads / a->kv_heads;
+    const long long rows = (long long)a->rows * group;     // of one key head
+    const bool tc = a->dtype == CME_BF16 && a->head_dim >= 64 && group <= 128;
+    CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
+    CME_REQUIRE(backend != 1 + PAGED_TC || tc, CME_ERR_UNSUPPORTED,
+                "paged attention: the tcgen05 kernel takes bf16, head sizes 64 and 128 and up to 128 query heads per key head");
+    if (backend) plan->kernel = backend - 1;
+    else if (rows <= 16ll * a->seqs) plan->kernel = PAGED_SINGLE;
+    else plan->kernel = PAGED_ROWS;
+    plan->row_tile = plan->kernel == PAGED_SINGLE ? 16 : plan->kernel == PAGED_ROWS ? 64 : 128 / group * group;
+    const long long tiles = rows / plan->row_tile + std::min(a->seqs, a->rows);      // each sequence adds less than one
+    const int key_tile = plan->kernel == PAGED_TC ? PAGED_TC_KEYS : paged_mma_key_tile(a->dtype, a->head_dim);
+    const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
+    const int key_tiles = std::max(1, cme_cdiv(longest, key_tile));
+    const long long ctas = tiles * a->kv_heads;
+    const int resident = plan->kernel == PAGED_SINGLE ? 2 : plan->kernel == PAGED_ROWS ? 1 : a->head_dim == 64 ? 4 : 2;
+    int parts = splits < 0 ? -splits : splits;
+    if (!parts) parts = ctas ? (int)std::min((long long)key_tiles, (2ll * sms * resident - 1) / ctas / 2 + 1) : 1;
+    parts = std::max(1, std::min(parts, MAX_SPLITS));
+    plan->cluster = plan->kernel == PAGED_SINGLE && splits >= 0 && parts <= 8 && parts > 1;
+    if (plan->cluster) {                                   // 2, 4 or 8 CTAs
+        int c = 2;
+        while (c < parts) c *= 2;
+        parts = c;
+    }
+    plan->splits = parts;
+    plan->split_keys = cme_cdiv(key_tiles, parts) * key_tile;
+    CME_REQUIRE(tiles * parts < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many rows");
+    plan->tiles = (int)tiles;
+    return CME_OK;
+}
+
+long long ws_bytes(const CmePaged* a, const PagedPlan& p) {
+    if (p.splits == 1 || p.cluster) return 0;
+    const long long parts = (long long)a->rows * a->heads * p.splits;
+    return ((parts * 2 + 3) / 4 * 4 + parts * a->head_dim) * 4;
+}
+
+int check_attention(const CmePaged* a) {
+    const int rc = check_cache(a, "paged attention");
+    if (rc) return rc;
+    CME_REQUIRE(a->heads > 0 && a->heads % a->kv_heads == 0, CME_ERR_SHAPE, "paged attention: %d heads do not share %d key heads evenly",
+                a->heads, a->kv_heads);
+    CME_REQUIRE(a->scale > 0.f && a->scale < INFINITY, CME_ERR_SHAPE, "paged attention: the scale has to be positive and finite");
+    return CME_OK;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encoder() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* sym = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(sym);
+    });
+    return fn;
+}
+
+}  // namespace
+
+// Map over (column, slot, head, page) with box (box_cols, box_rows, 1, 1).  Page num_pages lies behind it: such a box is filled with zeros.
+int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long long page_stride, long long head_stride,
+                   long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+    EncodeTiledFn enc = encoder();
+    CME_REQUIRE(enc != nullptr, CME_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const long long e = a->dtype == CME_F32 ? 4 : 2;
+    cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->page, (cuuint64_t)a->kv_heads, (cuuint64_t)std::max(1, a->num_pages)};
+    // the stride along a dimension of one entry leads nowhere
+    cuuint64_t strides[3] = {(cuuint64_t)(slot_stride * e), (cuuint64_t)((a->kv_heads > 1 ? head_stride : a->head_dim) * e),
+                             (cuuint64_t)((a->num_pages > 1 ? page_stride : a->head_dim) * e)};
+    cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(out, a->dtype == CME_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                     const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CME_REQUIRE(r == CUDA_SUCCESS, CME_ERR_CUDA, "paged cache: cuTensorMapEncodeTiled failed (%d): strides %lld %lld %lld", (int)r,
+                page_stride, head_stride, slot_stride);
+    return CME_OK;
+}
+
+CME_API int cme_paged_append(const CmePaged* a, void* stream) {
+    const int rc = check_cache(a, "cache append");
+    if (rc) return rc;
+    if (a->rows == 0 || a->seqs == 0 || a->num_pages == 0 || a->width == 0) return CME_OK;
+    const int elem = a->dtype == CME_F32 ? 4 : 2;
+    int head_log = 0;
+    while ((16 << head_log) < a->head_dim * elem) ++head_log;
+    const bool wide = (a->kv_heads << head_log) > APPEND_UNROLL * 32;
+    const dim3 grid(cme_cdiv(a->rows, APPEND_WARPS));
+    auto* kernel = wide ? paged_append_kernel<true> : paged_append_kernel<false>;
+    CME_CUDA(cme_launch_dependent(kernel, grid, dim3(APPEND_WARPS * 32), 0, (cudaStream_t)stream, *a, paged_div(a->page), elem, head_log));
+    CME_LAUNCH_CHECK();
+    return CME_OK;
+}
+
+// What a call will take: {kernel, row tile, row tiles, parts, joined in a cluster, keys of a part}.
+CME_API int cme_paged_attention_plan(const CmePaged* a, int backend, int splits, int sms, int* out) {
+    PagedPlan p{};
+    int rc = check_attention(a);
+    if (rc || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
+    out[0] = p.kernel; out[1] = p.row_tile; out[2] = p.tiles; out[3] = p.splits; out[4] = p.cluster; out[5] = p.split_keys;
+    return CME_OK;
+}
+
+// Scratch of a call, in bytes.
+CME_API int cme_paged_attention_ws_bytes(const CmePaged* a, int backend, int splits, long long* out) {
+    PagedPlan p{};
+    int rc, sms;
+    if ((rc = check_attention(a)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
+    *out = ws_bytes(a, p);
+    return CME_OK;
+}
+
+CME_API int cme_paged_attention(const CmePaged* a, int backend, int splits, void* stream) {
+    PagedPlan p{};
+    int rc, sms;
+    if ((rc = check_attention(a)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
+    if (a->rows == 0 || a->seqs == 0) return CME_OK;
+    CmePaged none = *a;
+    if (a->num_pages == 0) {                               // a cache without memory: no key is there, and nothing is loaded
+        none.max_len = 0;
+        none.k = none.v = const_cast<void*>(a->q);
+        a = &none;
+    }
+    CME_REQUIRE(ws_bytes(a, p) <= a->ws_bytes, CME_ERR_SHAPE, "paged attention: %lld bytes of scratch, %lld are needed", a->ws_bytes,
+                ws_bytes(a, p));
+    cudaStream_t st = (cudaStream_t)stream;
+    if ((rc = p.kernel == PAGED_TC ? paged_attention_tc(a, p, st) : paged_attention_mma(a, p, st))) return rc;
+    return p.splits > 1 && !p.cluster ? paged_join(a, p.splits, st) : CME_OK;
+}

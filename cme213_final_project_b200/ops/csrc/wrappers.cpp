@@ -11,6 +11,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
@@ -19,7 +20,10 @@
 
 #include "attention_desc.h"
 #include "gemm_desc.h"
+#include "paged_desc.h"
+#include "token_desc.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -47,6 +51,10 @@ struct Native {
     int (*cme_dact_colsum)(int, const void*, const void*, void*, void*, float*, int, int, int, int, void*);
     int (*cme_embedding_fwd)(int, const int*, const void*, const void*, void*, int, int, int, int, void*);
     int (*cme_embedding_bwd)(int, const int*, const void*, void*, void*, int, int, int, int, int, void*);
+    int (*cme_paged_append)(const CmePaged*, void*);
+    int (*cme_paged_attention_ws_bytes)(const CmePaged*, int, int, long long*);
+    int (*cme_paged_attention)(const CmePaged*, int, int, void*);
+    int (*cme_next_token)(const CmeToken*, void*);
 } lib;
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -366,6 +374,160 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* a, Py_ssize_t) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Generation: the paged cache, attention over it, the next token
+// ---------------------------------------------------------------------------------------------------------------------
+// A tensor on the current device with so many dimensions, whose last one is contiguous; undefined for None where that is allowed.
+at::Tensor strided(PyObject* o, const char* what, int dims, bool optional = false) {
+    if (optional && o == Py_None) return at::Tensor();
+    if (!THPVariable_Check(o)) fail(PyExc_TypeError, "native ops take tensors");
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_cuda() || t.get_device() != c10::cuda::current_device())
+        fail(native_error, std::string(what) + " has to be on the current CUDA device");
+    if (t.dim() != dims) fail(native_error, std::string(what) + " has to have " + std::to_string(dims) + " dimensions");
+    if (t.size(-1) > 1 && t.stride(-1) != 1) fail(native_error, std::string(what) + " has to be contiguous along its last dimension");
+    return t;
+}
+void same_type(const at::Tensor& t, at::ScalarType type, const char* what, const char* name) {
+    if (t.scalar_type() != type) fail(native_error, std::string(what) + " has to be " + name);
+}
+at::Tensor whole_numbers(PyObject* o, const char* what, int dims, bool optional = false) {
+    const at::Tensor t = strided(o, what, dims, optional);
+    if (t.defined()) same_type(t, at::kInt, what, "int32");
+    return t;
+}
+void has_size(const at::Tensor& t, int dim, long long n, const char* what) {
+    if (t.size(dim) != n)
+        fail(native_error, std::string(what) + " has size " + std::to_string(t.size(dim)) + " along dimension " + std::to_string(dim) +
+                               ", not " + std::to_string(n));
+}
+
+// a: cache_k, cache_v, pages, offsets, lengths; x: new rows [rows, heads, head_dim] of the cache's type
+CmePaged paged(const at::Tensor& x, PyObject* const* a) {
+    const at::Tensor k = strided(a[0], "cache_k", 4), v = strided(a[1], "cache_v", 4);
+    const at::Tensor pages = whole_numbers(a[2], "pages", 2), offsets = whole_numbers(a[3], "offsets", 1),
+                     lengths = whole_numbers(a[4], "lengths", 1);
+    CmePaged d;
+    std::memset(&d, 0, sizeof d);
+    d.dtype = dtype(x);
+    if (k.scalar_type() != x.scalar_type() || v.scalar_type() != x.scalar_type())
+        fail(native_error, "the cache has to have the type of the new rows");
+    for (int i = 0; i < 4; ++i) has_size(v, i, k.size(i), "cache_v");
+    d.seqs = int32(pages.size(0)); d.width = int32(pages.size(1));
+    has_size(offsets, 0, (long long)d.seqs + 1, "offsets");
+    has_size(lengths, 0, d.seqs, "lengths");
+    d.num_pages = int32(k.size(0)); d.kv_heads = int32(k.size(1)); d.page = int32(k.size(2)); d.head_dim = int32(k.size(3));
+    has_size(x, 2, d.head_dim, "the new rows");
+    d.rows = int32(x.size(0));
+    d.max_len = INT32_MAX;
+    d.q = ptr(x); d.q_token = x.stride(0); d.q_head = x.stride(1);
+    d.k = ptr(k); d.k_page_stride = k.stride(0); d.k_head_stride = k.stride(1); d.k_slot_stride = k.stride(2);
+    d.v = ptr(v); d.v_page_stride = v.stride(0); d.v_head_stride = v.stride(1); d.v_slot_stride = v.stride(2);
+    d.pages = (const int*)ptr(pages); d.pages_ld = pages.stride(0);
+    d.offsets = (const int*)ptr(offsets);
+    d.lengths = (const int*)ptr(lengths);
+    return d;
+}
+
+// (k, v, cache_k, cache_v, pages, offsets, lengths)
+PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const at::Tensor k = strided(a[0], "k", 3), v = strided(a[1], "v", 3);
+    CmePaged d = paged(k, a + 2);
+    if (v.scalar_type() != k.scalar_type()) fail(native_error, "v has to have the type of k");
+    for (int i = 0; i < 3; ++i) has_size(v, i, k.size(i), "v");
+    has_size(k, 1, d.kv_heads, "k");
+    d.heads = d.kv_heads;
+    d.nv = ptr(v); d.v_token = v.stride(0); d.v_head = v.stride(1);
+    run([&](void* st) { return lib.cme_paged_append(&d, st); });
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, cache_k, cache_v, pages, offsets, lengths, scale | None, max_len | None, backend, splits)
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const at::Tensor q = strided(a[0], "q", 3);
+    CmePaged d = paged(q, a + 1);
+    d.heads = int32(q.size(1));
+    d.scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)d.head_dim)) : real(a[6]);
+    if (a[7] != Py_None) d.max_len = int32(whole(a[7]));
+    const int backend = int32(whole(a[8])), splits = int32(whole(a[9]));
+    const at::Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({d.rows, d.heads}, q.options().dtype(at::kFloat));
+    d.o = ptr(out);
+    d.lse = (float*)ptr(lse);
+    check(lib.cme_paged_attention_ws_bytes(&d, backend, splits, &d.ws_bytes));
+    at::Tensor ws;
+    if (d.ws_bytes) {
+        ws = floats((d.ws_bytes + 3) / 4, q);
+        d.ws = (float*)ptr(ws);
+    }
+    run([&](void* st) { return lib.cme_paged_attention(&d, backend, splits, st); });
+    return pack(out, lse);
+    END_HANDLE_TH_ERRORS
+}
+
+// (logits, history | None, lengths | None, prompts | None, repetition | None, presence | None, frequency | None, bias_ids | None,
+//  bias_values | None, temperature | None, allowed | None, noise | None, processed)
+PyObject* next_token(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const at::Tensor logits = strided(a[0], "logits", 2);
+    CmeToken d;
+    std::memset(&d, 0, sizeof d);
+    d.dtype = dtype(logits);
+    d.rows = int32(logits.size(0)); d.vocab = int32(logits.size(1));
+    d.logits = ptr(logits); d.logits_ld = logits.stride(0);
+    if (d.rows > 1 && d.logits_ld < d.vocab) fail(native_error, "the rows of logits may not overlap");
+    if (d.rows <= 1) d.logits_ld = std::max<long long>(d.logits_ld, d.vocab);
+    // one number per row
+    auto per_row = [&](PyObject* o, const char* what, at::ScalarType type) -> const void* {
+        const at::Tensor t = strided(o, what, 1, true);
+        if (!t.defined()) return nullptr;
+        same_type(t, type, what, type == at::kInt ? "int32" : "fp32");
+        has_size(t, 0, d.rows, what);
+        return ptr(t);
+    };
+    if (const at::Tensor h = whole_numbers(a[1], "history", 2, true); h.defined()) {
+        has_size(h, 0, d.rows, "history");
+        if (a[2] == Py_None) fail(native_error, "a history needs its lengths");
+        d.history = (const int*)ptr(h); d.history_ld = h.stride(0); d.history_len = int32(h.size(1));
+    }
+    d.lengths = (const int*)per_row(a[2], "lengths", at::kInt);
+    d.prompts = (const int*)per_row(a[3], "prompts", at::kInt);
+    d.repetition = (const float*)per_row(a[4], "repetition", at::kFloat);
+    d.presence = (const float*)per_row(a[5], "presence", at::kFloat);
+    d.frequency = (const float*)per_row(a[6], "frequency", at::kFloat);
+    d.temperature = (const float*)per_row(a[9], "temperature", at::kFloat);
+    if ((a[7] == Py_None) != (a[8] == Py_None)) fail(native_error, "bias_ids and bias_values belong together");
+    if (const at::Tensor ids = whole_numbers(a[7], "bias_ids", 2, true); ids.defined()) {
+        const at::Tensor values = strided(a[8], "bias_values", 2);
+        same_type(values, at::kFloat, "bias_values", "fp32");
+        has_size(ids, 0, d.rows, "bias_ids");
+        has_size(values, 0, d.rows, "bias_values");
+        has_size(values, 1, ids.size(1), "bias_values");
+        if (!ids.is_contiguous() || !values.is_contiguous()) fail(native_error, "biases have to be contiguous");
+        d.bias_ids = (const int*)ptr(ids); d.bias_values = (const float*)ptr(values); d.biases = int32(ids.size(1));
+    }
+    if (const at::Tensor m = whole_numbers(a[10], "allowed", 2, true); m.defined()) {
+        if (m.size(0) != 1) has_size(m, 0, d.rows, "allowed");
+        has_size(m, 1, ((long long)d.vocab + 31) / 32, "allowed");
+        d.allowed = (const int*)ptr(m); d.allowed_ld = m.size(0) == 1 ? 0 : m.stride(0);
+    }
+    if (const at::Tensor g = strided(a[11], "noise", 2, true); g.defined()) {
+        same_type(g, at::kFloat, "noise", "fp32");
+        has_size(g, 0, d.rows, "noise");
+        has_size(g, 1, d.vocab, "noise");
+        if (!g.is_contiguous()) fail(native_error, "noise has to be contiguous");
+        d.noise = (const float*)ptr(g);
+    }
+    const at::Tensor token = at::empty({d.rows}, logits.options().dtype(at::kInt)), logprob = floats(d.rows, logits);
+    const at::Tensor processed = truth(a[12]) ? at::empty({d.rows, d.vocab}, logits.options()) : at::Tensor();
+    d.token = (int*)ptr(token); d.logprob = (float*)ptr(logprob); d.processed = ptr(processed);
+    run([&](void* st) { return lib.cme_next_token(&d, st); });
+    return pack(token, logprob, processed);
+    END_HANDLE_TH_ERRORS
+}
+
 // The steps of ops.gemm before its native call: shapes, the result, column sums and the descriptor, 5 of the 18 us that the call
 // took as Python statements.  Returns (out, column sums | None, descriptor in a bytearray, behind which lies the count that
 // colsum_slabs points to).
@@ -490,6 +652,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     GET(cme_last_error); GET(cme_cross_entropy); GET(cme_attention_fwd); GET(cme_attention_bwd); GET(cme_attention_path);
     GET(cme_attention_gemm_ws_bytes); GET(cme_layernorm_fwd); GET(cme_layernorm_bwd_blocks); GET(cme_layernorm_bwd);
     GET(cme_bias_act_residual); GET(cme_colsum_splits); GET(cme_dact_colsum); GET(cme_embedding_fwd); GET(cme_embedding_bwd);
+    GET(cme_paged_append); GET(cme_paged_attention_ws_bytes); GET(cme_paged_attention); GET(cme_next_token);
 #undef GET
     lib = next;
     Py_XSETREF(native_error, Py_NewRef(a[0]));
@@ -506,7 +669,7 @@ PyObject* counted(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 }
 PyMethodDef methods[] = {METHOD(bind, 2), METHOD(init, 1), METHOD(gemm_prepare, 19), METHOD(cross_entropy, 5), METHOD(attention_fwd, 9), METHOD(attention_bwd, 15),
                          METHOD(layernorm_fwd, 6), METHOD(layernorm_bwd, 9), METHOD(bias_act_residual, 5), METHOD(dact_colsum, 6),
-                         METHOD(embedding_fwd, 3), METHOD(embedding_bwd, 7), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(embedding_fwd, 3), METHOD(embedding_bwd, 7), METHOD(cache_append, 7), METHOD(paged_attention, 10), METHOD(next_token, 13), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_wrappers", nullptr, -1, methods};
 
 }  // namespace
