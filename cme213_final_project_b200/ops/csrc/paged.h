@@ -18,6 +18,8 @@ enum PagedKernel : int { PAGED_SINGLE = 0, PAGED_ROWS = 1, PAGED_TC = 2 };
 
 int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long long page_stride, long long head_stride,
                    long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle);
+// Q as (column, head, token, -): a box of `group` heads and `tokens` tokens, so that its rows lie token by token.
+int paged_make_q_map(CUtensorMap* out, const CmePaged* a, int group, int tokens);
 int paged_attention_mma(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
 int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
 int paged_join(const CmePaged* a, int splits, cudaStream_t st);      // the parts in a->ws to a->o and a->lse

@@ -100,14 +100,14 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
                 "paged attention: the tcgen05 kernel takes bf16, head sizes 64 and 128 and up to 128 query heads per key head");
     if (backend) plan->kernel = backend - 1;
     else if (rows <= 16ll * a->seqs) plan->kernel = PAGED_SINGLE;
-    else plan->kernel = PAGED_ROWS;
-    plan->row_tile = plan->kernel == PAGED_SINGLE ? 16 : plan->kernel == PAGED_ROWS ? 64 : 128 / group * group;
+    else plan->kernel = tc ? PAGED_TC : PAGED_ROWS;
+    plan->row_tile = plan->kernel == PAGED_SINGLE ? 16 : plan->kernel == PAGED_ROWS ? 64 : (a->head_dim == 64 ? 1 : 2) * (128 / group * group);
     const long long tiles = rows / plan->row_tile + std::min(a->seqs, a->rows);      // each sequence adds less than one
     const int key_tile = plan->kernel == PAGED_TC ? PAGED_TC_KEYS : paged_mma_key_tile(a->dtype, a->head_dim);
     const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
     const int key_tiles = std::max(1, cme_cdiv(longest, key_tile));
     const long long ctas = tiles * a->kv_heads;
-    const int resident = plan->kernel == PAGED_SINGLE ? 2 : plan->kernel == PAGED_ROWS ? 1 : a->head_dim == 64 ? 4 : 2;
+    const int resident = plan->kernel == PAGED_SINGLE ? 2 : plan->kernel == PAGED_ROWS ? 1 : a->head_dim == 64 ? 4 : 1;
     int parts = splits < 0 ? -splits : splits;
     if (!parts) parts = ctas ? (int)std::min((long long)key_tiles, (2ll * sms * resident - 1) / ctas / 2 + 1) : 1;
     parts = std::max(1, std::min(parts, MAX_SPLITS));
@@ -174,6 +174,21 @@ int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long l
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     CME_REQUIRE(r == CUDA_SUCCESS, CME_ERR_CUDA, "paged cache: cuTensorMapEncodeTiled failed (%d): strides %lld %lld %lld", (int)r,
                 page_stride, head_stride, slot_stride);
+    return CME_OK;
+}
+
+int paged_make_q_map(CUtensorMap* out, const CmePaged* a, int group, int tokens) {
+    EncodeTiledFn enc = encoder();
+    CME_REQUIRE(enc != nullptr, CME_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->heads, (cuuint64_t)a->rows, 1};
+    cuuint64_t strides[3] = {(cuuint64_t)(a->heads > 1 ? a->q_head : a->head_dim) * 2, (cuuint64_t)(a->rows > 1 ? a->q_token : a->head_dim) * 2,
+                             (cuuint64_t)a->head_dim * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)group, (cuuint32_t)tokens, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(a->q), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CME_REQUIRE(r == CUDA_SUCCESS, CME_ERR_CUDA, "paged attention: the map of q failed (%d): strides %lld %lld", (int)r, a->q_token, a->q_head);
     return CME_OK;
 }
 

@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 from cme213_final_project_b200 import ops
 
 BF16, F32 = torch.bfloat16, torch.float32
-BACKENDS = ["single", "rows"]
+BACKENDS = ["single", "rows", "tc"]
 SINGLES = [(1, 1), (1, 2), (1, 63), (1, 64), (1, 65), (1, 129), (1, 700)]
 CHUNKS = [(1, 1), (5, 5), (17, 130), (64, 64), (130, 300), (0, 77), (33, 33), (200, 457)]
 
