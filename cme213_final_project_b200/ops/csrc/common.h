@@ -84,6 +84,11 @@ static_assert(!cme_index32(1ll << 31) && cme_index32((1ll << 31) - 1) && (1ll <<
 // saved is the launch gap between consecutive kernels.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Lets the next kernel of the stream (launched through cme_launch_dependent) be scheduled as soon as every CTA of this one has come here or
+// ended, so that its set-up runs under this one's end.  It still waits for this kernel's completion in pdl_wait().  A kernel that
+// allocates tensor memory calls this after the allocation: the next kernel's CTAs could take what its own still need.
+__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t cme_launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                                         Args&&... args) {

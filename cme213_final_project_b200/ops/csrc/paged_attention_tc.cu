@@ -180,6 +180,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    pdl_release();
 
     constexpr uint32_t idesc_s = make_idesc(1, false, false, 128, KEYS);      // Q K^T: both K-major
     constexpr uint32_t idesc_o = make_idesc(1, false, true, 128, D);          // P V: V is MN-major
@@ -352,7 +353,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 m_ref = mx;
             }
             if (j > 0 && __any_sync(0xffffffffu, raise)) {
-                // (with one buffer S_j came after P_{j-1} V_{j-1})
+                // (with one buffer S_j came after P_{j-1} V_{j-1}; with two after P_{j-2} V_{j-2}, so that the parity is that of j - 1)
                 if (C::BUFFERS > 1 && !mbar_wait(&pv_done[half], (j - 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
@@ -404,7 +405,12 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
             l += s0 + s1;
         }
-        if (ok && nkv > 0) ok = C::BUFFERS > 1 ? mbar_wait(&pv_done[half], (nkv - 1) & 1, abort_flag) : mbar_wait(s_full, nkv & 1, abort_flag);
+        if (ok && nkv > 0) {
+            // With two buffers S_{nkv-1} says that P V is complete up to block nkv - 3 only, and one parity does not tell a phase from the
+            // next but one: the last two are awaited one by one.
+            if (C::BUFFERS > 1) ok = (nkv < 2 || mbar_wait(&pv_done[half], (nkv - 2) & 1, abort_flag)) && mbar_wait(&pv_done[half], (nkv - 1) & 1, abort_flag);
+            else ok = mbar_wait(s_full, nkv & 1, abort_flag);
+        }
         if (ok) {
             tc_fence_after();
             const int rr = t.first + row, tok = rr / p.group;

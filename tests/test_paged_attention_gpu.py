@@ -235,6 +235,25 @@ def test_cache_beyond_32_bits(backend):
     check((q, *small, table, offsets, lengths), got)
 
 
+@pytest.mark.parametrize("D,dtype", [(128, F32), (64, F32), (128, BF16), (64, BF16)])
+@pytest.mark.parametrize("splits", [0, 1, 2, 8, -1])
+def test_many_long_sequences(D, dtype, splits):
+    """Enough keys that their tiles come out of memory in any order; two of the sequences against 64 bits."""
+    seqs, page, KV = 16, 16, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    lengths = [2048 + 131 * b for b in range(seqs)]
+    width = -(-lengths[-1] // page)
+    table = torch.randperm(seqs * width, generator=g, device="cuda").to(torch.int32).view(seqs, width)
+    ck, cv = (torch.randn(seqs * width, KV, page, D, generator=g, device="cuda", dtype=dtype) for _ in range(2))
+    q = torch.randn(seqs, KV, D, generator=g, device="cuda", dtype=dtype)
+    offsets = torch.arange(seqs + 1, dtype=torch.int32).cuda()
+    lens = torch.tensor(lengths, dtype=torch.int32).cuda()
+    for _ in range(3):
+        out, lse = ops.paged_attention(q, ck, cv, table, offsets, lens, backend="single", splits=splits)
+    for b in (1, 14):
+        check((q[b:b + 1], ck, cv, table[b:b + 1], offsets[:2], lens[b:b + 1]), (out[b:b + 1], lse[b:b + 1]))
+
+
 def test_another_stream_and_a_graph():
     args = make(SINGLES, 4, 2, 64, 16, BF16, seed=7)
     want = ops.paged_attention(*args)
@@ -251,12 +270,15 @@ def test_another_stream_and_a_graph():
     assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1])
 
 
-def test_the_same_bits_every_time():
-    for pairs in (SINGLES, CHUNKS):
-        args = make(pairs, 4, 2, 64, 16, BF16, seed=8)
-        for splits in (0, -5):
-            a, b = (ops.paged_attention(*args, splits=splits) for _ in range(2))
-            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (128, F32)])
+def test_the_same_bits_every_time(D, dtype):
+    for pairs in (SINGLES, CHUNKS, [(700, 900)] * 3):
+        args = make(pairs, 4, 2, D, 16, dtype, seed=8)
+        for splits in (0, 1, -5):
+            first = ops.paged_attention(*args, splits=splits)
+            for _ in range(40):
+                out, lse = ops.paged_attention(*args, splits=splits)
+                assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
