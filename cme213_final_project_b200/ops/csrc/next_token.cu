@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(256) next_token_kernel(const CmeToken p, int c
     k.before = reinterpret_cast<int*>(dyn + words + 1);
     k.count = k.before + words;
     k.bias = k.count + records;
+    pdl_release();
     pdl_wait();
     // ---------------- marks and records ----------------
     if (words) {

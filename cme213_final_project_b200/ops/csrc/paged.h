@@ -10,11 +10,15 @@ struct PagedPlan {
     int kernel;          // PAGED_*
     int row_tile;        // rows (tokens x query heads of one key head) of a CTA
     int tiles;           // row tiles of all sequences at the most
-    int splits;          // parts that the keys of a row tile are divided into
-    int cluster;         // non-zero: the parts are one cluster's CTAs, which join them through shared memory
-    int split_keys;      // keys of a part otherwise (multiple of the key tile); the parts are joined through `ws`
+    int splits;          // parts that the keys of a row tile are divided into; stream: CTAs
+    int split_keys;      // keys of a part (multiple of the key tile; rows and tc)
 };
-enum PagedKernel : int { PAGED_SINGLE = 0, PAGED_ROWS = 1, PAGED_TC = 2 };
+enum PagedKernel : int {
+    PAGED_CLUSTER = 0,   // up to 16 rows a tile; the parts are one cluster's CTAs, which join them through shared memory
+    PAGED_STREAM = 1,    // up to 16 rows a tile; all tiles' keys in a row, divided among the CTAs; joined through `ws`
+    PAGED_ROWS = 2,      // 64 rows; joined through `ws`, as are the next one's
+    PAGED_TC = 3,        // tcgen05, 128 rows (head size 128: 256)
+};
 
 int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long long page_stride, long long head_stride,
                    long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle);
@@ -25,6 +29,7 @@ int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st
 int paged_join(const CmePaged* a, int splits, cudaStream_t st);      // the parts in a->ws to a->o and a->lse
 // Keys of the tiles that the kernels walk in.
 int paged_mma_key_tile(int dtype, int head_dim);
+int paged_mma_ctas(int dtype, int head_dim);               // of the kernels for up to 16 rows, on an SM
 constexpr int PAGED_TC_KEYS = 64;
 
 // Division by a page size that the host knows, for 0 <= x < 2^31: x / d = (x * m) >> s with m = ceil(2^s / d) and s = 31 + ceil(log2 d)

@@ -16,6 +16,7 @@ constexpr int APPEND_UNROLL = 4;           // 16-byte pieces per lane of keys, a
 
 template <bool WIDE>                       // whether a token has more pieces than one round of a warp takes
 __global__ void __launch_bounds__(APPEND_WARPS * 32) paged_append_kernel(const CmePaged a, PagedDiv page_div, int elem, int head_log) {
+    pdl_release();
     pdl_wait();
     const int token = blockIdx.x * APPEND_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (token >= a.rows) return;
@@ -89,34 +90,47 @@ int check_cache(const CmePaged* a, const char* what) {
 
 constexpr int MAX_SPLITS = 128;
 
-// backend: 0 by the rule, 1 + PagedKernel otherwise.  splits: 0 by the rule; k parts (in a cluster where the kernel has that form), -k
-// parts through scratch.
+// backend: 0 by the rule, 1 up to 16 rows a tile, 2 rows, 3 tc.  splits: 0 by the rule; up to 16 rows: a cluster of so many CTAs (1, 2, 4
+// or 8), negative: the stream; others: parts of the keys.
 int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* plan) {
     const int group = a->heads / a->kv_heads;
     const long long rows = (long long)a->rows * group;     // of one key head
     const bool tc = a->dtype == CME_BF16 && a->head_dim >= 64 && group <= 128;
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
-    CME_REQUIRE(backend != 1 + PAGED_TC || tc, CME_ERR_UNSUPPORTED,
+    CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
                 "paged attention: the tcgen05 kernel takes bf16, head sizes 64 and 128 and up to 128 query heads per key head");
-    if (backend) plan->kernel = backend - 1;
-    else if (rows <= 16ll * a->seqs) plan->kernel = PAGED_SINGLE;
-    else plan->kernel = tc ? PAGED_TC : PAGED_ROWS;
-    plan->row_tile = plan->kernel == PAGED_SINGLE ? 16 : plan->kernel == PAGED_ROWS ? 64 : (a->head_dim == 64 ? 1 : 2) * (128 / group * group);
+    if (!backend) backend = rows <= 16ll * a->seqs ? 1 : tc ? 3 : 2;
+    plan->row_tile = backend == 1 ? 16 : backend == 2 ? 64 : (a->head_dim == 64 ? 1 : 2) * (128 / group * group);
     const long long tiles = rows / plan->row_tile + std::min(a->seqs, a->rows);      // each sequence adds less than one
-    const int key_tile = plan->kernel == PAGED_TC ? PAGED_TC_KEYS : paged_mma_key_tile(a->dtype, a->head_dim);
+    const int key_tile = backend == 3 ? PAGED_TC_KEYS : paged_mma_key_tile(a->dtype, a->head_dim);
     const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
     const int key_tiles = std::max(1, cme_cdiv(longest, key_tile));
     const long long ctas = tiles * a->kv_heads;
-    const int resident = plan->kernel == PAGED_SINGLE ? 2 : plan->kernel == PAGED_ROWS ? 1 : a->head_dim == 64 ? 4 : 1;
-    int parts = splits < 0 ? -splits : splits;
-    if (!parts) parts = ctas ? (int)std::min((long long)key_tiles, (2ll * sms * resident - 1) / ctas / 2 + 1) : 1;
-    parts = std::max(1, std::min(parts, MAX_SPLITS));
-    plan->cluster = plan->kernel == PAGED_SINGLE && splits >= 0 && parts <= 8 && parts > 1;
-    if (plan->cluster) {                                   // 2, 4 or 8 CTAs
-        int c = 2;
-        while (c < parts) c *= 2;
-        parts = c;
+    int parts = std::min(splits < 0 ? -splits : splits, MAX_SPLITS);
+    if (backend == 1) {
+        const int slots = sms * paged_mma_ctas(a->dtype, a->head_dim);
+        // As many CTAs of a cluster as let all run at once; the stream from where a CTA would have more than eight key tiles in its turns (head
+        // size 64, lengths from half of the longest on, us, cluster / stream: 96 items of up to 1024 keys 8.5 / 10.1, of 4096 21.9 / 20.5;
+        // 384 items of 256 9.9 / 11.2, of 1024 23.0 / 21.4.  128: 32 items of 4096 14.1 / 17.7, 8 of 16384 33.6 / 21.8).
+        int c = 1;
+        while (c < 8 && c < key_tiles && ctas * c * 2 <= slots) c *= 2;
+        const long long turns = ctas ? (ctas * c + slots - 1) / slots : 1;
+        const bool cluster = splits ? splits > 0 : turns * cme_cdiv(key_tiles, c) <= 8;
+        plan->kernel = cluster ? PAGED_CLUSTER : PAGED_STREAM;
+        if (cluster) {
+            const int want = splits ? parts : c;
+            parts = 1;
+            while (parts < want && parts < 8) parts *= 2;
+        } else {
+            CME_REQUIRE(ctas * (key_tiles + 8ll) < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many keys");
+            parts = (int)std::min((long long)slots, std::max(1ll, ctas * key_tiles));
+        }
+    } else {
+        plan->kernel = backend == 2 ? PAGED_ROWS : PAGED_TC;
+        const int resident = backend == 2 ? 1 : a->head_dim == 64 ? 4 : 1;
+        if (!parts) parts = ctas ? (int)std::min((long long)key_tiles, std::max(1ll, (long long)sms * resident / ctas)) : 1;
     }
+    parts = std::max(1, parts);
     plan->splits = parts;
     plan->split_keys = cme_cdiv(key_tiles, parts) * key_tile;
     CME_REQUIRE(tiles * parts < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many rows");
@@ -125,9 +139,9 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
 }
 
 long long ws_bytes(const CmePaged* a, const PagedPlan& p) {
-    if (p.splits == 1 || p.cluster) return 0;
-    const long long parts = (long long)a->rows * a->heads * p.splits;
-    return ((parts * 2 + 3) / 4 * 4 + parts * a->head_dim) * 4;
+    if (p.kernel == PAGED_CLUSTER || (p.kernel != PAGED_STREAM && p.splits == 1)) return 0;
+    const long long parts = p.kernel == PAGED_STREAM ? p.splits * 32ll : (long long)a->rows * a->heads * p.splits;
+    return ((parts * 2 + 3) / 4 * 4 + parts * a->head_dim + (p.kernel == PAGED_STREAM ? p.splits * 8ll : 0)) * 4;
 }
 
 int check_attention(const CmePaged* a) {
@@ -207,12 +221,12 @@ CME_API int cme_paged_append(const CmePaged* a, void* stream) {
     return CME_OK;
 }
 
-// What a call will take: {kernel, row tile, row tiles, parts, joined in a cluster, keys of a part}.
+// What a call will take: {kernel, row tile, row tiles, parts, keys of a part}.
 CME_API int cme_paged_attention_plan(const CmePaged* a, int backend, int splits, int sms, int* out) {
     PagedPlan p{};
     int rc = check_attention(a);
     if (rc || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
-    out[0] = p.kernel; out[1] = p.row_tile; out[2] = p.tiles; out[3] = p.splits; out[4] = p.cluster; out[5] = p.split_keys;
+    out[0] = p.kernel; out[1] = p.row_tile; out[2] = p.tiles; out[3] = p.splits; out[4] = p.split_keys;
     return CME_OK;
 }
 
@@ -240,5 +254,5 @@ CME_API int cme_paged_attention(const CmePaged* a, int backend, int splits, void
                 ws_bytes(a, p));
     cudaStream_t st = (cudaStream_t)stream;
     if ((rc = p.kernel == PAGED_TC ? paged_attention_tc(a, p, st) : paged_attention_mma(a, p, st))) return rc;
-    return p.splits > 1 && !p.cluster ? paged_join(a, p.splits, st) : CME_OK;
+    return p.splits > 1 && p.kernel >= PAGED_ROWS ? paged_join(a, p.splits, st) : CME_OK;
 }
