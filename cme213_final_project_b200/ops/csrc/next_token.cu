@@ -4,10 +4,10 @@
 //     token = argmax of x (+ noise, where temperature > 0), the lowest index of equals;   logprob = x[token] - logsumexp(x)
 // Every step is one rounded operation, in this order, so that equal values stay equal and the lowest index decides.
 //
-// What bounds it: the bytes of a row (logits, noise, processed).  Only tokens of the history or with a bias need more than the division
-// and the mask.  A bitmap of the vocabulary in shared memory marks them, and the number of marks before one is its place among
-// the records (count, bias), of which there are as many as marked tokens: 6 KB of marks for 50304 tokens and one byte of them to look at
-// for eight logits, where counts for the whole vocabulary would take 200 KB to clear and read.
+// What bounds it: the bytes of a row (logits, noise, processed); with few rows, the chain of loads and barriers before them.  Most tokens
+// need the division and the mask only.  Those of the history or with a bias are marked, one bit each in shared memory, and left out of the
+// pass (done inside it, a marked token costs its warp 100 instructions); afterwards a thread each does all steps of them.  The number of marks before a token is its place among the records (count, bias, token): 12 KB of marks and numbers and as many
+// records as entries for 50304 tokens, where counts by token take 200 KB, or have to be made and cleared 8192 at a time.
 // A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary; maxima, sums and picks are joined in the first one's
 // shared memory.
 #include "common.h"
@@ -22,6 +22,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_CLUSTER = 8;
+constexpr size_t MAX_SMEM = 160 * 1024;    // of marks and records
 
 // Running softmax statistics and the pick of some tokens.
 struct Pick {
@@ -35,11 +36,12 @@ __device__ __forceinline__ bool above(float y, int at, float best, int best_at) 
     if (y != y || best != best) return y != y && (best == best || at < best_at);
     return y > best || (y == best && at < best_at);
 }
-__device__ __forceinline__ float exp_of(float x) {
+__device__ __forceinline__ float exp2_of(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * LOG2E));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * LOG2E); }
 __device__ __forceinline__ Pick join(const Pick& a, const Pick& b) {
     Pick r;
     r.m = fmaxf(a.m, b.m);
@@ -62,81 +64,261 @@ __device__ __forceinline__ Pick shfl_xor(const Pick& p, int o) {
     return r;
 }
 
-// The marked tokens of a slice and their records, in shared memory.
-struct Marks {
-    unsigned* bits;          // [words + 1]
-    int* before;             // [words] marks in the words before
-    int* count;              // [marks] times generated; bit 31: in the history
-    int* bias;               // [marks] last entry of the biases, or -1
-    __device__ __forceinline__ int place(int local) const {
-        return before[local >> 5] + __popc(bits[local >> 5] & ((1u << (local & 31)) - 1u));
-    }
-};
+constexpr int KEPT = 4;          // entries of a history that a thread keeps in registers
+constexpr int STAGES = 4;        // of a thread's ring of loads
 
-// Entries of the history that are tokens of [v0, v1); f(local index, was it generated).
-template <typename F> __device__ __forceinline__ void for_history(const CmeToken& p, int row, int v0, int v1, F&& f) {
-    if (!p.history) return;
-    const int n = max(0, min(p.lengths[row], p.history_len)), given = p.prompts ? p.prompts[row] : 0;
-    const int* h = p.history + row * p.history_ld;
-    for (int j = threadIdx.x; j < n; j += blockDim.x) {
-        const int id = h[j];
-        if (id >= v0 && id < v1) f(id - v0, j >= given);
-    }
-}
-template <typename F> __device__ __forceinline__ void for_biases(const CmeToken& p, int row, int v0, int v1, F&& f) {
-    if (!p.bias_ids) return;
-    const int* ids = p.bias_ids + (long long)row * p.biases;
-    for (int j = threadIdx.x; j < p.biases; j += blockDim.x) {
-        const int id = ids[j];
-        if (id >= v0 && id < v1) f(id - v0, j);
-    }
-}
-
+// Eight tokens of a thread: bf16 sixteen bytes in a row, fp32 twice sixteen bytes, a warp's width apart.
 template <typename T> struct Vec;
 template <> struct Vec<__nv_bfloat16> {
-    static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* f) { unpack8(__ldcs(reinterpret_cast<const uint4*>(p)), f); }
-    static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) { __stcs(reinterpret_cast<uint4*>(p), pack8(f)); }
+    static constexpr int N = 8, PIECES = 1;
+    typedef uint4 Raw;
+    static __device__ __forceinline__ void unpack(const Raw* r, float* f) { unpack8(r[0], f); }
+    static __device__ __forceinline__ Raw pack(const float* f, int) { return pack8(f); }
 };
 template <> struct Vec<float> {
-    static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const float* p, float* f) {
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    static constexpr int N = 4, PIECES = 2;
+    typedef float4 Raw;
+    static __device__ __forceinline__ void unpack(const Raw* r, float* f) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { f[4 * i] = r[i].x; f[4 * i + 1] = r[i].y; f[4 * i + 2] = r[i].z; f[4 * i + 3] = r[i].w; }
     }
-    static __device__ __forceinline__ void store(float* p, const float* f) {
-        __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
+    static __device__ __forceinline__ Raw pack(const float* f, int i) { return make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]); }
+};
+// The largest of three: a NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// The largest of the warp (the first a NaN if one is).
+__device__ __forceinline__ float warp_max_nan(float x) {
+    float y;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float warp_max_num(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float y;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// x / t, correctly rounded, for many x: with r = 1 / t correctly rounded and a quotient q that is off by one last place at the most, q + (x - q t) r
+// rounds to the right one (Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990), if t's
+// digits are not all ones and nothing under- or overflows; other x and t take the division itself.
+struct Divisor {
+    float t, r;
+    bool fine;
+    __device__ __forceinline__ explicit Divisor(float v) : t(v), r(1.f / v) {
+        fine = v > 0x1p-60f && v < 0x1p60f && (__float_as_uint(v) & 0x7fffffu) != 0x7fffffu;
+    }
+    __device__ __forceinline__ void apply8(float* x) const {
+        const F32x2 r2 = f2_splat(r), t2 = f2_splat(-t);
+        float q[8];
+        // smallest and largest magnitude; a NaN shows in the largest
+        float low = fabsf(x[0]), high = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            low = min3(low, fabsf(x[e]), fabsf(x[e + 1]));
+            high = max3_nan(high, fabsf(x[e]), fabsf(x[e + 1]));
+            const F32x2 v = f2_pack(x[e], x[e + 1]);
+            F32x2 d = f2_mul(v, r2);
+            d = f2_fma(f2_fma(d, t2, v), r2, d);
+            d = f2_fma(f2_fma(d, t2, v), r2, d);
+            f2_unpack(d, q[e], q[e + 1]);
+        }
+        if (fine && low > 0x1p-60f && high < 0x1p60f) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = q[e];
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 8; ++e) {                  // (one division in the code; the registers are moved round)
+                const float d = __fdiv_rn(x[0], t);
+#pragma unroll
+                for (int k = 0; k < 7; ++k) x[k] = x[k + 1];
+                x[7] = d;
+            }
+        }
     }
 };
+
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
 
 // VECTOR: logits, processed and noise have their 16-byte boundaries at the same elements of a row.
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(256) next_token_kernel(const CmeToken p, int cluster, int slice, int words, int records) {
+__global__ void __launch_bounds__(256, 4) next_token_kernel(const CmeToken p, int cluster, int slice, int words, int records, bool biased) {
+    // [words + 1] marks, [words] marks in the words before, then for each mark [records]: times generated (bit 31: in the history), last bias
+    // + 1, index in the slice
     extern __shared__ __align__(16) unsigned dyn[];
     __shared__ Pick parts[8], mine;
     __shared__ int scan[8], total;
-    constexpr int N = VECTOR ? Vec<T>::N : 1;
-    const int rank = blockIdx.x % cluster, row = blockIdx.x / cluster;
+    constexpr int N = VECTOR ? Vec<T>::N : 1, PIECES = Vec<T>::PIECES;
+    const int rank = blockIdx.x % cluster, row = blockIdx.x / cluster, tid = threadIdx.x, threads = blockDim.x;
     const int v0 = min(p.vocab, rank * slice), v1 = min(p.vocab, v0 + slice);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    Marks k;
-    k.bits = dyn;
-    k.before = reinterpret_cast<int*>(dyn + words + 1);
-    k.count = k.before + words;
-    k.bias = k.count + records;
-    pdl_release();
+    const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
+    unsigned* const marks = dyn;
+    int* const before = reinterpret_cast<int*>(marks + words + 1);
+    int* const count = before + words;
+    int* const bias = count + records;
+    int* const which = bias + records;
     pdl_wait();
-    // ---------------- marks and records ----------------
+    // What does not depend on one another is on its way together: the row's numbers, its history, its first logits.
+    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f;
+    const float freq = p.frequency ? p.frequency[row] : 0.f, temp = p.temperature ? p.temperature[row] : 1.f;
+    const int told = p.history ? max(0, min(p.lengths[row], p.history_len)) : 0, given = p.history && p.prompts ? p.prompts[row] : 0;
+    const int* hist = p.history + row * p.history_ld;
+    int kept[KEPT];
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+        const int j = tid + k * threads;
+        kept[k] = p.history && j < p.history_len ? hist[j] : -1;
+    }
+    const T* src = static_cast<const T*>(p.logits) + row * p.logits_ld;
+    T* dst = p.processed ? static_cast<T*>(p.processed) + (long long)row * p.vocab : nullptr;
+    const float* noise = p.noise && temp > 0.f ? p.noise + (long long)row * p.vocab : nullptr;
+    const unsigned* allowed = p.allowed ? reinterpret_cast<const unsigned*>(p.allowed) + row * p.allowed_ld : nullptr;
+    const int all_words = (p.vocab + 31) >> 5;
+
+    const bool divides = temp > 0.f && p.temperature;
+    const Divisor by(divides ? temp : 1.f);
+    // A warp shares its maximum and the value to beat, so that few groups change them (a new largest of k groups comes once in k; with values
+    // of a lane's own, some lane of 32 has one in most groups).  The loops over tokens go up, so that a tie leaves the lower index.
+    Pick best = nothing();
+    float to_beat = -INFINITY;
+    // Values x of n tokens and the same with noise, y; -inf: not to be looked at.  Whole warps; token(e): its index; `any_order`: a tie may be won.
+    auto take = [&](const float* x, const float* y, auto number, auto&& token, bool any_order) {
+        constexpr int n = decltype(number)::value;
+        float mx = x[0], top = y[0];
+        if constexpr (n > 1) {
+#pragma unroll
+            for (int e = 0; e < n; e += 2) { mx = max3(mx, x[e], x[e + 1]); top = max3_nan(top, y[e], y[e + 1]); }
+        }
+        if (__any_sync(0xffffffffu, mx > best.m || !(top < to_beat || (top == to_beat && !any_order)))) {      // a NaN too
+            mx = warp_max_num(mx);
+            if (mx > best.m) {
+                best.s *= exp_of(best.m - mx);             // (nothing yet: exp(-inf) = 0)
+                best.m = mx;
+            }
+            if (__any_sync(0xffffffffu, top != top)) {     // a NaN, of a logit or of noise that is not finite (which counts only where x does)
+#pragma unroll
+                for (int e = 0; e < n; ++e) {
+                    if (x[e] != -INFINITY && y[e] != -INFINITY && above(y[e], token(e), best.y, best.at)) {
+                        best.y = y[e];
+                        best.x = x[e];
+                        best.at = token(e);
+                    }
+                }
+            } else if (top > best.y || (any_order && top == best.y && top != -INFINITY)) {
+                int at = token(n - 1);
+                float xv = x[n - 1];
+#pragma unroll
+                for (int e = n - 2; e >= 0; --e) if (y[e] == top) { at = token(e); xv = x[e]; }
+                if (top > best.y || at < best.at) { best.y = top; best.x = xv; best.at = at; }
+            }
+            to_beat = warp_max_nan(best.y);
+        }
+        const float use = best.m == -INFINITY ? 0.f : best.m;
+        if constexpr (n == 1) {
+            best.s += exp_of(x[0] - use);
+        } else {
+            const F32x2 shift = f2_splat(-use), scale = f2_splat(LOG2E);
+            F32x2 sum = f2_splat(0.f);
+#pragma unroll
+            for (int e = 0; e < n; e += 2) {
+                float a, b;
+                f2_unpack(f2_mul(f2_add(f2_pack(x[e], x[e + 1]), shift), scale), a, b);
+                sum = f2_add(sum, f2_pack(exp2_of(a), exp2_of(b)));
+            }
+            float a, b;
+            f2_unpack(sum, a, b);
+            best.s += a + b;
+        }
+    };
+    auto not_allowed = [&](int v, int n) -> unsigned {     // bits [v, v + n), n <= 8
+        if (!allowed) return 0;
+        const int w = v >> 5;
+        unsigned b = __ldg(allowed + w) >> (v & 31);
+        if ((v & 31) + n > 32 && w + 1 < all_words) b |= __ldg(allowed + w + 1) << (32 - (v & 31));
+        return ~b & ((1u << n) - 1u);
+    };
+
+    // the first element on a 16-byte boundary, then groups, then what is left; marks of a group are whole bits of one byte
+    const int head = VECTOR ? (int)((N - (row * p.logits_ld + v0) % N) % N) : v1 - v0;
+    const int a0 = min(v1, v0 + head), groups = VECTOR ? (v1 - a0) / N : 0;      // (of sixteen bytes)
+    const int origin = VECTOR ? v0 + head - N : v0;        // of the marks
+    // f(index from the origin on, was it generated) for the entries of the history, f(index from the origin on, entry) for those of the biases
+    auto for_history = [&](auto&& f) {
+#pragma unroll
+        for (int k = 0; k < KEPT; ++k) {
+            const int j = tid + k * threads;
+            if (j < told && kept[k] >= v0 && kept[k] < v1) f(kept[k] - origin, j >= given);
+        }
+        for (int j = tid + KEPT * threads; j < told; j += threads) {
+            const int id = hist[j];
+            if (id >= v0 && id < v1) f(id - origin, j >= given);
+        }
+    };
+    auto for_biases = [&](auto&& f) {
+        if (!biased) return;
+        const int* ids = p.bias_ids + (long long)row * p.biases;
+        for (int j = tid; j < p.biases; j += threads) {
+            const int id = ids[j];
+            if (id >= v0 && id < v1) f(id - origin, j);
+        }
+    };
+    typedef typename Vec<T>::Raw Raw;
+    const int stride = threads * PIECES, first = warp * 32 * PIECES + lane;      // a thread's groups: first, + 32 ..., a stride further ...
+    // A thread's loads travel through a ring of its own in shared memory, STAGES - 1 turns ahead: with one turn ahead in registers, 64 bytes a
+    // thread are on their way, and 1024 rows of 50304 in fp32 run at 3.9 TB/s.
+    uint4* const ring = reinterpret_cast<uint4*>(dyn + (words ? (2 * words + 1 + 3 * records + 3) / 4 * 4 : 0)) + tid;
+    const int pieces = PIECES + (p.noise ? 2 : 0);         // of 16 bytes, a turn
+    auto fetch = [&](int turn) {
+        if constexpr (VECTOR) {
+            uint4* to = ring + turn % STAGES * pieces * threads;
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) {
+                const int j = first + turn * stride + k * 32;
+                if (j < groups) {
+                    copy16(to + k * threads, src + a0 + j * N);
+                    if (noise) {
+#pragma unroll
+                        for (int e = 0; e < N / 4; ++e) copy16(to + (PIECES + k * (N / 4) + e) * threads, noise + a0 + j * N + e * 4);
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t) fetch(t);
+    float early = 0.f, early_noise = 0.f;                  // one by one, a thread's first token
+    if (!VECTOR && v0 + tid < v1) {
+        early = to_f32<T>(src[v0 + tid]);
+        if (noise) early_noise = noise[v0 + tid];
+    }
+    auto place = [&](int l) { return before[l >> 5] + __popc(marks[l >> 5] & ((1u << (l & 31)) - 1u)); };
     if (words) {
-        for (int i = threadIdx.x; i <= words; i += blockDim.x) k.bits[i] = 0;
+        for (int i = tid; i <= words; i += threads) marks[i] = 0;
+        for (int i = tid; i < 2 * records; i += threads) count[i] = 0;
         __syncthreads();
-        for_history(p, row, v0, v1, [&](int v, bool) { atomicOr(&k.bits[v >> 5], 1u << (v & 31)); });
-        for_biases(p, row, v0, v1, [&](int v, int) { atomicOr(&k.bits[v >> 5], 1u << (v & 31)); });
+        for_history([&](int l, bool) { atomicOr(&marks[l >> 5], 1u << (l & 31)); });
+        for_biases([&](int l, int) { atomicOr(&marks[l >> 5], 1u << (l & 31)); });
         __syncthreads();
         // marks before each word: a thread's own words, then the threads before it
-        const int each = (words + blockDim.x - 1) / blockDim.x, w0 = min(words, (int)threadIdx.x * each), w1 = min(words, w0 + each);
+        const int each = (words + threads - 1) / threads, w0 = min(words, tid * each), w1 = min(words, w0 + each);
         int sum = 0;
-        for (int w = w0; w < w1; ++w) sum += __popc(k.bits[w]);
+        for (int w = w0; w < w1; ++w) sum += __popc(marks[w]);
         int upto = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -147,124 +329,133 @@ __global__ void __launch_bounds__(256) next_token_kernel(const CmeToken p, int c
         __syncthreads();
         int at = upto - sum;
         for (int w = 0; w < warp; ++w) at += scan[w];
-        if (threadIdx.x == blockDim.x - 1) total = at + sum;
-        for (int w = w0; w < w1; ++w) { k.before[w] = at; at += __popc(k.bits[w]); }
-        __syncthreads();
-        for (int i = threadIdx.x; i < total; i += blockDim.x) { k.count[i] = 0; k.bias[i] = -1; }
+        if (tid == threads - 1) total = at + sum;
+        for (int w = w0; w < w1; ++w) { before[w] = at; at += __popc(marks[w]); }
         __syncthreads();
         // whole numbers: any order of the additions gives the same
-        for_history(p, row, v0, v1, [&](int v, bool made) {
-            int* c = &k.count[k.place(v)];
-            atomicOr(c, (int)0x80000000);
-            if (made) atomicAdd(c, 1);
+        for_history([&](int l, bool made) {
+            const int at = place(l);
+            which[at] = l;
+            atomicOr(&count[at], (int)0x80000000);
+            if (made) atomicAdd(&count[at], 1);
         });
-        for_biases(p, row, v0, v1, [&](int v, int j) { atomicMax(&k.bias[k.place(v)], j); });
-        __syncthreads();
+        for_biases([&](int l, int j) {
+            const int at = place(l);
+            which[at] = l;
+            atomicMax(&bias[at], j + 1);
+        });
     }
-    // ---------------- the row ----------------
-    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f;
-    const float freq = p.frequency ? p.frequency[row] : 0.f, temp = p.temperature ? p.temperature[row] : 1.f;
-    const bool warm = temp > 0.f;
-    const T* src = static_cast<const T*>(p.logits) + row * p.logits_ld;
-    T* dst = p.processed ? static_cast<T*>(p.processed) + (long long)row * p.vocab : nullptr;
-    const float* noise = p.noise && warm ? p.noise + (long long)row * p.vocab : nullptr;
-    const unsigned* allowed = p.allowed ? reinterpret_cast<const unsigned*>(p.allowed) + row * p.allowed_ld : nullptr;
-    Pick best = nothing();
-    // bits [v, v + n) of a row of words, n <= 8
-    const int all_words = (p.vocab + 31) >> 5;
-    auto allowed_bits = [&](int v, int n) {
-        const int w = v >> 5;
-        unsigned b = __ldg(allowed + w) >> (v & 31);
-        if ((v & 31) + n > 32 && w + 1 < all_words) b |= __ldg(allowed + w + 1) << (32 - (v & 31));
-        return b;
-    };
-    auto group = [&](int v, float* x, const float* g, auto count) {
-        constexpr int n = decltype(count)::value;
-        if (words) {
-            const int local = v - v0;
-            unsigned marked = __funnelshift_r(k.bits[local >> 5], k.bits[(local >> 5) + 1], local & 31) & ((1u << n) - 1u);
-            while (marked) {
-                const int i = __ffs(marked) - 1;
-                marked &= marked - 1;
-                const int at = k.place(local + i);
-                const int c = k.count[at], j = k.bias[at];
-                float t = 0.f;
-#pragma unroll
-                for (int e = 0; e < n; ++e) if (e == i) t = x[e];      // (registers have no index)
-                if (c < 0) t = t > 0.f ? __fdiv_rn(t, rep) : __fmul_rn(t, rep);
-                const int made = c & 0x7fffffff;
-                if (made) { t = __fsub_rn(t, __fmul_rn(freq, (float)made)); t = __fsub_rn(t, pres); }
-                if (j >= 0) t = __fadd_rn(t, p.bias_values[(long long)row * p.biases + j]);
-#pragma unroll
-                for (int e = 0; e < n; ++e) if (e == i) x[e] = t;
+    // tokens [from, to) one by one, whole warps
+    auto singles = [&](int from, int to) {
+        for (int b = from + warp * 32; b < to; b += threads) {
+            const int v = b + lane;
+            float x = -INFINITY, g = 0.f;
+            if (v < to) {
+                x = !VECTOR && v == v0 + tid ? early : to_f32<T>(src[v]);
+                if (noise) g = !VECTOR && v == v0 + tid ? early_noise : noise[v];
+                if (divides) x = __fdiv_rn(x, temp);
+                const int l = v - origin;
+                if (not_allowed(v, 1) || (words && (marks[l >> 5] >> (l & 31)) & 1)) x = -INFINITY;
+                if (dst) dst[v] = from_f32<T>(x);
             }
-        }
-        if (warm && p.temperature) {
-#pragma unroll
-            for (int e = 0; e < n; ++e) x[e] = __fdiv_rn(x[e], temp);
-        }
-        if (allowed) {
-            const unsigned ok = allowed_bits(v, n);
-#pragma unroll
-            for (int e = 0; e < n; ++e) if (!((ok >> e) & 1)) x[e] = -INFINITY;
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int e = 1; e < n; ++e) mx = fmaxf(mx, x[e]);
-        if (mx > best.m) {
-            best.s *= exp_of(best.m - mx);                 // (nothing yet: exp(-inf) = 0)
-            best.m = mx;
-        }
-        const float use = best.m == -INFINITY ? 0.f : best.m;
-#pragma unroll
-        for (int e = 0; e < n; ++e) {
-            best.s += exp_of(x[e] - use);
-            const float y = g && x[e] != -INFINITY ? __fadd_rn(x[e], g[e]) : x[e];
-            if (y > best.y || (y != y && best.y == best.y)) { best.y = y; best.x = x[e]; best.at = v + e; }
+            const float y = noise ? __fadd_rn(x, g) : x;
+            take(&x, &y, std::integral_constant<int, 1>{}, [&](int) { return v; }, false);
         }
     };
-    auto single = [&](int v) {
-        float x = to_f32<T>(src[v]);
-        const float g = noise ? noise[v] : 0.f;
-        group(v, &x, noise ? &g : nullptr, std::integral_constant<int, 1>{});
-        if (dst) dst[v] = from_f32<T>(x);
-    };
+    singles(v0, a0);
     if constexpr (VECTOR) {
-        // the first element of the slice on a 16-byte boundary, then groups, then what is left
-        const int head = (int)((N - (row * p.logits_ld + v0) % N) % N), a0 = min(v1, v0 + head), groups = (v1 - a0) / N;
-        if ((int)threadIdx.x < a0 - v0) single(v0 + threadIdx.x);
-        for (int i = threadIdx.x; i < groups; i += blockDim.x) {
-            const int v = a0 + i * N;
-            float x[N], g[N];
-            Vec<T>::load(src + v, x);
+        const uint8_t* bytes = reinterpret_cast<const uint8_t*>(marks);
+        auto eight = [&](int i, const Raw* r, const float4* g) {       // groups i (and i + 32)
+            float x[8];
+            Vec<T>::unpack(r, x);
+            if (divides) by.apply8(x);
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) {
+                const int j = i + k * 32;
+                unsigned no = 0xff;
+                if (j < groups) {
+                    no = allowed ? not_allowed(a0 + j * N, N) : 0;
+                    if (words) no |= N == 8 ? bytes[j + 1] : bytes[(j + 1) >> 1] >> ((j + 1) & 1) * 4;
+                }
+                if (no & ((1u << N) - 1u)) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) if ((no >> e) & 1) x[k * N + e] = -INFINITY;
+                }
+                if (dst && j < groups) __stcs(reinterpret_cast<Raw*>(dst + a0) + j, Vec<T>::pack(x, k));
+            }
+            auto token = [&](int e) { return a0 + (i + e / N * 32) * N + e % N; };
+            if (noise) {
+                const float* f = reinterpret_cast<const float*>(g);
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) f2_unpack(f2_add(f2_pack(x[e], x[e + 1]), f2_pack(f[e], f[e + 1])), y[e], y[e + 1]);
+                take(x, y, std::integral_constant<int, 8>{}, token, false);
+            } else {
+                take(x, x, std::integral_constant<int, 8>{}, token, false);
+            }
+        };
+        for (int turn = 0, i = first; i - lane < groups; ++turn, i += stride) {
+            fetch(turn + STAGES - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            const uint4* from = ring + turn % STAGES * pieces * threads;
+            Raw r[PIECES];
+            float4 g[2];
+#pragma unroll
+            for (int k = 0; k < PIECES; ++k) r[k] = *reinterpret_cast<const Raw*>(from + k * threads);
             if (noise) {
 #pragma unroll
-                for (int e = 0; e < N; e += 4) Vec<float>::load(noise + v + e, g + e);
+                for (int k = 0; k < 2; ++k) g[k] = *reinterpret_cast<const float4*>(from + (PIECES + k) * threads);
             }
-            group(v, x, noise ? g : nullptr, std::integral_constant<int, N>{});
-            if (dst) Vec<T>::store(dst + v, x);
+            eight(i, r, g);
         }
-        if (a0 + groups * N + (int)threadIdx.x < v1) single(a0 + groups * N + threadIdx.x);
-    } else {
-        for (int v = v0 + threadIdx.x; v < v1; v += blockDim.x) single(v);
+        singles(a0 + groups * N, v1);
     }
+    if (words) {
+        __syncthreads();                                   // the counts are made; what the pass wrote for marked tokens is overwritten
+        for (int b = warp * 32; b < total; b += threads) {
+            const int i = b + lane;
+            int v = 0;
+            float x = -INFINITY, g = 0.f;
+            if (i < total) {
+                const int c = count[i], made = c & 0x7fffffff, j = bias[i] - 1;
+                v = origin + which[i];
+                x = to_f32<T>(src[v]);
+                if (noise) g = noise[v];
+                if (c < 0) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+                if (made) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)made)), pres);
+                if (j >= 0) x = __fadd_rn(x, p.bias_values[(long long)row * p.biases + j]);
+                if (divides) x = __fdiv_rn(x, temp);
+                if (not_allowed(v, 1)) x = -INFINITY;
+                if (dst) dst[v] = from_f32<T>(x);
+            }
+            const float y = noise ? __fadd_rn(x, g) : x;
+            take(&x, &y, std::integral_constant<int, 1>{}, [&](int) { return v; }, true);
+        }
+    }
+    // (earlier, CTAs of the next kernel would crowd on the SMs that are done first: 1024 rows of 50304 183 us)
+    pdl_release();
     // ---------------- joins ----------------
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = join(best, shfl_xor(best, o));
     if (lane == 0) parts[warp] = best;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < warps; ++w) best = join(best, parts[w]);
-        mine = best;
+    if (warp == 0) {
+        best = lane < warps ? parts[lane] : nothing();
+#pragma unroll
+        for (int o = 4; o; o >>= 1) best = join(best, shfl_xor(best, o));
+        if (lane == 0) mine = best;
     }
     if (cluster > 1) {
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();
-        if (rank == 0 && threadIdx.x == 0)
-            for (int r = 1; r < cluster; ++r) best = join(best, *cl.map_shared_rank(&mine, r));
+        if (rank == 0 && warp == 0) {
+            best = lane < cluster ? *cl.map_shared_rank(&mine, lane) : nothing();
+#pragma unroll
+            for (int o = 4; o; o >>= 1) best = join(best, shfl_xor(best, o));
+        }
         cl.sync();
     }
-    if (rank == 0 && threadIdx.x == 0) {
+    if (rank == 0 && tid == 0) {
         const bool none = best.at == INT_MAX;
         p.token[row] = none ? -1 : best.at;
         p.logprob[row] = none ? -INFINITY : best.x - best.m - logf(best.s);
@@ -284,28 +475,31 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
     // As many CTAs as keep the SMs busy, with no fewer than 2048 tokens each.
     int cluster = 1;
     while (cluster < MAX_CLUSTER && (long long)p->rows * cluster < 4ll * sms && p->vocab / (2 * cluster) >= 2048) cluster *= 2;
-    const bool marks = (p->history && p->history_len) || (p->bias_ids && p->biases);
+    const bool biased = p->bias_ids && p->biases;
+    const bool marks = biased || (p->history && p->history_len);
     int slice, words, records;
     size_t smem;
-    for (;; cluster *= 2) {
+    for (;; cluster *= 2) {                                // smaller slices where a CTA's records would not fit
         slice = (cme_cdiv(p->vocab, cluster) + 31) / 32 * 32;
-        words = marks ? slice / 32 : 0;
-        records = marks ? (int)std::min((long long)slice, (long long)(p->history ? p->history_len : 0) + (p->bias_ids ? p->biases : 0)) : 0;
-        smem = marks ? ((size_t)2 * words + 1 + 2 * (size_t)records) * 4 : 0;
-        if (smem <= 200 * 1024) break;
+        words = marks ? slice / 32 + 1 : 0;                // (marks start up to eight tokens before the slice)
+        records = marks ? (int)std::min((long long)slice, (long long)(p->history ? p->history_len : 0) + (biased ? p->biases : 0)) : 0;
+        smem = marks ? ((size_t)2 * words + 1 + 3 * (size_t)records) * 4 : 0;
+        if (smem <= MAX_SMEM) break;
         CME_REQUIRE(cluster < MAX_CLUSTER, CME_ERR_LIMIT, "next token: a history of %d with a vocabulary of %d", p->history_len, p->vocab);
     }
     CME_REQUIRE((long long)p->rows * cluster < (1ll << 31), CME_ERR_LIMIT, "next token: too many rows");
     const int n = p->dtype == CME_F32 ? 4 : 8;
     auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
-    // rows of logits start at the same place between 16-byte boundaries as rows of noise and of the processed logits
-    const bool vector = al16(p->logits) && al16(p->processed) && al16(p->noise) && p->logits_ld % n == p->vocab % n;
+    // In groups of sixteen bytes, where there is more than a turn or two of them and rows of logits start at the same place between 16-byte boundaries as rows of noise and of the processed logits
+    const bool vector = slice >= 1024 && al16(p->logits) && al16(p->processed) && al16(p->noise) && p->logits_ld % n == p->vocab % n;
     auto* kernel = p->dtype == CME_F32 ? (vector ? next_token_kernel<float, true> : next_token_kernel<float, false>)
                                        : (vector ? next_token_kernel<__nv_bfloat16, true> : next_token_kernel<__nv_bfloat16, false>);
-    if (smem > 48 * 1024) CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    const int threads = slice <= 1024 ? 128 : 256;
+    if (vector) smem = (smem + 15) / 16 * 16 + (size_t)STAGES * threads * 16 * ((p->dtype == CME_F32 ? 2 : 1) + (p->noise ? 2 : 0));
+    if (smem > 48 * 1024) CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p->rows * cluster));
-    cfg.blockDim = dim3(slice <= 1024 ? 128 : 256);
+    cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute at[2];
@@ -316,7 +510,7 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    CME_CUDA(cudaLaunchKernelEx(&cfg, kernel, *p, cluster, slice, words, records));
+    CME_CUDA(cudaLaunchKernelEx(&cfg, kernel, *p, cluster, slice, words, records, biased));
     CME_LAUNCH_CHECK();
     return CME_OK;
 }

@@ -127,6 +127,14 @@ def test_lowest_index_of_equals(dtype):
     x[1, [8999, 4500, 77]] = 2.0
     x[2, [8999, 8998]] = 1.0
     assert ops.next_token(x)[0].tolist() == [0, 77, 8998]
+    # equals in what is done one by one (the ends of a row off the 16-byte boundaries, tokens of the history) and in groups
+    x = torch.zeros(9, 4099, dtype=dtype, device="cuda")
+    history = torch.tensor([[5], [4000], [0], [4098], [77], [1], [2], [3], [4]], dtype=torch.int32).cuda()
+    assert ops.next_token(x, history=history, lengths=torch.ones(9, dtype=torch.int32).cuda())[0].tolist() == [0] * 9
+    for row in range(9):
+        x[row, row:] = 1.0
+        x[row, 4000] = 1.0
+    assert ops.next_token(x, history=history, lengths=torch.ones(9, dtype=torch.int32).cuda())[0].tolist() == list(range(9))
 
 
 @pytest.mark.parametrize("V", [50, 9000])
