@@ -31,7 +31,7 @@ constexpr float RESCALE_THRESHOLD = 8.f;
 
 template <int D> struct Cfg;
 template <> struct Cfg<64> {
-    static constexpr int HALVES = 1, STAGES = 2, BUFFERS = 1, CTAS = 4, COLS = 128;
+    static constexpr int HALVES = 1, STAGES = 3, BUFFERS = 1, CTAS = 3, COLS = 128;
 };
 template <> struct Cfg<128> {
     static constexpr int HALVES = 2, STAGES = 4, BUFFERS = 2, CTAS = 1, COLS = 512;
@@ -41,7 +41,7 @@ template <int D> struct Sizes : Cfg<D> {
     static constexpr int SLABS = D / 64;                              // 64 columns = 128 bytes each
     static constexpr int Q_SLAB = 128 * 128, KV_SLAB = KEYS * 128;
     static constexpr int Q_BYTES = SLABS * Q_SLAB, KV_BYTES = SLABS * KV_SLAB;
-    static constexpr int LOADER = 4 * C::HALVES + (C::HALVES > 1 ? C::HALVES : 0);      // with one half, the warp that issues the MMAs loads too
+    static constexpr int LOADER = 5 * C::HALVES;                      // four warps of softmax and one that issues MMAs for each half, one that loads
     static constexpr int THREADS = (LOADER + 1) * 32;
     static constexpr int SMEM = C::HALVES * Q_BYTES + 2 * C::STAGES * KV_BYTES + 256;
     static constexpr int HALF_COLS = C::COLS / C::HALVES;            // S buffers, then O
@@ -89,14 +89,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint64_t* q_full = bars;
     uint64_t* k_full = bars + 1;              // [stage]
     uint64_t* v_full = k_full + C::STAGES;
-    uint64_t* k_empty = v_full + C::STAGES;   // (two halves only) their products are complete
+    uint64_t* k_empty = v_full + C::STAGES;   // its products are complete
     uint64_t* v_empty = k_empty + C::STAGES;
-    uint64_t* s_full = v_empty + C::STAGES;   // [half][buffer] S_j is ready; with one buffer O is complete up to block j - 1 too
+    uint64_t* s_full = v_empty + C::STAGES;   // [half][buffer] S_j is ready (one buffer: and P V complete up to block j - 1, two: j - 2)
     uint64_t* p_ready = s_full + C::HALVES * C::BUFFERS;      // [half] S_j read, P_j written over it, O rescaled (128 arrivals)
     uint64_t* pv_done = p_ready + C::HALVES;  // [half] P_j V_j complete
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + C::HALVES);
+    uint64_t* o_done = pv_done + C::HALVES;   // [half] the last one
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + C::HALVES);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((1 + 4 * C::STAGES + C::HALVES * (C::BUFFERS + 2)) * 8 + 8 <= 256, "barriers");
+    static_assert((1 + 4 * C::STAGES + C::HALVES * (C::BUFFERS + 3)) * 8 + 8 <= 256, "barriers");
 
     const CmePaged& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -113,6 +114,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             for (int b = 0; b < C::BUFFERS; ++b) mbar_init(&s_full[h * C::BUFFERS + b], 1);
             mbar_init(&p_ready[h], 128);
             mbar_init(&pv_done[h], 1);
+            mbar_init(&o_done[h], 1);
         }
         fence_barrier_init();
         prefetch_tmap(&tmQ);
@@ -120,18 +122,22 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         prefetch_tmap(&tmV);
     }
     __syncwarp();                             // the loading lanes see the barriers
+    if (warp == 0) { tmem_alloc(tmem_slot, C::COLS); tmem_relinquish(); }
     pdl_wait();
-    // late tiles, which see the most keys, first
-    const int head = blockIdx.y, split = blockIdx.x % p.splits;
-    const PagedTile t = paged_find_tile(a, p.tiles - 1 - blockIdx.x / p.splits, p.group, p.row_tile);
-    if (t.rows == 0) return;
+    // late tiles, which see the most keys, first, of all heads
+    const int head = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads, split = at % p.splits;
+    const PagedTile t = paged_find_tile(a, p.tiles - 1 - at / p.splits, p.group, p.row_tile);
+    if (t.rows == 0) {
+        if (warp == 0) { __syncwarp(); tmem_dealloc(*tmem_slot, C::COLS); }
+        return;
+    }
     const int limit = max(0, min(t.length, t.length - t.n + (t.first + t.rows - 1) / p.group + 1));
     const int begin = (int)min((long long)limit, (long long)split * p.split_keys);
     const int end = (int)min((long long)limit, (long long)begin + p.split_keys);
     const int nkv = cme_cdiv_dev(end - begin, KEYS);
     const int halves = t.rows > p.half_rows ? C::HALVES : 1;           // with rows
 
-    // One lane per box and slab: `which` 0 keys, 1 values.  Of tile j's boxes lane b's page and slot:
+    // Of tile j's boxes lane b's page and slot (the lanes of a warp count to eight, again and again)
     const int b = lane & 7;
     auto lookup = [&](int j, int& page, int& slot) {
         const int key = begin + j * KEYS + b * p.box;
@@ -144,38 +150,47 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (page < 0 || page >= a.num_pages) page = a.num_pages;
         }
     };
-    auto expect = [&](int j, uint64_t* bar) {
-        const int boxes = cme_cdiv_dev(min(KEYS, end - begin - j * KEYS), p.box);
-        mbar_arrive_expect_tx(bar, (uint32_t)(boxes * p.box * D * 2));
-    };
-    auto load_q = [&]() {
-        const int rows = C::HALVES > 1 && halves > 1 ? 2 : 1;
-        mbar_arrive_expect_tx(q_full, (uint32_t)(rows * p.half_rows * D * 2));
-        for (int h = 0; h < rows; ++h)
-            for (int s = 0; s < C::SLABS; ++s)
-                tma_load_4d(smem_u32(sQ) + h * C::Q_BYTES + s * C::Q_SLAB, &tmQ, q_full, s * 64, head * p.group,
-                            t.token0 + (t.first + h * p.half_rows) / p.group, 0);
-    };
-
-    int page0, slot0, page1, slot1;
-    if constexpr (C::HALVES == 1) {
-        if (warp == C::LOADER && nkv > 0) {                            // the first loads run under the TMEM allocation
-            if (elect_one()) load_q();
-            lookup(0, page0, slot0);
-            lookup(1, page1, slot1);
-            const int which = (lane >> 3) & 1;
-            if (lane == 0) { expect(0, &k_full[0]); expect(0, &v_full[0]); if (nkv > 1) { expect(1, &k_full[1]); expect(1, &v_full[1]); } }
-            __syncwarp();
-            if (lane < 16) {
-                uint64_t* full = which ? v_full : k_full;
-                const CUtensorMap* map = which ? &tmV : &tmK;
-                const uint32_t dst = smem_u32(which ? sV : sK) + b * p.box * 128;
-                if (page0 >= 0) tma_load_4d(dst, map, &full[0], 0, slot0, head, page0);
-                if (page1 >= 0) tma_load_4d(dst + C::KV_BYTES, map, &full[1], 0, slot1, head, page1);
+    // The warp that loads: lanes 0-15 keys, 16-31 values, a lane one box and slab of each tile.  It looks up the next tile's pages while it
+    // waits for a stage.  (Done by the warp that issues the MMAs, the loads of a tile held these up by 2500 clocks.)
+    int page0 = -1, slot0 = 0, loaded = 0;
+    auto load_tiles = [&](int upto) {
+        const int slab = (lane >> 3) & 1;
+        const bool values = lane >= 16;
+        const uint32_t dst = smem_u32(values ? sV : sK) + slab * C::KV_SLAB + b * p.box * 128;
+        for (; loaded < upto; ++loaded) {
+            const int s = loaded % C::STAGES;
+            int page1, slot1;
+            lookup(loaded + 1, page1, slot1);
+            bool free = true;
+            if (loaded >= C::STAGES) {
+                const uint32_t parity = (loaded / C::STAGES - 1) & 1;
+                free = mbar_wait(&k_empty[s], parity, abort_flag) && mbar_wait(&v_empty[s], parity, abort_flag);
             }
+            if (!__all_sync(0xffffffffu, free)) return false;
+            if ((lane & 15) == 0) {
+                const int boxes = cme_cdiv_dev(min(KEYS, end - begin - loaded * KEYS), p.box);
+                mbar_arrive_expect_tx(values ? &v_full[s] : &k_full[s], (uint32_t)(boxes * p.box * D * 2));
+            }
+            __syncwarp();
+            if (page0 >= 0 && slab < C::SLABS)
+                tma_load_4d(dst + s * C::KV_BYTES, values ? &tmV : &tmK, values ? &v_full[s] : &k_full[s], slab * 64, slot0, head, page0);
+            page0 = page1;
+            slot0 = slot1;
         }
+        return true;
+    };
+    if (warp == C::LOADER && nkv > 0) {
+        if (elect_one()) {
+            mbar_arrive_expect_tx(q_full, (uint32_t)(halves * p.half_rows * D * 2));
+            for (int h = 0; h < halves; ++h)
+                for (int s = 0; s < C::SLABS; ++s)
+                    tma_load_4d(smem_u32(sQ) + h * C::Q_BYTES + s * C::Q_SLAB, &tmQ, q_full, s * 64, head * p.group,
+                                t.token0 + (t.first + h * p.half_rows) / p.group, 0);
+        }
+        __syncwarp();
+        lookup(0, page0, slot0);
+        load_tiles(min(nkv, C::STAGES));
     }
-    if (warp == 0) { tmem_alloc(tmem_slot, C::COLS); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -201,94 +216,35 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool ok = true;
 
     if (warp >= 4 * C::HALVES) {
-        if constexpr (C::HALVES == 1) {
-            // ---------------- loads and MMAs (one warp) ----------------
-            const uint32_t tmem_S = tmem_base, tmem_O = tmem_base + KEYS;
-            if (nkv > 0) {
-                ok = mbar_wait(q_full, 0, abort_flag) && mbar_wait(&k_full[0], 0, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (ok) {
-                    tc_fence_after();
-                    if (elect_one()) { issue_s(0, 0, tmem_S); mma_commit(s_full); }
-                }
-            }
-            lookup(2, page0, slot0);                         // K of tile j + 2; V of tile j + 1 has the page of the turn before
-            for (int j = 0; j < nkv && ok; ++j) {
-                ok = mbar_wait(p_ready, j & 1, abort_flag) && mbar_wait(&v_full[j & 1], (j >> 1) & 1, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) { issue_pv(j, tmem_O, tmem_S); mma_commit(j + 1 < nkv ? pv_done : s_full); }
-                if (j + 1 == nkv) break;                     // s_full's phase nkv: O is complete
-                // S_j has been read, so its MMAs and with them those of P_{j-1} V_{j-1} are complete: refill their tiles while
-                // the product just issued runs
-                if (lane == 0) {
-                    if (j + 2 < nkv) expect(j + 2, &k_full[j & 1]);
-                    if (j >= 1) expect(j + 1, &v_full[(j + 1) & 1]);
-                }
-                __syncwarp();
-                if (lane < 8 && page0 >= 0) tma_load_4d(smem_u32(sK) + (j & 1) * C::KV_BYTES + b * p.box * 128, &tmK, &k_full[j & 1], 0, slot0, head, page0);
-                if (j >= 1 && lane < 8 && page1 >= 0)
-                    tma_load_4d(smem_u32(sV) + ((j + 1) & 1) * C::KV_BYTES + b * p.box * 128, &tmV, &v_full[(j + 1) & 1], 0, slot1, head, page1);
-                page1 = page0;
-                slot1 = slot0;
-                lookup(j + 3, page0, slot0);
-                ok = mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag) && mbar_wait(pv_done, j & 1, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) { issue_s(0, j + 1, tmem_S); mma_commit(s_full); }
-            }
-        } else if (warp == C::LOADER) {
-            // ---------------- loads ----------------
-            if (nkv > 0 && elect_one()) load_q();
-            const int slab = (lane >> 3) & 1;
-            const bool values = lane >= 16;
-            const uint32_t dst = smem_u32(values ? sV : sK) + slab * C::KV_SLAB + b * p.box * 128;
-            uint64_t* full = values ? v_full : k_full;
-            const CUtensorMap* map = values ? &tmV : &tmK;
-            lookup(0, page0, slot0);
-            for (int j = 0; j < nkv; ++j) {
-                const int s = j % C::STAGES;
-                lookup(j + 1, page1, slot1);
-                if (j >= C::STAGES) ok = mbar_wait(&k_empty[s], (j / C::STAGES - 1) & 1, abort_flag) && mbar_wait(&v_empty[s], (j / C::STAGES - 1) & 1, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                if (lane == 0) { expect(j, &k_full[s]); expect(j, &v_full[s]); }
-                __syncwarp();
-                if (page0 >= 0) tma_load_4d(dst + s * C::KV_BYTES, map, &full[s], slab * 64, slot0, head, page0);
-                page0 = page1;
-                slot0 = slot1;
-            }
+        if (warp == C::LOADER) {
+            ok = load_tiles(nkv);
         } else if (elect_one()) {
             // ---------------- MMAs of one half (one thread) ----------------
             const int half = warp - 4 * C::HALVES;
             const uint32_t tmem_S = tmem_base + half * C::HALF_COLS, tmem_O = tmem_S + C::BUFFERS * KEYS;
             if (half < halves) {
+                // PTX orders two MMAs only if they accumulate in the same place, and S_j takes the columns of the P before it there: it is issued
+                // once that P V is complete.
                 auto scores = [&](int j) {
-                    issue_s(half, j, tmem_S + (j & 1) * KEYS);
-                    mma_commit(&s_full[half * C::BUFFERS + (j & 1)]);
+                    if (!mbar_wait(&k_full[j % C::STAGES], (j / C::STAGES) & 1, abort_flag) ||
+                        (j >= C::BUFFERS && !mbar_wait(&pv_done[half], (j - C::BUFFERS) & 1, abort_flag))) return false;
+                    tc_fence_after();
+                    issue_s(half, j, tmem_S + (C::BUFFERS > 1 ? (j & 1) * KEYS : 0));
+                    mma_commit(&s_full[half * C::BUFFERS + (C::BUFFERS > 1 ? j & 1 : 0)]);
                     mma_commit(&k_empty[j % C::STAGES]);
+                    return true;
                 };
-                ok = nkv > 0 && mbar_wait(q_full, 0, abort_flag) && mbar_wait(&k_full[0], 0, abort_flag);
-                if (ok) { tc_fence_after(); scores(0); }
+                if (nkv > 0) ok = mbar_wait(q_full, 0, abort_flag) && scores(0);
                 for (int j = 0; j < nkv && ok; ++j) {
-                    if (j + 1 < nkv) {
-                        // S_{j+1} takes the columns of P_{j-1}: PTX orders two MMAs only if they accumulate in the same place
-                        ok = mbar_wait(&k_full[(j + 1) % C::STAGES], ((j + 1) / C::STAGES) & 1, abort_flag) &&
-                             (j < 1 || mbar_wait(&pv_done[half], (j - 1) & 1, abort_flag));
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(j + 1);
-                    }
+                    if (C::BUFFERS > 1 && j + 1 < nkv && !scores(j + 1)) { ok = false; break; }
                     ok = mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1, abort_flag) && mbar_wait(&p_ready[half], j & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    issue_pv(j, tmem_O, tmem_S + (j & 1) * KEYS);
-                    mma_commit(&pv_done[half]);
+                    issue_pv(j, tmem_O, tmem_S + (C::BUFFERS > 1 ? (j & 1) * KEYS : 0));
+                    mma_commit(j + 1 < nkv ? &pv_done[half] : &o_done[half]);
                     mma_commit(&v_empty[j % C::STAGES]);
+                    if (C::BUFFERS == 1 && j + 1 < nkv) ok = scores(j + 1);
                 }
-                ok = ok || nkv == 0;
             } else {
                 for (int j = 0; j < nkv && ok; ++j) {        // no rows: only hands the tiles back
                     const int s = j % C::STAGES;
@@ -354,7 +310,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             }
             if (j > 0 && __any_sync(0xffffffffu, raise)) {
                 // (with one buffer S_j came after P_{j-1} V_{j-1}; with two after P_{j-2} V_{j-2}, so that the parity is that of j - 1)
-                if (C::BUFFERS > 1 && !mbar_wait(&pv_done[half], (j - 1) & 1, abort_flag)) { ok = false; break; }
+                if (!mbar_wait(&pv_done[half], (j - 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {         // 16 columns at a time: the score row stays in registers
@@ -405,12 +361,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
             l += s0 + s1;
         }
-        if (ok && nkv > 0) {
-            // With two buffers S_{nkv-1} says that P V is complete up to block nkv - 3 only, and one parity does not tell a phase from the
-            // next but one: the last two are awaited one by one.
-            if (C::BUFFERS > 1) ok = (nkv < 2 || mbar_wait(&pv_done[half], (nkv - 2) & 1, abort_flag)) && mbar_wait(&pv_done[half], (nkv - 1) & 1, abort_flag);
-            else ok = mbar_wait(s_full, nkv & 1, abort_flag);
-        }
+        // (a barrier of its own: the parity of pv_done does not tell the last phase from the one before the one before)
+        if (ok && nkv > 0) ok = mbar_wait(&o_done[half], 0, abort_flag);
         if (ok) {
             tc_fence_after();
             const int rr = t.first + row, tok = rr / p.group;
@@ -482,7 +434,7 @@ template <int D> int launch(const CmePaged* a, const PagedPlan& plan, TcParams& 
     if ((rc = paged_make_q_map(&mq, a, p.group, p.half_rows / p.group))) return rc;
     if ((rc = paged_make_map(&mk, a, a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits), a->kv_heads), dim3(C::THREADS), (size_t)C::SMEM, st,
+    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits) * a->kv_heads), dim3(C::THREADS), (size_t)C::SMEM, st,
                                   mq, mk, mv, p));
     CME_LAUNCH_CHECK();
     return CME_OK;

@@ -127,13 +127,13 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
         }
     } else {
         plan->kernel = backend == 2 ? PAGED_ROWS : PAGED_TC;
-        const int resident = backend == 2 ? 1 : a->head_dim == 64 ? 4 : 1;
+        const int resident = backend == 2 ? 1 : a->head_dim == 64 ? 3 : 1;
         if (!parts) parts = ctas ? (int)std::min((long long)key_tiles, std::max(1ll, (long long)sms * resident / ctas)) : 1;
     }
     parts = std::max(1, parts);
     plan->splits = parts;
     plan->split_keys = cme_cdiv(key_tiles, parts) * key_tile;
-    CME_REQUIRE(tiles * parts < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many rows");
+    CME_REQUIRE(tiles * parts * a->kv_heads < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many rows");
     plan->tiles = (int)tiles;
     return CME_OK;
 }
