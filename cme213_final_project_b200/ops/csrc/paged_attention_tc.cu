@@ -43,7 +43,7 @@ template <int D> struct Sizes : Cfg<D> {
     static constexpr int Q_BYTES = SLABS * Q_SLAB, KV_BYTES = SLABS * KV_SLAB;
     static constexpr int LOADER = 5 * C::HALVES;                      // four warps of softmax and one that issues MMAs for each half, one that loads
     static constexpr int THREADS = (LOADER + 1) * 32;
-    static constexpr int SMEM = C::HALVES * Q_BYTES + 2 * C::STAGES * KV_BYTES + 256;
+    static constexpr int SMEM = C::HALVES * Q_BYTES + 2 * C::STAGES * KV_BYTES + 384;
     static constexpr int HALF_COLS = C::COLS / C::HALVES;            // S buffers, then O
     static_assert(C::BUFFERS * KEYS + D <= HALF_COLS && C::CTAS * C::COLS <= 512, "tensor memory");
     static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
@@ -95,9 +95,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint64_t* p_ready = s_full + C::HALVES * C::BUFFERS;      // [half] S_j read, P_j written over it, O rescaled (128 arrivals)
     uint64_t* pv_done = p_ready + C::HALVES;  // [half] P_j V_j complete
     uint64_t* o_done = pv_done + C::HALVES;   // [half] the last one
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + C::HALVES);
+    uint64_t* turn = o_done + C::HALVES;      // (two halves only) [softmax warp] it may take its turn at the exponentials
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + (C::HALVES > 1 ? 8 : 0));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((1 + 4 * C::STAGES + C::HALVES * (C::BUFFERS + 3)) * 8 + 8 <= 256, "barriers");
+    static_assert((1 + 4 * C::STAGES + C::HALVES * (C::BUFFERS + 3) + 8) * 8 + 8 <= 384, "barriers");
 
     const CmePaged& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -116,6 +117,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             mbar_init(&pv_done[h], 1);
             mbar_init(&o_done[h], 1);
         }
+        for (int w = 0; w < (C::HALVES > 1 ? 8 : 0); ++w) mbar_init(&turn[w], 1);
         fence_barrier_init();
         prefetch_tmap(&tmQ);
         prefetch_tmap(&tmK);
@@ -124,8 +126,12 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     __syncwarp();                             // the loading lanes see the barriers
     if (warp == 0) { tmem_alloc(tmem_slot, C::COLS); tmem_relinquish(); }
     pdl_wait();
-    // late tiles, which see the most keys, first, of all heads
-    const int head = blockIdx.x % a.kv_heads, at = blockIdx.x / a.kv_heads, split = at % p.splits;
+    // Late tiles, which see the most keys, first: of all heads, or (two halves, which take more keys a clock out of L2) head by head, so that
+    // fewer heads' keys are in use at a time (us, all heads / head by head: 16 chunks of GPT-2 small 31.9 / 34.2, two of 2048 over 8192 with head
+    // size 128 352 / 331).
+    const int of_head = p.tiles * p.splits;
+    const int head = C::HALVES > 1 ? blockIdx.x / of_head : blockIdx.x % a.kv_heads;
+    const int at = C::HALVES > 1 ? blockIdx.x % of_head : blockIdx.x / a.kv_heads, split = at % p.splits;
     const PagedTile t = paged_find_tile(a, p.tiles - 1 - at / p.splits, p.group, p.row_tile);
     if (t.rows == 0) {
         if (warp == 0) { __syncwarp(); tmem_dealloc(*tmem_slot, C::COLS); }
@@ -199,16 +205,17 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
     constexpr uint32_t idesc_s = make_idesc(1, false, false, 128, KEYS);      // Q K^T: both K-major
     constexpr uint32_t idesc_o = make_idesc(1, false, true, 128, D);          // P V: V is MN-major
+    const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024), k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
+    const uint64_t v_desc = make_smem_desc(smem_u32(sV), C::KV_SLAB, 1024);
     auto issue_s = [&](int half, int j, uint32_t tmem_S) {
-        const uint64_t qd = make_smem_desc(smem_u32(sQ) + half * C::Q_BYTES, 0, 1024);
-        const uint64_t kd = make_smem_desc(smem_u32(sK) + (j % C::STAGES) * C::KV_BYTES, 0, 1024);
+        const uint64_t qd = desc_at(q_desc, (half * C::Q_BYTES) >> 4), kd = desc_at(k_desc, ((j % C::STAGES) * C::KV_BYTES) >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
             mma_f16_ss(tmem_S, desc_at(qd, ((k >> 2) * C::Q_SLAB + (k & 3) * 32) >> 4),
                        desc_at(kd, ((k >> 2) * C::KV_SLAB + (k & 3) * 32) >> 4), idesc_s, k > 0);
     };
     auto issue_pv = [&](int j, uint32_t tmem_O, uint32_t tmem_P) {
-        const uint64_t vd = make_smem_desc(smem_u32(sV) + (j % C::STAGES) * C::KV_BYTES, C::KV_SLAB, 1024);
+        const uint64_t vd = desc_at(v_desc, ((j % C::STAGES) * C::KV_BYTES) >> 4);
 #pragma unroll
         for (int k = 0; k < KEYS / 16; ++k)                  // A = P from tensor memory: 16 keys = 8 columns per step
             mma_f16_ts(tmem_O, tmem_P + k * 8, desc_at(vd, k * 2048 >> 4), idesc_o, j > 0 || k > 0);
@@ -324,6 +331,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 l *= alpha;
             }
             const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
+            // The two halves' warps of a scheduler take turns at the exponentials; left alone they fall into step, both wait for the tensor
+            // core, and then for one another.
+            if (C::HALVES > 1 && halves > 1 && half + j > 0 && !mbar_wait(&turn[warp], (half ? j : j - 1) & 1, abort_flag)) { ok = false; break; }
             // scale-and-shift and the row sum on packed pairs (one instruction per two keys); four independent chains
             const F32x2 sc2 = f2_splat(p.scale_log2), nm2 = f2_splat(-m_use);
             F32x2 sum2[4];
@@ -343,6 +353,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 for (int i = 0; i < 16; ++i) pw[i] = f2_to_bf2(x[2 * i], x[2 * i + 1]);
                 tmem_st16(tmem_S + c * 16, pw);
             }
+            if (C::HALVES > 1 && halves > 1 && lane == 0) mbar_arrive(&turn[warp ^ 4]);
             if (k0 + KEYS > end) {
                 // values behind the end may be anything, NaN too, which a probability of zero does not stop: zeros take their place
                 const int s = j % C::STAGES;
