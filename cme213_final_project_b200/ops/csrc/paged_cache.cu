@@ -90,6 +90,30 @@ int check_cache(const CmePaged* a, const char* what) {
 
 constexpr int MAX_SPLITS = 128;
 
+// Estimated time of a form, in us: turns of its CTAs on the GPU, key tiles of a turn, time of a key tile (of its own size and rows, measured with
+// the keys in L2 and all SMs busy), and what its parts cost that are joined through scratch (written and read once more, at 3 TB/s,
+// and a launch).  The host does not know the sequences: they are taken to be as long as the longest, and to share the new tokens evenly.
+// Measured / estimated: 12 heads of 64, 128 tokens over 4096 in 4 sequences: tc in 1, 4, 8 parts 72 / 79, 32 / 32, 31 / 27, stream 62 / 70;
+// 4 heads of 128 in fp32, 256 over 512 in 8: rows 66 / 68, stream 97 / 91.
+struct Form {
+    int keys;                // of a tile
+    int slots;               // CTAs that run at a time
+    float tile_us;
+};
+Form form_of(const CmePaged* a, int backend, int sms) {
+    const bool f32 = a->dtype == CME_F32;
+    const int d = a->head_dim;
+    if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 64 ? 3 : 1), d == 64 ? 1.15f : 1.0f};
+    const int keys = paged_mma_key_tile(a->dtype, d);
+    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : 1.4f) : d == 32 ? 0.8f : d == 64 ? 1.4f : 1.2f};
+    return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 7.5f : 4.5f) : d == 128 ? 2.6f : 1.8f};
+}
+float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
+    const long long ctas = tiles * a->kv_heads * parts, turns = (ctas + f.slots - 1) / f.slots;
+    const double joined = parts > 1 ? 4.0 + (double)a->rows * a->heads * parts * (a->head_dim + 2) * 8 / 3e6 : 0.0;
+    return (float)(5.0 + (double)turns * cme_cdiv(key_tiles, parts) * f.tile_us + joined);
+}
+
 // backend: 0 by the rule, 1 up to 16 rows a tile, 2 rows, 3 tc.  splits: 0 by the rule; up to 16 rows: a cluster of so many CTAs (1, 2, 4
 // or 8), negative: the stream; others: parts of the keys.
 int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* plan) {
@@ -99,23 +123,53 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
     CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
                 "paged attention: the tcgen05 kernel takes bf16, head sizes 64 and 128 and up to 128 query heads per key head");
-    if (!backend) backend = rows <= 16ll * a->seqs ? 1 : tc ? 3 : 2;
-    plan->row_tile = backend == 1 ? 16 : backend == 2 ? 64 : (a->head_dim == 64 ? 1 : 2) * (128 / group * group);
-    const long long tiles = rows / plan->row_tile + std::min(a->seqs, a->rows);      // each sequence adds less than one
-    const int key_tile = backend == 3 ? PAGED_TC_KEYS : paged_mma_key_tile(a->dtype, a->head_dim);
+    auto row_tile = [&](int b) { return b == 1 ? 16 : b == 2 ? 64 : (a->head_dim == 64 ? 1 : 2) * (128 / group * group); };
+    auto tiles_of = [&](int b) { return rows / row_tile(b) + std::min(a->seqs, a->rows); };      // at the most: each sequence adds less than one
+    auto even_tiles = [&](int b) { return a->seqs ? a->seqs * ((rows + (long long)a->seqs * row_tile(b) - 1) / ((long long)a->seqs * row_tile(b))) : 0; };
     const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
-    const int key_tiles = std::max(1, cme_cdiv(longest, key_tile));
-    const long long ctas = tiles * a->kv_heads;
+    auto key_tiles_of = [&](const Form& f) { return std::max(1, cme_cdiv(longest, f.keys)); };
+    auto best_parts = [&](int b, float* us) {              // of rows and tc
+        const Form f = form_of(a, b, sms);
+        const int n = key_tiles_of(f);
+        int best = 1;
+        *us = estimate(a, f, even_tiles(b), n, 1);
+        for (int parts = 2; parts <= std::min(n, MAX_SPLITS); parts += (parts + 3) / 4) {
+            const float t = estimate(a, f, even_tiles(b), n, parts);
+            if (t < *us) { *us = t; best = parts; }
+        }
+        return best;
+    };
+    // Up to 16 rows a tile: as many CTAs of a cluster as let all run at once; the stream from where a CTA would have more than eight key
+    // tiles in its turns (head size 64, lengths from half of the longest on, us, cluster / stream: 96 items of up to 1024 keys 8.5 /
+    // 10.1, of 4096 21.9 / 20.5; 384 items of 256 9.9 / 11.2, of 1024 23.0 / 21.4.  128: 32 items of 4096 14.1 / 17.7, 8 of 16384 33.6 / 21.8).
+    const Form one = form_of(a, 1, sms);
+    const int one_keys = key_tiles_of(one);
+    auto cluster_of = [&](long long items, int* c) {       // the cluster's size, and the key tiles of a CTA's turns
+        for (*c = 1; *c < 8 && *c < one_keys && items * *c * 2 <= one.slots;) *c *= 2;
+        return (items * *c + one.slots - 1) / one.slots * cme_cdiv(one_keys, *c);
+    };
+    if (!backend) {
+        backend = 1;
+        if (rows > 16ll * a->seqs) {                       // (else a row tile has all rows of a sequence: its keys are read once)
+            const int many = tc ? 3 : 2;
+            const long long items = even_tiles(1) * a->kv_heads;
+            int c;
+            const long long turns = cluster_of(items, &c);
+            float us;
+            best_parts(many, &us);
+            // (two more tiles an item of the stream, as its kernel reckons)
+            const float few = turns <= 8 ? 4.5f + (float)turns * one.tile_us : 6.f + (float)((items * (one_keys + 2) + one.slots - 1) / one.slots) * one.tile_us;
+            if (us < few) backend = many;
+        }
+    }
+    const Form f = form_of(a, backend, sms);
+    const long long tiles = tiles_of(backend), ctas = tiles * a->kv_heads;
+    const int key_tiles = key_tiles_of(f);
+    plan->row_tile = row_tile(backend);
     int parts = std::min(splits < 0 ? -splits : splits, MAX_SPLITS);
     if (backend == 1) {
-        const int slots = sms * paged_mma_ctas(a->dtype, a->head_dim);
-        // As many CTAs of a cluster as let all run at once; the stream from where a CTA would have more than eight key tiles in its turns (head
-        // size 64, lengths from half of the longest on, us, cluster / stream: 96 items of up to 1024 keys 8.5 / 10.1, of 4096 21.9 / 20.5;
-        // 384 items of 256 9.9 / 11.2, of 1024 23.0 / 21.4.  128: 32 items of 4096 14.1 / 17.7, 8 of 16384 33.6 / 21.8).
-        int c = 1;
-        while (c < 8 && c < key_tiles && ctas * c * 2 <= slots) c *= 2;
-        const long long turns = ctas ? (ctas * c + slots - 1) / slots : 1;
-        const bool cluster = splits ? splits > 0 : turns * cme_cdiv(key_tiles, c) <= 8;
+        int c;
+        const bool cluster = cluster_of(ctas, &c) <= 8 ? splits >= 0 : splits > 0;
         plan->kernel = cluster ? PAGED_CLUSTER : PAGED_STREAM;
         if (cluster) {
             const int want = splits ? parts : c;
@@ -123,16 +177,16 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
             while (parts < want && parts < 8) parts *= 2;
         } else {
             CME_REQUIRE(ctas * (key_tiles + 8ll) < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many keys");
-            parts = (int)std::min((long long)slots, std::max(1ll, ctas * key_tiles));
+            parts = (int)std::min((long long)f.slots, std::max(1ll, ctas * key_tiles));
         }
     } else {
         plan->kernel = backend == 2 ? PAGED_ROWS : PAGED_TC;
-        const int resident = backend == 2 ? 1 : a->head_dim == 64 ? 3 : 1;
-        if (!parts) parts = ctas ? (int)std::min((long long)key_tiles, std::max(1ll, (long long)sms * resident / ctas)) : 1;
+        float us;
+        if (!parts) parts = best_parts(backend, &us);
     }
     parts = std::max(1, parts);
     plan->splits = parts;
-    plan->split_keys = cme_cdiv(key_tiles, parts) * key_tile;
+    plan->split_keys = cme_cdiv(key_tiles, parts) * f.keys;
     CME_REQUIRE(tiles * parts * a->kv_heads < (1ll << 31), CME_ERR_LIMIT, "paged attention: too many rows");
     plan->tiles = (int)tiles;
     return CME_OK;
