@@ -11,6 +11,7 @@ Layers (each only calls downward):
 * ``parallel``    -- data-parallel gradient synchronisation (blocking, bucketed overlap, fused peer-memory)
 * ``utils``       -- device timers, NVTX ranges, clock sampling, log-line formats
 * ``train``       -- the command-line training driver
+* ``generate``    -- text from a trained model: a paged cache, prompts in chunks, one token a step
 """
 
 __version__ = "0.1.0"
