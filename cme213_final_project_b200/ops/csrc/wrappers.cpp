@@ -9,6 +9,7 @@
 // The library's entry points arrive as addresses (bind), so this module links to torch only and always calls the library
 // that ops/__init__.py has loaded.  The GIL is released around the native calls, as ctypes does.
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -109,6 +110,10 @@ bool truth(PyObject* o) {
 }
 at::Tensor like(const at::Tensor& t) { return at::empty(t.sizes(), t.options()); }
 at::Tensor floats(long long n, const at::Tensor& t) { return at::empty({n}, t.options().dtype(at::kFloat)); }
+// As at::empty on t's device, without its way through the dispatcher, for calls that a step of generation makes over and over.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& t) {
+    return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
+}
 
 PyObject* wrap(const at::Tensor& t) {
     if (!t.defined()) Py_RETURN_NONE;
@@ -453,13 +458,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t) {
     d.scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)d.head_dim)) : real(a[6]);
     if (a[7] != Py_None) d.max_len = int32(whole(a[7]));
     const int backend = int32(whole(a[8])), splits = int32(whole(a[9]));
-    const at::Tensor out = at::empty(q.sizes(), q.options()), lse = at::empty({d.rows, d.heads}, q.options().dtype(at::kFloat));
+    const at::Tensor out = fresh(q.sizes(), q.scalar_type(), q), lse = fresh({d.rows, d.heads}, at::kFloat, q);
     d.o = ptr(out);
     d.lse = (float*)ptr(lse);
     check(lib.cme_paged_attention_ws_bytes(&d, backend, splits, &d.ws_bytes));
     at::Tensor ws;
     if (d.ws_bytes) {
-        ws = floats((d.ws_bytes + 3) / 4, q);
+        ws = fresh({(d.ws_bytes + 3) / 4}, at::kFloat, q);
         d.ws = (float*)ptr(ws);
     }
     run([&](void* st) { return lib.cme_paged_attention(&d, backend, splits, st); });
@@ -520,8 +525,8 @@ PyObject* next_token(PyObject*, PyObject* const* a, Py_ssize_t) {
         if (!g.is_contiguous()) fail(native_error, "noise has to be contiguous");
         d.noise = (const float*)ptr(g);
     }
-    const at::Tensor token = at::empty({d.rows}, logits.options().dtype(at::kInt)), logprob = floats(d.rows, logits);
-    const at::Tensor processed = truth(a[12]) ? at::empty({d.rows, d.vocab}, logits.options()) : at::Tensor();
+    const at::Tensor token = fresh({d.rows}, at::kInt, logits), logprob = fresh({d.rows}, at::kFloat, logits);
+    const at::Tensor processed = truth(a[12]) ? fresh({d.rows, d.vocab}, logits.scalar_type(), logits) : at::Tensor();
     d.token = (int*)ptr(token); d.logprob = (float*)ptr(logprob); d.processed = ptr(processed);
     run([&](void* st) { return lib.cme_next_token(&d, st); });
     return pack(token, logprob, processed);
