@@ -7,7 +7,7 @@
 // make up one tile.  A page that is not there is a box behind the cache, which TMA fills with zeros, and a bit in the row's mask.
 // What bounds it: the exponentials (16 a clock and SM: 512 clocks for 128 rows x 64 keys) and, with head size 128, as many clocks of the
 // tensor pipe; one hides behind the other only if several tiles of rows are on their way at a time.
-//   head size 64   128 rows a CTA, four CTAs an SM (128 columns of tensor memory each): a tile's chain of steps, its start and its end run
+//   head size 64   128 rows a CTA, three CTAs an SM (128 columns of tensor memory each): a tile's chain of steps, its start and its end run
 //                  under the others'.
 //   head size 128  256 rows a CTA, one CTA an SM, two buffers of scores for each half: S_{j+1} is made while softmax_j runs.  Both halves
 //                  read the same keys: with 128 rows a CTA the tiles of K and V would come out of L2 at 53 bytes a clock and SM.
@@ -15,6 +15,7 @@
 #include "paged.h"
 #include "sm100_ptx.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 using namespace sm100;
@@ -46,7 +47,7 @@ template <int D> struct Sizes : Cfg<D> {
     static constexpr int SMEM = C::HALVES * Q_BYTES + 2 * C::STAGES * KV_BYTES + 384;
     static constexpr int HALF_COLS = C::COLS / C::HALVES;            // S buffers, then O
     static_assert(C::BUFFERS * KEYS + D <= HALF_COLS && C::CTAS * C::COLS <= 512, "tensor memory");
-    static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");
+    static_assert(C::CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory");      // (1 KB of each CTA is the system's)
 };
 
 struct TcParams {
@@ -429,6 +430,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (warp == 0) { tc_fence_after(); tmem_dealloc(tmem_base, C::COLS); }
 }
 
+// Shared memory of a CTA that keeps more than `each` of them off an SM.  Where CTAs are few the hardware still puts several on one SM
+// (chunks of GPT-2 small, 1 / 2 / 8 sequences, us: 19.3 / 19.0 / 25.6, spread over the SMs 17.6 / 17.1 / 24.5).
+constexpr int spread(int each) { return 228 * 1024 / (each + 1); }
+
 template <int D> int launch(const CmePaged* a, const PagedPlan& plan, TcParams& p, cudaStream_t st) {
     using C = Sizes<D>;
     auto* kernel = paged_attn_tc_kernel<D>;
@@ -436,7 +441,7 @@ template <int D> int launch(const CmePaged* a, const PagedPlan& plan, TcParams& 
     int dev = 0;
     CME_CUDA(cudaGetDevice(&dev));
     if (!attr[dev % CME_MAX_DEVICES]) {
-        CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::CTAS > 1 ? spread(1) : C::SMEM));
         attr[dev % CME_MAX_DEVICES] = true;
     }
     p.half_rows = p.row_tile / C::HALVES;
@@ -445,7 +450,11 @@ template <int D> int launch(const CmePaged* a, const PagedPlan& plan, TcParams& 
     if ((rc = paged_make_q_map(&mq, a, p.group, p.half_rows / p.group))) return rc;
     if ((rc = paged_make_map(&mk, a, a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits) * a->kv_heads), dim3(C::THREADS), (size_t)C::SMEM, st,
+    int sms;
+    if ((rc = cme_num_sms(&sms))) return rc;
+    const long long ctas = (long long)plan.tiles * plan.splits * a->kv_heads, each = std::max(1ll, (ctas + sms - 1) / sms);
+    const int smem = each < C::CTAS ? spread((int)each) : C::SMEM;
+    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits) * a->kv_heads), dim3(C::THREADS), (size_t)smem, st,
                                   mq, mk, mv, p));
     CME_LAUNCH_CHECK();
     return CME_OK;
