@@ -6,8 +6,9 @@
 // tile, so that a key is read once for all of them.  Two forms:
 //   single  up to 16 rows a tile, each of four warps takes a quarter of every key tile and keeps its own m, l and sums; they are
 //           joined at the end.  For single tokens, which are bound by the bytes of the cache.
-//   rows    64 rows a CTA, 16 a warp, every warp takes all keys.  For chunks that the tcgen05 kernel does not take.
-// The fifth warp looks up the pages and loads key tiles by TMA, one box per page (or key tile), several tiles ahead.
+//   rows    64 rows a CTA, 16 a warp; in fp32 and head sizes above 32 two warps share 16 rows and take every other 16 keys.  For chunks
+//           that the tcgen05 kernel does not take.
+// The last warp looks up the pages and loads key tiles by TMA, one box per page (or key tile), several tiles ahead.
 // fp32 operands of the matrix instructions are split into two tf32 numbers each (x = hi + lo, 11 bits each) and multiplied as hi hi + hi lo + lo hi: what is
 // left out is below 2^-22 of a product.  The tensor core's sums are kept short (one key tile, added up in fp32 registers), since it cuts
 // what it shifts out.
@@ -27,9 +28,9 @@ int* cme_attn_status_ptr();
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int THREADS = 160;               // rows kernel: four warps that compute, one that loads
 
 template <typename T, int D, bool ROWS> struct Cfg {
+    static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int ROW = D * (int)sizeof(T);                    // bytes of a key
     static constexpr int SLAB = ROW < 128 ? ROW : 128;                // bytes of a key in one swizzled slab
     static constexpr int SLABS = ROW / SLAB;
@@ -37,19 +38,21 @@ template <typename T, int D, bool ROWS> struct Cfg {
     static constexpr int KEYS = 4 * WARP_KEYS;                        // key tile
     static constexpr int TILE = KEYS * ROW;                           // bytes of its keys (and of its values)
     static constexpr int STAGES = ROW == 64 ? 4 : ROWS && ROW == 512 ? 2 : 3;      // (the rows' fragments take 64 KB then)
-    static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int FRAGS = F32 ? D * 128 : 0;                   // bytes of 16 rows' fragments in shared memory
-    // Up to 16 rows: CTAs of an SM, and groups of four warps, which take every other key tile.  Two CTAs' or two groups' chains of products
-    // and softmax run at a time; 64 KB tiles leave room for one CTA.
-    static constexpr int CTAS = ROW == 512 ? 1 : 2, GROUPS = ROW == 512 ? 2 : 1, WARPS = 4 * GROUPS;
-    static constexpr int JOIN_ROWS = 32 / WARPS;                      // joined at a time
+    // CTAs of an SM, and groups of four warps, which take every other key tile (rows: every other 16 keys of each).  Two CTAs' or two groups'
+    // chains of products and softmax run at a time; 64 KB tiles, or 64 rows' fragments of fp32, leave room for one CTA.  Rows, fp32, one
+    // group / two, us: 16 heads of 64, 512 tokens over 2048 in 4 sequences 469 / 384; 32 heads of 128 on 8, 500 over 2000 in 2 864 / 701;
+    // 12 heads of 64, 64 over 128 in one 11.9 / 11.4.  (Head size 32 has room for two CTAs.)
+    static constexpr int CTAS = ROWS ? (D == 32 ? 2 : 1) : ROW == 512 ? 1 : 2;
+    static constexpr int GROUPS = (ROWS ? F32 && D > 32 : ROW == 512) ? 2 : 1, WARPS = 4 * GROUPS;
+    static constexpr int JOIN_ROWS = 32 / WARPS;                      // joined at a time (up to 16 rows)
     static_assert(STAGES <= 4, "words kept for the stages");
 };
 
 struct MmaParams {
     CmePaged a;
     PagedDiv page;
-    int group, box, box_log, splits, split_keys;
+    int group, box, box_log, splits, split_keys, tiles;
     float scale_log2;
     float* part_o;                         // [rows, heads, splits, head_dim] sums of a part; stream: [CTA, 2, 16, head_dim]
     float2* part_ml;                       // [rows, heads, splits] its m (log2 units) and l; stream: [CTA, 2, 16]
@@ -482,7 +485,7 @@ __device__ __forceinline__ int row_sees(const MmaParams& p, const PagedTile& t, 
 // Many rows: 16 a warp, every warp takes all keys
 // ------------------------------------------------------------------------------------------------------
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Cfg<T, D, true>::WARPS * 32 + 32, Cfg<T, D, true>::CTAS)
 paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const MmaParams p) {
     using C = Cfg<T, D, true>;
     constexpr int NT = D / 8;
@@ -500,7 +503,7 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     const CmePaged& a = p.a;
     if (threadIdx.x == 0) {
         *ld.abort_flag = 0;
-        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&ld.full[s], 1); mbar_init(&ld.empty[s], 4); }
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&ld.full[s], 1); mbar_init(&ld.empty[s], C::WARPS); }
         fence_barrier_init();
         prefetch_tmap(&tmK);
         prefetch_tmap(&tmV);
@@ -508,23 +511,27 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     pdl_release();
     pdl_wait();
     const int split = blockIdx.x % p.splits, head = blockIdx.y;
-    const PagedTile t = paged_find_tile(a, blockIdx.x / p.splits, p.group, 64);
+    // late tiles, which see the most keys, first
+    const PagedTile t = paged_find_tile(a, p.tiles - 1 - (int)(blockIdx.x / p.splits), p.group, 64);
     __syncthreads();
     if (t.rows == 0) return;
     // keys [0, limit) are seen by the last row; this CTA takes [begin, end)
     const int limit = max(0, min(t.length, row_sees(p, t, t.rows - 1)));
     const int begin = (int)min((long long)limit, (long long)split * p.split_keys);
     const int end = (int)min((long long)limit, (long long)begin + p.split_keys);
-    if (warp == 4) {
+    if (warp == C::WARPS) {
         ld.tiles(p, &tmK, &tmV, t.seq, head, begin, end);
         ld.drain();
     } else {
-        const int row0 = warp * 16 + (lane >> 2), tq = lane & 3;       // this thread's rows: row0, row0 + 8
+        const int of = warp & 3, group = warp >> 2;                    // its 16 rows, and which of the keys it takes
+        const int row0 = of * 16 + (lane >> 2), tq = lane & 3;         // this thread's rows: row0, row0 + 8
         Rows<T, C, D, 1> q;
         q.load(row_of_q<T>(p, t, head, row0), row_of_q<T>(p, t, head, row0 + 8), 0);
-        q.publish(sQ + warp * C::FRAGS, 0);
+        q.publish(sQ + of * C::FRAGS, 0);                              // (both groups write the same)
         const int see0 = min(end, row_sees(p, t, row0)), see1 = min(end, row_sees(p, t, row0 + 8));
-        const int see_first = min(end, row_sees(p, t, warp * 16));
+        const int see_first = min(end, row_sees(p, t, of * 16));
+        const int last = min(t.rows, of * 16 + 16) - 1;
+        const int seen = last < of * 16 ? 0 : min(end, row_sees(p, t, last));      // no row of the warp sees keys from here on
         WarpState<C, D> w;
         w.clear();
         int it = 0;
@@ -532,20 +539,45 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
             const int s = it % C::STAGES;
             if (!mbar_wait(&ld.full[s], (it / C::STAGES) & 1, ld.abort_flag)) break;
             const uint32_t there = ld.there[s];
-            if (k0 + C::KEYS > end) clear_values<C>(ld.sV + s * C::TILE, end - k0, C::KEYS);
+            if (k0 < seen && k0 + C::KEYS > end) clear_values<C>(ld.sV + s * C::TILE, end - k0, C::KEYS);
 #pragma unroll 1
-            for (int key0 = 0; key0 < C::KEYS && k0 + key0 < end; key0 += C::WARP_KEYS)
+            for (int key0 = group * C::WARP_KEYS; key0 < C::KEYS && k0 + key0 < seen; key0 += C::GROUPS * C::WARP_KEYS)
                 attend(w, q, smem_u32(ld.sK) + s * C::TILE, smem_u32(ld.sV) + s * C::TILE, key0, k0, see0, see1,
                        there != 0xffffffffu || k0 + key0 + C::WARP_KEYS > see_first, there, p.box_log, p.scale_log2);
             __syncwarp();
             if (lane == 0) mbar_arrive(&ld.empty[s]);
         }
         w.finish();
+        if constexpr (C::GROUPS > 1) {
+            // the second group's part of the rows through the tiles' memory, which nobody reads any more
+            static_assert((NT * 4 + 4) * 512 <= 2 * C::STAGES * C::TILE, "memory of the tiles");
+            float* x = reinterpret_cast<float*>(smem) + (threadIdx.x & 127);
+            named_bar_sync(1, C::WARPS * 32);
+            if (group) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) { x[r * 256] = w.m[r]; x[r * 256 + 128] = w.l[r]; }
+#pragma unroll
+                for (int i = 0; i < NT * 4; ++i) x[(4 + i) * 128] = w.o[i >> 2][i & 3];
+            }
+            named_bar_sync(1, C::WARPS * 32);
+            if (!group) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float m = x[r * 256], mm = fmaxf(w.m[r], m), f0 = part_factor(w.m[r], mm), f1 = part_factor(m, mm);
+                    w.m[r] = mm;
+                    w.l[r] = fmaf(f1, x[r * 256 + 128], f0 * w.l[r]);
+#pragma unroll
+                    for (int d = 0; d < NT; ++d)
+#pragma unroll
+                        for (int i = 2 * r; i < 2 * r + 2; ++i) w.o[d][i] = fmaf(f1, x[(4 + d * 4 + i) * 128], f0 * w.o[d][i]);
+                }
+            }
+        }
         T* out = static_cast<T*>(a.o);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int row = row0 + 8 * r;
-            if (row >= t.rows) continue;
+            if (group || row >= t.rows) continue;
             long long at = row_at(p, t, head, row);
             if (p.splits == 1) {
                 const float inv = inverse(w.l[r]);
@@ -984,7 +1016,7 @@ template <typename T, int D, bool ROWS, auto Kernel>
 int launch(dim3 grid, const CmePaged* a, int cluster, const MmaParams& p, cudaStream_t st) {
     using C = Cfg<T, D, ROWS>;
     constexpr int SMEM = smem_bytes<T, D, ROWS>();
-    static_assert(SMEM <= 227 * 1024 && (ROWS || C::CTAS * (SMEM + 1024) <= 228 * 1024), "shared memory of a CTA");
+    static_assert(SMEM <= 227 * 1024 && C::CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of a CTA");
     static bool attr[CME_MAX_DEVICES] = {};               // function attributes are per device
     int dev = 0;
     CME_CUDA(cudaGetDevice(&dev));
@@ -999,7 +1031,7 @@ int launch(dim3 grid, const CmePaged* a, int cluster, const MmaParams& p, cudaSt
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, C::SLAB / (int)sizeof(T), p.box, swizzle))) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(ROWS ? THREADS : C::WARPS * 32 + 32);
+    cfg.blockDim = dim3(C::WARPS * 32 + 32);
     cfg.dynamicSmemBytes = SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -1059,6 +1091,7 @@ int paged_attention_mma(const CmePaged* a, const PagedPlan& plan, cudaStream_t s
     while (p.box < tile && a->page % (p.box * 2) == 0) { p.box *= 2; ++p.box_log; }
     p.splits = plan.splits;
     p.split_keys = plan.split_keys;
+    p.tiles = plan.tiles;
     p.scale_log2 = a->scale * LOG2E;
     // scratch: m and l of the parts (16-byte aligned by their size), their sums; stream: a record for each CTA before them
     const long long parts = plan.kernel == PAGED_STREAM ? plan.splits * 32ll : (long long)a->rows * a->heads * plan.splits;

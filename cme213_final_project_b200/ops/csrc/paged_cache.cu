@@ -94,7 +94,7 @@ constexpr int MAX_SPLITS = 128;
 // the keys in L2 and all SMs busy), and what its parts cost that are joined through scratch (written and read once more, at 3 TB/s,
 // and a launch).  The host does not know the sequences: they are taken to be as long as the longest, and to share the new tokens evenly.
 // Measured / estimated: 12 heads of 64, 128 tokens over 4096 in 4 sequences: tc in 1, 4, 8 parts 72 / 79, 32 / 32, 31 / 27, stream 62 / 70;
-// 4 heads of 128 in fp32, 256 over 512 in 8: rows 66 / 68, stream 97 / 91.
+// 4 heads of 128 in fp32, 256 over 512 in 8: rows 56 / 55, stream 97 / 104; 12 heads of 64 in fp32, 256 over 512 in 8: rows 82 / 84, stream 109 / 110.
 struct Form {
     int keys;                // of a tile
     int slots;               // CTAs that run at a time
@@ -105,8 +105,8 @@ Form form_of(const CmePaged* a, int backend, int sms) {
     const int d = a->head_dim;
     if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 64 ? 3 : 1), d == 64 ? 1.15f : 1.0f};
     const int keys = paged_mma_key_tile(a->dtype, d);
-    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : 1.4f) : d == 32 ? 0.8f : d == 64 ? 1.4f : 1.2f};
-    return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 7.5f : 4.5f) : d == 128 ? 2.6f : 1.8f};
+    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 32 ? 0.8f : d == 64 ? 1.4f : 1.2f};
+    return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.2f : d == 64 ? 3.3f : 4.5f) : d == 128 ? 2.6f : 1.8f};
 }
 float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
     const long long ctas = tiles * a->kv_heads * parts, turns = (ctas + f.slots - 1) / f.slots;
