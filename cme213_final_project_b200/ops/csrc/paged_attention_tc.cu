@@ -93,13 +93,15 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint64_t* k_empty = v_full + C::STAGES;   // its products are complete
     uint64_t* v_empty = k_empty + C::STAGES;
     uint64_t* s_full = v_empty + C::STAGES;   // [half][buffer] S_j is ready (one buffer: and P V complete up to block j - 1, two: j - 2)
-    uint64_t* p_ready = s_full + C::HALVES * C::BUFFERS;      // [half] S_j read, P_j written over it, O rescaled (128 arrivals)
-    uint64_t* pv_done = p_ready + C::HALVES;  // [half] P_j V_j complete
+    // [half][buffer] S_j read, P_j written over it, O rescaled (128 arrivals).  A barrier for each buffer: with two of them a warp may be a step
+    // ahead of another one, whose arrival its own for S_{j+1} must not stand in for; S_{j+2} comes when P_j V_j is complete.
+    uint64_t* p_ready = s_full + C::HALVES * C::BUFFERS;
+    uint64_t* pv_done = p_ready + C::HALVES * C::BUFFERS;     // [half] P_j V_j complete
     uint64_t* o_done = pv_done + C::HALVES;   // [half] the last one
     uint64_t* turn = o_done + C::HALVES;      // (two halves only) [softmax warp] it may take its turn at the exponentials
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + (C::HALVES > 1 ? 8 : 0));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((1 + 4 * C::STAGES + C::HALVES * (C::BUFFERS + 3) + 8) * 8 + 8 <= 384, "barriers");
+    static_assert((1 + 4 * C::STAGES + C::HALVES * (2 * C::BUFFERS + 2) + 8) * 8 + 8 <= 384, "barriers");
 
     const CmePaged& a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -113,8 +115,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             mbar_init(&v_empty[s], C::HALVES);
         }
         for (int h = 0; h < C::HALVES; ++h) {
-            for (int b = 0; b < C::BUFFERS; ++b) mbar_init(&s_full[h * C::BUFFERS + b], 1);
-            mbar_init(&p_ready[h], 128);
+            for (int b = 0; b < C::BUFFERS; ++b) {
+                mbar_init(&s_full[h * C::BUFFERS + b], 1);
+                mbar_init(&p_ready[h * C::BUFFERS + b], 128);
+            }
             mbar_init(&pv_done[h], 1);
             mbar_init(&o_done[h], 1);
         }
@@ -245,7 +249,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 if (nkv > 0) ok = mbar_wait(q_full, 0, abort_flag) && scores(0);
                 for (int j = 0; j < nkv && ok; ++j) {
                     if (C::BUFFERS > 1 && j + 1 < nkv && !scores(j + 1)) { ok = false; break; }
-                    ok = mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1, abort_flag) && mbar_wait(&p_ready[half], j & 1, abort_flag);
+                    ok = mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1, abort_flag) &&
+                         (C::BUFFERS > 1 ? mbar_wait(&p_ready[half * C::BUFFERS + (j & 1)], (j >> 1) & 1, abort_flag)
+                                         : mbar_wait(&p_ready[half], j & 1, abort_flag));
                     if (!ok) break;
                     tc_fence_after();
                     issue_pv(j, tmem_O, tmem_S + (C::BUFFERS > 1 ? (j & 1) * KEYS : 0));
@@ -368,7 +374,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_ready[half]);
+            mbar_arrive(&p_ready[C::BUFFERS > 1 ? half * C::BUFFERS + (j & 1) : half]);
             float s0, s1;
             f2_unpack(f2_add(f2_add(sum2[0], sum2[1]), f2_add(sum2[2], sum2[3])), s0, s1);
             l += s0 + s1;

@@ -282,6 +282,27 @@ def test_the_same_bits_every_time(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_whose_maximum_rises_with_every_tile(D, dtype):
+    """32 rows of every 128, a warp's, see scores that grow by 6.4 (9.2 in log2 units) from one 64 keys to the next, so that their sums are
+    scaled down for every tile; the others' scores stay flat, and their warps could run ahead."""
+    args = make([(500, 1500), (130, 700), (60, 900)], 4, 1, D, 16, dtype, seed=11)
+    q, ck, cv, pages, offsets, lengths = args
+    q.mul_(2 ** -7)
+    q[..., 0] = 0
+    rows = torch.arange(q.shape[0] * 4, device="cuda").view(-1, 4)
+    for b in range(3):
+        lo, hi = offsets[b].item(), offsets[b + 1].item()
+        steep = (rows[lo:hi] - lo * 4) // 32 % 4 == 1
+        q[lo:hi, :, 0][steep] = D ** 0.5 / 10
+        for t in range(lengths[b].item()):
+            ck[pages[b, t // 16].item(), :, t % 16, 0] = t
+    for backend in (["tc"] if dtype == BF16 else []) + ["rows", "single", "auto"]:
+        for splits in (0, 1):
+            check(args, ops.paged_attention(*args, backend=backend, splits=splits))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D,kv_heads,page,token_major", [(64, 12, 16, False), (128, 3, 8, True), (32, 1, 48, False), (128, 40, 16, False)])
 @pytest.mark.parametrize("seqs", [1, 9, 70])
 def test_append(dtype, D, kv_heads, page, token_major, seqs):
