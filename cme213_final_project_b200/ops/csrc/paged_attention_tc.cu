@@ -8,7 +8,9 @@
 // What bounds it: the exponentials (16 a clock and SM: 512 clocks for 128 rows x 64 keys) and, with head size 128, as many clocks of the
 // tensor pipe; one hides behind the other only if several tiles of rows are on their way at a time.
 //   head size 64   128 rows a CTA, three CTAs an SM (128 columns of tensor memory each): a tile's chain of steps, its start and its end run
-//                  under the others'.
+//                  under the others'.  Where that many CTAs are not there, two an SM at the most, with two buffers of scores (256 columns): a
+//                  tile's steps are shorter, all SMs' together fewer (1 / 8 / 16 chunks of GPT-2 small, us: 16.4 / 20.4 / 31.8, three an SM
+//                  17.6 / 24.5 / 31.9; 512 tokens over 4096 in 4 sequences 73.5 / 65.4).
 //   head size 128  256 rows a CTA, one CTA an SM, two buffers of scores for each half: S_{j+1} is made while softmax_j runs.  Both halves
 //                  read the same keys: with 128 rows a CTA the tiles of K and V would come out of L2 at 53 bytes a clock and SM.
 // Every mbarrier wait is bounded; on expiry the CTA flags the status word, frees TMEM and returns.
@@ -30,15 +32,18 @@ constexpr int KEYS = PAGED_TC_KEYS;
 // bf16 then holds exactly)
 constexpr float RESCALE_THRESHOLD = 8.f;
 
-template <int D> struct Cfg;
-template <> struct Cfg<64> {
+template <int D, bool FEW> struct Cfg;
+template <> struct Cfg<64, false> {
     static constexpr int HALVES = 1, STAGES = 3, BUFFERS = 1, CTAS = 3, COLS = 128;
 };
-template <> struct Cfg<128> {
+template <> struct Cfg<64, true> {
+    static constexpr int HALVES = 1, STAGES = 3, BUFFERS = 2, CTAS = 2, COLS = 256;
+};
+template <> struct Cfg<128, false> {
     static constexpr int HALVES = 2, STAGES = 4, BUFFERS = 2, CTAS = 1, COLS = 512;
 };
-template <int D> struct Sizes : Cfg<D> {
-    using C = Cfg<D>;
+template <int D, bool FEW> struct Sizes : Cfg<D, FEW> {
+    using C = Cfg<D, FEW>;
     static constexpr int SLABS = D / 64;                              // 64 columns = 128 bytes each
     static constexpr int Q_SLAB = 128 * 128, KV_SLAB = KEYS * 128;
     static constexpr int Q_BYTES = SLABS * Q_SLAB, KV_BYTES = SLABS * KV_SLAB;
@@ -73,11 +78,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
-template <int D>
-__global__ void __launch_bounds__(Sizes<D>::THREADS, Sizes<D>::CTAS)
+template <int D, bool FEW>
+__global__ void __launch_bounds__(Sizes<D, FEW>::THREADS, Sizes<D, FEW>::CTAS)
 paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const TcParams p) {
-    using C = Sizes<D>;
+    using C = Sizes<D, FEW>;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {             // swizzled tiles need a 1024-byte aligned base
         if (threadIdx.x == 0 && p.status) atomicExch(p.status, CME_ERR_SHAPE);
@@ -440,9 +445,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 // (chunks of GPT-2 small, 1 / 2 / 8 sequences, us: 19.3 / 19.0 / 25.6, spread over the SMs 17.6 / 17.1 / 24.5).
 constexpr int spread(int each) { return 228 * 1024 / (each + 1); }
 
-template <int D> int launch(const CmePaged* a, const PagedPlan& plan, TcParams& p, cudaStream_t st) {
-    using C = Sizes<D>;
-    auto* kernel = paged_attn_tc_kernel<D>;
+template <int D, bool FEW> int launch(const CmePaged* a, const PagedPlan& plan, long long ctas, int sms, TcParams& p, cudaStream_t st) {
+    using C = Sizes<D, FEW>;
+    auto* kernel = paged_attn_tc_kernel<D, FEW>;
     static bool attr[CME_MAX_DEVICES] = {};               // function attributes are per device
     int dev = 0;
     CME_CUDA(cudaGetDevice(&dev));
@@ -456,11 +461,9 @@ template <int D> int launch(const CmePaged* a, const PagedPlan& plan, TcParams& 
     if ((rc = paged_make_q_map(&mq, a, p.group, p.half_rows / p.group))) return rc;
     if ((rc = paged_make_map(&mk, a, a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
-    int sms;
-    if ((rc = cme_num_sms(&sms))) return rc;
-    const long long ctas = (long long)plan.tiles * plan.splits * a->kv_heads, each = std::max(1ll, (ctas + sms - 1) / sms);
+    const long long each = std::max(1ll, (ctas + sms - 1) / sms);
     const int smem = each < C::CTAS ? spread((int)each) : C::SMEM;
-    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits) * a->kv_heads), dim3(C::THREADS), (size_t)smem, st,
+    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)ctas), dim3(C::THREADS), (size_t)smem, st,
                                   mq, mk, mv, p));
     CME_LAUNCH_CHECK();
     return CME_OK;
@@ -486,5 +489,9 @@ int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st
     p.part_o = a->ws + (parts * 2 + 3) / 4 * 4;
     p.status = cme_attn_status_ptr();
     CME_REQUIRE(p.status != nullptr, CME_ERR_CUDA, "paged attention: device state unavailable");
-    return a->head_dim == 64 ? launch<64>(a, plan, p, st) : launch<128>(a, plan, p, st);
+    int sms;
+    if (const int rc = cme_num_sms(&sms)) return rc;
+    const long long ctas = (long long)plan.tiles * plan.splits * a->kv_heads;
+    if (a->head_dim == 128) return launch<128, false>(a, plan, ctas, sms, p, st);
+    return ctas <= sms * 2ll ? launch<64, true>(a, plan, ctas, sms, p, st) : launch<64, false>(a, plan, ctas, sms, p, st);
 }
