@@ -32,7 +32,7 @@ int paged_mma_key_tile(int dtype, int head_dim);
 int paged_mma_ctas(int dtype, int head_dim);               // of the kernels for up to 16 rows, on an SM
 constexpr int PAGED_TC_KEYS = 64;
 
-// Division by a page size that the host knows, for 0 <= x < 2^31: x / d = (x * m) >> s with m = ceil(2^s / d) and s = 31 + ceil(log2 d)
+// Division by a number that the host knows, for 0 <= x < 2^31: x / d = (x * m) >> s with m = ceil(2^s / d) and s = 31 + ceil(log2 d)
 // (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994).
 struct PagedDiv {
     unsigned long long m;
@@ -92,6 +92,52 @@ __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile
         }
         base += __shfl_sync(0xffffffffu, upto, 31);
     }
+    return t;
+}
+
+// As paged_find_tile, counting the tiles by what they see: most key tiles of `keys` keys first, equal ones by sequence.  Up to 32 sequences.
+__device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, int tile, int group, int row_tile, int keys) {
+    const int b = threadIdx.x & 31, each = row_tile / group;           // (whole tokens)
+    PagedTile t{0, 0, 0, 0, 0, 0};
+    int lo = 0, hi = 0, length = 0;
+    if (b < a.seqs) {
+        lo = a.offsets[b];
+        hi = a.offsets[b + 1];
+        length = (int)min((long long)max(0, min(a.lengths[b], a.max_len)), (long long)a.width * a.page);
+    }
+    lo = max(0, min(lo, a.rows));
+    hi = max(lo, min(hi, a.rows));
+    const int n = hi - lo, own = (n + each - 1) / each;
+    // tiles of the sequence that see x key tiles at least; they are its last ones
+    auto count = [&](int x) {
+        const long long need = (long long)(x - 1) * keys + 1;          // keys
+        if (x <= 0) return own;
+        if (length < need) return 0;
+        const int more = (int)max(1ll, need - length + n);             // of the new tokens (<= n)
+        return own - (more + each - 1) / each + 1;
+    };
+    if (tile >= (int)__reduce_add_sync(0xffffffffu, own)) return t;
+    int x = 0, most = __reduce_max_sync(0xffffffffu, n > 0 ? length / keys + 1 : 0);      // the tile sees between x and `most` key tiles
+    while (x < most) {
+        const int mid = (x + most + 1) >> 1;
+        if ((int)__reduce_add_sync(0xffffffffu, count(mid)) > tile) x = mid;
+        else most = mid - 1;
+    }
+    const int above = count(x + 1), same = count(x) - above;
+    tile -= (int)__reduce_add_sync(0xffffffffu, above);
+    int upto = same;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (b >= o) upto += v;
+    }
+    const int src = __ffs(__ballot_sync(0xffffffffu, tile < upto)) - 1;
+    t.seq = src;
+    t.first = __shfl_sync(0xffffffffu, (own - above - 1 - (tile - (upto - same))) * row_tile, src);
+    t.token0 = __shfl_sync(0xffffffffu, lo, src);
+    t.n = __shfl_sync(0xffffffffu, n, src);
+    t.length = __shfl_sync(0xffffffffu, length, src);
+    t.rows = (int)min((long long)row_tile, (long long)t.n * group - t.first);
     return t;
 }
 

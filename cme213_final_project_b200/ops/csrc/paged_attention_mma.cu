@@ -51,8 +51,8 @@ template <typename T, int D, bool ROWS> struct Cfg {
 
 struct MmaParams {
     CmePaged a;
-    PagedDiv page;
-    int group, box, box_log, splits, split_keys, tiles;
+    PagedDiv page, heads, parts;           // slots of a page; key heads and splits (rows)
+    int group, box, box_log, splits, split_keys, tiles, by_keys;
     float scale_log2;
     float* part_o;                         // [rows, heads, splits, head_dim] sums of a part; stream: [CTA, 2, 16, head_dim]
     float2* part_ml;                       // [rows, heads, splits] its m (log2 units) and l; stream: [CTA, 2, 16]
@@ -510,9 +510,10 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     }
     pdl_release();
     pdl_wait();
-    const int split = blockIdx.x % p.splits, head = blockIdx.y;
-    // late tiles, which see the most keys, first
-    const PagedTile t = paged_find_tile(a, p.tiles - 1 - (int)(blockIdx.x / p.splits), p.group, 64);
+    // Where not all CTAs run at once, tiles that see the most keys first (above 32 sequences: late tiles), of all heads: fp32, 16 sequences of
+    // up to 400 tokens over 1500, 12 heads of 64 240 / 206 us.
+    const int at = p.heads.div(blockIdx.x), head = blockIdx.x - at * a.kv_heads, tile = p.parts.div(at), split = at - tile * p.splits;
+    const PagedTile t = p.by_keys ? paged_find_tile_by_keys(a, tile, p.group, 64, C::KEYS) : paged_find_tile(a, p.tiles - 1 - tile, p.group, 64);
     __syncthreads();
     if (t.rows == 0) return;
     // keys [0, limit) are seen by the last row; this CTA takes [begin, end)
@@ -1047,9 +1048,17 @@ int launch(dim3 grid, const CmePaged* a, int cluster, const MmaParams& p, cudaSt
     return CME_OK;
 }
 
-template <typename T, int D> int launch_any(const CmePaged* a, const PagedPlan& plan, const MmaParams& p, cudaStream_t st) {
+template <typename T, int D> int launch_any(const CmePaged* a, const PagedPlan& plan, MmaParams& p, cudaStream_t st) {
+    if (plan.kernel == PAGED_ROWS) {
+        int sms;
+        if (const int rc = cme_num_sms(&sms)) return rc;
+        const unsigned ctas = (unsigned)(plan.tiles * plan.splits) * a->kv_heads;
+        p.by_keys = a->seqs <= 32 && ctas > (unsigned)sms * Cfg<T, D, true>::CTAS;
+        p.heads = paged_div(a->kv_heads);
+        p.parts = paged_div(plan.splits);
+        return launch<T, D, true, paged_attn_rows_kernel<T, D>>(dim3(ctas), a, 1, p, st);
+    }
     const dim3 grid((unsigned)(plan.tiles * plan.splits), a->kv_heads);
-    if (plan.kernel == PAGED_ROWS) return launch<T, D, true, paged_attn_rows_kernel<T, D>>(grid, a, 1, p, st);
     if (plan.kernel == PAGED_CLUSTER) return launch<T, D, false, paged_attn_single_kernel<T, D, true>>(grid, a, plan.splits, p, st);
     const int rc = launch<T, D, false, paged_attn_single_kernel<T, D, false>>(dim3(plan.splits), a, 1, p, st);
     if (rc) return rc;

@@ -57,8 +57,8 @@ template <int D, bool FEW> struct Sizes : Cfg<D, FEW> {
 
 struct TcParams {
     CmePaged a;
-    PagedDiv page;
-    int group, row_tile, half_rows, box, box_log, splits, split_keys, tiles;
+    PagedDiv page, heads, parts;           // slots of a page; key heads whose tiles are taken together; splits
+    int group, row_tile, half_rows, box, box_log, splits, split_keys, tiles, by_keys;
     float scale_log2;
     float* part_o;
     float2* part_ml;
@@ -136,13 +136,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     __syncwarp();                             // the loading lanes see the barriers
     if (warp == 0) { tmem_alloc(tmem_slot, C::COLS); tmem_relinquish(); }
     pdl_wait();
-    // Late tiles, which see the most keys, first: of all heads, or (two halves, which take more keys a clock out of L2) head by head, so that
-    // fewer heads' keys are in use at a time (us, all heads / head by head: 16 chunks of GPT-2 small 31.9 / 34.2, two of 2048 over 8192 with head
-    // size 128 352 / 331).
-    const int of_head = p.tiles * p.splits;
-    const int head = C::HALVES > 1 ? blockIdx.x / of_head : blockIdx.x % a.kv_heads;
-    const int at = C::HALVES > 1 ? blockIdx.x % of_head : blockIdx.x / a.kv_heads, split = at % p.splits;
-    const PagedTile t = paged_find_tile(a, p.tiles - 1 - at / p.splits, p.group, p.row_tile);
+    // Where not all CTAs run at once, tiles that see the most keys first (above 32 sequences: late tiles); of all heads, or (two halves, which
+    // take more keys a clock out of L2) of one to four, so that fewer heads' keys are in use at a time.  us, late tiles first / most keys
+    // first: 16 chunks of GPT-2 small 31.9 / 26.3, 16 of 1024 77 / 72; head size 128 (there head by head), two of up to 2048 over 8192 328 /
+    // 321, four 396 / 377.
+    const int at = p.heads.div(blockIdx.x), head = blockIdx.y * p.heads.d + blockIdx.x - at * p.heads.d;
+    const int tile = p.parts.div(at), split = at - tile * p.splits;
+    const PagedTile t = p.by_keys ? paged_find_tile_by_keys(a, tile, p.group, p.row_tile, KEYS)
+                                     : paged_find_tile(a, p.tiles - 1 - tile, p.group, p.row_tile);
     if (t.rows == 0) {
         if (warp == 0) { __syncwarp(); tmem_dealloc(*tmem_slot, C::COLS); }
         return;
@@ -462,8 +463,9 @@ template <int D, bool FEW> int launch(const CmePaged* a, const PagedPlan& plan, 
     if ((rc = paged_make_map(&mk, a, a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     const long long each = std::max(1ll, (ctas + sms - 1) / sms);
+    p.by_keys = a->seqs <= 32 && ctas > (long long)sms * C::CTAS;
     const int smem = each < C::CTAS ? spread((int)each) : C::SMEM;
-    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)ctas), dim3(C::THREADS), (size_t)smem, st,
+    CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits) * p.heads.d, a->kv_heads / p.heads.d), dim3(C::THREADS), (size_t)smem, st,
                                   mq, mk, mv, p));
     CME_LAUNCH_CHECK();
     return CME_OK;
@@ -483,6 +485,10 @@ int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st
     p.splits = plan.splits;
     p.split_keys = plan.split_keys;
     p.tiles = plan.tiles;
+    int heads = a->kv_heads;
+    if (a->head_dim == 128) for (heads = 4; a->kv_heads % heads; --heads) {}
+    p.heads = paged_div(heads);
+    p.parts = paged_div(plan.splits);
     p.scale_log2 = a->scale * LOG2E;
     const long long parts = (long long)a->rows * a->heads * plan.splits;
     p.part_ml = reinterpret_cast<float2*>(a->ws);
