@@ -11,6 +11,7 @@ namespace {
 // ------------------------------------------------------------------------------------------------------
 // Token i of a sequence's n new ones goes to position length - n + i.  A copy, so bytes bound it (read once, written once); one warp per
 // token, whose loads are on their way before it looks up where they go: offsets -> length -> page is a chain of three.
+// 16 prompts of 500 to 1024 tokens, 12 heads of 64: 14.6 us, 5.1 TB/s of 75 MB.  16 tokens: 2.3 us, a launch and the chain.
 constexpr int APPEND_WARPS = 4;
 constexpr int APPEND_UNROLL = 4;           // 16-byte pieces per lane of keys, and as many of values, at a time
 
