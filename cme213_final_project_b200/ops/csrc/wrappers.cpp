@@ -114,6 +114,17 @@ at::Tensor floats(long long n, const at::Tensor& t) { return at::empty({n}, t.op
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& t) {
     return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
 }
+// Two results of a call in one piece of memory, the second behind the first: an allocation takes half a microsecond.
+void fresh_pair(at::Tensor& a, at::IntArrayRef a_sizes, at::ScalarType a_type, at::Tensor& b, at::IntArrayRef b_sizes, at::ScalarType b_type,
+                const at::Tensor& t) {
+    const long long a_size = c10::elementSize(a_type), b_size = c10::elementSize(b_type);
+    const long long b_at = (c10::multiply_integers(a_sizes) * a_size + 15) / 16 * 16;
+    a = fresh({(b_at + c10::multiply_integers(b_sizes) * b_size + a_size - 1) / a_size}, a_type, t);
+    b = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(a.storage()), a.key_set(), c10::scalarTypeToTypeMeta(b_type));
+    b.unsafeGetTensorImpl()->set_storage_offset(b_at / b_size);
+    b.unsafeGetTensorImpl()->set_sizes_contiguous(b_sizes);
+    a.unsafeGetTensorImpl()->set_sizes_contiguous(a_sizes);
+}
 
 PyObject* wrap(const at::Tensor& t) {
     if (!t.defined()) Py_RETURN_NONE;
@@ -382,12 +393,12 @@ PyObject* embedding_bwd(PyObject*, PyObject* const* a, Py_ssize_t) {
 // ---------------------------------------------------------------------------------------------------------------------
 // Generation: the paged cache, attention over it, the next token
 // ---------------------------------------------------------------------------------------------------------------------
-// A tensor on the current device with so many dimensions, whose last one is contiguous; undefined for None where that is allowed.
-at::Tensor strided(PyObject* o, const char* what, int dims, bool optional = false) {
+// A tensor on device `device`, the current one, with so many dimensions, whose last one is contiguous; undefined for None where that is allowed.
+at::Tensor strided(int device, PyObject* o, const char* what, int dims, bool optional = false) {
     if (optional && o == Py_None) return at::Tensor();
     if (!THPVariable_Check(o)) fail(PyExc_TypeError, "native ops take tensors");
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || t.get_device() != c10::cuda::current_device())
+    if (!t.is_cuda() || t.get_device() != device)
         fail(native_error, std::string(what) + " has to be on the current CUDA device");
     if (t.dim() != dims) fail(native_error, std::string(what) + " has to have " + std::to_string(dims) + " dimensions");
     if (t.size(-1) > 1 && t.stride(-1) != 1) fail(native_error, std::string(what) + " has to be contiguous along its last dimension");
@@ -396,8 +407,8 @@ at::Tensor strided(PyObject* o, const char* what, int dims, bool optional = fals
 void same_type(const at::Tensor& t, at::ScalarType type, const char* what, const char* name) {
     if (t.scalar_type() != type) fail(native_error, std::string(what) + " has to be " + name);
 }
-at::Tensor whole_numbers(PyObject* o, const char* what, int dims, bool optional = false) {
-    const at::Tensor t = strided(o, what, dims, optional);
+at::Tensor whole_numbers(int device, PyObject* o, const char* what, int dims, bool optional = false) {
+    const at::Tensor t = strided(device, o, what, dims, optional);
     if (t.defined()) same_type(t, at::kInt, what, "int32");
     return t;
 }
@@ -408,10 +419,10 @@ void has_size(const at::Tensor& t, int dim, long long n, const char* what) {
 }
 
 // a: cache_k, cache_v, pages, offsets, lengths; x: new rows [rows, heads, head_dim] of the cache's type
-CmePaged paged(const at::Tensor& x, PyObject* const* a) {
-    const at::Tensor k = strided(a[0], "cache_k", 4), v = strided(a[1], "cache_v", 4);
-    const at::Tensor pages = whole_numbers(a[2], "pages", 2), offsets = whole_numbers(a[3], "offsets", 1),
-                     lengths = whole_numbers(a[4], "lengths", 1);
+CmePaged paged(int device, const at::Tensor& x, PyObject* const* a) {
+    const at::Tensor k = strided(device, a[0], "cache_k", 4), v = strided(device, a[1], "cache_v", 4);
+    const at::Tensor pages = whole_numbers(device, a[2], "pages", 2), offsets = whole_numbers(device, a[3], "offsets", 1),
+                     lengths = whole_numbers(device, a[4], "lengths", 1);
     CmePaged d;
     std::memset(&d, 0, sizeof d);
     d.dtype = dtype(x);
@@ -437,8 +448,9 @@ CmePaged paged(const at::Tensor& x, PyObject* const* a) {
 // (k, v, cache_k, cache_v, pages, offsets, lengths)
 PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t) {
     HANDLE_TH_ERRORS
-    const at::Tensor k = strided(a[0], "k", 3), v = strided(a[1], "v", 3);
-    CmePaged d = paged(k, a + 2);
+    const int device = c10::cuda::current_device();
+    const at::Tensor k = strided(device, a[0], "k", 3), v = strided(device, a[1], "v", 3);
+    CmePaged d = paged(device, k, a + 2);
     if (v.scalar_type() != k.scalar_type()) fail(native_error, "v has to have the type of k");
     for (int i = 0; i < 3; ++i) has_size(v, i, k.size(i), "v");
     has_size(k, 1, d.kv_heads, "k");
@@ -452,13 +464,15 @@ PyObject* cache_append(PyObject*, PyObject* const* a, Py_ssize_t) {
 // (q, cache_k, cache_v, pages, offsets, lengths, scale | None, max_len | None, backend, splits)
 PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t) {
     HANDLE_TH_ERRORS
-    const at::Tensor q = strided(a[0], "q", 3);
-    CmePaged d = paged(q, a + 1);
+    const int device = c10::cuda::current_device();
+    const at::Tensor q = strided(device, a[0], "q", 3);
+    CmePaged d = paged(device, q, a + 1);
     d.heads = int32(q.size(1));
     d.scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)d.head_dim)) : real(a[6]);
     if (a[7] != Py_None) d.max_len = int32(whole(a[7]));
     const int backend = int32(whole(a[8])), splits = int32(whole(a[9]));
-    const at::Tensor out = fresh(q.sizes(), q.scalar_type(), q), lse = fresh({d.rows, d.heads}, at::kFloat, q);
+    at::Tensor out, lse;
+    fresh_pair(out, q.sizes(), q.scalar_type(), lse, {d.rows, d.heads}, at::kFloat, q);
     d.o = ptr(out);
     d.lse = (float*)ptr(lse);
     check(lib.cme_paged_attention_ws_bytes(&d, backend, splits, &d.ws_bytes));
@@ -476,7 +490,8 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t) {
 //  bias_values | None, temperature | None, allowed | None, noise | None, processed)
 PyObject* next_token(PyObject*, PyObject* const* a, Py_ssize_t) {
     HANDLE_TH_ERRORS
-    const at::Tensor logits = strided(a[0], "logits", 2);
+    const int device = c10::cuda::current_device();
+    const at::Tensor logits = strided(device, a[0], "logits", 2);
     CmeToken d;
     std::memset(&d, 0, sizeof d);
     d.dtype = dtype(logits);
@@ -486,13 +501,13 @@ PyObject* next_token(PyObject*, PyObject* const* a, Py_ssize_t) {
     if (d.rows <= 1) d.logits_ld = std::max<long long>(d.logits_ld, d.vocab);
     // one number per row
     auto per_row = [&](PyObject* o, const char* what, at::ScalarType type) -> const void* {
-        const at::Tensor t = strided(o, what, 1, true);
+        const at::Tensor t = strided(device, o, what, 1, true);
         if (!t.defined()) return nullptr;
         same_type(t, type, what, type == at::kInt ? "int32" : "fp32");
         has_size(t, 0, d.rows, what);
         return ptr(t);
     };
-    if (const at::Tensor h = whole_numbers(a[1], "history", 2, true); h.defined()) {
+    if (const at::Tensor h = whole_numbers(device, a[1], "history", 2, true); h.defined()) {
         has_size(h, 0, d.rows, "history");
         if (a[2] == Py_None) fail(native_error, "a history needs its lengths");
         d.history = (const int*)ptr(h); d.history_ld = h.stride(0); d.history_len = int32(h.size(1));
@@ -504,8 +519,8 @@ PyObject* next_token(PyObject*, PyObject* const* a, Py_ssize_t) {
     d.frequency = (const float*)per_row(a[6], "frequency", at::kFloat);
     d.temperature = (const float*)per_row(a[9], "temperature", at::kFloat);
     if ((a[7] == Py_None) != (a[8] == Py_None)) fail(native_error, "bias_ids and bias_values belong together");
-    if (const at::Tensor ids = whole_numbers(a[7], "bias_ids", 2, true); ids.defined()) {
-        const at::Tensor values = strided(a[8], "bias_values", 2);
+    if (const at::Tensor ids = whole_numbers(device, a[7], "bias_ids", 2, true); ids.defined()) {
+        const at::Tensor values = strided(device, a[8], "bias_values", 2);
         same_type(values, at::kFloat, "bias_values", "fp32");
         has_size(ids, 0, d.rows, "bias_ids");
         has_size(values, 0, d.rows, "bias_values");
@@ -513,19 +528,20 @@ PyObject* next_token(PyObject*, PyObject* const* a, Py_ssize_t) {
         if (!ids.is_contiguous() || !values.is_contiguous()) fail(native_error, "biases have to be contiguous");
         d.bias_ids = (const int*)ptr(ids); d.bias_values = (const float*)ptr(values); d.biases = int32(ids.size(1));
     }
-    if (const at::Tensor m = whole_numbers(a[10], "allowed", 2, true); m.defined()) {
+    if (const at::Tensor m = whole_numbers(device, a[10], "allowed", 2, true); m.defined()) {
         if (m.size(0) != 1) has_size(m, 0, d.rows, "allowed");
         has_size(m, 1, ((long long)d.vocab + 31) / 32, "allowed");
         d.allowed = (const int*)ptr(m); d.allowed_ld = m.size(0) == 1 ? 0 : m.stride(0);
     }
-    if (const at::Tensor g = strided(a[11], "noise", 2, true); g.defined()) {
+    if (const at::Tensor g = strided(device, a[11], "noise", 2, true); g.defined()) {
         same_type(g, at::kFloat, "noise", "fp32");
         has_size(g, 0, d.rows, "noise");
         has_size(g, 1, d.vocab, "noise");
         if (!g.is_contiguous()) fail(native_error, "noise has to be contiguous");
         d.noise = (const float*)ptr(g);
     }
-    const at::Tensor token = fresh({d.rows}, at::kInt, logits), logprob = fresh({d.rows}, at::kFloat, logits);
+    at::Tensor token, logprob;
+    fresh_pair(token, {d.rows}, at::kInt, logprob, {d.rows}, at::kFloat, logits);
     const at::Tensor processed = truth(a[12]) ? fresh({d.rows, d.vocab}, logits.scalar_type(), logits) : at::Tensor();
     d.token = (int*)ptr(token); d.logprob = (float*)ptr(logprob); d.processed = ptr(processed);
     run([&](void* st) { return lib.cme_next_token(&d, st); });
