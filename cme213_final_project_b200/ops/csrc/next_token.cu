@@ -474,30 +474,36 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
     if (p->rows == 0) return CME_OK;
     int sms, rc;
     if ((rc = cme_num_sms(&sms))) return rc;
-    // As many CTAs as keep the SMs busy, with no fewer than 2048 tokens each.
-    int cluster = 1;
-    while (cluster < MAX_CLUSTER && (long long)p->rows * cluster < 4ll * sms && p->vocab / (2 * cluster) >= 2048) cluster *= 2;
-    const bool biased = p->bias_ids && p->biases;
-    const bool marks = biased || (p->history && p->history_len);
-    int slice, words, records;
-    size_t smem;
-    for (;; cluster *= 2) {                                // smaller slices where a CTA's records would not fit
+    const bool biased = p->bias_ids && p->biases, marks = biased || (p->history && p->history_len);
+    const int n = p->dtype == CME_F32 ? 4 : 8;
+    auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+    const bool aligned = al16(p->logits) && al16(p->processed) && al16(p->noise) && p->logits_ld % n == p->vocab % n;
+    int slice, words, records, threads;
+    bool vector;
+    size_t tables, smem;
+    auto lay_out = [&](int cluster) {
         slice = (cme_cdiv(p->vocab, cluster) + 31) / 32 * 32;
         words = marks ? slice / 32 + 1 : 0;                // (marks start up to eight tokens before the slice)
         records = marks ? (int)std::min((long long)slice, (long long)(p->history ? p->history_len : 0) + (biased ? p->biases : 0)) : 0;
-        smem = marks ? ((size_t)2 * words + 1 + 3 * (size_t)records) * 4 : 0;
-        if (smem <= MAX_SMEM) break;
-        CME_REQUIRE(cluster < MAX_CLUSTER, CME_ERR_LIMIT, "next token: a history of %d with a vocabulary of %d", p->history_len, p->vocab);
+        tables = smem = marks ? ((size_t)2 * words + 1 + 3 * (size_t)records) * 4 : 0;
+        // In groups of sixteen bytes, where there is more than a turn or two of them and rows of logits start at the same place between
+        // 16-byte boundaries as rows of noise and of the processed logits
+        vector = slice >= 1024 && aligned;
+        threads = slice <= 1024 ? 128 : 256;
+        if (vector) smem = (smem + 15) / 16 * 16 + (size_t)STAGES * threads * 16 * ((p->dtype == CME_F32 ? 2 : 1) + (p->noise ? 2 : 0));
+    };
+    // As many CTAs as run at a time, with no fewer than 2048 tokens each: a second turn costs as much as a row's length (us, one CTA / two for
+    // a row: 319 rows of 6186 10.7 / 18.0, 200 of 50304 in fp32, two / four 28.0 / 34.5).  Smaller slices where a CTA's records would not fit.
+    int cluster = MAX_CLUSTER;
+    for (; cluster > 1; cluster /= 2) {
+        lay_out(cluster);
+        if (p->vocab / cluster >= 2048 && (long long)p->rows * cluster <= (long long)sms * std::min<size_t>(4, 227 * 1024 / (smem + 1024))) break;
     }
+    for (lay_out(cluster); tables > MAX_SMEM; lay_out(cluster *= 2))
+        CME_REQUIRE(cluster < MAX_CLUSTER, CME_ERR_LIMIT, "next token: a history of %d with a vocabulary of %d", p->history_len, p->vocab);
     CME_REQUIRE((long long)p->rows * cluster < (1ll << 31), CME_ERR_LIMIT, "next token: too many rows");
-    const int n = p->dtype == CME_F32 ? 4 : 8;
-    auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
-    // In groups of sixteen bytes, where there is more than a turn or two of them and rows of logits start at the same place between 16-byte boundaries as rows of noise and of the processed logits
-    const bool vector = slice >= 1024 && al16(p->logits) && al16(p->processed) && al16(p->noise) && p->logits_ld % n == p->vocab % n;
     auto* kernel = p->dtype == CME_F32 ? (vector ? next_token_kernel<float, true> : next_token_kernel<float, false>)
                                        : (vector ? next_token_kernel<__nv_bfloat16, true> : next_token_kernel<__nv_bfloat16, false>);
-    const int threads = slice <= 1024 ? 128 : 256;
-    if (vector) smem = (smem + 15) / 16 * 16 + (size_t)STAGES * threads * 16 * ((p->dtype == CME_F32 ? 2 : 1) + (p->noise ? 2 : 0));
     if (smem > 48 * 1024) CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p->rows * cluster));
