@@ -435,7 +435,7 @@ def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Opti
 
     ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_len``: no length is larger (default: what the table
     holds); the number of parts that the keys are divided into goes by it.  ``backend``: ``auto`` | ``single`` (few rows) | ``rows`` |
-    ``tc`` (tcgen05: bf16, head sizes 64 and 128); ``splits``: parts of the keys, 0 = by the rule, negative = joined
+    ``tc`` (tcgen05: bf16); ``splits``: parts of the keys, 0 = by the rule, negative = joined
     through scratch memory in any case."""
     return _native().paged_attention(q, cache_k, cache_v, pages, offsets, lengths, scale, max_len, _PAGED_BACKENDS[backend], splits)
 

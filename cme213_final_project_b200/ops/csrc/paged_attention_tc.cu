@@ -1,4 +1,4 @@
-// Attention of chunks of new tokens over a paged cache on tcgen05 (bf16, head sizes 64 and 128): scores, probabilities and sums of
+// Attention of chunks of new tokens over a paged cache on tcgen05 (bf16): scores, probabilities and sums of
 // 128 rows live in tensor memory; a row is a token and one of the query heads that share the key head, token by token.
 //
 //     S_j = Q K_j^T (TMEM) -> registers -> online softmax -> P_j (bf16 pairs over the columns of S_j) -> O += P_j V_j (TMEM)
@@ -11,6 +11,8 @@
 //                  under the others'.  Where that many CTAs are not there, two an SM at the most, with two buffers of scores (256 columns): a
 //                  tile's steps are shorter, all SMs' together fewer (1 / 8 / 16 chunks of GPT-2 small, us: 16.4 / 20.4 / 31.8, three an SM
 //                  17.6 / 24.5 / 31.9; 512 tokens over 4096 in 4 sequences 73.5 / 65.4).
+//   head size 32   as 64: the boxes reach over the head's end, where TMA puts zeros, and the sums' second half is left.  What bounds the steps
+//                  is the same (1566 tokens over 6081, 12 heads: 74 us, with warp-level products 94).
 //   head size 128  256 rows a CTA, one CTA an SM, two buffers of scores for each half: S_{j+1} is made while softmax_j runs.  Both halves
 //                  read the same keys: with 128 rows a CTA the tiles of K and V would come out of L2 at 53 bytes a clock and SM.
 // 16 chunks of GPT-2 small, 1 to 511 tokens over up to 1024: 26.3 us, 187 TFLOP/s; two of 1500 to 2048 over 8192, 32 heads of 128 on 8: 321 us,
@@ -111,6 +113,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     static_assert((1 + 4 * C::STAGES + C::HALVES * (2 * C::BUFFERS + 2) + 8) * 8 + 8 <= 384, "barriers");
 
     const CmePaged& a = p.a;
+    const int cols = D == 64 ? a.head_dim : D;                         // of the head (32 or 64)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (warp == C::LOADER && elect_one()) {
         *abort_flag = 0;
@@ -335,7 +338,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 if (!mbar_wait(&pv_done[half], (j - 1) & 1, abort_flag)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {         // 16 columns at a time: the score row stays in registers
+                for (int c = 0; c < cols / 16; ++c) {      // 16 columns at a time: the score row stays in registers
                     uint32_t o[16];
                     tmem_ld16(tmem_O + c * 16, o);
                     tmem_wait_ld();
@@ -398,7 +401,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 uint8_t* stage = sQ + half * C::Q_BYTES + (warp & 3) * 4096;
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
+                for (int c = 0; c < cols / 32; ++c) {
                     uint32_t o32[32];
                     if (nkv > 0) { tmem_ld32(tmem_O + c * 32, o32); tmem_wait_ld(); }
                     float* o = reinterpret_cast<float*>(o32);
@@ -414,8 +417,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 for (int i = 0; i < D / 8; ++i) {
                     const int src = i * 32 + lane, r = src / (D / 8), c = src % (D / 8);
                     const long long to = __shfl_sync(0xffffffffu, mine ? at : -1ll, r);
-                    if (to >= 0)
-                        *reinterpret_cast<uint4*>(out + to * D + c * 8) =
+                    if (to >= 0 && c * 8 < cols)
+                        *reinterpret_cast<uint4*>(out + to * cols + c * 8) =
                             *reinterpret_cast<const uint4*>(stage + (c >> 3) * C::Q_SLAB + swz(r, c & 7));
                 }
                 if (mine) a.lse[at] = l == 0.f ? -INFINITY : m_ref == -INFINITY ? l : (m_ref + log2f(l)) / LOG2E;
@@ -423,14 +426,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 const long long part = at * p.splits + split;
                 if (nkv > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
+                    for (int c = 0; c < cols / 32; ++c) {
                         uint32_t o[32];
                         tmem_ld32(tmem_O + c * 32, o);
                         tmem_wait_ld();
                         if (mine) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<uint4*>(p.part_o + part * D + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                                *reinterpret_cast<uint4*>(p.part_o + part * cols + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                         }
                     }
                 }

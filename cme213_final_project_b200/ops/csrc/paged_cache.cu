@@ -104,9 +104,9 @@ struct Form {
 Form form_of(const CmePaged* a, int backend, int sms) {
     const bool f32 = a->dtype == CME_F32;
     const int d = a->head_dim;
-    if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 64 ? 3 : 1), d == 64 ? 1.15f : 1.0f};
+    if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 3), d == 128 ? 1.0f : 1.15f};
     const int keys = paged_mma_key_tile(a->dtype, d);
-    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 32 ? 0.8f : d == 64 ? 1.4f : 1.2f};
+    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 32 ? 1.0f : d == 64 ? 1.4f : 1.2f};
     return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.2f : d == 64 ? 3.3f : 4.5f) : d == 128 ? 2.6f : 1.8f};
 }
 float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
@@ -120,11 +120,11 @@ float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles,
 int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* plan) {
     const int group = a->heads / a->kv_heads;
     const long long rows = (long long)a->rows * group;     // of one key head
-    const bool tc = a->dtype == CME_BF16 && a->head_dim >= 64 && group <= 128;
+    const bool tc = a->dtype == CME_BF16 && group <= 128;
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
     CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
-                "paged attention: the tcgen05 kernel takes bf16, head sizes 64 and 128 and up to 128 query heads per key head");
-    auto row_tile = [&](int b) { return b == 1 ? 16 : b == 2 ? 64 : (a->head_dim == 64 ? 1 : 2) * (128 / group * group); };
+                "paged attention: the tcgen05 kernel takes bf16 and up to 128 query heads per key head");
+    auto row_tile = [&](int b) { return b == 1 ? 16 : b == 2 ? 64 : (a->head_dim == 128 ? 2 : 1) * (128 / group * group); };
     auto tiles_of = [&](int b) { return rows / row_tile(b) + std::min(a->seqs, a->rows); };      // at the most: each sequence adds less than one
     auto even_tiles = [&](int b) { return a->seqs ? a->seqs * ((rows + (long long)a->seqs * row_tile(b) - 1) / ((long long)a->seqs * row_tile(b))) : 0; };
     const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
@@ -152,12 +152,16 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
     if (!backend) {
         backend = 1;
         if (rows > 16ll * a->seqs) {                       // (else a row tile has all rows of a sequence: its keys are read once)
-            const int many = tc ? 3 : 2;
+            int many = tc ? 3 : 2;
             const long long items = even_tiles(1) * a->kv_heads;
             int c;
             const long long turns = cluster_of(items, &c);
             float us;
             best_parts(many, &us);
+            // head size 32 wins less on the tensor cores (us, 12 heads, rows / tc: 64 tokens over 256 in 32 sequences 9.5 / 13.6, 512 over 8192
+            // in one 45 / 36, 1100 over 4166 in 5 184 / 141)
+            float rows_us;
+            if (tc && a->head_dim == 32 && (best_parts(2, &rows_us), rows_us < us)) { many = 2; us = rows_us; }
             // (two more tiles an item of the stream, as its kernel reckons)
             const float few = turns <= 8 ? 4.5f + (float)turns * one.tile_us : 6.f + (float)((items * (one_keys + 2) + one.slots - 1) / one.slots) * one.tile_us;
             if (us < few) backend = many;

@@ -281,6 +281,19 @@ def test_the_same_bits_every_time(D, dtype):
                 assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
 
 
+@pytest.mark.parametrize("heads,kv_heads,page", [(4, 4, 16), (6, 2, 8), (8, 1, 48), (3, 1, 128)])
+@pytest.mark.parametrize("drop", [0, 3])
+def test_heads_of_32_on_the_tensor_core_kernel(heads, kv_heads, page, drop):
+    args = make(CHUNKS, heads, kv_heads, 32, page, BF16, seed=heads, drop=drop, token_major=kv_heads == 2)
+    for splits in (0, 1, 3):
+        check(args, ops.paged_attention(*args, backend="tc", splits=splits))
+    many = make([(700, 900)] * 12, heads, kv_heads, 32, page, BF16, seed=heads)          # three CTAs an SM
+    first = ops.paged_attention(*many, backend="tc", splits=1)
+    check(many, first)
+    for _ in range(20):
+        assert all(torch.equal(x, y) for x, y in zip(first, ops.paged_attention(*many, backend="tc", splits=1)))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D", [64, 128])
 def test_rows_whose_maximum_rises_with_every_tile(D, dtype):
