@@ -6,7 +6,7 @@
 // tile, so that a key is read once for all of them.  Two forms:
 //   single  up to 16 rows a tile, each of four warps takes a quarter of every key tile and keeps its own m, l and sums; they are
 //           joined at the end.  For single tokens, which are bound by the bytes of the cache.
-//   rows    64 rows a CTA, 16 a warp; in fp32 and head sizes above 32 two warps share 16 rows and take every other 16 keys.  For chunks
+//   rows    64 rows a CTA, 16 a warp; in fp32 and head sizes above 32 two warps share 16 rows and take every other 16 or 32 keys.  For chunks
 //           that the tcgen05 kernel does not take.
 // The last warp looks up the pages and loads key tiles by TMA, one box per page (or key tile), several tiles ahead.
 // fp32 operands of the matrix instructions are split into two tf32 numbers each (x = hi + lo, 11 bits each) and multiplied as hi hi + hi lo + lo hi: what is
@@ -34,12 +34,12 @@ template <typename T, int D, bool ROWS> struct Cfg {
     static constexpr int ROW = D * (int)sizeof(T);                    // bytes of a key
     static constexpr int SLAB = ROW < 128 ? ROW : 128;                // bytes of a key in one swizzled slab
     static constexpr int SLABS = ROW / SLAB;
-    static constexpr int WARP_KEYS = ROW <= 128 ? 32 : 16;            // keys that a warp takes at a time
-    static constexpr int KEYS = 4 * WARP_KEYS;                        // key tile
+    static constexpr int WARP_KEYS = ROW <= 128 || (ROWS && F32 && D == 64) ? 32 : 16;      // keys that a warp takes at a time
+    static constexpr int KEYS = ROW <= 128 ? 128 : 64;                // key tile
     static constexpr int TILE = KEYS * ROW;                           // bytes of its keys (and of its values)
     static constexpr int STAGES = ROW == 64 ? 4 : ROWS && ROW == 512 ? 2 : 3;      // (the rows' fragments take 64 KB then)
     static constexpr int FRAGS = F32 ? D * 128 : 0;                   // bytes of 16 rows' fragments in shared memory
-    // CTAs of an SM, and groups of four warps, which take every other key tile (rows: every other 16 keys of each).  Two CTAs' or two groups'
+    // CTAs of an SM, and groups of four warps, which take every other key tile (rows: every other WARP_KEYS keys of each).  Two CTAs' or two groups'
     // chains of products and softmax run at a time; 64 KB tiles, or 64 rows' fragments of fp32, leave room for one CTA.  Rows, fp32, one
     // group / two, us: 16 heads of 64, 512 tokens over 2048 in 4 sequences 469 / 384; 32 heads of 128 on 8, 500 over 2000 in 2 864 / 701;
     // 12 heads of 64, 64 over 128 in one 11.9 / 11.4.  (Head size 32 has room for two CTAs.)
@@ -204,7 +204,7 @@ __device__ __forceinline__ void attend(WarpState<C, D>& w, const R& q, uint32_t 
         float sl[NK][4];                                   // the products with a low part
 #pragma unroll
         for (int n = 0; n < NK; ++n) sl[n][0] = sl[n][1] = sl[n][2] = sl[n][3] = 0.f;
-#pragma unroll 2
+#pragma unroll
         for (int ks = 0; ks < KS; ks += 2) {
             float4 f[4];
 #pragma unroll
@@ -486,8 +486,8 @@ __device__ __forceinline__ int row_sees(const MmaParams& p, const PagedTile& t, 
 // ------------------------------------------------------------------------------------------------------
 // What bounds it in fp32: three tf32 products an element at 8 clocks an instruction and scheduler (92 TFLOP/s of the product asked for), and beside
 // them 4 instructions to split each element of K and V, which every warp does for itself.  16 heads of 64, 512 tokens over 2048 in 4
-// sequences: 378 us, 40 TFLOP/s.  (Two tiles of 16 rows a warp, which split half as often: 344 us there, but 13.0 for 11.4 with 64 tokens
-// over 128 and 36 for 28 with head size 32.)
+// sequences: 351 us, 43 TFLOP/s.  (Two tiles of 16 rows a warp, which split half as often, when it took 378: 344 us there, but 13.0 for 11.4 with
+// 64 tokens over 128 and 36 for 28 with head size 32.)
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<T, D, true>::WARPS * 32 + 32, Cfg<T, D, true>::CTAS)
 paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const MmaParams p) {

@@ -107,7 +107,7 @@ Form form_of(const CmePaged* a, int backend, int sms) {
     if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 3), d == 128 ? 1.0f : 1.15f};
     const int keys = paged_mma_key_tile(a->dtype, d);
     if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 32 ? 1.0f : d == 64 ? 1.4f : 1.2f};
-    return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.2f : d == 64 ? 3.3f : 4.5f) : d == 128 ? 2.6f : 1.8f};
+    return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.0f : d == 64 ? 3.0f : 4.5f) : d == 128 ? 2.6f : 1.8f};
 }
 float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
     const long long ctas = tiles * a->kv_heads * parts, turns = (ctas + f.slots - 1) / f.slots;
