@@ -91,11 +91,12 @@ int check_cache(const CmePaged* a, const char* what) {
 
 constexpr int MAX_SPLITS = 128;
 
-// Estimated time of a form, in us: turns of its CTAs on the GPU, key tiles of a turn, time of a key tile (of its own size and rows, measured with
+// Estimated time of a form, in us: turns of its CTAs on the GPU, key tiles of a turn (two more where there are several: starts and ends), time
+// of a key tile (of its own size and rows, measured with
 // the keys in L2 and all SMs busy), and what its parts cost that are joined through scratch (written and read once more, at 3 TB/s,
 // and a launch).  The host does not know the sequences: they are taken to be as long as the longest, and to share the new tokens evenly.
-// Measured / estimated: 12 heads of 64, 128 tokens over 4096 in 4 sequences: tc in 1, 4, 8 parts 72 / 79, 32 / 32, 31 / 27, stream 62 / 70;
-// 4 heads of 128 in fp32, 256 over 512 in 8: rows 56 / 55, stream 97 / 104; 12 heads of 64 in fp32, 256 over 512 in 8: rows 82 / 84, stream 109 / 110.
+// Measured / estimated: 12 heads of 64, 128 tokens over 4096 in 4 sequences: tc in 1, 4, 8 parts 72 / 79, 32 / 32, 31 / 27, stream 62 / 72;
+// 4 heads of 128 in fp32, 256 over 512 in 8: rows 56 / 53, stream 97 / 107; 12 heads of 64 in fp32, 256 over 512 in 8: rows 72 / 95, stream 109 / 113.
 struct Form {
     int keys;                // of a tile
     int slots;               // CTAs that run at a time
@@ -106,13 +107,13 @@ Form form_of(const CmePaged* a, int backend, int sms) {
     const int d = a->head_dim;
     if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 3), d == 128 ? 1.0f : 1.15f};
     const int keys = paged_mma_key_tile(a->dtype, d);
-    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 32 ? 1.0f : d == 64 ? 1.4f : 1.2f};
+    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 64 ? 1.4f : 1.2f};
     return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.0f : d == 64 ? 3.0f : 4.5f) : d == 128 ? 2.6f : 1.8f};
 }
 float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
     const long long ctas = tiles * a->kv_heads * parts, turns = (ctas + f.slots - 1) / f.slots;
     const double joined = parts > 1 ? 4.0 + (double)a->rows * a->heads * parts * (a->head_dim + 2) * 8 / 3e6 : 0.0;
-    return (float)(5.0 + (double)turns * cme_cdiv(key_tiles, parts) * f.tile_us + joined);
+    return (float)(5.0 + (double)turns * (cme_cdiv(key_tiles, parts) + 2 * (turns > 1)) * f.tile_us + joined);
 }
 
 // backend: 0 by the rule, 1 up to 16 rows a tile, 2 rows, 3 tc.  splits: 0 by the rule; up to 16 rows: a cluster of so many CTAs (1, 2, 4
@@ -153,7 +154,8 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
         backend = 1;
         if (rows > 16ll * a->seqs) {                       // (else a row tile has all rows of a sequence: its keys are read once)
             int many = tc ? 3 : 2;
-            const long long items = even_tiles(1) * a->kv_heads;
+            // (a sequence's last tile of rows is half full on average)
+            const long long items = (rows / 16 + a->seqs / 2) * a->kv_heads;
             int c;
             const long long turns = cluster_of(items, &c);
             float us;
@@ -163,7 +165,9 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
             float rows_us;
             if (tc && a->head_dim == 32 && (best_parts(2, &rows_us), rows_us < us)) { many = 2; us = rows_us; }
             // (two more tiles an item of the stream, as its kernel reckons)
-            const float few = turns <= 8 ? 4.5f + (float)turns * one.tile_us : 6.f + (float)((items * (one_keys + 2) + one.slots - 1) / one.slots) * one.tile_us;
+            const float tiles = turns <= 8 ? (float)((items * c + one.slots - 1) / one.slots) * (float)longest / (float)(one.keys * c)
+                                           : (float)((items * (one_keys + 2) + one.slots - 1) / one.slots);
+            const float few = (turns <= 8 ? 4.5f : 6.f) + tiles * one.tile_us;
             if (us < few) backend = many;
         }
     }
