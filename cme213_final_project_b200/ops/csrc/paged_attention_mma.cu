@@ -616,7 +616,7 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 //            finished there, the others' parts are left in scratch (at most two a CTA) and joined by a small kernel.
 //   cluster  a CTA has one part of one item, and up to eight CTAs join theirs through shared memory: one launch, for few items.
 // Single tokens, bf16: one sequence of 701, 12 heads of 64 5.2 us (a launch, three dependent lookups, a tile, the join); 64 of up to 1024, 16
-// heads of 64 32 us, 4.2 TB/s of 135 MB; 16 of 2000 to 32768, 32 heads of 128 on 8 163 us, 6.2 TB/s.  fp32: 32 of up to 2048, 4 heads of 128
+// heads of 64 31 us, 4.3 TB/s of 135 MB; 16 of 2000 to 32768, 32 heads of 128 on 8 163 us, 6.2 TB/s.  fp32: 32 of up to 2048, 4 heads of 128
 // 34 us, 3.9 TB/s.
 constexpr int REC_INTS = 8;                // of an item that ends in a CTA other than it began in: first CTA or -1, rows, token0, first, head
 
@@ -934,7 +934,8 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     if (threadIdx.x == 0 && *ld.abort_flag && p.status) atomicExch(p.status, CME_ERR_TIMEOUT);
 }
 
-// Joins the parts of the items that several CTAs of the stream had: block (c, y) those of the item that ends in CTA c, rows y, y + 4, ...
+// Joins the parts of the items that several CTAs of the stream had: block (c, y) those of the item that ends in CTA c, rows 4 y to 4 y + 3, or,
+// of items in many parts, rows y, y + 4, ...
 template <typename T, int D>
 __global__ void __launch_bounds__(128) paged_stream_join_kernel(const MmaParams p) {
     constexpr int COLS = D / 4, GROUPS = 128 / COLS;       // threads of a row, and how many of its parts are added at a time
@@ -951,8 +952,40 @@ __global__ void __launch_bounds__(128) paged_stream_join_kernel(const MmaParams 
     t.token0 = rec[2];
     t.first = rec[3];
     const int head = rec[4], group = threadIdx.x / COLS, c = threadIdx.x % COLS * 4;
+    auto slot_of = [&](int k, int row) { return (k * 2ll + (k != c1)) * 16 + row; };
+    constexpr int FEW = 8;
+    if (c1 - c0 < FEW) {
+        // A warp a row, all loads at once (64 sequences of up to 1024, 16 heads of 64: 31.3 us, in the way of many parts 32.2)
+        const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+        if (row >= t.rows) return;
+        float2 ml[FEW];
+        float4 x[FEW];
+#pragma unroll
+        for (int k = 0; k < FEW; ++k) {
+            ml[k] = make_float2(-INFINITY, 0.f);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c0 + k <= c1) {
+                ml[k] = p.part_ml[slot_of(c0 + k, row)];
+                if (lane < COLS) x[k] = *reinterpret_cast<const float4*>(p.part_o + slot_of(c0 + k, row) * D + lane * 4);
+            }
+        }
+        float mm = -INFINITY, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < FEW; ++k) mm = fmaxf(mm, ml[k].x);
+#pragma unroll
+        for (int k = 0; k < FEW; ++k) {
+            const float f = part_factor(ml[k].x, mm);
+            l = fmaf(f, ml[k].y, l);
+            add4(v, f, x[k]);
+        }
+        const long long at = row_at(p, t, head, row);
+        if (lane < COLS) store4(static_cast<T*>(p.a.o) + at * D + lane * 4, v, inverse(l));
+        if (lane == 0) p.a.lse[at] = log_sum(mm, l);
+        return;
+    }
     for (int row = blockIdx.y; row < t.rows; row += 4) {
-        auto slot = [&](int k) { return (k * 2ll + (k != c1)) * 16 + row; };
+        auto slot = [&](int k) { return slot_of(k, row); };
         float mm = -INFINITY;
         for (int k = c0 + threadIdx.x; k <= c1; k += 128) mm = fmaxf(mm, p.part_ml[slot(k)].x);
         mm = block_max(mm, scratch);
