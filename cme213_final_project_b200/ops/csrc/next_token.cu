@@ -25,6 +25,7 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_CLUSTER = 8;
 constexpr size_t MAX_SMEM = 160 * 1024;    // of marks and records
+constexpr size_t MAX_RING = 65 * 1024;     // of the loads under way
 
 // Running softmax statistics and the pick of some tokens.
 struct Pick {
@@ -490,6 +491,7 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
         // 16-byte boundaries as rows of noise and of the processed logits
         vector = slice >= 1024 && aligned;
         threads = slice <= 1024 ? 128 : 256;
+        static_assert(STAGES * 256 * 16 * 4 + 16 <= MAX_RING, "ring");
         if (vector) smem = (smem + 15) / 16 * 16 + (size_t)STAGES * threads * 16 * ((p->dtype == CME_F32 ? 2 : 1) + (p->noise ? 2 : 0));
     };
     // As many CTAs as run at a time, with no fewer than 2048 tokens each: a second turn costs as much as a row's length (us, one CTA / two for
@@ -504,7 +506,13 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
     CME_REQUIRE((long long)p->rows * cluster < (1ll << 31), CME_ERR_LIMIT, "next token: too many rows");
     auto* kernel = p->dtype == CME_F32 ? (vector ? next_token_kernel<float, true> : next_token_kernel<float, false>)
                                        : (vector ? next_token_kernel<__nv_bfloat16, true> : next_token_kernel<__nv_bfloat16, false>);
-    if (smem > 48 * 1024) CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static bool attr[2][2][CME_MAX_DEVICES] = {};         // function attributes are per device
+    int dev = 0;
+    CME_CUDA(cudaGetDevice(&dev));
+    if (bool& set = attr[p->dtype == CME_F32][vector][dev % CME_MAX_DEVICES]; !set) {
+        CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MAX_SMEM + MAX_RING)));
+        set = true;
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(p->rows * cluster));
     cfg.blockDim = dim3(threads);
