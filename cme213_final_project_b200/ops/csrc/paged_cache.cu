@@ -96,7 +96,7 @@ constexpr int MAX_SPLITS = 128;
 // the keys in L2 and all SMs busy), and what its parts cost that are joined through scratch (written and read once more, at 3 TB/s,
 // and a launch).  The host does not know the sequences: they are taken to be as long as the longest, and to share the new tokens evenly.
 // Measured / estimated: 12 heads of 64, 128 tokens over 4096 in 4 sequences: tc in 1, 4, 8 parts 72 / 79, 32 / 32, 31 / 27, stream 62 / 72;
-// 4 heads of 128 in fp32, 256 over 512 in 8: rows 56 / 53, stream 97 / 107; 12 heads of 64 in fp32, 256 over 512 in 8: rows 72 / 95, stream 109 / 113.
+// 4 heads of 128 in fp32, 256 over 512 in 8: rows 56 / 53, stream 97 / 107; 12 heads of 64 in fp32, 256 over 512 in 8: rows 72 / 98, stream 109 / 113.
 struct Form {
     int keys;                // of a tile
     int slots;               // CTAs that run at a time
@@ -111,9 +111,10 @@ Form form_of(const CmePaged* a, int backend, int sms) {
     return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.0f : d == 64 ? 3.0f : 4.5f) : d == 128 ? 2.6f : 1.8f};
 }
 float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
-    const long long ctas = tiles * a->kv_heads * parts, turns = (ctas + f.slots - 1) / f.slots;
+    const long long ctas = tiles * a->kv_heads * parts;
+    const double turns = ctas <= f.slots ? 1.0 : (double)ctas / f.slots + 0.5;         // (the shortest last: half a turn at the end)
     const double joined = parts > 1 ? 4.0 + (double)a->rows * a->heads * parts * (a->head_dim + 2) * 8 / 3e6 : 0.0;
-    return (float)(5.0 + (double)turns * (cme_cdiv(key_tiles, parts) + 2 * (turns > 1)) * f.tile_us + joined);
+    return (float)(5.0 + turns * (cme_cdiv(key_tiles, parts) + 2 * (turns > 1)) * f.tile_us + joined);
 }
 
 // backend: 0 by the rule, 1 up to 16 rows a tile, 2 rows, 3 tc.  splits: 0 by the rule; up to 16 rows: a cluster of so many CTAs (1, 2, 4
