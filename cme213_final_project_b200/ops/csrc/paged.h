@@ -49,6 +49,9 @@ inline PagedDiv paged_div(int d) {
     return p;
 }
 
+// Whether paged_find_tile_by_keys takes the call.
+inline bool paged_by_keys(const CmePaged* a, int group) { return a->seqs <= 32 && (long long)a->rows * group < (1ll << 30); }
+
 #ifdef __CUDACC__
 
 // What a CTA works on: rows [first, first + rows) of a sequence's tokens x group, for one key head.
@@ -95,9 +98,10 @@ __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile
     return t;
 }
 
-// As paged_find_tile, counting the tiles by what they see: most key tiles of `keys` keys first, equal ones by sequence.  Up to 32 sequences.
+// As paged_find_tile, counting the tiles by what they see: most key tiles of `keys` keys first, equal ones by sequence.  Up to 32 sequences
+// and 2^30 rows.
 __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, int tile, int group, int row_tile, int keys) {
-    const int b = threadIdx.x & 31, each = row_tile / group;           // (whole tokens)
+    const int b = threadIdx.x & 31;
     PagedTile t{0, 0, 0, 0, 0, 0};
     int lo = 0, hi = 0, length = 0;
     if (b < a.seqs) {
@@ -107,14 +111,14 @@ __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, 
     }
     lo = max(0, min(lo, a.rows));
     hi = max(lo, min(hi, a.rows));
-    const int n = hi - lo, own = (n + each - 1) / each;
+    const int n = hi - lo, own = (n * group + row_tile - 1) / row_tile;
     // tiles of the sequence that see x key tiles at least; they are its last ones
     auto count = [&](int x) {
         const long long need = (long long)(x - 1) * keys + 1;          // keys
         if (x <= 0) return own;
         if (length < need) return 0;
         const int more = (int)max(1ll, need - length + n);             // of the new tokens (<= n)
-        return own - (more + each - 1) / each + 1;
+        return own - ((more - 1) * group + row_tile) / row_tile + 1;   // without those that end before the first row of token more - 1
     };
     if (tile >= (int)__reduce_add_sync(0xffffffffu, own)) return t;
     int x = 0, most = __reduce_max_sync(0xffffffffu, n > 0 ? length / keys + 1 : 0);      // the tile sees between x and `most` key tiles

@@ -1093,7 +1093,7 @@ template <typename T, int D> int launch_any(const CmePaged* a, const PagedPlan& 
         int sms;
         if (const int rc = cme_num_sms(&sms)) return rc;
         const unsigned ctas = (unsigned)(plan.tiles * plan.splits) * a->kv_heads;
-        p.by_keys = a->seqs <= 32 && ctas > (unsigned)sms * Cfg<T, D, true>::CTAS;
+        p.by_keys = paged_by_keys(a, p.group) && ctas > (unsigned)sms * Cfg<T, D, true>::CTAS;
         p.heads = paged_div(a->kv_heads);
         p.parts = paged_div(plan.splits);
         return launch<T, D, true, paged_attn_rows_kernel<T, D>>(dim3(ctas), a, 1, p, st);

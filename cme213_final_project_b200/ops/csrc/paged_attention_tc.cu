@@ -468,7 +468,7 @@ template <int D, bool FEW> int launch(const CmePaged* a, const PagedPlan& plan, 
     if ((rc = paged_make_map(&mk, a, a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, 64, p.box, CU_TENSOR_MAP_SWIZZLE_128B))) return rc;
     const long long each = std::max(1ll, (ctas + sms - 1) / sms);
-    p.by_keys = a->seqs <= 32 && ctas > (long long)sms * C::CTAS;
+    p.by_keys = paged_by_keys(a, p.group) && ctas > (long long)sms * C::CTAS;
     const int smem = each < C::CTAS ? spread((int)each) : C::SMEM;
     CME_CUDA(cme_launch_dependent(kernel, dim3((unsigned)(plan.tiles * plan.splits) * p.heads.d, a->kv_heads / p.heads.d), dim3(C::THREADS), (size_t)smem, st,
                                   mq, mk, mv, p));

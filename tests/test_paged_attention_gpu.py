@@ -294,6 +294,17 @@ def test_heads_of_32_on_the_tensor_core_kernel(heads, kv_heads, page, drop):
         assert all(torch.equal(x, y) for x, y in zip(first, ops.paged_attention(*many, backend="tc", splits=1)))
 
 
+@pytest.mark.parametrize("D,dtype", [(32, BF16), (64, F32), (128, F32)])
+@pytest.mark.parametrize("heads,kv_heads", [(15, 3), (3, 1), (14, 2), (130, 1), (65, 1)])
+def test_tiles_in_the_order_of_their_keys(heads, kv_heads, D, dtype):
+    """More tiles of rows than run at a time, whose ends lie inside a token's heads, or which are a part of one."""
+    pairs = [(n * 16 * kv_heads // heads + 1, l) for n, l in ((130, 700), (0, 50), (70, 500), (170, 640), (1, 3), (100, 110), (160, 900), (7, 0))] * 4
+    pairs = [(min(n, l) if l else n, l) for n, l in pairs]
+    args = make(pairs, heads, kv_heads, D, 16, dtype, seed=heads)
+    for splits in (1, 2):
+        check(args, ops.paged_attention(*args, backend="rows", splits=splits))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("D", [64, 128])
 def test_rows_whose_maximum_rises_with_every_tile(D, dtype):
