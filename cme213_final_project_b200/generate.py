@@ -75,6 +75,14 @@ class PagedCache:
         self.lengths[b] = 0
         self.table[b] = -1
 
+    def clear(self) -> None:
+        """All sequences are over."""
+        for b in reversed(range(len(self.owned))):
+            self.free += reversed(self.owned[b])
+            self.owned[b] = []
+            self.lengths[b] = 0
+        self.table.fill_(-1)
+
 
 @dataclass
 class Sampling:
@@ -144,9 +152,11 @@ class Generator:
         return gemm(x, P["tok_embed"], b_trans=True) if cfg.tied_embeddings else gemm(x, P["Wout"])
 
     def prefill(self, prompts: Sequence[Sequence[int]], chunk: int = 512) -> torch.Tensor:
-        """Take the prompts into the cache, up to ``chunk`` tokens of each at a time; logits after each prompt's last token."""
+        """Start new sequences: take the prompts into the cache, up to ``chunk`` tokens of each at a time; logits after each prompt's last
+        token.  What the cache held, of an earlier call or of one that failed, is given back first."""
         if len(prompts) != self.seqs or any(len(p) == 0 for p in prompts):
             raise ValueError(f"{self.seqs} prompts with a token at least are needed")
+        self.cache.clear()
         device = self.cache.table.device
         out = None
         done = [0] * self.seqs
@@ -170,8 +180,8 @@ class Generator:
     # -- a run ------------------------------------------------------------------------------------
     def generate(self, prompts: Sequence[Sequence[int]], max_new: int, sampling: Optional[Sampling] = None, seed: int = 0,
                  chunk: int = 512, cuda_graph: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
-        """``max_new`` tokens after each prompt: ``(tokens [seqs, max_new], log-probabilities)`` on the device.  -1 where the
-        sampling's mask left no token (and from there on)."""
+        """``max_new`` tokens after each prompt, as new sequences: ``(tokens [seqs, max_new], log-probabilities)`` on the device.  -1
+        where the sampling's mask left no token (and from there on)."""
         from . import ops
         s, cfg, device = sampling or Sampling(), self.cfg, self.cache.table.device
         if max(len(p) for p in prompts) + max_new > cfg.seq_len + 1:

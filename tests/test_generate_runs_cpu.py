@@ -1,0 +1,121 @@
+"""Runs of a generator on the CPU, with the operators replaced by plain torch: what a call does may not depend on the calls before it."""
+import pytest
+import torch
+
+from cme213_final_project_b200 import ops
+from cme213_final_project_b200.arena import ArenaLayout, init_flat
+from cme213_final_project_b200.config import ModelConfig
+from cme213_final_project_b200.generate import CacheFull, Generator, Sampling
+
+PROMPTS = [[1, 2, 3, 4, 5], list(range(20)), [7], [(i * 7) % 33 for i in range(31)]]
+
+
+def plain_layernorm(x, gamma, beta, eps):
+    return (torch.nn.functional.layer_norm(x, x.shape[-1:], gamma, beta, eps),)
+
+
+def plain_gemm(a, b, *, b_trans=False, bias=None, act=None, residual=None, allow_tf32=True):
+    y = a @ (b.T if b_trans else b)
+    y = y if bias is None else y + bias
+    y = torch.nn.functional.gelu(y) if act else y
+    return y if residual is None else y + residual
+
+
+def places(n, offsets, lengths):
+    """(row, sequence, position) of all new tokens."""
+    offs = offsets.tolist()
+    assert offs[0] == 0 and offs[-1] == n
+    for b, length in enumerate(lengths.tolist()):
+        for row in range(offs[b], offs[b + 1]):
+            yield row, b, length - offs[b + 1] + row
+
+
+def plain_append(k, v, cache_k, cache_v, pages, offsets, lengths):
+    P = cache_k.shape[2]
+    for row, b, pos in places(k.shape[0], offsets, lengths):
+        at = pages[b, pos // P]
+        assert at >= 0
+        cache_k[at, :, pos % P], cache_v[at, :, pos % P] = k[row], v[row]
+
+
+def plain_attention(q, cache_k, cache_v, pages, offsets, lengths):
+    P, out = cache_k.shape[2], torch.empty_like(q)
+    for row, b, pos in places(q.shape[0], offsets, lengths):
+        at = torch.arange(pos + 1)
+        page = pages[b].long()[at // P]
+        k, v = cache_k[page, :, at % P], cache_v[page, :, at % P]          # [keys, heads, head_dim]
+        p = torch.softmax(torch.einsum("hd,thd->ht", q[row], k) * q.shape[-1] ** -0.5, 1)
+        out[row] = torch.einsum("ht,thd->hd", p, v)
+    return out, None
+
+
+def plain_next_token(logits, *, history, lengths, prompts, temperature, repetition, presence, frequency, noise=None, allowed=None,
+                     bias_ids=None, bias_values=None):
+    x = logits.clone()
+    for r in range(x.shape[0]):
+        told = history[r, :lengths[r]].tolist()
+        assert all(0 <= t < x.shape[1] for t in told)
+        for t in set(told):
+            x[r, t] = x[r, t] / repetition[r] if x[r, t] > 0 else x[r, t] * repetition[r]
+        for t in told[prompts[r]:]:
+            x[r, t] -= frequency[r]
+        for t in set(told[prompts[r]:]):
+            x[r, t] -= presence[r]
+        if temperature[r] > 0:
+            x[r] /= temperature[r]
+    token = (x if noise is None else x + noise).argmax(1)
+    return token.to(torch.int32), torch.log_softmax(x, 1).gather(1, token[:, None])[:, 0], None
+
+
+@pytest.fixture(autouse=True)
+def on_the_cpu(monkeypatch):
+    for name, f in (("add", torch.add), ("layernorm_fwd", plain_layernorm), ("gemm", plain_gemm), ("cache_append", plain_append),
+                    ("paged_attention", plain_attention), ("next_token", plain_next_token)):
+        monkeypatch.setattr(ops, name, f)
+
+
+def generator(seqs=4, **kw):
+    cfg = ModelConfig(mode="gpt", vocab_size=33, seq_len=48, hidden=64, heads=2, ff=64, layers=2, batch_size=1, activation="gelu",
+                      causal=True, head_layout="split", tied_embeddings=True, final_layernorm=True, init="normal")
+    layout = ArenaLayout(cfg)
+    return Generator(cfg, layout, init_flat(layout, 3) * 6.0, seqs, page=8, **kw)
+
+
+def run(g, prompts, new=8, **kw):
+    return g.generate(prompts, new, cuda_graph=False, **kw)
+
+
+def same(a, b):
+    return torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_prompts_are_taken_in_anew_each_time():
+    g = generator()
+    first = g.prefill(PROMPTS)
+    assert torch.equal(g.prefill(PROMPTS), first) and g.cache.lengths == [len(p) for p in PROMPTS]
+    assert torch.equal(g.prefill(PROMPTS[::-1], 7), generator().prefill(PROMPTS[::-1], 7))
+    assert torch.equal(g.prefill(PROMPTS), first)
+
+
+@pytest.mark.parametrize("sampling", [None, Sampling(0.0, 1.3, 0.2, 0.4), Sampling(1.0)])
+def test_a_run_does_not_depend_on_the_runs_before_it(sampling):
+    other = [[9], [8, 8], list(range(30)), [1]]
+    want = [run(generator(), p, sampling=sampling) for p in (PROMPTS, other)]
+    assert want[0][0].unique().numel() > 3                 # (a model that says one thing only would show nothing)
+    g = generator()
+    for p, w in ((PROMPTS, want[0]), (other, want[1]), (other, want[1]), (PROMPTS, want[0])):
+        assert same(run(g, p, sampling=sampling), w)
+
+
+def test_as_many_runs_as_one_likes():
+    g = generator()
+    for _ in range(6):                                     # (a cache that kept them would be full after the second)
+        run(g, PROMPTS, 17)
+    assert sorted([p for o in g.cache.owned for p in o] + g.cache.free) == list(range(g.cache.k.shape[1]))
+
+
+def test_a_run_after_one_that_failed():
+    g = generator(pages=9)
+    with pytest.raises(CacheFull):
+        run(g, PROMPTS, 16)
+    assert same(run(g, PROMPTS, 2), run(generator(), PROMPTS, 2))
