@@ -156,6 +156,8 @@ class Generator:
         token.  What the cache held, of an earlier call or of one that failed, is given back first."""
         if len(prompts) != self.seqs or any(len(p) == 0 for p in prompts):
             raise ValueError(f"{self.seqs} prompts with a token at least are needed")
+        if chunk < 1:
+            raise ValueError(f"a chunk of {chunk} tokens: one at least is needed")
         self.cache.clear()
         device = self.cache.table.device
         out = None

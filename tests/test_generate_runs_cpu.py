@@ -119,3 +119,14 @@ def test_a_run_after_one_that_failed():
     with pytest.raises(CacheFull):
         run(g, PROMPTS, 16)
     assert same(run(g, PROMPTS, 2), run(generator(), PROMPTS, 2))
+
+
+@pytest.mark.parametrize("chunk", [0, -1, -512])
+def test_a_chunk_has_a_token_at_least(chunk):
+    g = generator()
+    first = run(g, PROMPTS, 2)
+    for call in (lambda: g.prefill(PROMPTS, chunk), lambda: run(g, PROMPTS, 2, chunk=chunk)):
+        with pytest.raises(ValueError, match="chunk"):
+            call()
+        assert g.cache.lengths == [len(p) + 1 for p in PROMPTS]            # refused before anything has changed
+    assert same(run(g, PROMPTS, 2, chunk=1), run(generator(), PROMPTS, 2, chunk=1)) and first[0].shape == (4, 2)
