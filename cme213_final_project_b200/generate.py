@@ -186,6 +186,8 @@ class Generator:
         where the sampling's mask left no token (and from there on)."""
         from . import ops
         s, cfg, device = sampling or Sampling(), self.cfg, self.cache.table.device
+        if max_new < 1:
+            raise ValueError(f"max_new of {max_new}: one token at least is needed")
         if max(len(p) for p in prompts) + max_new > cfg.seq_len + 1:
             raise ValueError(f"prompts of up to {max(map(len, prompts))} tokens and {max_new} more: the model's positions end at {cfg.seq_len}")
         logits = self.prefill(prompts, chunk)

@@ -130,3 +130,12 @@ def test_a_chunk_has_a_token_at_least(chunk):
             call()
         assert g.cache.lengths == [len(p) + 1 for p in PROMPTS]            # refused before anything has changed
     assert same(run(g, PROMPTS, 2, chunk=1), run(generator(), PROMPTS, 2, chunk=1)) and first[0].shape == (4, 2)
+
+
+@pytest.mark.parametrize("new", [0, -1, -40])
+def test_a_run_has_a_token_at_least(new):
+    g = generator()
+    run(g, PROMPTS, 2)
+    with pytest.raises(ValueError, match="max_new"):
+        run(g, PROMPTS[::-1], new)
+    assert g.cache.lengths == [len(p) + 1 for p in PROMPTS]                # refused before anything has changed
