@@ -75,6 +75,15 @@ class PagedCache:
         self.lengths[b] = 0
         self.table[b] = -1
 
+    def fits(self, lengths: Sequence[int]) -> None:
+        """Raises what :meth:`grow` would if sequences of these lengths were all that is there."""
+        for b, n in enumerate(lengths):
+            if n > self.max_len:
+                raise ValueError(f"sequence {b}: {n} tokens, {self.max_len} at the most")
+        need, pages = sum(-(-n // self.page) for n in lengths), self.k.shape[1]
+        if need > pages:
+            raise CacheFull(f"{need} pages are needed, the cache has {pages}")
+
     def clear(self) -> None:
         """All sequences are over."""
         for b in reversed(range(len(self.owned))):
@@ -158,6 +167,7 @@ class Generator:
             raise ValueError(f"{self.seqs} prompts with a token at least are needed")
         if chunk < 1:
             raise ValueError(f"a chunk of {chunk} tokens: one at least is needed")
+        self.cache.fits([len(p) for p in prompts])
         self.cache.clear()
         device = self.cache.table.device
         out = None
@@ -190,9 +200,10 @@ class Generator:
             raise ValueError(f"max_new of {max_new}: one token at least is needed")
         if max(len(p) for p in prompts) + max_new > cfg.seq_len + 1:
             raise ValueError(f"prompts of up to {max(map(len, prompts))} tokens and {max_new} more: the model's positions end at {cfg.seq_len}")
+        self.cache.fits([len(p) + max_new - 1 for p in prompts])          # (the last token's key is not needed)
         logits = self.prefill(prompts, chunk)
         start = list(self.cache.lengths)
-        self.cache.grow([max_new - 1] * self.seqs)                        # (the last token's key is not needed)
+        self.cache.grow([max_new - 1] * self.seqs)
         i32 = lambda v: torch.tensor(v, dtype=torch.int32).to(device)
         given = i32(start)
         history = torch.zeros(self.seqs, cfg.seq_len + 1, dtype=torch.int32, device=device)

@@ -139,3 +139,19 @@ def test_a_run_has_a_token_at_least(new):
     with pytest.raises(ValueError, match="max_new"):
         run(g, PROMPTS[::-1], new)
     assert g.cache.lengths == [len(p) + 1 for p in PROMPTS]                # refused before anything has changed
+
+
+def test_what_has_no_room_is_refused_before_anything_changes():
+    g = generator(pages=12)
+    first = run(g, PROMPTS, 2)
+    held = [list(o) for o in g.cache.owned]
+    with pytest.raises(CacheFull):
+        run(g, PROMPTS, 16)                                # room for the prompts, not for what follows
+    with pytest.raises(CacheFull):
+        g.prefill([list(range(30))] * 4, 7)                # for the first chunks only
+    with pytest.raises(ValueError):
+        g.prefill([[1], [2], [3], [4] * 49], 7)            # beyond the model's positions
+    assert [list(o) for o in g.cache.owned] == held and g.cache.lengths == [len(p) + 1 for p in PROMPTS]
+    assert same(run(g, PROMPTS, 2), first)
+    logits = g.prefill([[k] * (8 * k) for k in (1, 2, 4, 5)])         # every page
+    assert logits.shape == (4, 33) and not g.cache.free
