@@ -165,6 +165,8 @@ class Generator:
         token.  What the cache held, of an earlier call or of one that failed, is given back first."""
         if len(prompts) != self.seqs or any(len(p) == 0 for p in prompts):
             raise ValueError(f"{self.seqs} prompts with a token at least are needed")
+        if any(not 0 <= t < self.cfg.vocab_size for p in prompts for t in p):
+            raise ValueError(f"prompts have to have tokens of the vocabulary, 0 to {self.cfg.vocab_size - 1}")
         if chunk < 1:
             raise ValueError(f"a chunk of {chunk} tokens: one at least is needed")
         self.cache.fits([len(p) for p in prompts])

@@ -155,3 +155,13 @@ def test_what_has_no_room_is_refused_before_anything_changes():
     assert same(run(g, PROMPTS, 2), first)
     logits = g.prefill([[k] * (8 * k) for k in (1, 2, 4, 5)])         # every page
     assert logits.shape == (4, 33) and not g.cache.free
+
+
+@pytest.mark.parametrize("token", [-1, 33, 10 ** 6])
+def test_prompts_have_tokens_of_the_vocabulary(token):
+    g = generator()
+    run(g, PROMPTS, 2)
+    for call in (g.prefill, lambda p: run(g, p, 2)):
+        with pytest.raises(ValueError, match="vocabulary"):
+            call([[1], [2, 3, token], [4], [5]])
+    assert g.cache.lengths == [len(p) + 1 for p in PROMPTS]                # refused before anything has changed
