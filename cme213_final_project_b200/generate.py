@@ -111,6 +111,8 @@ class Sampling:
             kw["bias_ids"] = torch.tensor([list(self.bias)] * rows, dtype=torch.int32, device=device)
             kw["bias_values"] = torch.tensor([list(self.bias.values())] * rows, dtype=torch.float32, device=device)
         if self.allowed is not None:
+            if any(not 0 <= t < vocab for t in self.allowed):
+                raise ValueError(f"allowed tokens have to be of the vocabulary, 0 to {vocab - 1}")
             bits = torch.zeros(-(-vocab // 32) * 32, dtype=torch.int64)
             bits[torch.as_tensor(list(self.allowed), dtype=torch.int64)] = 1
             words = (bits.view(-1, 32) << torch.arange(32)).sum(1)
@@ -202,6 +204,7 @@ class Generator:
             raise ValueError(f"max_new of {max_new}: one token at least is needed")
         if max(len(p) for p in prompts) + max_new > cfg.seq_len + 1:
             raise ValueError(f"prompts of up to {max(map(len, prompts))} tokens and {max_new} more: the model's positions end at {cfg.seq_len}")
+        kw = s.tensors(self.seqs, cfg.vocab_size, device)
         self.cache.fits([len(p) + max_new - 1 for p in prompts])          # (the last token's key is not needed)
         logits = self.prefill(prompts, chunk)
         start = list(self.cache.lengths)
@@ -214,7 +217,6 @@ class Generator:
         told = given.clone()                                              # tokens of a sequence so far, on the device
         rows, noise = torch.arange(self.seqs, device=device), None
         offsets = i32(list(range(self.seqs + 1)))
-        kw = s.tensors(self.seqs, cfg.vocab_size, device)
         uniform = torch.Generator(device=device).manual_seed(seed)
         if s.temperature > 0:
             noise = torch.empty(self.seqs, cfg.vocab_size, device=device)

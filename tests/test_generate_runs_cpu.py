@@ -165,3 +165,9 @@ def test_prompts_have_tokens_of_the_vocabulary(token):
         with pytest.raises(ValueError, match="vocabulary"):
             call([[1], [2, 3, token], [4], [5]])
     assert g.cache.lengths == [len(p) + 1 for p in PROMPTS]                # refused before anything has changed
+
+
+@pytest.mark.parametrize("token", [-1, 33, 63, 64, 10 ** 6])
+def test_allowed_tokens_are_of_the_vocabulary(token):
+    with pytest.raises(ValueError, match="vocabulary"):
+        Sampling(allowed=[3, token]).tensors(2, 33, "cpu")
