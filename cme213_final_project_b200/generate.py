@@ -276,7 +276,7 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--repetition", type=float, default=1.0)
     p.add_argument("--presence", type=float, default=0.0)
     p.add_argument("--frequency", type=float, default=0.0)
-    p.add_argument("--allow", help="only these characters may come (with --data)")
+    p.add_argument("--allow", help="only these characters of the corpus may come (with --data)")
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--chunk", type=int, default=512, help="tokens of a prompt that are taken in at a time")
     p.add_argument("--page", type=int, default=16, help="slots of a cache page")
@@ -304,9 +304,15 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
         prompts = [tok.encode(t).tolist() if tok else [int(i) for i in t.split(",")] for t in texts]
         if any(not 0 <= t < cfg.vocab_size for p in prompts for t in p) or not all(prompts):
             raise ValueError("prompts have to have tokens of the model's vocabulary")
+        allowed = None
+        if a.allow is not None:
+            if tok is None:
+                raise ValueError("--allow names characters: it needs --data")
+            allowed = tok.encode(a.allow).tolist()
+            if not allowed or len(allowed) < len(a.allow.encode("utf-8")):
+                raise ValueError(f"--allow has to name characters of {a.data}")
         if not torch.cuda.is_available():
             raise ValueError("generation needs a GPU")
-        allowed = tok.encode(a.allow).tolist() if a.allow and tok else None
         dtype = torch.bfloat16 if a.compute_dtype == "bf16" else torch.float32
         # (on the device tensors start at multiples of 64 elements, as the engine lays them)
         aligned = ArenaLayout(cfg, align=64)

@@ -171,3 +171,19 @@ def test_prompts_have_tokens_of_the_vocabulary(token):
 def test_allowed_tokens_are_of_the_vocabulary(token):
     with pytest.raises(ValueError, match="vocabulary"):
         Sampling(allowed=[3, token]).tensors(2, 33, "cpu")
+
+
+@pytest.mark.parametrize("allow,data", [("ab", False), ("abz", True), ("z", True), ("aé", True), ("", True)])
+def test_the_command_takes_only_characters_that_can_come(allow, data, tmp_path, capsys):
+    from cme213_final_project_b200.checkpoint import save_checkpoint
+    from cme213_final_project_b200.generate import main
+    text, ck = tmp_path / "text.txt", tmp_path / "model.ck"
+    text.write_text("abc abc")
+    cfg = ModelConfig(mode="gpt", vocab_size=4, seq_len=8, hidden=32, heads=1, ff=32, layers=1, batch_size=1, activation="gelu", causal=True,
+                      head_layout="split", tied_embeddings=True, final_layernorm=True, init="normal")
+    layout = ArenaLayout(cfg)
+    flat = init_flat(layout, 1)
+    save_checkpoint(str(ck), layout, flat, flat * 0, flat * 0, 0)
+    args = ["--checkpoint", str(ck), "--allow", allow, "--prompt", "ab" if data else "0,1", "--max-new", "2"]
+    assert main(args + (["--data", str(text)] if data else [])) == 1
+    assert "--allow" in capsys.readouterr().err
