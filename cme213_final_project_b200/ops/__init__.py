@@ -433,8 +433,10 @@ def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Opti
     ``[tokens, heads]``.  Keys on pages that are not there do not take part; a row without any key gets zeros and ``-inf``.
     What the cache holds beyond a sequence's length may be anything, within it the values have to be finite.
 
-    ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_len``: no length is larger (default: what the table
-    holds); the number of parts that the keys are divided into goes by it.  ``backend``: ``auto`` | ``single`` (few rows) | ``rows`` |
+    ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_len``: keys from this position on do not take part (default: what
+    the table holds); the number of parts that the keys are divided into goes by it.  Where a length passes it, new tokens keep their
+    positions, as in :func:`cache_append`, and see the keys below it up to their own; a sequence none of whose new tokens has a
+    position below it counts as that long.  ``backend``: ``auto`` | ``single`` (few rows) | ``rows`` |
     ``tc`` (tcgen05: bf16); ``splits``: parts of the keys, 0 = by the rule, negative = joined
     through scratch memory in any case."""
     return _native().paged_attention(q, cache_k, cache_v, pages, offsets, lengths, scale, max_len, _PAGED_BACKENDS[backend], splits)

@@ -58,13 +58,23 @@ inline bool paged_by_keys(const CmePaged* a, int group) { return a->seqs <= 32 &
 struct PagedTile {
     int seq, first, rows;        // rows == 0: the tile does not exist
     int token0, n, length;       // the sequence's first row of q, its new tokens, its tokens
+    int held;                    // keys of them that the table and max_len hold
 };
+
+// length and held of a sequence with n new tokens.  Where a length passes what is held, the new tokens keep their positions (cache_append
+// writes those that have a place): each sees all keys that are held up to its own.  Where none of them has a place, the length counts as what is held.
+__device__ __forceinline__ void paged_length(const CmePaged& a, int len, int n, int& length, int& held) {
+    held = (int)min((long long)a.width * a.page, (long long)a.max_len);
+    length = max(0, len);
+    if (length - n >= held) length = held;
+    held = min(held, length);
+}
 
 // Finds row tile `tile`, counting ceil(new tokens x group / row_tile) tiles per sequence.  Whole warps call it; every warp gets
 // the answer.  offsets and lengths that make no sense cannot lead outside of the buffers: they are cut to them.
 __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile, int group, int row_tile) {
     const int lane = threadIdx.x & 31;
-    PagedTile t{0, 0, 0, 0, 0, 0};
+    PagedTile t{};
     int base = 0;
     for (int b0 = 0; b0 < a.seqs; b0 += 32) {
         const int b = b0 + lane;
@@ -87,8 +97,7 @@ __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile
             t.seq = b0 + src;
             t.token0 = __shfl_sync(0xffffffffu, lo, src);
             t.n = __shfl_sync(0xffffffffu, n, src);
-            const long long most = (long long)a.width * a.page;
-            t.length = (int)min((long long)max(0, min(__shfl_sync(0xffffffffu, len, src), a.max_len)), most);
+            paged_length(a, __shfl_sync(0xffffffffu, len, src), t.n, t.length, t.held);
             t.first = first;
             t.rows = (int)min((long long)row_tile, (long long)t.n * group - first);
             return t;
@@ -102,26 +111,28 @@ __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile
 // and 2^30 rows.
 __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, int tile, int group, int row_tile, int keys) {
     const int b = threadIdx.x & 31;
-    PagedTile t{0, 0, 0, 0, 0, 0};
-    int lo = 0, hi = 0, length = 0;
+    PagedTile t{};
+    int lo = 0, hi = 0, len = 0, length, held;
     if (b < a.seqs) {
         lo = a.offsets[b];
         hi = a.offsets[b + 1];
-        length = (int)min((long long)max(0, min(a.lengths[b], a.max_len)), (long long)a.width * a.page);
+        len = a.lengths[b];
     }
     lo = max(0, min(lo, a.rows));
     hi = max(lo, min(hi, a.rows));
-    const int n = hi - lo, own = (n * group + row_tile - 1) / row_tile;
+    const int n = hi - lo;
+    paged_length(a, len, n, length, held);
+    const int own = (n * group + row_tile - 1) / row_tile;
     // tiles of the sequence that see x key tiles at least; they are its last ones
     auto count = [&](int x) {
         const long long need = (long long)(x - 1) * keys + 1;          // keys
         if (x <= 0) return own;
-        if (length < need) return 0;
+        if (held < need) return 0;
         const int more = (int)max(1ll, need - length + n);             // of the new tokens (<= n)
         return own - ((more - 1) * group + row_tile) / row_tile + 1;   // without those that end before the first row of token more - 1
     };
     if (tile >= (int)__reduce_add_sync(0xffffffffu, own)) return t;
-    int x = 0, most = __reduce_max_sync(0xffffffffu, n > 0 ? length / keys + 1 : 0);      // the tile sees between x and `most` key tiles
+    int x = 0, most = __reduce_max_sync(0xffffffffu, n > 0 ? held / keys + 1 : 0);      // the tile sees between x and `most` key tiles
     while (x < most) {
         const int mid = (x + most + 1) >> 1;
         if ((int)__reduce_add_sync(0xffffffffu, count(mid)) > tile) x = mid;
@@ -141,6 +152,7 @@ __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, 
     t.token0 = __shfl_sync(0xffffffffu, lo, src);
     t.n = __shfl_sync(0xffffffffu, n, src);
     t.length = __shfl_sync(0xffffffffu, length, src);
+    t.held = __shfl_sync(0xffffffffu, held, src);
     t.rows = (int)min((long long)row_tile, (long long)t.n * group - t.first);
     return t;
 }

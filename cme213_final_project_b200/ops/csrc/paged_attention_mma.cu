@@ -521,7 +521,7 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     __syncthreads();
     if (t.rows == 0) return;
     // keys [0, limit) are seen by the last row; this CTA takes [begin, end)
-    const int limit = max(0, min(t.length, row_sees(p, t, t.rows - 1)));
+    const int limit = max(0, min(t.held, row_sees(p, t, t.rows - 1)));
     const int begin = (int)min((long long)limit, (long long)split * p.split_keys);
     const int end = (int)min((long long)limit, (long long)begin + p.split_keys);
     if (warp == C::WARPS) {
@@ -637,10 +637,10 @@ struct Walk {
         t.seq = seq = b;
         t.token0 = lo;
         t.n = hi - lo;
-        t.length = (int)min((long long)max(0, min(a.lengths[b], a.max_len)), (long long)a.width * a.page);
+        paged_length(a, a.lengths[b], t.n, t.length, t.held);
         t.first = t.rows = 0;
         tiles = (int)(((long long)t.n * p.group + 15) / 16);
-        keys = max(1, cme_cdiv_dev(t.length, C::KEYS)) + ITEM_COST;
+        keys = max(1, cme_cdiv_dev(t.held, C::KEYS)) + ITEM_COST;
     }
     // Takes share `part` of `parts` of the whole; returns how many key tiles a share has.  Whole warps.
     template <typename C> __device__ __forceinline__ int start(const MmaParams& p, int part, int parts) {
@@ -687,7 +687,7 @@ struct Walk {
             if (k1 > 0) {
                 t.first = tile * 16;
                 t.rows = (int)min(16ll, (long long)t.n * p.group - t.first);
-                const int limit = max(0, min(t.length, row_sees(p, t, t.rows - 1)));
+                const int limit = max(0, min(t.held, row_sees(p, t, t.rows - 1)));
                 part.t = t;
                 part.head = head;
                 part.begin = (int)min((long long)limit, (long long)k0 * C::KEYS);
@@ -749,7 +749,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     if constexpr (CLUSTER) {
         part.t = paged_find_tile(a, blockIdx.x / p.splits, p.group, 16);
         part.head = blockIdx.y;
-        const int limit = max(0, min(part.t.length, row_sees(p, part.t, part.t.rows - 1)));
+        const int limit = max(0, min(part.t.held, row_sees(p, part.t, part.t.rows - 1)));
         const int span = cme_cdiv_dev(cme_cdiv_dev(limit, C::KEYS), p.splits) * C::KEYS;
         part.begin = (int)min((long long)limit, (long long)(blockIdx.x % p.splits) * span);
         part.end = (int)min((long long)limit, (long long)part.begin + span);

@@ -9,7 +9,7 @@ struct CmePaged {
     int page, width, num_pages;          // slots of a page, columns of the table, pages of the cache
     int dtype;                           // CME_BF16 or CME_F32, of everything but lse
     int rows;                            // new tokens of all sequences
-    int max_len;                         // no length is larger (lengths are cut to it and to what the table holds)
+    int max_len;                         // keys from this position on do not take part, as those beyond the table
     float scale;                         // of the scores
     long long q_token, q_head;           // strides of q (attention) or of the new keys (append)
     long long v_token, v_head;           // strides of the new values (append)
