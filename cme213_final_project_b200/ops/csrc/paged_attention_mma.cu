@@ -645,11 +645,15 @@ struct Walk {
     // Takes share `part` of `parts` of the whole; returns how many key tiles a share has.  Whole warps.
     template <typename C> __device__ __forceinline__ int start(const MmaParams& p, int part, int parts) {
         const int lane = threadIdx.x & 31, each = (p.a.seqs + 31) / 32;
-        int sum = 0;
+        long long own = 0;
         for (int i = 0; i < each; ++i) {                   // a lane's sequences
             const int b = lane * each + i;
-            if (b < p.a.seqs) { load_seq<C>(p, b); sum += tiles * p.a.kv_heads * keys; }
+            if (b < p.a.seqs) { load_seq<C>(p, b); own += (long long)tiles * p.a.kv_heads * keys; }
         }
+        // Sequences that share rows, which no offsets in order make, can have more than 31 bits of tiles: none is taken then.
+        const unsigned high = __reduce_add_sync(0xffffffffu, (unsigned)min(own >> 16, 1ll << 16)), low = __reduce_add_sync(0xffffffffu, (unsigned)own & 0xffffu);
+        if (((unsigned long long)high << 16) + low > INT_MAX) return 1;
+        const int sum = (int)own;
         int upto = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -657,7 +661,8 @@ struct Walk {
             if (lane >= o) upto += v;
         }
         // (share * part passes 31 bits only where nothing is left)
-        const int all = __shfl_sync(0xffffffffu, upto, 31), share = (all + parts - 1) / parts, first = (int)min((long long)all, (long long)share * part);
+        const int all = __shfl_sync(0xffffffffu, upto, 31), share = (int)(((unsigned)all + parts - 1) / parts);
+        const int first = (int)min((long long)all, (long long)share * part);
         left = min(share, all - first);
         if (left <= 0) return share;
         const int who = __ffs(__ballot_sync(0xffffffffu, first < upto)) - 1;
