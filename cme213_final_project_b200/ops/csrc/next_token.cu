@@ -159,8 +159,9 @@ __device__ __forceinline__ void copy16(void* to, const void* from) {
 }
 
 // VECTOR: logits, processed and noise have their 16-byte boundaries at the same elements of a row.
-template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(256, 4) next_token_kernel(const CmeToken p, int cluster, int slice, int words, int records, bool biased) {
+// STEPS: a CTA takes its tokens in `steps` slices one after the other, where the marks and records of all of them would not fit.
+template <typename T, bool VECTOR, bool STEPS>
+__global__ void __launch_bounds__(256, 4) next_token_kernel(const CmeToken p, int cluster, int steps, int slice, int words, int records, bool biased) {
     // [words + 1] marks, [words] marks in the words before, then for each mark [records]: times generated (bit 31: in the history), last bias
     // + 1, index in the slice
     extern __shared__ __align__(16) unsigned dyn[];
@@ -168,7 +169,6 @@ __global__ void __launch_bounds__(256, 4) next_token_kernel(const CmeToken p, in
     __shared__ int scan[8], total;
     constexpr int N = VECTOR ? Vec<T>::N : 1, PIECES = Vec<T>::PIECES;
     const int rank = blockIdx.x % cluster, row = blockIdx.x / cluster, tid = threadIdx.x, threads = blockDim.x;
-    const int v0 = min(p.vocab, rank * slice), v1 = min(p.vocab, v0 + slice);
     const int lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
     unsigned* const marks = dyn;
     int* const before = reinterpret_cast<int*>(marks + words + 1);
@@ -256,183 +256,188 @@ __global__ void __launch_bounds__(256, 4) next_token_kernel(const CmeToken p, in
         return ~b & ((1u << n) - 1u);
     };
 
-    // the first element on a 16-byte boundary, then groups, then what is left; marks of a group are whole bits of one byte
-    const int head = VECTOR ? (int)((N - (row * p.logits_ld + v0) % N) % N) : v1 - v0;
-    const int a0 = min(v1, v0 + head), groups = VECTOR ? (v1 - a0) / N : 0;      // (of sixteen bytes)
-    const int origin = VECTOR ? v0 + head - N : v0;        // of the marks
-    // f(index from the origin on, was it generated) for the entries of the history, f(index from the origin on, entry) for those of the biases
-    auto for_history = [&](auto&& f) {
+    // slices of the CTA's tokens, in their order
+    for (int step = 0; step < (STEPS ? steps : 1); ++step) {
+        if (STEPS && step) __syncthreads();                // the last slice's marks and records are done with
+        const int v0 = min(p.vocab, (STEPS ? rank * steps + step : rank) * slice), v1 = min(p.vocab, v0 + slice);
+        // the first element on a 16-byte boundary, then groups, then what is left; marks of a group are whole bits of one byte
+        const int head = VECTOR ? (int)((N - (row * p.logits_ld + v0) % N) % N) : v1 - v0;
+        const int a0 = min(v1, v0 + head), groups = VECTOR ? (v1 - a0) / N : 0;      // (of sixteen bytes)
+        const int origin = VECTOR ? v0 + head - N : v0;        // of the marks
+        // f(index from the origin on, was it generated) for the entries of the history, f(index from the origin on, entry) for those of the biases
+        auto for_history = [&](auto&& f) {
 #pragma unroll
-        for (int k = 0; k < KEPT; ++k) {
-            const int j = tid + k * threads;
-            if (j < told && kept[k] >= v0 && kept[k] < v1) f(kept[k] - origin, j >= given);
-        }
-        for (int j = tid + KEPT * threads; j < told; j += threads) {
-            const int id = hist[j];
-            if (id >= v0 && id < v1) f(id - origin, j >= given);
-        }
-    };
-    auto for_biases = [&](auto&& f) {
-        if (!biased) return;
-        const int* ids = p.bias_ids + (long long)row * p.biases;
-        for (int j = tid; j < p.biases; j += threads) {
-            const int id = ids[j];
-            if (id >= v0 && id < v1) f(id - origin, j);
-        }
-    };
-    typedef typename Vec<T>::Raw Raw;
-    const int stride = threads * PIECES, first = warp * 32 * PIECES + lane;      // a thread's groups: first, + 32 ..., a stride further ...
-    // A thread's loads travel through a ring of its own in shared memory, STAGES - 1 turns ahead: with one turn ahead in registers, 64 bytes a
-    // thread are on their way, and 1024 rows of 50304 in fp32 run at 3.9 TB/s.
-    uint4* const ring = reinterpret_cast<uint4*>(dyn + (words ? (2 * words + 1 + 3 * records + 3) / 4 * 4 : 0)) + tid;
-    const int pieces = PIECES + (p.noise ? 2 : 0);         // of 16 bytes, a turn
-    auto fetch = [&](int turn) {
-        if constexpr (VECTOR) {
-            uint4* to = ring + turn % STAGES * pieces * threads;
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) {
-                const int j = first + turn * stride + k * 32;
-                if (j < groups) {
-                    copy16(to + k * threads, src + a0 + j * N);
-                    if (noise) {
-#pragma unroll
-                        for (int e = 0; e < N / 4; ++e) copy16(to + (PIECES + k * (N / 4) + e) * threads, noise + a0 + j * N + e * 4);
-                    }
-                }
+            for (int k = 0; k < KEPT; ++k) {
+                const int j = tid + k * threads;
+                if (j < told && kept[k] >= v0 && kept[k] < v1) f(kept[k] - origin, j >= given);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-    };
-#pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t) fetch(t);
-    float early = 0.f, early_noise = 0.f;                  // one by one, a thread's first token
-    if (!VECTOR && v0 + tid < v1) {
-        early = to_f32<T>(src[v0 + tid]);
-        if (noise) early_noise = noise[v0 + tid];
-    }
-    auto place = [&](int l) { return before[l >> 5] + __popc(marks[l >> 5] & ((1u << (l & 31)) - 1u)); };
-    if (words) {
-        for (int i = tid; i <= words; i += threads) marks[i] = 0;
-        for (int i = tid; i < 2 * records; i += threads) count[i] = 0;
-        __syncthreads();
-        for_history([&](int l, bool) { atomicOr(&marks[l >> 5], 1u << (l & 31)); });
-        for_biases([&](int l, int) { atomicOr(&marks[l >> 5], 1u << (l & 31)); });
-        __syncthreads();
-        // marks before each word: a thread's own words, then the threads before it
-        const int each = (words + threads - 1) / threads, w0 = min(words, tid * each), w1 = min(words, w0 + each);
-        int sum = 0;
-        for (int w = w0; w < w1; ++w) sum += __popc(marks[w]);
-        int upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        if (lane == 31) scan[warp] = upto;
-        __syncthreads();
-        int at = upto - sum;
-        for (int w = 0; w < warp; ++w) at += scan[w];
-        if (tid == threads - 1) total = at + sum;
-        for (int w = w0; w < w1; ++w) { before[w] = at; at += __popc(marks[w]); }
-        __syncthreads();
-        // whole numbers: any order of the additions gives the same
-        for_history([&](int l, bool made) {
-            const int at = place(l);
-            which[at] = l;
-            atomicOr(&count[at], (int)0x80000000);
-            if (made) atomicAdd(&count[at], 1);
-        });
-        for_biases([&](int l, int j) {
-            const int at = place(l);
-            which[at] = l;
-            atomicMax(&bias[at], j + 1);
-        });
-    }
-    // tokens [from, to) one by one, whole warps
-    auto singles = [&](int from, int to) {
-        for (int b = from + warp * 32; b < to; b += threads) {
-            const int v = b + lane;
-            float x = -INFINITY, g = 0.f;
-            if (v < to) {
-                x = !VECTOR && v == v0 + tid ? early : to_f32<T>(src[v]);
-                if (noise) g = !VECTOR && v == v0 + tid ? early_noise : noise[v];
-                if (divides) x = __fdiv_rn(x, temp);
-                const int l = v - origin;
-                if (not_allowed(v, 1) || (words && (marks[l >> 5] >> (l & 31)) & 1)) x = -INFINITY;
-                if (dst) dst[v] = from_f32<T>(x);
-            }
-            const float y = noise ? __fadd_rn(x, g) : x;
-            take(&x, &y, std::integral_constant<int, 1>{}, [&](int) { return v; }, false);
-        }
-    };
-    singles(v0, a0);
-    if constexpr (VECTOR) {
-        const uint8_t* bytes = reinterpret_cast<const uint8_t*>(marks);
-        auto eight = [&](int i, const Raw* r, const float4* g) {       // groups i (and i + 32)
-            float x[8];
-            Vec<T>::unpack(r, x);
-            if (divides) by.apply8(x);
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) {
-                const int j = i + k * 32;
-                unsigned no = 0xff;
-                if (j < groups) {
-                    no = allowed ? not_allowed(a0 + j * N, N) : 0;
-                    if (words) no |= N == 8 ? bytes[j + 1] : bytes[(j + 1) >> 1] >> ((j + 1) & 1) * 4;
-                }
-                if (no & ((1u << N) - 1u)) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e) if ((no >> e) & 1) x[k * N + e] = -INFINITY;
-                }
-                if (dst && j < groups) __stcs(reinterpret_cast<Raw*>(dst + a0) + j, Vec<T>::pack(x, k));
-            }
-            auto token = [&](int e) { return a0 + (i + e / N * 32) * N + e % N; };
-            if (noise) {
-                const float* f = reinterpret_cast<const float*>(g);
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) f2_unpack(f2_add(f2_pack(x[e], x[e + 1]), f2_pack(f[e], f[e + 1])), y[e], y[e + 1]);
-                take(x, y, std::integral_constant<int, 8>{}, token, false);
-            } else {
-                take(x, x, std::integral_constant<int, 8>{}, token, false);
+            for (int j = tid + KEPT * threads; j < told; j += threads) {
+                const int id = hist[j];
+                if (id >= v0 && id < v1) f(id - origin, j >= given);
             }
         };
-        for (int turn = 0, i = first; i - lane < groups; ++turn, i += stride) {
-            fetch(turn + STAGES - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-            const uint4* from = ring + turn % STAGES * pieces * threads;
-            Raw r[PIECES];
-            float4 g[2];
-#pragma unroll
-            for (int k = 0; k < PIECES; ++k) r[k] = *reinterpret_cast<const Raw*>(from + k * threads);
-            if (noise) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) g[k] = *reinterpret_cast<const float4*>(from + (PIECES + k) * threads);
+        auto for_biases = [&](auto&& f) {
+            if (!biased) return;
+            const int* ids = p.bias_ids + (long long)row * p.biases;
+            for (int j = tid; j < p.biases; j += threads) {
+                const int id = ids[j];
+                if (id >= v0 && id < v1) f(id - origin, j);
             }
-            eight(i, r, g);
+        };
+        typedef typename Vec<T>::Raw Raw;
+        const int stride = threads * PIECES, first = warp * 32 * PIECES + lane;      // a thread's groups: first, + 32 ..., a stride further ...
+        // A thread's loads travel through a ring of its own in shared memory, STAGES - 1 turns ahead: with one turn ahead in registers, 64 bytes a
+        // thread are on their way, and 1024 rows of 50304 in fp32 run at 3.9 TB/s.
+        uint4* const ring = reinterpret_cast<uint4*>(dyn + (words ? (2 * words + 1 + 3 * records + 3) / 4 * 4 : 0)) + tid;
+        const int pieces = PIECES + (p.noise ? 2 : 0);         // of 16 bytes, a turn
+        auto fetch = [&](int turn) {
+            if constexpr (VECTOR) {
+                uint4* to = ring + turn % STAGES * pieces * threads;
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) {
+                    const int j = first + turn * stride + k * 32;
+                    if (j < groups) {
+                        copy16(to + k * threads, src + a0 + j * N);
+                        if (noise) {
+#pragma unroll
+                            for (int e = 0; e < N / 4; ++e) copy16(to + (PIECES + k * (N / 4) + e) * threads, noise + a0 + j * N + e * 4);
+                        }
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+        };
+#pragma unroll
+        for (int t = 0; t < STAGES - 1; ++t) fetch(t);
+        float early = 0.f, early_noise = 0.f;                  // one by one, a thread's first token
+        if (!VECTOR && v0 + tid < v1) {
+            early = to_f32<T>(src[v0 + tid]);
+            if (noise) early_noise = noise[v0 + tid];
         }
-        singles(a0 + groups * N, v1);
-    }
-    if (words) {
-        __syncthreads();                                   // the counts are made; what the pass wrote for marked tokens is overwritten
-        for (int b = warp * 32; b < total; b += threads) {
-            const int i = b + lane;
-            int v = 0;
-            float x = -INFINITY, g = 0.f;
-            if (i < total) {
-                const int c = count[i], made = c & 0x7fffffff, j = bias[i] - 1;
-                v = origin + which[i];
-                x = to_f32<T>(src[v]);
-                if (noise) g = noise[v];
-                if (c < 0) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-                if (made) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)made)), pres);
-                if (j >= 0) x = __fadd_rn(x, p.bias_values[(long long)row * p.biases + j]);
-                if (divides) x = __fdiv_rn(x, temp);
-                if (not_allowed(v, 1)) x = -INFINITY;
-                if (dst) dst[v] = from_f32<T>(x);
+        auto place = [&](int l) { return before[l >> 5] + __popc(marks[l >> 5] & ((1u << (l & 31)) - 1u)); };
+        if (words) {
+            for (int i = tid; i <= words; i += threads) marks[i] = 0;
+            for (int i = tid; i < 2 * records; i += threads) count[i] = 0;
+            __syncthreads();
+            for_history([&](int l, bool) { atomicOr(&marks[l >> 5], 1u << (l & 31)); });
+            for_biases([&](int l, int) { atomicOr(&marks[l >> 5], 1u << (l & 31)); });
+            __syncthreads();
+            // marks before each word: a thread's own words, then the threads before it
+            const int each = (words + threads - 1) / threads, w0 = min(words, tid * each), w1 = min(words, w0 + each);
+            int sum = 0;
+            for (int w = w0; w < w1; ++w) sum += __popc(marks[w]);
+            int upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
             }
-            const float y = noise ? __fadd_rn(x, g) : x;
-            take(&x, &y, std::integral_constant<int, 1>{}, [&](int) { return v; }, true);
+            if (lane == 31) scan[warp] = upto;
+            __syncthreads();
+            int at = upto - sum;
+            for (int w = 0; w < warp; ++w) at += scan[w];
+            if (tid == threads - 1) total = at + sum;
+            for (int w = w0; w < w1; ++w) { before[w] = at; at += __popc(marks[w]); }
+            __syncthreads();
+            // whole numbers: any order of the additions gives the same
+            for_history([&](int l, bool made) {
+                const int at = place(l);
+                which[at] = l;
+                atomicOr(&count[at], (int)0x80000000);
+                if (made) atomicAdd(&count[at], 1);
+            });
+            for_biases([&](int l, int j) {
+                const int at = place(l);
+                which[at] = l;
+                atomicMax(&bias[at], j + 1);
+            });
+        }
+        // tokens [from, to) one by one, whole warps
+        auto singles = [&](int from, int to) {
+            for (int b = from + warp * 32; b < to; b += threads) {
+                const int v = b + lane;
+                float x = -INFINITY, g = 0.f;
+                if (v < to) {
+                    x = !VECTOR && v == v0 + tid ? early : to_f32<T>(src[v]);
+                    if (noise) g = !VECTOR && v == v0 + tid ? early_noise : noise[v];
+                    if (divides) x = __fdiv_rn(x, temp);
+                    const int l = v - origin;
+                    if (not_allowed(v, 1) || (words && (marks[l >> 5] >> (l & 31)) & 1)) x = -INFINITY;
+                    if (dst) dst[v] = from_f32<T>(x);
+                }
+                const float y = noise ? __fadd_rn(x, g) : x;
+                take(&x, &y, std::integral_constant<int, 1>{}, [&](int) { return v; }, false);
+            }
+        };
+        singles(v0, a0);
+        if constexpr (VECTOR) {
+            const uint8_t* bytes = reinterpret_cast<const uint8_t*>(marks);
+            auto eight = [&](int i, const Raw* r, const float4* g) {       // groups i (and i + 32)
+                float x[8];
+                Vec<T>::unpack(r, x);
+                if (divides) by.apply8(x);
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) {
+                    const int j = i + k * 32;
+                    unsigned no = 0xff;
+                    if (j < groups) {
+                        no = allowed ? not_allowed(a0 + j * N, N) : 0;
+                        if (words) no |= N == 8 ? bytes[j + 1] : bytes[(j + 1) >> 1] >> ((j + 1) & 1) * 4;
+                    }
+                    if (no & ((1u << N) - 1u)) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) if ((no >> e) & 1) x[k * N + e] = -INFINITY;
+                    }
+                    if (dst && j < groups) __stcs(reinterpret_cast<Raw*>(dst + a0) + j, Vec<T>::pack(x, k));
+                }
+                auto token = [&](int e) { return a0 + (i + e / N * 32) * N + e % N; };
+                if (noise) {
+                    const float* f = reinterpret_cast<const float*>(g);
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) f2_unpack(f2_add(f2_pack(x[e], x[e + 1]), f2_pack(f[e], f[e + 1])), y[e], y[e + 1]);
+                    take(x, y, std::integral_constant<int, 8>{}, token, false);
+                } else {
+                    take(x, x, std::integral_constant<int, 8>{}, token, false);
+                }
+            };
+            for (int turn = 0, i = first; i - lane < groups; ++turn, i += stride) {
+                fetch(turn + STAGES - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+                const uint4* from = ring + turn % STAGES * pieces * threads;
+                Raw r[PIECES];
+                float4 g[2];
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) r[k] = *reinterpret_cast<const Raw*>(from + k * threads);
+                if (noise) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) g[k] = *reinterpret_cast<const float4*>(from + (PIECES + k) * threads);
+                }
+                eight(i, r, g);
+            }
+            singles(a0 + groups * N, v1);
+        }
+        if (words) {
+            __syncthreads();                                   // the counts are made; what the pass wrote for marked tokens is overwritten
+            for (int b = warp * 32; b < total; b += threads) {
+                const int i = b + lane;
+                int v = 0;
+                float x = -INFINITY, g = 0.f;
+                if (i < total) {
+                    const int c = count[i], made = c & 0x7fffffff, j = bias[i] - 1;
+                    v = origin + which[i];
+                    x = to_f32<T>(src[v]);
+                    if (noise) g = noise[v];
+                    if (c < 0) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+                    if (made) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)made)), pres);
+                    if (j >= 0) x = __fadd_rn(x, p.bias_values[(long long)row * p.biases + j]);
+                    if (divides) x = __fdiv_rn(x, temp);
+                    if (not_allowed(v, 1)) x = -INFINITY;
+                    if (dst) dst[v] = from_f32<T>(x);
+                }
+                const float y = noise ? __fadd_rn(x, g) : x;
+                take(&x, &y, std::integral_constant<int, 1>{}, [&](int) { return v; }, true);
+            }
         }
     }
     // (earlier, CTAs of the next kernel would crowd on the SMs that are done first: 1024 rows of 50304 183 us)
@@ -482,8 +487,8 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
     int slice, words, records, threads;
     bool vector;
     size_t tables, smem;
-    auto lay_out = [&](int cluster) {
-        slice = (cme_cdiv(p->vocab, cluster) + 31) / 32 * 32;
+    auto lay_out = [&](int slices) {
+        slice = (cme_cdiv(p->vocab, slices) + 31) / 32 * 32;
         words = marks ? slice / 32 + 1 : 0;                // (marks start up to eight tokens before the slice)
         records = marks ? (int)std::min((long long)slice, (long long)(p->history ? p->history_len : 0) + (biased ? p->biases : 0)) : 0;
         tables = smem = marks ? ((size_t)2 * words + 1 + 3 * (size_t)records) * 4 : 0;
@@ -495,21 +500,25 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
         if (vector) smem = (smem + 15) / 16 * 16 + (size_t)STAGES * threads * 16 * ((p->dtype == CME_F32 ? 2 : 1) + (p->noise ? 2 : 0));
     };
     // As many CTAs as run at a time, with no fewer than 2048 tokens each: a second turn costs as much as a row's length (us, one CTA / two for
-    // a row: 319 rows of 6186 10.7 / 18.0, 200 of 50304 in fp32, two / four 28.0 / 34.5).  Smaller slices where a CTA's records would not fit.
-    int cluster = MAX_CLUSTER;
+    // a row: 319 rows of 6186 10.7 / 18.0, 200 of 50304 in fp32, two / four 28.0 / 34.5).  Smaller slices where a CTA's records would not fit, and
+    // from eight CTAs on several for each: a token of a slice has a record at the most, so that some number of them does.
+    int cluster = MAX_CLUSTER, steps = 1;
     for (; cluster > 1; cluster /= 2) {
         lay_out(cluster);
         if (p->vocab / cluster >= 2048 && (long long)p->rows * cluster <= (long long)sms * std::min<size_t>(4, 227 * 1024 / (smem + 1024))) break;
     }
-    for (lay_out(cluster); tables > MAX_SMEM; lay_out(cluster *= 2))
-        CME_REQUIRE(cluster < MAX_CLUSTER, CME_ERR_LIMIT, "next token: a history of %d with a vocabulary of %d", p->history_len, p->vocab);
+    for (lay_out(cluster); tables > MAX_SMEM; lay_out(cluster * steps)) (cluster < MAX_CLUSTER ? cluster : steps) *= 2;
     CME_REQUIRE((long long)p->rows * cluster < (1ll << 31), CME_ERR_LIMIT, "next token: too many rows");
-    auto* kernel = p->dtype == CME_F32 ? (vector ? next_token_kernel<float, true> : next_token_kernel<float, false>)
-                                       : (vector ? next_token_kernel<__nv_bfloat16, true> : next_token_kernel<__nv_bfloat16, false>);
-    static bool attr[2][2][CME_MAX_DEVICES] = {};         // function attributes are per device
+    auto of = [&](auto several) {
+        constexpr bool S = decltype(several)::value;
+        return p->dtype == CME_F32 ? (vector ? next_token_kernel<float, true, S> : next_token_kernel<float, false, S>)
+                                   : (vector ? next_token_kernel<__nv_bfloat16, true, S> : next_token_kernel<__nv_bfloat16, false, S>);
+    };
+    auto* kernel = steps > 1 ? of(std::true_type{}) : of(std::false_type{});
+    static bool attr[2][2][2][CME_MAX_DEVICES] = {};      // function attributes are per device
     int dev = 0;
     CME_CUDA(cudaGetDevice(&dev));
-    if (bool& set = attr[p->dtype == CME_F32][vector][dev % CME_MAX_DEVICES]; !set) {
+    if (bool& set = attr[steps > 1][p->dtype == CME_F32][vector][dev % CME_MAX_DEVICES]; !set) {
         CME_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MAX_SMEM + MAX_RING)));
         set = true;
     }
@@ -526,7 +535,7 @@ CME_API int cme_next_token(const CmeToken* p, void* stream) {
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    CME_CUDA(cudaLaunchKernelEx(&cfg, kernel, *p, cluster, slice, words, records, biased));
+    CME_CUDA(cudaLaunchKernelEx(&cfg, kernel, *p, cluster, steps, slice, words, records, biased));
     CME_LAUNCH_CHECK();
     return CME_OK;
 }
