@@ -651,8 +651,10 @@ struct Walk {
             if (b < p.a.seqs) { load_seq<C>(p, b); own += (long long)tiles * p.a.kv_heads * keys; }
         }
         // Sequences that share rows, which no offsets in order make, can have more than 31 bits of tiles: none is taken then.
-        const unsigned high = __reduce_add_sync(0xffffffffu, (unsigned)min(own >> 16, 1ll << 16)), low = __reduce_add_sync(0xffffffffu, (unsigned)own & 0xffffu);
-        if (((unsigned long long)high << 16) + low > INT_MAX) return 1;
+        if (__any_sync(0xffffffffu, own > INT_MAX / 32)) {
+            const unsigned high = __reduce_add_sync(0xffffffffu, (unsigned)min(own >> 16, 1ll << 16)), low = __reduce_add_sync(0xffffffffu, (unsigned)own & 0xffffu);
+            if (((unsigned long long)high << 16) + low > INT_MAX) return 1;
+        }
         const int sum = (int)own;
         int upto = sum;
 #pragma unroll
