@@ -58,16 +58,13 @@ inline bool paged_by_keys(const CmePaged* a, int group) { return a->seqs <= 32 &
 struct PagedTile {
     int seq, first, rows;        // rows == 0: the tile does not exist
     int token0, n, length;       // the sequence's first row of q, its new tokens, its tokens
-    int held;                    // keys of them that the table and max_len hold
 };
 
-// length and held of a sequence with n new tokens.  Where a length passes what is held, the new tokens keep their positions (cache_append
-// writes those that have a place): each sees all keys that are held up to its own.  Where none of them has a place, the length counts as what is held.
-__device__ __forceinline__ void paged_length(const CmePaged& a, int len, int n, int& length, int& held) {
-    held = (int)min((long long)a.width * a.page, (long long)a.max_len);
-    length = max(0, len);
-    if (length - n >= held) length = held;
-    held = min(held, length);
+// The length of a sequence with n new tokens.  Where it passes max_len (here no more than the table holds), the new tokens keep their positions
+// (cache_append writes those that have a place): each sees the keys below max_len up to its own.  Where none of them has a place, the length counts as max_len.
+__device__ __forceinline__ int paged_length(const CmePaged& a, int len, int n) {
+    len = max(0, len);
+    return len - n >= a.max_len ? a.max_len : len;
 }
 
 // Finds row tile `tile`, counting ceil(new tokens x group / row_tile) tiles per sequence.  Whole warps call it; every warp gets
@@ -97,7 +94,7 @@ __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile
             t.seq = b0 + src;
             t.token0 = __shfl_sync(0xffffffffu, lo, src);
             t.n = __shfl_sync(0xffffffffu, n, src);
-            paged_length(a, __shfl_sync(0xffffffffu, len, src), t.n, t.length, t.held);
+            t.length = paged_length(a, __shfl_sync(0xffffffffu, len, src), t.n);
             t.first = first;
             t.rows = (int)min((long long)row_tile, (long long)t.n * group - first);
             return t;
@@ -112,7 +109,7 @@ __device__ __forceinline__ PagedTile paged_find_tile(const CmePaged& a, int tile
 __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, int tile, int group, int row_tile, int keys) {
     const int b = threadIdx.x & 31;
     PagedTile t{};
-    int lo = 0, hi = 0, len = 0, length, held;
+    int lo = 0, hi = 0, len = 0;
     if (b < a.seqs) {
         lo = a.offsets[b];
         hi = a.offsets[b + 1];
@@ -120,8 +117,7 @@ __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, 
     }
     lo = max(0, min(lo, a.rows));
     hi = max(lo, min(hi, a.rows));
-    const int n = hi - lo;
-    paged_length(a, len, n, length, held);
+    const int n = hi - lo, length = paged_length(a, len, n), held = min(length, a.max_len);
     const int own = (n * group + row_tile - 1) / row_tile;
     // tiles of the sequence that see x key tiles at least; they are its last ones
     auto count = [&](int x) {
@@ -152,7 +148,6 @@ __device__ __forceinline__ PagedTile paged_find_tile_by_keys(const CmePaged& a, 
     t.token0 = __shfl_sync(0xffffffffu, lo, src);
     t.n = __shfl_sync(0xffffffffu, n, src);
     t.length = __shfl_sync(0xffffffffu, length, src);
-    t.held = __shfl_sync(0xffffffffu, held, src);
     t.rows = (int)min((long long)row_tile, (long long)t.n * group - t.first);
     return t;
 }

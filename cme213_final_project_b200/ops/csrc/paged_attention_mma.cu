@@ -476,9 +476,13 @@ template <typename T> __device__ __forceinline__ const T* row_of_q(const MmaPara
     const int rr = t.first + r, tok = rr / p.group;
     return static_cast<const T*>(p.a.q) + (t.token0 + tok) * p.a.q_token + (head * p.group + rr - tok * p.group) * p.a.q_head;
 }
-// Keys that row r of a tile sees.
+// Keys that row r of a tile sees, if there are so many.
 __device__ __forceinline__ int row_sees(const MmaParams& p, const PagedTile& t, int r) {
     return t.length - t.n + (t.first + r) / p.group + 1;
+}
+// Keys that a row of the tile sees: those of its last row.
+__device__ __forceinline__ int tile_sees(const MmaParams& p, const PagedTile& t) {
+    return max(0, min(p.a.max_len, row_sees(p, t, t.rows - 1)));
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -521,7 +525,7 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     __syncthreads();
     if (t.rows == 0) return;
     // keys [0, limit) are seen by the last row; this CTA takes [begin, end)
-    const int limit = max(0, min(t.held, row_sees(p, t, t.rows - 1)));
+    const int limit = tile_sees(p, t);
     const int begin = (int)min((long long)limit, (long long)split * p.split_keys);
     const int end = (int)min((long long)limit, (long long)begin + p.split_keys);
     if (warp == C::WARPS) {
@@ -637,10 +641,10 @@ struct Walk {
         t.seq = seq = b;
         t.token0 = lo;
         t.n = hi - lo;
-        paged_length(a, a.lengths[b], t.n, t.length, t.held);
+        t.length = paged_length(a, a.lengths[b], t.n);
         t.first = t.rows = 0;
         tiles = (int)(((long long)t.n * p.group + 15) / 16);
-        keys = max(1, cme_cdiv_dev(t.held, C::KEYS)) + ITEM_COST;
+        keys = max(1, cme_cdiv_dev(min(t.length, a.max_len), C::KEYS)) + ITEM_COST;
     }
     // Takes share `part` of `parts` of the whole; returns how many key tiles a share has.  Whole warps.
     template <typename C> __device__ __forceinline__ int start(const MmaParams& p, int part, int parts) {
@@ -694,7 +698,7 @@ struct Walk {
             if (k1 > 0) {
                 t.first = tile * 16;
                 t.rows = (int)min(16ll, (long long)t.n * p.group - t.first);
-                const int limit = max(0, min(t.held, row_sees(p, t, t.rows - 1)));
+                const int limit = tile_sees(p, t);
                 part.t = t;
                 part.head = head;
                 part.begin = (int)min((long long)limit, (long long)k0 * C::KEYS);
@@ -756,7 +760,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     if constexpr (CLUSTER) {
         part.t = paged_find_tile(a, blockIdx.x / p.splits, p.group, 16);
         part.head = blockIdx.y;
-        const int limit = max(0, min(part.t.held, row_sees(p, part.t, part.t.rows - 1)));
+        const int limit = tile_sees(p, part.t);
         const int span = cme_cdiv_dev(cme_cdiv_dev(limit, C::KEYS), p.splits) * C::KEYS;
         part.begin = (int)min((long long)limit, (long long)(blockIdx.x % p.splits) * span);
         part.end = (int)min((long long)limit, (long long)part.begin + span);

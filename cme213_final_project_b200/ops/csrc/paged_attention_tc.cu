@@ -153,7 +153,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (warp == 0) { __syncwarp(); tmem_dealloc(*tmem_slot, C::COLS); }
         return;
     }
-    const int limit = max(0, min(t.held, t.length - t.n + (t.first + t.rows - 1) / p.group + 1));
+    const int limit = max(0, min(a.max_len, t.length - t.n + (t.first + t.rows - 1) / p.group + 1));
     const int begin = (int)min((long long)limit, (long long)split * p.split_keys);
     const int end = (int)min((long long)limit, (long long)begin + p.split_keys);
     const int nkv = cme_cdiv_dev(end - begin, KEYS);

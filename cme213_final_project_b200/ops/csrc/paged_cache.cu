@@ -308,12 +308,13 @@ CME_API int cme_paged_attention(const CmePaged* a, int backend, int splits, void
     int rc, sms;
     if ((rc = check_attention(a)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
     if (a->rows == 0 || a->seqs == 0) return CME_OK;
-    CmePaged none = *a;
+    CmePaged held = *a;
+    held.max_len = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
     if (a->num_pages == 0) {                               // a cache without memory: no key is there, and nothing is loaded
-        none.max_len = 0;
-        none.k = none.v = const_cast<void*>(a->q);
-        a = &none;
+        held.max_len = 0;
+        held.k = held.v = const_cast<void*>(a->q);
     }
+    a = &held;
     CME_REQUIRE(ws_bytes(a, p) <= a->ws_bytes, CME_ERR_SHAPE, "paged attention: %lld bytes of scratch, %lld are needed", a->ws_bytes,
                 ws_bytes(a, p));
     cudaStream_t st = (cudaStream_t)stream;
