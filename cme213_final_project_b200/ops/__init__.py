@@ -431,7 +431,8 @@ def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Opti
     :func:`cache_append` for the cache and the tables).  ``heads`` is a multiple of the cache's heads, which as many query heads
     in a row share.  Returns ``(out, lse)``: ``[tokens, heads, head_dim]`` and the log-sum-exp of the scaled scores, fp32
     ``[tokens, heads]``.  Keys on pages that are not there do not take part; a row without any key gets zeros and ``-inf``.
-    What the cache holds beyond a sequence's length may be anything, within it the values have to be finite.
+    Both results lie in one allocation, which lives as long as either.  What the cache holds beyond a sequence's length may be
+    anything, within it the values have to be finite.
 
     ``scale``: of the scores, ``head_dim ** -0.5`` by default.  ``max_len``: keys from this position on do not take part (default: what
     the table holds); the number of parts that the keys are divided into goes by it.  Where a length passes it, new tokens keep their
@@ -445,7 +446,8 @@ def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Opti
 def next_token(logits, *, history=None, lengths=None, prompts=None, repetition=None, presence=None, frequency=None, bias_ids=None,
                bias_values=None, temperature=None, allowed=None, noise=None, processed: bool = False):
     """From ``logits`` (``[rows, vocab]``, bf16 or fp32) to each row's next token.  Returns ``(token, logprob, processed)``: int32
-    and fp32 ``[rows]``, and the processed logits in the type of ``logits`` (``None`` unless ``processed``).
+    and fp32 ``[rows]`` (one allocation, which lives as long as either), and the processed logits in the type of ``logits`` (``None``
+    unless ``processed``).
 
     In 32 bits and in this order: tokens of the row's ``history`` (int32 ``[rows, columns]``, the first ``lengths[row]`` of
     them; others than tokens are skipped) get ``x / r`` where x > 0, else ``x * r``, r = ``repetition``; those at ``prompts[row]``

@@ -10,8 +10,8 @@
 // records as entries for 50304 tokens, where counts by token take 200 KB, or have to be made and cleared 8192 at a time.
 // A row belongs to a cluster of 1 to 8 CTAs, each with a slice of the vocabulary; maxima, sums and picks are joined in the first one's
 // shared memory.
-// 64 rows of 65 tokens 5.1 us; 64 of 50304, bf16, 1024 tokens of history and 64 biases each 14.0 us; 1024 of 50304 in fp32 with noise and the
-// processed logits 124 us, 5.0 TB/s.
+// 64 rows of 65 tokens 5.4 us; 64 of 50304, bf16, 1024 tokens of history and 64 biases each 13.6 us; 1024 of 50304 in fp32 with noise and the
+// processed logits 127 to 130 us, 4.8 TB/s (calls one after the other; replayed as a graph 4.9, 13.6 and 125).
 #include "common.h"
 #include "token_desc.h"
 

@@ -9,8 +9,8 @@
 //   rows    64 rows a CTA, 16 a warp; in fp32 and head sizes above 32 two warps share 16 rows and take every other 16 or 32 keys.  For chunks
 //           that the tcgen05 kernel does not take.
 // The last warp looks up the pages and loads key tiles by TMA, one box per page (or key tile), several tiles ahead.
-// fp32 operands of the matrix instructions are split into two tf32 numbers each (x = hi + lo, 11 bits each) and multiplied as hi hi + hi lo + lo hi: what is
-// left out is below 2^-22 of a product.  The tensor core's sums are kept short (one key tile, added up in fp32 registers), since it cuts
+// fp32 operands of the matrix instructions are split into two tf32 numbers each (x = hi + lo, 11 bits each) and multiplied as hi hi + hi lo + lo hi.  What is
+// left out is 2^-21 of a product at the most: 2^-22 for lo lo, 2^-23 for what each operand's lo cuts off.  The tensor core's sums are kept short (one key tile, added up in fp32 registers), since it cuts
 // what it shifts out.
 // Every wait is bounded; on expiry the CTA flags the status word and returns.
 #include "paged.h"
@@ -97,7 +97,8 @@ __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x as the sum of two tf32 numbers: the nearest one (half away from zero) and what is left, cut off; 2^-21 of x is lost.  On the integer
+// x as the sum of two tf32 numbers: the nearest one (half away from zero), and what is left, up to 2^-11 of x, cut off to its 11 upper bits.
+// That is a multiple of x's last place of 13 bits at the most, which loses one last place, 2^-23 of x.  On the integer
 // pipe: the conversion instruction runs at an eighth of its rate.  NaN stays (in the low part, if its bits overflow).
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
@@ -315,7 +316,8 @@ __device__ __forceinline__ void attend(WarpState<C, D>& w, const R& q, uint32_t 
             for (int i = 0; i < 4; ++i) w.o[d][i] += acc[i] + low[i];
         }
     } else {
-        // probabilities as bf16, the operand's type; their sum l is of the unrounded ones
+        // Probabilities as bf16, the type of the other operand, V; their sum l is of the unrounded ones.  Errors against 64 bits are 0.0013 to 0.0022
+        // of a result's size, 0.0011 to 0.0017 with probabilities in 32 bits (the result's own rounding).
 #pragma unroll
         for (int n = 0; n < NK; n += 2) {
             const uint32_t pa[4] = {f2_to_bf2(sc[n][0], sc[n][1]), f2_to_bf2(sc[n][2], sc[n][3]),
@@ -619,9 +621,9 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
 //            lengths.  A CTA's loads run on into its next item while the last one's warps are joined.  An item that lies in one CTA is
 //            finished there, the others' parts are left in scratch (at most two a CTA) and joined by a small kernel.
 //   cluster  a CTA has one part of one item, and up to eight CTAs join theirs through shared memory: one launch, for few items.
-// Single tokens, bf16: one sequence of 701, 12 heads of 64 5.2 us (a launch, three dependent lookups, a tile, the join); 64 of up to 1024, 16
-// heads of 64 31 us, 4.3 TB/s of 135 MB; 16 of 2000 to 32768, 32 heads of 128 on 8 163 us, 6.2 TB/s.  fp32: 32 of up to 2048, 4 heads of 128
-// 34 us, 3.9 TB/s.
+// Single tokens, bf16, calls one after the other: one sequence of 701, 12 heads of 64 5.6 us (a launch, three dependent lookups, a tile, the join;
+// 5.0 as a graph); 64 of up to 1024, 16 heads of 64 31.8 us, 4.2 TB/s of 135 MB; 16 of 2000 to 32768, 32 heads of 128 on 8 166 us, 6.1 TB/s.  fp32: 32
+// of up to 2048, 4 heads of 128 34.3 us, 3.9 TB/s.
 constexpr int REC_INTS = 8;                // of an item that ends in a CTA other than it began in: first CTA or -1, rows, token0, first, head
 
 // Walks over the key tiles of all items, in the order sequence, tile of rows, key head, key tile.  What an item costs besides its tiles
