@@ -61,7 +61,8 @@ _PROTOTYPES = {
 _WRAPPED = ("cme_last_error", "cme_cross_entropy", "cme_attention_fwd", "cme_attention_bwd", "cme_attention_path",
             "cme_attention_gemm_ws_bytes", "cme_layernorm_fwd", "cme_layernorm_bwd_blocks", "cme_layernorm_bwd",
             "cme_bias_act_residual", "cme_colsum_splits", "cme_dact_colsum", "cme_embedding_fwd", "cme_embedding_bwd",
-            "cme_paged_append", "cme_paged_attention_ws_bytes", "cme_paged_attention", "cme_next_token")
+            "cme_paged_append", "cme_paged_attention_ws_bytes", "cme_paged_attention", "cme_next_token", "cme_paged_append8",
+            "cme_paged_attention8_ws_bytes", "cme_paged_attention8", "cme_beam_step_ws_bytes", "cme_beam_step", "cme_cache_reorder")
 _CTYPES = {"v": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "u": ctypes.c_uint}
 
 
@@ -408,12 +409,12 @@ def attention_bwd(q, k, v, out, lse, dout, B: int, H: int, T: int, layout: str =
 
 
 # --------------------------------------------------------------------------------------------------
-# Generation: a paged cache of keys and values, attention over it, the next token
+# Generation: a paged cache of keys and values, attention over it, the next token, beams
 # --------------------------------------------------------------------------------------------------
 _PAGED_BACKENDS = {"auto": 0, "single": 1, "rows": 2, "tc": 3}
 
 
-def cache_append(k, v, cache_k, cache_v, pages, offsets, lengths) -> None:
+def cache_append(k, v, cache_k, cache_v, pages, offsets, lengths, *, k_scales=None, v_scales=None) -> None:
     """Write new tokens' keys and values (``[tokens, kv_heads, head_dim]``, any strides of multiples of 16 bytes) into a paged cache.
 
     ``cache_k``, ``cache_v``: ``[pages, kv_heads, slots, head_dim]``, any strides of multiples of 16 bytes, slots a multiple of 8;
@@ -421,12 +422,23 @@ def cache_append(k, v, cache_k, cache_v, pages, offsets, lengths) -> None:
     ``p % slots`` of page ``pages[seq, p // slots]``; an entry outside the cache (-1) is a page that is not there.  ``offsets``
     (int32 ``[seqs + 1]``, from 0 to the number of tokens): the tokens of a sequence.  ``lengths`` (int32 ``[seqs]``): tokens of
     a sequence with the new ones, which come last.  A token without a place (page not there, position beyond the table) is dropped.
-    A page belongs to one sequence at a time as far as new tokens go; pages that are only read may be shared."""
-    _native().cache_append(k, v, cache_k, cache_v, pages, offsets, lengths)
+    A page belongs to one sequence at a time as far as new tokens go; pages that are only read may be shared.
+
+    With ``k_scales`` and ``v_scales`` (fp32 ``[pages, kv_heads, blocks]``) the cache is int8: slot s of a page and head stands for its
+    integers (-127 to 127) times the scale of block ``s // (slots / blocks)``, a multiple of 8 slots.  A block's scale is the
+    largest magnitude written to it times ``1 / 127``.  Where new tokens come to a block that holds earlier ones of their sequence and raise it, the
+    earlier ones' integers are rounded anew, so the cache depends on how tokens came in calls; a number is off by half of its scale, plus half of
+    each scale that its block had before.  Numbers are ``round(x * (1 / scale))`` and ``round(q * (old / new))``, each
+    operation rounded in 32 bits; where a scale would be below ``2 ** -100``, it and the integers are 0.  The first token of a block starts it
+    anew, whatever was there.  A NaN or infinity among a block's numbers makes all of its numbers NaN."""
+    if k_scales is None and v_scales is None:
+        _native().cache_append(k, v, cache_k, cache_v, pages, offsets, lengths)
+    else:
+        _native().cache_append8(k, v, cache_k, cache_v, pages, offsets, lengths, k_scales, v_scales)
 
 
 def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Optional[float] = None, max_len: Optional[int] = None,
-                    backend: str = "auto", splits: int = 0):
+                    backend: str = "auto", splits: int = 0, k_scales=None, v_scales=None):
     """Causal attention of new tokens, ``q`` = ``[tokens, heads, head_dim]``, over a paged cache that holds their keys too (see
     :func:`cache_append` for the cache and the tables).  ``heads`` is a multiple of the cache's heads, which as many query heads
     in a row share.  Returns ``(out, lse)``: ``[tokens, heads, head_dim]`` and the log-sum-exp of the scaled scores, fp32
@@ -439,7 +451,13 @@ def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Opti
     positions, as in :func:`cache_append`, and see the keys below it up to their own; a sequence none of whose new tokens has a
     position below it counts as that long.  ``backend``: ``auto`` | ``single`` (few rows) | ``rows`` |
     ``tc`` (tcgen05: bf16); ``splits``: parts of the keys, 0 = by the rule, negative = joined
-    through scratch memory in any case."""
+    through scratch memory in any case.
+
+    ``k_scales``, ``v_scales``: of an int8 cache, as :func:`cache_append` makes it; ``q`` and the result are bf16 or fp32 all the same.  Scales
+    of values below ``2 ** -100`` count as 0; those of blocks that no sequence has reached may be anything."""
+    if k_scales is not None or v_scales is not None:
+        return _native().paged_attention8(q, cache_k, cache_v, pages, offsets, lengths, scale, max_len, _PAGED_BACKENDS[backend], splits,
+                                          k_scales, v_scales)
     return _native().paged_attention(q, cache_k, cache_v, pages, offsets, lengths, scale, max_len, _PAGED_BACKENDS[backend], splits)
 
 
@@ -459,6 +477,33 @@ def next_token(logits, *, history=None, lengths=None, prompts=None, repetition=N
     log-sum-exp of the row (``-inf`` without a token).  ``repetition``, ``presence``, ``frequency``, ``temperature``: fp32 ``[rows]``."""
     return _native().next_token(logits, history, lengths, prompts, repetition, presence, frequency, bias_ids, bias_values, temperature,
                                 allowed, noise, processed)
+
+
+def beam_step(logits, scores, width: Optional[int] = None, *, finished=None, allowed=None):
+    """The ``width`` best continuations of each group of beams (1 to 32 of both; ``width`` is the number of beams by default).  Returns
+    ``(parents, tokens, scores)``, int32, int32 and fp32 ``[groups, width]``, best first (one allocation, which lives as long as any).
+
+    ``logits``: bf16 or fp32 ``[groups * beams, vocab]``, after each beam's last token; ``scores``: fp32 ``[groups, beams]``.  Token t
+    after beam b is worth ``scores[b] + logits[b, t] - logsumexp(logits[b])``, over the tokens whose bit of ``allowed`` (as
+    :func:`next_token` takes it) is set.  A beam of ``finished`` (bool ``[groups, beams]``) has one continuation: itself, with token -1
+    and its score.  Ordered by these values as real numbers (not by their rounded ones); equals by beam, then by token.  A beam
+    whose score is not finite, and one without a finite log-sum-exp (no token allowed, a NaN or ``inf`` among its logits), has none.
+    Where a group has fewer than ``width``, the others are ``(place % beams, -1, -inf)``."""
+    return _native().beam_step(logits, scores, width, finished, allowed)
+
+
+def cache_reorder(cache_k, cache_v, pages, spare, parents, lengths, *, k_scales=None, v_scales=None):
+    """Let each beam go on from its parent's past in a paged cache.  Returns ``(pages, spare)`` anew (int32, one allocation).
+
+    ``cache_k``, ``cache_v``: ``[layers, pages, kv_heads, slots, head_dim]`` with ``k_scales``, ``v_scales``
+    (``[layers, pages, kv_heads, blocks]``) if they are int8.  ``pages`` (int32 ``[groups * beams, columns]``): as :func:`cache_append`
+    takes it; ``parents`` (int32 ``[groups, beams]``): a number within the group, others than those stand for the beam itself;
+    ``lengths`` (int32 ``[groups]``): tokens of each beam of a group.  Pages that the length fills are shared: the beam's table names its
+    parent's.  Of the last, partly filled one each beam has its own: where the parent is another beam, its filled slots are copied to
+    page ``spare[beam]`` (int32 ``[groups * beams]``), which the new table names, and the page that the table named before becomes the new
+    spare one.  Table entries behind the length stay.  Spare pages, last pages and pages behind them have to belong to one beam
+    each.  Where the parent's last page is not there, the beam has none either; without a spare page it has none (-1)."""
+    return _native().cache_reorder(cache_k, cache_v, pages, spare, parents, lengths, k_scales, v_scales)
 
 
 def launch_count() -> int:

@@ -1,0 +1,545 @@
+// One step of a search with beams: of all continuations of a group's beams, the `width` best.
+//
+//     value(beam, token) = score[beam] + x[token] - log sum exp x;      a finished beam has one continuation, itself, with its score
+//
+// The order is that of the values as real numbers; equal ones: lower beam, lower token.  Within a beam that is the order of x.  Between beams
+// it hangs on the log-sum-exps, whose 32-bit sums are off by some 2^-20; so every pair of different beams that decides something is held
+// against a bound of that error, and where one is closer, the log-sum-exps of its beams are made anew in 64 bits.  Equal rows have equal
+// ones then, too.
+//
+// Two launches: `scan` goes once over the logits, a CTA a slice of a row: sum of exponentials and the `width` largest; `merge`, a CTA a group,
+// joins the slices and picks.  Up to 256 tokens (characters) a row is a warp's, in 64 bits, and one launch does both.
+// In scan a thread keeps the sum and the largest of its elements only, which costs no branch; the width-th largest of the best of those bounds
+// what can be chosen from below, and the few threads that hold something above it look through their elements again.
+// What bounds it: the bytes of the logits.
+//
+// The bound of a log-sum-exp's error: an exponential's argument x - r is rounded twice and multiplied by a rounded log2 e, 2.5 * 2^-24 of |x - r|, which
+// weighted by the softmax comes to 2.5 * 2^-24 (log vocab + RAISE) at the most (a reference r is one of the x, and none above r + RAISE
+// goes by it; the mean distance from the largest x is at most log vocab, as the entropy is); the
+// exponential itself is good to 2^-22; four additions in 32 bits a sum of eight, 4 * 2^-24; the rest is added in 64 bits.
+#include "common.h"
+#include "beam_desc.h"
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_WIDTH = 32, MAX_BEAMS = 32;
+constexpr int SCAN = 256;                  // threads of a scan CTA
+constexpr int CAP = 1024;                  // elements above the bound that a scan CTA can hold
+constexpr int MERGE = 512;                 // threads of a merge CTA
+constexpr int SURVIVORS = MAX_WIDTH * MAX_WIDTH;
+constexpr int SMALL_VOCAB = 256;
+constexpr float RAISE = 8.f;
+
+struct Cand { float x; int token; };
+// What a slice of a row comes to; behind it [width] candidates, best first.
+struct Part {
+    double sum;                            // of exp(x - ref)
+    float ref;
+    int count, pad[4];
+};
+static_assert(sizeof(Part) == 32 && sizeof(Cand) == 8, "layout of the scratch");
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.x > b.x || (a.x == b.x && a.token < b.token); }
+
+// The row's elements [v0, v1) as this thread's share of sixteen bytes each: f(first token, values, how many).  Every call of a thread's walks
+// over the same elements.
+template <typename T> struct Slice {
+    static constexpr int N = 16 / (int)sizeof(T);
+    const T* src;
+    const unsigned* allowed;
+    int v0, v1, a0, groups;
+
+    __device__ __forceinline__ Slice(const CmeBeams& p, int row, int from, int to) : v0(from), v1(to) {
+        src = static_cast<const T*>(p.logits) + row * p.logits_ld;
+        allowed = p.allowed ? reinterpret_cast<const unsigned*>(p.allowed) + row * p.allowed_ld : nullptr;
+        const int off = (int)((reinterpret_cast<uintptr_t>(src + v0) / sizeof(T)) % N);
+        a0 = min(v1, v0 + (off ? N - off : 0));
+        groups = (v1 - a0) / N;
+    }
+    __device__ __forceinline__ bool is_allowed(int t) const { return !allowed || (__ldg(allowed + (t >> 5)) >> (t & 31)) & 1; }
+    __device__ __forceinline__ float at(int t) const { return is_allowed(t) ? to_f32<T>(src[t]) : -INFINITY; }
+    static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+        if constexpr (N == 8) unpack8(v, x);
+        else { x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w); }
+    }
+    template <int THREADS, typename F> __device__ __forceinline__ void each(F&& f) const {
+        constexpr int AHEAD = 4;
+        for (int g0 = threadIdx.x; g0 < groups; g0 += THREADS * AHEAD) {
+            uint4 raw[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+                if (g0 + u * THREADS < groups) raw[u] = *reinterpret_cast<const uint4*>(src + a0 + (g0 + u * THREADS) * N);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int t = a0 + (g0 + u * THREADS) * N;
+                if (g0 + u * THREADS >= groups) break;
+                float x[N];
+                unpack(raw[u], x);
+                if (allowed) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[e] = is_allowed(t + e) ? x[e] : -INFINITY;
+                }
+                f(t, x, std::integral_constant<int, N>{});
+            }
+        }
+        // the ends, one by one
+        const int head = a0 - v0, tail = a0 + groups * N, rest = head + v1 - tail;
+        if ((int)threadIdx.x < rest) {
+            const int t = (int)threadIdx.x < head ? v0 + (int)threadIdx.x : tail + (int)threadIdx.x - head;
+            const float x[1] = {at(t)};
+            f(t, x, std::integral_constant<int, 1>{});
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------------
+// Scan
+// ------------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int slices, int slice) {
+    constexpr int WARPS = SCAN / 32;
+    __shared__ float tops[WARPS * 8];
+    __shared__ double sums[WARPS];
+    __shared__ float refs[WARPS], bound_s;
+    __shared__ Cand held[CAP];
+    __shared__ int count;
+    __shared__ Cand round_best[WARPS];
+    pdl_wait();
+    const int row = blockIdx.x / slices, part = blockIdx.x - row * slices, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    char* out = static_cast<char*>(p.ws) + (long long)blockIdx.x * (sizeof(Part) + p.width * sizeof(Cand));
+    Part* result = reinterpret_cast<Part*>(out);
+    Cand* list = reinterpret_cast<Cand*>(result + 1);
+    if ((p.finished && p.finished[row]) || !finite(p.scores[row])) {         // nothing of the row counts
+        if (tid == 0) *result = Part{0.0, 0.f, 0, {0, 0, 0, 0}};
+        return;
+    }
+    const int v0 = min((long long)p.vocab, (long long)part * slice), v1 = min((long long)p.vocab, (long long)v0 + slice);
+    const Slice<T> s(p, row, v0, v1);
+    // A thread's sum has a reference of its own, the largest of its first elements, and a new one only where that is passed by much.
+    float ref = -INFINITY, top = -INFINITY;
+    double sum = 0.0;
+    s.template each<SCAN>([&](int, const float* x, auto number) {
+        constexpr int n = decltype(number)::value;
+        float m = x[0];
+#pragma unroll
+        for (int e = 1; e < n; ++e) m = fmaxf(m, x[e]);
+        top = fmaxf(top, m);
+        if (m > ref + RAISE || (ref == -INFINITY && m > ref)) {
+            if (ref > -INFINITY) sum *= exp((double)ref - (double)m);         // (else it is 0, or NaN)
+            ref = m;
+        }
+        const float use = ref == -INFINITY ? 0.f : ref;
+        float part = 0.f;
+        if constexpr (n == 1) {
+            part = ex2((x[0] - use) * LOG2E);
+        } else {
+            const F32x2 shift = f2_splat(-use), scale = f2_splat(LOG2E);
+            F32x2 acc = f2_splat(0.f);
+#pragma unroll
+            for (int e = 0; e < n; e += 2) {
+                float a, b;
+                f2_unpack(f2_mul(f2_add(f2_pack(x[e], x[e + 1]), shift), scale), a, b);
+                acc = f2_add(acc, f2_pack(ex2(a), ex2(b)));
+            }
+            float a, b;
+            f2_unpack(acc, a, b);
+            part = a + b;
+        }
+        sum += (double)part;
+    });
+    // (a NaN or +inf among the logits makes the sum a NaN, by which the row is left out)
+    float all = ref;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+    if (lane == 0) refs[warp] = all;
+    // each warp's largest 2 ceil(width / warps) of its threads' largest
+    const int per_warp = 2 * ((p.width + WARPS - 1) / WARPS);
+    float left = top;
+    for (int k = 0; k < per_warp; ++k) {
+        float m = left;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int who = __ffs(__ballot_sync(0xffffffffu, left == m)) - 1;
+        if (lane == 0) tops[warp * per_warp + k] = m;
+        if (lane == who) left = -INFINITY;
+    }
+    if (tid == 0) { count = 0; bound_s = -INFINITY; }
+    __syncthreads();
+    float block_ref = refs[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) block_ref = fmaxf(block_ref, refs[w]);
+    if (ref != block_ref && ref > -INFINITY) sum *= exp((double)ref - (double)block_ref);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+    // the width-th largest of what the warps gave: so many elements are as large at least
+    const int given = WARPS * per_warp;
+    if (tid < given) {
+        const float v = tops[tid];
+        int above = 0;
+        for (int k = 0; k < given; ++k) above += tops[k] > v || (tops[k] == v && k < tid);
+        if (above == p.width - 1) bound_s = v;
+    }
+    __syncthreads();
+    const float bound = bound_s;
+    if (tid == 0) {
+        double total = 0.0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) total += sums[w];
+        *result = Part{total, block_ref, 0, {0, 0, 0, 0}};
+    }
+    if (top >= bound && top > -INFINITY) {
+        s.template each<SCAN>([&](int t, const float* x, auto number) {
+            constexpr int n = decltype(number)::value;
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                if (x[e] >= bound && x[e] > -INFINITY) {
+                    const int at = atomicAdd(&count, 1);
+                    if (at < CAP) held[at] = Cand{x[e], t + e};
+                }
+            }
+        });
+    }
+    __syncthreads();
+    const int n = count;
+    if (n <= CAP) {
+        for (int i = tid; i < n; i += SCAN) {
+            const Cand c = held[i];
+            int rank = 0;
+            for (int k = 0; k < n; ++k) rank += before(held[k], c);
+            if (rank < p.width) list[rank] = c;
+        }
+        if (tid == 0) result->count = min(n, p.width);
+        return;
+    }
+    // Too many equals: one after the other, each the best behind the last one.
+    Cand last{INFINITY, -1};
+    int found = 0;
+    for (; found < p.width; ++found) {
+        Cand best{-INFINITY, INT_MAX};
+        s.template each<SCAN>([&](int t, const float* x, auto number) {
+            constexpr int n = decltype(number)::value;
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                const Cand c{x[e], t + e};
+                if (before(last, c) && before(c, best)) best = c;
+            }
+        });
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const Cand c{__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.token, o)};
+            if (before(c, best)) best = c;
+        }
+        __syncthreads();
+        if (lane == 0) round_best[warp] = best;
+        __syncthreads();
+        best = round_best[0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) if (before(round_best[w], best)) best = round_best[w];
+        if (!(best.x > -INFINITY)) break;
+        if (tid == 0) list[found] = best;
+        last = best;
+    }
+    if (tid == 0) result->count = found;
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Selection
+// ------------------------------------------------------------------------------------------------------
+struct Select {
+    double value[SURVIVORS];
+    int beam[SURVIVORS], token[SURVIVORS];
+    double lse[MAX_BEAMS], score[MAX_BEAMS];
+    double slack;                          // twice the largest error of a log-sum-exp
+    int counted;
+    unsigned close;                        // beams of which a pair is too close
+    double heads[MERGE];
+    int last;                              // list of the bound
+};
+
+// Of `lists` lists, best first, list l of beam l / per_beam: count_of(l) candidates at(l, k).  All threads of the block; `width` outputs of the group.
+// False: some order is not certain; sel.close has the beams.
+template <int THREADS, typename Count, typename At>
+__device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, int per_beam, Count&& count_of, At&& at) {
+    const int tid = threadIdx.x;
+    const double slack = sel.slack;
+    auto value = [&](int l, int k) {
+        const int b = l / per_beam;
+        const Cand c = at(l, k);
+        return c.token < 0 ? sel.score[b] : sel.score[b] + ((double)c.x - sel.lse[b]);
+    };
+    // The width-th best of the lists' first ones bounds the choice from below.  Of equal values those of the list before come first: a list
+    // of a lower beam, or of lower tokens.  With slack 0 no more than `width` lists are that good, so all that is chosen from fits.
+    __syncthreads();
+    if (tid == 0) { sel.counted = 0; sel.close = 0; sel.last = -1; }
+    for (int l = tid; l < lists; l += THREADS) sel.heads[l] = count_of(l) ? value(l, 0) : -INFINITY;
+    __syncthreads();
+    if (lists > p.width) {
+        for (int l = tid; l < lists; l += THREADS) {
+            const double v = sel.heads[l];
+            int above = 0;
+            for (int k = 0; k < lists; ++k) above += sel.heads[k] > v || (sel.heads[k] == v && k < l);
+            if (above == p.width - 1) sel.last = l;
+        }
+        __syncthreads();
+    }
+    const int bound_list = sel.last < 0 ? lists : sel.last;
+    const double bound = sel.last < 0 ? -INFINITY : sel.heads[sel.last] - slack;
+    for (int l = tid; l < lists; l += THREADS) {
+        const int n = count_of(l);
+        for (int k = 0; k < n; ++k) {
+            const double v = value(l, k);
+            if (!(v > bound || (v == bound && (slack > 0.0 || l < bound_list || (l == bound_list && k == 0))))) break;
+            const int i = atomicAdd(&sel.counted, 1);
+            if (i < SURVIVORS) { sel.value[i] = v; sel.beam[i] = l / per_beam; sel.token[i] = at(l, k).token; }
+        }
+    }
+    __syncthreads();
+    const int n = sel.counted;
+    if (n > SURVIVORS) {                   // many near one another
+        if (tid == 0) sel.close = 0xffffffffu;
+        __syncthreads();
+        return false;
+    }
+    const int outs = p.width;
+    for (int i = tid; i < n; i += THREADS) {
+        const double v = sel.value[i];
+        const int b = sel.beam[i], t = sel.token[i];
+        int rank = 0;
+        unsigned near = 0;
+        for (int k = 0; k < n; ++k) {
+            const double u = sel.value[k];
+            const int c = sel.beam[k];
+            rank += u > v || (u == v && (c < b || (c == b && sel.token[k] < t)));
+            if (c != b && fabs(u - v) <= slack) near |= 1u << c;
+        }
+        if (rank < outs) {
+            if (near && slack > 0.0) atomicOr(&sel.close, near | 1u << b);
+            const long long o = (long long)group * outs + rank;
+            p.parents[o] = b;
+            p.tokens[o] = t;
+            p.out[o] = (float)v;
+        }
+    }
+    for (int i = n + tid; i < outs; i += THREADS) {
+        const long long o = (long long)group * outs + i;
+        p.parents[o] = i % p.beams;
+        p.tokens[o] = -1;
+        p.out[o] = -INFINITY;
+    }
+    __syncthreads();
+    return sel.close == 0;
+}
+
+// The log-sum-exp of a row in 64 bits, whatever its place in memory: the whole block.
+template <int THREADS, typename T> __device__ double exact_lse(const CmeBeams& p, int row, double* scratch) {
+    const Slice<T> s(p, row, 0, p.vocab);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float m = -INFINITY;
+    for (int t = tid; t < p.vocab; t += THREADS) m = fmaxf(m, s.at(t));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    __syncthreads();
+    if (lane == 0) scratch[warp] = m;
+    __syncthreads();
+    double top = scratch[0];
+    for (int w = 1; w < THREADS / 32; ++w) top = fmax(top, scratch[w]);
+    double sum = 0.0;
+    for (int t = tid; t < p.vocab; t += THREADS) {
+        const double x = s.at(t);
+        if (x > -INFINITY) sum += exp(x - top);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) scratch[warp] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < THREADS / 32; ++w) sum += scratch[w];
+    return top + log(sum);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int slices) {
+    __shared__ Select sel;
+    __shared__ double scratch[MERGE / 32];
+    __shared__ double error[MAX_BEAMS];
+    __shared__ int counts[MERGE];
+    pdl_wait();
+    const int group = blockIdx.x, tid = threadIdx.x, lists = p.beams * slices;
+    const long long stride = sizeof(Part) + p.width * sizeof(Cand);
+    auto part_at = [&](int l) -> const Part* {
+        return reinterpret_cast<const Part*>(static_cast<const char*>(p.ws) + ((long long)group * p.beams * slices + l) * stride);
+    };
+    if (tid < p.beams) {
+        const long long row = (long long)group * p.beams + tid;
+        const float score = p.scores[row];
+        const bool over = p.finished && p.finished[row];
+        double ref = -INFINITY, sum = 0.0;
+        for (int k = 0; k < slices; ++k) {
+            const Part* part = part_at(tid * slices + k);
+            if (!(part->sum > 0.0 || part->sum != part->sum)) continue;       // nothing in it (a NaN goes on)
+            const double r = part->ref;
+            if (r > ref) { sum = sum == 0.0 ? 0.0 : sum * exp(ref - r); ref = r; }
+            sum += part->sum * exp(r - ref);
+        }
+        const double lse = ref + log(sum);
+        const bool fine = finite(score) && (over || (sum > 0.0 && fabs(lse) < INFINITY));
+        sel.score[tid] = fine ? (double)score : -INFINITY;
+        sel.lse[tid] = fine && !over ? lse : 0.0;
+        error[tid] = fine && !over ? 0x1p-21 + 2.5 * 0x1p-24 * (log((double)p.vocab) + RAISE) : 0.0;
+        for (int k = 0; k < slices; ++k) counts[tid * slices + k] = !fine ? 0 : over ? k == 0 : part_at(tid * slices + k)->count;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        double e = 0.0;
+        for (int b = 0; b < p.beams; ++b) e = fmax(e, error[b]);
+        sel.slack = 2.0 * e;
+    }
+    __syncthreads();
+    auto count_of = [&](int l) { return counts[l]; };
+    auto at = [&](int l, int k) {
+        const long long row = (long long)group * p.beams + l / slices;
+        return p.finished && p.finished[row] ? Cand{0.f, -1} : reinterpret_cast<const Cand*>(part_at(l) + 1)[k];
+    };
+    if (pick<MERGE>(sel, p, group, lists, slices, count_of, at)) return;
+    const unsigned close = sel.close;
+    for (int b = 0; b < p.beams; ++b) {
+        const long long row = (long long)group * p.beams + b;
+        if (!(close >> b & 1) || sel.score[b] == -INFINITY || (p.finished && p.finished[row])) continue;
+        const double lse = exact_lse<MERGE, T>(p, (int)row, scratch);
+        __syncthreads();
+        if (tid == 0) sel.lse[b] = lse;
+    }
+    if (tid == 0) sel.slack = 0.0;
+    __syncthreads();
+    pick<MERGE>(sel, p, group, lists, slices, count_of, at);
+}
+
+// Few tokens: a warp a row, in 64 bits.
+constexpr int SMALL = 256;
+template <typename T>
+__global__ void __launch_bounds__(SMALL) beam_small_kernel(const CmeBeams p) {
+    constexpr int WARPS = SMALL / 32, EACH = SMALL_VOCAB / 32;
+    __shared__ Select sel;
+    __shared__ Cand best[MAX_BEAMS][MAX_WIDTH];
+    __shared__ int counts[MAX_BEAMS];
+    pdl_release();
+    pdl_wait();
+    const int group = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) sel.slack = 0.0;
+    for (int b = warp; b < p.beams; b += WARPS) {
+        const long long row = (long long)group * p.beams + b;
+        const float score = p.scores[row];
+        const bool over = p.finished && p.finished[row];
+        const Slice<T> s(p, (int)row, 0, p.vocab);
+        float x[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) x[e] = e * 32 + lane < p.vocab ? s.at(e * 32 + lane) : -INFINITY;
+        float m = -INFINITY;
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) m = fmaxf(m, x[e]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll 1
+        for (int e = 0; e * 32 < p.vocab; ++e) {
+            const float v = e * 32 + lane < p.vocab ? s.at(e * 32 + lane) : -INFINITY;
+            if (v != -INFINITY) sum += exp((double)v - (double)m);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double lse = (double)m + log(sum);
+        const bool fine = finite(score) && (over || (sum > 0.0 && fabs(lse) < INFINITY));
+        int n = 0;
+        if (fine && over) {
+            n = 1;
+            if (lane == 0) best[b][0] = Cand{0.f, -1};
+        } else if (fine) {
+            for (; n < p.width; ++n) {
+                Cand c{-INFINITY, INT_MAX};
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) if (x[e] > c.x) c = Cand{x[e], e * 32 + lane};
+#pragma unroll
+                for (int o = 16; o; o >>= 1) {
+                    const Cand d{__shfl_xor_sync(0xffffffffu, c.x, o), __shfl_xor_sync(0xffffffffu, c.token, o)};
+                    if (before(d, c)) c = d;
+                }
+                if (c.x == -INFINITY) break;
+                if (lane == 0) best[b][n] = c;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) if (e * 32 + lane == c.token) x[e] = -INFINITY;
+            }
+        }
+        if (lane == 0) {
+            sel.score[b] = fine ? (double)score : -INFINITY;
+            sel.lse[b] = fine && !over ? lse : 0.0;
+            counts[b] = n;
+        }
+    }
+    __syncthreads();
+    pick<SMALL>(sel, p, group, p.beams, 1, [&](int l) { return counts[l]; }, [&](int l, int k) { return best[l][k]; });
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------------------
+int check(const CmeBeams* a) {
+    CME_REQUIRE(a->dtype == CME_F32 || a->dtype == CME_BF16, CME_ERR_UNSUPPORTED, "beam step: unsupported dtype");
+    CME_REQUIRE(a->groups >= 0 && a->vocab > 0, CME_ERR_SHAPE, "beam step: bad sizes");
+    CME_REQUIRE(a->beams > 0 && a->beams <= MAX_BEAMS && a->width > 0 && a->width <= MAX_WIDTH, CME_ERR_LIMIT,
+                "beam step: %d beams and a width of %d (1 to 32 of both)", a->beams, a->width);
+    CME_REQUIRE((long long)a->groups * a->beams * 256 < (1ll << 31), CME_ERR_LIMIT, "beam step: too many rows");
+    return CME_OK;
+}
+// Slices of a row.
+int slices_of(const CmeBeams* a, int sms) {
+    const long long rows = std::max(1ll, (long long)a->groups * a->beams);
+    const long long wanted = (sms * 8ll + rows - 1) / rows, fit = MERGE / a->beams, by_size = std::max(1, a->vocab / 2048);
+    return (int)std::max(1ll, std::min(std::min(wanted, by_size), std::min(fit, 32ll)));
+}
+template <typename T> int launch(const CmeBeams* a, int sms, cudaStream_t st) {
+    if (a->vocab <= SMALL_VOCAB) {
+        CME_CUDA(cme_launch_dependent(beam_small_kernel<T>, dim3(a->groups), dim3(SMALL), 0, st, *a));
+        CME_LAUNCH_CHECK();
+        return CME_OK;
+    }
+    const int slices = slices_of(a, sms), slice = cme_cdiv(cme_cdiv(a->vocab, slices), 8) * 8;
+    CME_CUDA(cme_launch_dependent(beam_scan_kernel<T>, dim3(a->groups * a->beams * slices), dim3(SCAN), 0, st, *a, slices, slice));
+    CME_LAUNCH_CHECK();
+    CME_CUDA(cme_launch_dependent(beam_merge_kernel<T>, dim3(a->groups), dim3(MERGE), 0, st, *a, slices));
+    CME_LAUNCH_CHECK();
+    return CME_OK;
+}
+
+}  // namespace
+
+// Scratch of a call, in bytes.
+CME_API int cme_beam_step_ws_bytes(const CmeBeams* a, long long* out) {
+    int rc, sms;
+    if ((rc = check(a)) || (rc = cme_num_sms(&sms))) return rc;
+    *out = a->vocab <= SMALL_VOCAB ? 0 : (long long)a->groups * a->beams * slices_of(a, sms) * (long long)(sizeof(Part) + a->width * sizeof(Cand));
+    return CME_OK;
+}
+
+CME_API int cme_beam_step(const CmeBeams* a, void* stream) {
+    int sms;
+    long long need;
+    int rc = cme_beam_step_ws_bytes(a, &need);
+    if (rc || (rc = cme_num_sms(&sms))) return rc;
+    if (a->groups == 0) return CME_OK;
+    CME_REQUIRE(need <= a->ws_bytes && (reinterpret_cast<uintptr_t>(a->ws) & 15) == 0, CME_ERR_SHAPE, "beam step: %lld bytes of scratch, %lld are needed",
+                a->ws_bytes, need);
+    return a->dtype == CME_F32 ? launch<float>(a, sms, (cudaStream_t)stream) : launch<__nv_bfloat16>(a, sms, (cudaStream_t)stream);
+}

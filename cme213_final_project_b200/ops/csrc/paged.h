@@ -21,16 +21,22 @@ enum PagedKernel : int {
 };
 
 int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long long page_stride, long long head_stride,
-                   long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle);
+                   long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle, bool q8 = false);
 // Q as (column, head, token, -): a box of `group` heads and `tokens` tokens, so that its rows lie token by token.
 int paged_make_q_map(CUtensorMap* out, const CmePaged* a, int group, int tokens);
 int paged_attention_mma(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
+int paged_attention8_mma(const CmePaged* a, const CmePagedScales* scales, const PagedPlan& plan, cudaStream_t st);
 int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
 int paged_join(const CmePaged* a, int splits, cudaStream_t st);      // the parts in a->ws to a->o and a->lse
 // Keys of the tiles that the kernels walk in.
-int paged_mma_key_tile(int dtype, int head_dim);
-int paged_mma_ctas(int dtype, int head_dim);               // of the kernels for up to 16 rows, on an SM
+int paged_mma_key_tile(int dtype, int head_dim, bool q8);
+int paged_mma_ctas(int dtype, int head_dim, bool q8);      // of the kernels for up to 16 rows, on an SM
 constexpr int PAGED_TC_KEYS = 64;
+
+// The smallest scale of 8-bit integers: where less would be needed (numbers below 2^-93), a block is all zeros, its scale too.
+constexpr float PAGED_SMALLEST_SCALE = 0x1p-100f;
+// Checks of the cache's side of a call (scales: null for a cache of the rows' type).
+int paged_check_cache(const CmePaged* a, const CmePagedScales* scales, const char* what);
 
 // Division by a number that the host knows, for 0 <= x < 2^31: x / d = (x * m) >> s with m = ceil(2^s / d) and s = 31 + ceil(log2 d)
 // (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994).

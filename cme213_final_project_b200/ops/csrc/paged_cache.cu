@@ -71,23 +71,31 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) paged_append_kernel(const C
 // ------------------------------------------------------------------------------------------------------
 // Checks, and the choice of a kernel
 // ------------------------------------------------------------------------------------------------------
-int check_cache(const CmePaged* a, const char* what) {
+}  // namespace
+
+int paged_check_cache(const CmePaged* a, const CmePagedScales* scales, const char* what) {
     CME_REQUIRE(a->dtype == CME_F32 || a->dtype == CME_BF16, CME_ERR_UNSUPPORTED, "%s: unsupported dtype", what);
     CME_REQUIRE(a->head_dim == 32 || a->head_dim == 64 || a->head_dim == 128, CME_ERR_SHAPE, "%s: head size %d is not 32, 64 or 128",
                 what, a->head_dim);
     CME_REQUIRE(a->page >= 8 && a->page % 8 == 0, CME_ERR_SHAPE, "%s: pages of %d slots (a multiple of 8 is needed)", what, a->page);
     CME_REQUIRE(a->seqs >= 0 && a->rows >= 0 && a->kv_heads > 0 && a->kv_heads <= 65535 && a->width >= 0 && a->num_pages >= 0 &&
                 a->max_len >= 0, CME_ERR_SHAPE, "%s: bad sizes", what);
-    const int per16 = a->dtype == CME_F32 ? 4 : 8;
-    auto ok = [&](const void* p, long long s0, long long s1, long long s2) {
-        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % per16 == 0 && s1 % per16 == 0 && s2 % per16 == 0;
+    if (scales)
+        CME_REQUIRE(scales->block >= 8 && scales->block % 8 == 0 && a->page % scales->block == 0, CME_ERR_SHAPE,
+                    "%s: scales of %d slots (a multiple of 8 that divides a page is needed)", what, scales->block);
+    const int per16 = a->dtype == CME_F32 ? 4 : 8, cached = scales ? 16 : per16;
+    auto ok = [&](int n, const void* p, long long s0, long long s1, long long s2) {
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s0 % n == 0 && s1 % n == 0 && s2 % n == 0;
     };
-    CME_REQUIRE(ok(a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride) && ok(a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride),
+    CME_REQUIRE(ok(cached, a->k, a->k_page_stride, a->k_head_stride, a->k_slot_stride) &&
+                ok(cached, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride),
                 CME_ERR_SHAPE, "%s: the cache has to start, and its strides have to be, at multiples of 16 bytes", what);
-    CME_REQUIRE(ok(a->q, a->q_token, a->q_head, 0) && ok(a->nv, a->v_token, a->v_head, 0), CME_ERR_SHAPE,
+    CME_REQUIRE(ok(per16, a->q, a->q_token, a->q_head, 0) && ok(per16, a->nv, a->v_token, a->v_head, 0), CME_ERR_SHAPE,
                 "%s: new rows have to start, and their strides have to be, at multiples of 16 bytes", what);
     return CME_OK;
 }
+
+namespace {
 
 constexpr int MAX_SPLITS = 128;
 
@@ -102,12 +110,17 @@ struct Form {
     int slots;               // CTAs that run at a time
     float tile_us;
 };
-Form form_of(const CmePaged* a, int backend, int sms) {
+Form form_of(const CmePaged* a, bool q8, int backend, int sms) {
     const bool f32 = a->dtype == CME_F32;
     const int d = a->head_dim;
+    if (q8) {
+        const int keys = paged_mma_key_tile(a->dtype, d, true);
+        if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d, true), d == 128 ? 1.6f : d == 64 ? 1.2f : 1.0f};
+        return {keys, sms * 2, d == 128 ? 5.0f : d == 64 ? 3.2f : 2.4f};
+    }
     if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 3), d == 128 ? 1.0f : 1.15f};
-    const int keys = paged_mma_key_tile(a->dtype, d);
-    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 64 ? 1.4f : 1.2f};
+    const int keys = paged_mma_key_tile(a->dtype, d, false);
+    if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d, false), f32 ? (d == 128 ? 2.8f : d == 64 ? 2.0f : 1.4f) : d == 64 ? 1.4f : 1.2f};
     return {keys, sms * (d == 32 ? (f32 ? 2 : 3) : 1), f32 ? (d == 128 ? 6.0f : d == 64 ? 3.0f : 4.5f) : d == 128 ? 2.6f : 1.8f};
 }
 float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles, int parts) {
@@ -119,10 +132,10 @@ float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles,
 
 // backend: 0 by the rule, 1 up to 16 rows a tile, 2 rows, 3 tc.  splits: 0 by the rule; up to 16 rows: a cluster of so many CTAs (1, 2, 4
 // or 8), negative: the stream; others: parts of the keys.
-int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* plan) {
+int make_plan(const CmePaged* a, bool q8, int backend, int splits, int sms, PagedPlan* plan) {
     const int group = a->heads / a->kv_heads;
     const long long rows = (long long)a->rows * group;     // of one key head
-    const bool tc = a->dtype == CME_BF16 && group <= 128;
+    const bool tc = a->dtype == CME_BF16 && group <= 128 && !q8;
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
     CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
                 "paged attention: the tcgen05 kernel takes bf16 and up to 128 query heads per key head");
@@ -132,7 +145,7 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
     const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
     auto key_tiles_of = [&](const Form& f) { return std::max(1, cme_cdiv(longest, f.keys)); };
     auto best_parts = [&](int b, float* us) {              // of rows and tc
-        const Form f = form_of(a, b, sms);
+        const Form f = form_of(a, q8, b, sms);
         const int n = key_tiles_of(f);
         int best = 1;
         *us = estimate(a, f, even_tiles(b), n, 1);
@@ -145,7 +158,7 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
     // Up to 16 rows a tile: as many CTAs of a cluster as let all run at once; the stream from where a CTA would have more than eight key
     // tiles in its turns (head size 64, lengths from half of the longest on, us, cluster / stream: 96 items of up to 1024 keys 8.5 /
     // 10.1, of 4096 21.9 / 20.5; 384 items of 256 9.9 / 11.2, of 1024 23.0 / 21.4.  128: 32 items of 4096 14.1 / 17.7, 8 of 16384 33.6 / 21.8).
-    const Form one = form_of(a, 1, sms);
+    const Form one = form_of(a, q8, 1, sms);
     const int one_keys = key_tiles_of(one);
     auto cluster_of = [&](long long items, int* c) {       // the cluster's size, and the key tiles of a CTA's turns
         for (*c = 1; *c < 8 && *c < one_keys && items * *c * 2 <= one.slots;) *c *= 2;
@@ -172,7 +185,7 @@ int make_plan(const CmePaged* a, int backend, int splits, int sms, PagedPlan* pl
             if (us < few) backend = many;
         }
     }
-    const Form f = form_of(a, backend, sms);
+    const Form f = form_of(a, q8, backend, sms);
     const long long tiles = tiles_of(backend), ctas = tiles * a->kv_heads;
     const int key_tiles = key_tiles_of(f);
     plan->row_tile = row_tile(backend);
@@ -208,8 +221,8 @@ long long ws_bytes(const CmePaged* a, const PagedPlan& p) {
     return ((parts * 2 + 3) / 4 * 4 + parts * a->head_dim + (p.kernel == PAGED_STREAM ? p.splits * 8ll : 0)) * 4;
 }
 
-int check_attention(const CmePaged* a) {
-    const int rc = check_cache(a, "paged attention");
+int check_attention(const CmePaged* a, const CmePagedScales* scales) {
+    const int rc = paged_check_cache(a, scales, "paged attention");
     if (rc) return rc;
     CME_REQUIRE(a->heads > 0 && a->heads % a->kv_heads == 0, CME_ERR_SHAPE, "paged attention: %d heads do not share %d key heads evenly",
                 a->heads, a->kv_heads);
@@ -237,17 +250,17 @@ EncodeTiledFn encoder() {
 
 // Map over (column, slot, head, page) with box (box_cols, box_rows, 1, 1).  Page num_pages lies behind it: such a box is filled with zeros.
 int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long long page_stride, long long head_stride,
-                   long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
+                   long long slot_stride, int box_cols, int box_rows, CUtensorMapSwizzle swizzle, bool q8) {
     EncodeTiledFn enc = encoder();
     CME_REQUIRE(enc != nullptr, CME_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const long long e = a->dtype == CME_F32 ? 4 : 2;
+    const long long e = q8 ? 1 : a->dtype == CME_F32 ? 4 : 2;
     cuuint64_t dims[4] = {(cuuint64_t)a->head_dim, (cuuint64_t)a->page, (cuuint64_t)a->kv_heads, (cuuint64_t)std::max(1, a->num_pages)};
     // the stride along a dimension of one entry leads nowhere
     cuuint64_t strides[3] = {(cuuint64_t)(slot_stride * e), (cuuint64_t)((a->kv_heads > 1 ? head_stride : a->head_dim) * e),
                              (cuuint64_t)((a->num_pages > 1 ? page_stride : a->head_dim) * e)};
     cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
-    CUresult r = enc(out, a->dtype == CME_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+    CUresult r = enc(out, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : a->dtype == CME_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                      const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     CME_REQUIRE(r == CUDA_SUCCESS, CME_ERR_CUDA, "paged cache: cuTensorMapEncodeTiled failed (%d): strides %lld %lld %lld", (int)r,
@@ -271,7 +284,7 @@ int paged_make_q_map(CUtensorMap* out, const CmePaged* a, int group, int tokens)
 }
 
 CME_API int cme_paged_append(const CmePaged* a, void* stream) {
-    const int rc = check_cache(a, "cache append");
+    const int rc = paged_check_cache(a, nullptr, "cache append");
     if (rc) return rc;
     if (a->rows == 0 || a->seqs == 0 || a->num_pages == 0 || a->width == 0) return CME_OK;
     const int elem = a->dtype == CME_F32 ? 4 : 2;
@@ -285,28 +298,26 @@ CME_API int cme_paged_append(const CmePaged* a, void* stream) {
     return CME_OK;
 }
 
-// What a call will take: {kernel, row tile, row tiles, parts, keys of a part}.
-CME_API int cme_paged_attention_plan(const CmePaged* a, int backend, int splits, int sms, int* out) {
+namespace {
+
+int plan_of(const CmePaged* a, const CmePagedScales* scales, int backend, int splits, int sms, int* out) {
     PagedPlan p{};
-    int rc = check_attention(a);
-    if (rc || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
+    int rc = check_attention(a, scales);
+    if (rc || (rc = make_plan(a, scales != nullptr, backend, splits, sms, &p))) return rc;
     out[0] = p.kernel; out[1] = p.row_tile; out[2] = p.tiles; out[3] = p.splits; out[4] = p.split_keys;
     return CME_OK;
 }
-
-// Scratch of a call, in bytes.
-CME_API int cme_paged_attention_ws_bytes(const CmePaged* a, int backend, int splits, long long* out) {
+int scratch_of(const CmePaged* a, const CmePagedScales* scales, int backend, int splits, long long* out) {
     PagedPlan p{};
     int rc, sms;
-    if ((rc = check_attention(a)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
+    if ((rc = check_attention(a, scales)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, scales != nullptr, backend, splits, sms, &p))) return rc;
     *out = ws_bytes(a, p);
     return CME_OK;
 }
-
-CME_API int cme_paged_attention(const CmePaged* a, int backend, int splits, void* stream) {
+int attend(const CmePaged* a, const CmePagedScales* scales, int backend, int splits, cudaStream_t st) {
     PagedPlan p{};
     int rc, sms;
-    if ((rc = check_attention(a)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, backend, splits, sms, &p))) return rc;
+    if ((rc = check_attention(a, scales)) || (rc = cme_num_sms(&sms)) || (rc = make_plan(a, scales != nullptr, backend, splits, sms, &p))) return rc;
     if (a->rows == 0 || a->seqs == 0) return CME_OK;
     CmePaged held = *a;
     held.max_len = (int)std::min((long long)a->max_len, (long long)a->width * a->page);
@@ -317,7 +328,33 @@ CME_API int cme_paged_attention(const CmePaged* a, int backend, int splits, void
     a = &held;
     CME_REQUIRE(ws_bytes(a, p) <= a->ws_bytes, CME_ERR_SHAPE, "paged attention: %lld bytes of scratch, %lld are needed", a->ws_bytes,
                 ws_bytes(a, p));
-    cudaStream_t st = (cudaStream_t)stream;
-    if ((rc = p.kernel == PAGED_TC ? paged_attention_tc(a, p, st) : paged_attention_mma(a, p, st))) return rc;
+    rc = scales ? paged_attention8_mma(a, scales, p, st) : p.kernel == PAGED_TC ? paged_attention_tc(a, p, st) : paged_attention_mma(a, p, st);
+    if (rc) return rc;
     return p.splits > 1 && p.kernel >= PAGED_ROWS ? paged_join(a, p.splits, st) : CME_OK;
+}
+
+}  // namespace
+
+// What a call will take: {kernel, row tile, row tiles, parts, keys of a part}.
+CME_API int cme_paged_attention_plan(const CmePaged* a, int backend, int splits, int sms, int* out) {
+    return plan_of(a, nullptr, backend, splits, sms, out);
+}
+CME_API int cme_paged_attention8_plan(const CmePaged* a, const CmePagedScales* scales, int backend, int splits, int sms, int* out) {
+    return plan_of(a, scales, backend, splits, sms, out);
+}
+
+// Scratch of a call, in bytes.
+CME_API int cme_paged_attention_ws_bytes(const CmePaged* a, int backend, int splits, long long* out) {
+    return scratch_of(a, nullptr, backend, splits, out);
+}
+CME_API int cme_paged_attention8_ws_bytes(const CmePaged* a, const CmePagedScales* scales, int backend, int splits, long long* out) {
+    return scratch_of(a, scales, backend, splits, out);
+}
+
+CME_API int cme_paged_attention(const CmePaged* a, int backend, int splits, void* stream) {
+    return attend(a, nullptr, backend, splits, (cudaStream_t)stream);
+}
+// Over a cache of 8-bit integers.
+CME_API int cme_paged_attention8(const CmePaged* a, const CmePagedScales* scales, int backend, int splits, void* stream) {
+    return attend(a, scales, backend, splits, (cudaStream_t)stream);
 }

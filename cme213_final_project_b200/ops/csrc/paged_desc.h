@@ -24,3 +24,11 @@ struct CmePaged {
     void* o; float* lse;                 // [rows, heads, head_dim] and [rows, heads]
     float* ws; long long ws_bytes;       // scratch of cme_paged_attention_ws_bytes() bytes
 };
+
+// Scales of a cache of 8-bit integers (whose CmePaged has the type of the new rows, and strides of the cache in bytes): slot s of a page and
+// head stands for its integers times [page, head, s / block].
+struct CmePagedScales {
+    float* k; float* v;
+    int block;                           // slots of a scale: a multiple of 8 that divides a page
+    long long k_page, k_head, v_page, v_head;    // strides, in elements
+};

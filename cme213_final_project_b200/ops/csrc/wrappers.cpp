@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "attention_desc.h"
+#include "beam_desc.h"
 #include "gemm_desc.h"
 #include "paged_desc.h"
 #include "token_desc.h"
@@ -56,6 +57,12 @@ struct Native {
     int (*cme_paged_attention_ws_bytes)(const CmePaged*, int, int, long long*);
     int (*cme_paged_attention)(const CmePaged*, int, int, void*);
     int (*cme_next_token)(const CmeToken*, void*);
+    int (*cme_paged_append8)(const CmePaged*, const CmePagedScales*, void*);
+    int (*cme_paged_attention8_ws_bytes)(const CmePaged*, const CmePagedScales*, int, int, long long*);
+    int (*cme_paged_attention8)(const CmePaged*, const CmePagedScales*, int, int, void*);
+    int (*cme_beam_step_ws_bytes)(const CmeBeams*, long long*);
+    int (*cme_beam_step)(const CmeBeams*, void*);
+    int (*cme_cache_reorder)(const CmeReorder*, void*);
 } lib;
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -419,15 +426,19 @@ void has_size(const at::Tensor& t, int dim, long long n, const char* what) {
 }
 
 // a: cache_k, cache_v, pages, offsets, lengths; x: new rows [rows, heads, head_dim] of the cache's type
-CmePaged paged(int device, const at::Tensor& x, PyObject* const* a) {
+CmePaged paged(int device, const at::Tensor& x, PyObject* const* a, bool q8 = false) {
     const at::Tensor k = strided(device, a[0], "cache_k", 4), v = strided(device, a[1], "cache_v", 4);
     const at::Tensor pages = whole_numbers(device, a[2], "pages", 2), offsets = whole_numbers(device, a[3], "offsets", 1),
                      lengths = whole_numbers(device, a[4], "lengths", 1);
     CmePaged d;
     std::memset(&d, 0, sizeof d);
     d.dtype = dtype(x);
-    if (k.scalar_type() != x.scalar_type() || v.scalar_type() != x.scalar_type())
-        fail(native_error, "the cache has to have the type of the new rows");
+    if (q8) {
+        same_type(k, at::kChar, "cache_k", "int8 (it has scales)");
+        same_type(v, at::kChar, "cache_v", "int8 (it has scales)");
+    } else if (k.scalar_type() != x.scalar_type() || v.scalar_type() != x.scalar_type()) {
+        fail(native_error, k.scalar_type() == at::kChar ? "an int8 cache needs its scales" : "the cache has to have the type of the new rows");
+    }
     for (int i = 0; i < 4; ++i) has_size(v, i, k.size(i), "cache_v");
     d.seqs = int32(pages.size(0)); d.width = int32(pages.size(1));
     has_size(offsets, 0, (long long)d.seqs + 1, "offsets");
@@ -483,6 +494,172 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t) {
     }
     run([&](void* st) { return lib.cme_paged_attention(&d, backend, splits, st); });
     return pack(out, lse);
+    END_HANDLE_TH_ERRORS
+}
+
+// k_scales, v_scales of the cache of d
+CmePagedScales paged_scales(int device, const CmePaged& d, PyObject* const* a) {
+    if (a[0] == Py_None || a[1] == Py_None) fail(native_error, "k_scales and v_scales belong together");
+    const at::Tensor k = strided(device, a[0], "k_scales", 3), v = strided(device, a[1], "v_scales", 3);
+    same_type(k, at::kFloat, "k_scales", "fp32");
+    same_type(v, at::kFloat, "v_scales", "fp32");
+    CmePagedScales s;
+    std::memset(&s, 0, sizeof s);
+    for (const at::Tensor* t : {&k, &v}) {
+        has_size(*t, 0, d.num_pages, "the scales");
+        has_size(*t, 1, d.kv_heads, "the scales");
+    }
+    has_size(v, 2, k.size(2), "v_scales");
+    if (k.size(2) < 1 || d.page % k.size(2)) fail(native_error, "the scales of a page have to stand for equal numbers of its slots");
+    s.block = int32(d.page / k.size(2));
+    s.k = (float*)ptr(k); s.k_page = k.stride(0); s.k_head = k.stride(1);
+    s.v = (float*)ptr(v); s.v_page = v.stride(0); s.v_head = v.stride(1);
+    return s;
+}
+
+// (k, v, cache_k, cache_v, pages, offsets, lengths, k_scales, v_scales)
+PyObject* cache_append8(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const int device = c10::cuda::current_device();
+    const at::Tensor k = strided(device, a[0], "k", 3), v = strided(device, a[1], "v", 3);
+    CmePaged d = paged(device, k, a + 2, true);
+    if (v.scalar_type() != k.scalar_type()) fail(native_error, "v has to have the type of k");
+    for (int i = 0; i < 3; ++i) has_size(v, i, k.size(i), "v");
+    has_size(k, 1, d.kv_heads, "k");
+    d.heads = d.kv_heads;
+    d.nv = ptr(v); d.v_token = v.stride(0); d.v_head = v.stride(1);
+    const CmePagedScales s = paged_scales(device, d, a + 7);
+    run([&](void* st) { return lib.cme_paged_append8(&d, &s, st); });
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, cache_k, cache_v, pages, offsets, lengths, scale | None, max_len | None, backend, splits, k_scales, v_scales)
+PyObject* paged_attention8(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const int device = c10::cuda::current_device();
+    const at::Tensor q = strided(device, a[0], "q", 3);
+    CmePaged d = paged(device, q, a + 1, true);
+    const CmePagedScales s = paged_scales(device, d, a + 10);
+    d.heads = int32(q.size(1));
+    d.scale = a[6] == Py_None ? (float)(1.0 / std::sqrt((double)d.head_dim)) : real(a[6]);
+    if (a[7] != Py_None) d.max_len = int32(whole(a[7]));
+    const int backend = int32(whole(a[8])), splits = int32(whole(a[9]));
+    at::Tensor out, lse;
+    fresh_pair(out, q.sizes(), q.scalar_type(), lse, {d.rows, d.heads}, at::kFloat, q);
+    d.o = ptr(out);
+    d.lse = (float*)ptr(lse);
+    check(lib.cme_paged_attention8_ws_bytes(&d, &s, backend, splits, &d.ws_bytes));
+    at::Tensor ws;
+    if (d.ws_bytes) {
+        ws = fresh({(d.ws_bytes + 3) / 4}, at::kFloat, q);
+        d.ws = (float*)ptr(ws);
+    }
+    run([&](void* st) { return lib.cme_paged_attention8(&d, &s, backend, splits, st); });
+    return pack(out, lse);
+    END_HANDLE_TH_ERRORS
+}
+
+// (logits, scores, width | None, finished | None, allowed | None)
+PyObject* beam_step(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const int device = c10::cuda::current_device();
+    const at::Tensor logits = strided(device, a[0], "logits", 2), scores = strided(device, a[1], "scores", 2);
+    CmeBeams d;
+    std::memset(&d, 0, sizeof d);
+    d.dtype = dtype(logits);
+    same_type(scores, at::kFloat, "scores", "fp32");
+    if (!scores.is_contiguous()) fail(native_error, "scores have to be contiguous");
+    d.groups = int32(scores.size(0)); d.beams = int32(scores.size(1)); d.vocab = int32(logits.size(1));
+    has_size(logits, 0, (long long)d.groups * d.beams, "logits");
+    d.logits = ptr(logits); d.logits_ld = logits.stride(0);
+    if (logits.size(0) > 1 && d.logits_ld < d.vocab) fail(native_error, "the rows of logits may not overlap");
+    d.scores = (const float*)ptr(scores);
+    d.width = a[2] == Py_None ? d.beams : int32(whole(a[2]));
+    if (const at::Tensor f = strided(device, a[3], "finished", 2, true); f.defined()) {
+        same_type(f, at::kBool, "finished", "bool");
+        has_size(f, 0, d.groups, "finished");
+        has_size(f, 1, d.beams, "finished");
+        if (!f.is_contiguous()) fail(native_error, "finished has to be contiguous");
+        d.finished = (const unsigned char*)ptr(f);
+    }
+    if (const at::Tensor m = whole_numbers(device, a[4], "allowed", 2, true); m.defined()) {
+        if (m.size(0) != 1) has_size(m, 0, logits.size(0), "allowed");
+        has_size(m, 1, ((long long)d.vocab + 31) / 32, "allowed");
+        d.allowed = (const int*)ptr(m); d.allowed_ld = m.size(0) == 1 ? 0 : m.stride(0);
+    }
+    check(lib.cme_beam_step_ws_bytes(&d, &d.ws_bytes));
+    // the three results in one piece of memory
+    const long long n = (long long)d.groups * d.width;
+    at::Tensor all = fresh({3, d.groups, d.width}, at::kInt, logits), ws;
+    d.parents = (int*)ptr(all); d.tokens = d.parents + n; d.out = (float*)(d.tokens + n);
+    if (d.ws_bytes) {
+        ws = fresh({(d.ws_bytes + 3) / 4}, at::kFloat, logits);
+        d.ws = ptr(ws);
+    }
+    run([&](void* st) { return lib.cme_beam_step(&d, st); });
+    auto part = [&](int i, at::ScalarType type) {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset(i * n);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous({d.groups, d.width});
+        return t;
+    };
+    return pack(part(0, at::kInt), part(1, at::kInt), part(2, at::kFloat));
+    END_HANDLE_TH_ERRORS
+}
+
+// (cache_k, cache_v, pages, spare, parents, lengths, k_scales | None, v_scales | None)
+PyObject* cache_reorder(PyObject*, PyObject* const* a, Py_ssize_t) {
+    HANDLE_TH_ERRORS
+    const int device = c10::cuda::current_device();
+    const at::Tensor pages = whole_numbers(device, a[2], "pages", 2), spare = whole_numbers(device, a[3], "spare", 1),
+                     parents = whole_numbers(device, a[4], "parents", 2), lengths = whole_numbers(device, a[5], "lengths", 1);
+    CmeReorder d;
+    std::memset(&d, 0, sizeof d);
+    d.groups = int32(parents.size(0)); d.beams = int32(parents.size(1)); d.width = int32(pages.size(1));
+    const long long seqs = (long long)d.groups * d.beams;
+    has_size(pages, 0, seqs, "pages");
+    has_size(spare, 0, seqs, "spare");
+    has_size(lengths, 0, d.groups, "lengths");
+    if (!parents.is_contiguous()) fail(native_error, "parents have to be contiguous");
+    if ((a[6] == Py_None) != (a[7] == Py_None)) fail(native_error, "k_scales and v_scales belong together");
+    const char* names[4] = {"cache_k", "cache_v", "k_scales", "v_scales"};
+    for (int i = 0; i < 4; ++i) {
+        PyObject* o = i < 2 ? a[i] : a[i + 4];
+        const at::Tensor t = strided(device, o, names[i], i < 2 ? 5 : 4, i >= 2);
+        if (!t.defined()) break;
+        const bool q8 = a[6] != Py_None;
+        if (i >= 2) same_type(t, at::kFloat, names[i], "fp32");
+        else if (q8) same_type(t, at::kChar, names[i], "int8 (it has scales)");
+        else if (t.scalar_type() == at::kChar) fail(native_error, "an int8 cache needs its scales");
+        else dtype(t);
+        const long long e = t.element_size();
+        if (i == 0) {
+            d.layers = int32(t.size(0)); d.num_pages = int32(t.size(1)); d.slots = int32(t.size(3));
+            if (t.size(2) < 1 || d.slots < 1 || t.size(4) < 1) fail(native_error, "the cache has to have heads, slots and columns");
+        } else {
+            has_size(t, 0, d.layers, names[i]);
+            has_size(t, 1, d.num_pages, names[i]);
+            has_size(t, 2, d.t[0].heads, names[i]);
+            if (i == 1) { has_size(t, 3, d.slots, names[i]); has_size(t, 4, d.t[0].row_bytes / e, names[i]); }
+            else if (t.size(3) < 1 || d.slots % t.size(3)) fail(native_error, "the scales of a page have to stand for equal numbers of its slots");
+        }
+        CmePages& p = d.t[d.tensors++];
+        p.base = (char*)ptr(t);
+        p.heads = int32(t.size(2));
+        p.layer = t.stride(0) * e; p.page = t.stride(1) * e; p.head = t.stride(2) * e;
+        p.row = (i < 2 ? t.stride(3) : 1) * e;
+        p.row_bytes = int32(i < 2 ? t.size(4) * e : e);
+        p.per = i < 2 ? 1 : int32(d.slots / t.size(3));
+    }
+    d.pages = (const int*)ptr(pages); d.pages_ld = pages.stride(0);
+    if (spare.numel() > 1 && spare.stride(0) != 1) fail(native_error, "spare has to be contiguous");
+    d.spare = (const int*)ptr(spare); d.parents = (const int*)ptr(parents); d.lengths = (const int*)ptr(lengths);
+    at::Tensor new_pages, new_spare;
+    fresh_pair(new_pages, {seqs, d.width}, at::kInt, new_spare, {seqs}, at::kInt, pages);
+    d.new_pages = (int*)ptr(new_pages); d.new_spare = (int*)ptr(new_spare);
+    run([&](void* st) { return lib.cme_cache_reorder(&d, st); });
+    return pack(new_pages, new_spare);
     END_HANDLE_TH_ERRORS
 }
 
@@ -674,6 +851,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     GET(cme_attention_gemm_ws_bytes); GET(cme_layernorm_fwd); GET(cme_layernorm_bwd_blocks); GET(cme_layernorm_bwd);
     GET(cme_bias_act_residual); GET(cme_colsum_splits); GET(cme_dact_colsum); GET(cme_embedding_fwd); GET(cme_embedding_bwd);
     GET(cme_paged_append); GET(cme_paged_attention_ws_bytes); GET(cme_paged_attention); GET(cme_next_token);
+    GET(cme_paged_append8); GET(cme_paged_attention8_ws_bytes); GET(cme_paged_attention8);
+    GET(cme_beam_step_ws_bytes); GET(cme_beam_step); GET(cme_cache_reorder);
 #undef GET
     lib = next;
     Py_XSETREF(native_error, Py_NewRef(a[0]));
@@ -690,7 +869,8 @@ PyObject* counted(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 }
 PyMethodDef methods[] = {METHOD(bind, 2), METHOD(init, 1), METHOD(gemm_prepare, 19), METHOD(cross_entropy, 5), METHOD(attention_fwd, 9), METHOD(attention_bwd, 15),
                          METHOD(layernorm_fwd, 6), METHOD(layernorm_bwd, 9), METHOD(bias_act_residual, 5), METHOD(dact_colsum, 6),
-                         METHOD(embedding_fwd, 3), METHOD(embedding_bwd, 7), METHOD(cache_append, 7), METHOD(paged_attention, 10), METHOD(next_token, 13), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(embedding_fwd, 3), METHOD(embedding_bwd, 7), METHOD(cache_append, 7), METHOD(paged_attention, 10), METHOD(next_token, 13),
+                         METHOD(cache_append8, 9), METHOD(paged_attention8, 12), METHOD(beam_step, 5), METHOD(cache_reorder, 8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_wrappers", nullptr, -1, methods};
 
 }  // namespace
