@@ -26,6 +26,7 @@ int paged_make_map(CUtensorMap* out, const CmePaged* a, const void* base, long l
 int paged_make_q_map(CUtensorMap* out, const CmePaged* a, int group, int tokens);
 int paged_attention_mma(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
 int paged_attention8_mma(const CmePaged* a, const CmePagedScales* scales, const PagedPlan& plan, cudaStream_t st);
+int paged_attention8_tc(const CmePaged* a, const CmePagedScales* scales, const PagedPlan& plan, cudaStream_t st);
 int paged_attention_tc(const CmePaged* a, const PagedPlan& plan, cudaStream_t st);
 int paged_join(const CmePaged* a, int splits, cudaStream_t st);      // the parts in a->ws to a->o and a->lse
 // Keys of the tiles that the kernels walk in.

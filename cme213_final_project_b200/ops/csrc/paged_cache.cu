@@ -115,6 +115,7 @@ Form form_of(const CmePaged* a, bool q8, int backend, int sms) {
     const int d = a->head_dim;
     if (q8) {
         const int keys = paged_mma_key_tile(a->dtype, d, true);
+        if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 2), d == 128 ? 1.1f : 1.2f};
         if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d, true), d == 128 ? 1.6f : d == 64 ? 1.2f : 1.0f};
         return {keys, sms * 2, d == 128 ? 5.0f : d == 64 ? 3.2f : 2.4f};
     }
@@ -135,7 +136,7 @@ float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles,
 int make_plan(const CmePaged* a, bool q8, int backend, int splits, int sms, PagedPlan* plan) {
     const int group = a->heads / a->kv_heads;
     const long long rows = (long long)a->rows * group;     // of one key head
-    const bool tc = a->dtype == CME_BF16 && group <= 128 && !q8;
+    const bool tc = a->dtype == CME_BF16 && group <= 128;
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
     CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
                 "paged attention: the tcgen05 kernel takes bf16 and up to 128 query heads per key head");
@@ -328,7 +329,8 @@ int attend(const CmePaged* a, const CmePagedScales* scales, int backend, int spl
     a = &held;
     CME_REQUIRE(ws_bytes(a, p) <= a->ws_bytes, CME_ERR_SHAPE, "paged attention: %lld bytes of scratch, %lld are needed", a->ws_bytes,
                 ws_bytes(a, p));
-    rc = scales ? paged_attention8_mma(a, scales, p, st) : p.kernel == PAGED_TC ? paged_attention_tc(a, p, st) : paged_attention_mma(a, p, st);
+    if (scales) rc = p.kernel == PAGED_TC ? paged_attention8_tc(a, scales, p, st) : paged_attention8_mma(a, scales, p, st);
+    else rc = p.kernel == PAGED_TC ? paged_attention_tc(a, p, st) : paged_attention_mma(a, p, st);
     if (rc) return rc;
     return p.splits > 1 && p.kernel >= PAGED_ROWS ? paged_join(a, p.splits, st) : CME_OK;
 }

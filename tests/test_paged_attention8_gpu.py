@@ -139,7 +139,7 @@ def test_chunks(dtype, D, heads, kv_heads, page, block):
     check(args, scales, ops.paged_attention(*args, **scales))
 
 
-@pytest.mark.parametrize("dtype,backend", [(BF16, "single"), (BF16, "rows"), (F32, "single"), (F32, "rows")])
+@pytest.mark.parametrize("dtype,backend", [(BF16, "single"), (BF16, "rows"), (BF16, "tc"), (F32, "single"), (F32, "rows")])
 @pytest.mark.parametrize("splits", [1, 2, 3, 8, 13, -1, -2, -7])
 @pytest.mark.parametrize("D", [32, 64, 128])
 @pytest.mark.parametrize("pairs", [SINGLES, CHUNKS])
@@ -160,7 +160,7 @@ def test_pages_that_are_not_there(dtype, pairs, drop, page):
         check(args[:3] + (table,) + args[4:], scales, ops.paged_attention(*args[:3], table, *args[4:], **scales))
 
 
-@pytest.mark.parametrize("dtype,backend", [(BF16, "single"), (BF16, "rows"), (F32, "single"), (F32, "rows"), (BF16, "auto")])
+@pytest.mark.parametrize("dtype,backend", [(BF16, "single"), (BF16, "rows"), (F32, "single"), (F32, "rows"), (BF16, "tc")])
 def test_rows_without_keys(dtype, backend):
     args, scales = make([(1, 1), (3, 3), (20, 20), (2, 0), (1, 0)], 4, 2, 64, 16, 16, dtype)
     args = args[:5] + (torch.tensor([1, 2, 5, 0, 0], dtype=torch.int32).cuda(),)
