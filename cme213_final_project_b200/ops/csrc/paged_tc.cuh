@@ -56,10 +56,10 @@ template <> struct Cfg<128, false, false> {
 };
 // (RAW: stages of the 8-bit tiles)
 template <> struct Cfg<64, true, true> {
-    static constexpr int HALVES = 1, STAGES = 2, BUFFERS = 2, CTAS = 2, COLS = 256, RAW = 4;
+    static constexpr int HALVES = 1, STAGES = 3, BUFFERS = 2, CTAS = 2, COLS = 256, RAW = 3;
 };
 template <> struct Cfg<128, false, true> {
-    static constexpr int HALVES = 2, STAGES = 2, BUFFERS = 2, CTAS = 1, COLS = 512, RAW = 4;
+    static constexpr int HALVES = 2, STAGES = 3, BUFFERS = 2, CTAS = 1, COLS = 512, RAW = 3;
 };
 template <int D, bool FEW, bool Q8_> struct Sizes : Cfg<D, FEW, Q8_> {
     using C = Cfg<D, FEW, Q8_>;
