@@ -16,7 +16,7 @@
 // The bound of a log-sum-exp's error: an exponential's argument x - r is rounded twice and multiplied by a rounded log2 e, 2.5 * 2^-24 of |x - r|, which
 // weighted by the softmax comes to 2.5 * 2^-24 (log vocab + RAISE) at the most (a reference r is one of the x, and none above r + RAISE
 // goes by it; the mean distance from the largest x is at most log vocab, as the entropy is); the
-// exponential itself is good to 2^-22; four additions in 32 bits a sum of eight, 4 * 2^-24; the rest is added in 64 bits.
+// exponential itself is good to 2^-22; a term takes part in at most eight additions in 32 bits, 8 * 2^-24; the rest is added in 64 bits.
 #include "common.h"
 #include "beam_desc.h"
 
@@ -52,8 +52,8 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.x > b.x || (a.x == b.x && a.token < b.token); }
 
-// The row's elements [v0, v1) as this thread's share of sixteen bytes each: f(first token, values, how many).  Every call of a thread's walks
-// over the same elements.
+// The row's elements [v0, v1), four times sixteen bytes of a thread's share at a time: f(values, token of value i, how many); -inf where nothing is
+// (left).  Every call of a thread's walks over the same elements.
 template <typename T> struct Slice {
     static constexpr int N = 16 / (int)sizeof(T);
     const T* src;
@@ -80,25 +80,23 @@ template <typename T> struct Slice {
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u)
                 if (g0 + u * THREADS < groups) raw[u] = *reinterpret_cast<const uint4*>(src + a0 + (g0 + u * THREADS) * N);
+            float x[AHEAD * N];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const int t = a0 + (g0 + u * THREADS) * N;
-                if (g0 + u * THREADS >= groups) break;
-                float x[N];
-                unpack(raw[u], x);
-                if (allowed) {
+                const bool in = g0 + u * THREADS < groups;
+                unpack(raw[u], x + u * N);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) x[e] = is_allowed(t + e) ? x[e] : -INFINITY;
-                }
-                f(t, x, std::integral_constant<int, N>{});
+                for (int e = 0; e < N; ++e) x[u * N + e] = in && (!allowed || is_allowed(t + e)) ? x[u * N + e] : -INFINITY;
             }
+            f(x, [&](int i) { return a0 + (g0 + i / N * THREADS) * N + i % N; }, std::integral_constant<int, AHEAD * N>{});
         }
         // the ends, one by one
         const int head = a0 - v0, tail = a0 + groups * N, rest = head + v1 - tail;
         if ((int)threadIdx.x < rest) {
             const int t = (int)threadIdx.x < head ? v0 + (int)threadIdx.x : tail + (int)threadIdx.x - head;
             const float x[1] = {at(t)};
-            f(t, x, std::integral_constant<int, 1>{});
+            f(x, [&](int) { return t; }, std::integral_constant<int, 1>{});
         }
     }
 };
@@ -129,7 +127,7 @@ __global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int s
     // A thread's sum has a reference of its own, the largest of its first elements, and a new one only where that is passed by much.
     float ref = -INFINITY, top = -INFINITY;
     double sum = 0.0;
-    s.template each<SCAN>([&](int, const float* x, auto number) {
+    s.template each<SCAN>([&](const float* x, auto&&, auto number) {
         constexpr int n = decltype(number)::value;
         float m = x[0];
 #pragma unroll
@@ -144,16 +142,22 @@ __global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int s
         if constexpr (n == 1) {
             part = ex2((x[0] - use) * LOG2E);
         } else {
+            constexpr int CHAINS = n / 8;                  // of four pairs each: 3 additions, then 1 or 2, and the pair's
             const F32x2 shift = f2_splat(-use), scale = f2_splat(LOG2E);
-            F32x2 acc = f2_splat(0.f);
+            F32x2 acc[CHAINS];
 #pragma unroll
             for (int e = 0; e < n; e += 2) {
                 float a, b;
                 f2_unpack(f2_mul(f2_add(f2_pack(x[e], x[e + 1]), shift), scale), a, b);
-                acc = f2_add(acc, f2_pack(ex2(a), ex2(b)));
+                const F32x2 y = f2_pack(ex2(a), ex2(b));
+                acc[e / 2 % CHAINS] = e / 2 < CHAINS ? y : f2_add(acc[e / 2 % CHAINS], y);
             }
+#pragma unroll
+            for (int step = 1; step < CHAINS; step *= 2)
+#pragma unroll
+                for (int c = 0; c + step < CHAINS; c += 2 * step) acc[c] = f2_add(acc[c], acc[c + step]);
             float a, b;
-            f2_unpack(acc, a, b);
+            f2_unpack(acc[0], a, b);
             part = a + b;
         }
         sum += (double)part;
@@ -200,13 +204,13 @@ __global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int s
         *result = Part{total, block_ref, 0, {0, 0, 0, 0}};
     }
     if (top >= bound && top > -INFINITY) {
-        s.template each<SCAN>([&](int t, const float* x, auto number) {
+        s.template each<SCAN>([&](const float* x, auto&& token, auto number) {
             constexpr int n = decltype(number)::value;
 #pragma unroll
             for (int e = 0; e < n; ++e) {
                 if (x[e] >= bound && x[e] > -INFINITY) {
                     const int at = atomicAdd(&count, 1);
-                    if (at < CAP) held[at] = Cand{x[e], t + e};
+                    if (at < CAP) held[at] = Cand{x[e], token(e)};
                 }
             }
         });
@@ -228,11 +232,11 @@ __global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int s
     int found = 0;
     for (; found < p.width; ++found) {
         Cand best{-INFINITY, INT_MAX};
-        s.template each<SCAN>([&](int t, const float* x, auto number) {
+        s.template each<SCAN>([&](const float* x, auto&& token, auto number) {
             constexpr int n = decltype(number)::value;
 #pragma unroll
             for (int e = 0; e < n; ++e) {
-                const Cand c{x[e], t + e};
+                const Cand c{x[e], token(e)};
                 if (before(last, c) && before(c, best)) best = c;
             }
         });
@@ -296,14 +300,13 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, int p
     }
     const int bound_list = sel.last < 0 ? lists : sel.last;
     const double bound = sel.last < 0 ? -INFINITY : sel.heads[sel.last] - slack;
-    for (int l = tid; l < lists; l += THREADS) {
-        const int n = count_of(l);
-        for (int k = 0; k < n; ++k) {
-            const double v = value(l, k);
-            if (!(v > bound || (v == bound && (slack > 0.0 || l < bound_list || (l == bound_list && k == 0))))) break;
-            const int i = atomicAdd(&sel.counted, 1);
-            if (i < SURVIVORS) { sel.value[i] = v; sel.beam[i] = l / per_beam; sel.token[i] = at(l, k).token; }
-        }
+    for (int i = tid; i < lists * p.width; i += THREADS) {
+        const int l = i / p.width, k = i - l * p.width;
+        if (k >= count_of(l) || sel.heads[l] < bound) continue;
+        const double v = value(l, k);
+        if (!(v > bound || (v == bound && (slack > 0.0 || l < bound_list || (l == bound_list && k == 0))))) continue;
+        const int c = atomicAdd(&sel.counted, 1);
+        if (c < SURVIVORS) { sel.value[c] = v; sel.beam[c] = l / per_beam; sel.token[c] = at(l, k).token; }
     }
     __syncthreads();
     const int n = sel.counted;
@@ -374,45 +377,51 @@ template <typename T>
 __global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int slices) {
     __shared__ Select sel;
     __shared__ double scratch[MERGE / 32];
-    __shared__ double error[MAX_BEAMS];
     __shared__ int counts[MERGE];
+    __shared__ double sums[MERGE];
+    __shared__ float refs[MERGE];
+    __shared__ unsigned char over_s[MAX_BEAMS];
     pdl_wait();
     const int group = blockIdx.x, tid = threadIdx.x, lists = p.beams * slices;
     const long long stride = sizeof(Part) + p.width * sizeof(Cand);
     auto part_at = [&](int l) -> const Part* {
         return reinterpret_cast<const Part*>(static_cast<const char*>(p.ws) + ((long long)group * p.beams * slices + l) * stride);
     };
+    for (int l = tid; l < lists; l += MERGE) {
+        const Part part = *part_at(l);
+        sums[l] = part.sum;
+        refs[l] = part.ref;
+        counts[l] = part.count;
+    }
+    float score = 0.f;
+    bool over = false;
     if (tid < p.beams) {
         const long long row = (long long)group * p.beams + tid;
-        const float score = p.scores[row];
-        const bool over = p.finished && p.finished[row];
-        double ref = -INFINITY, sum = 0.0;
-        for (int k = 0; k < slices; ++k) {
-            const Part* part = part_at(tid * slices + k);
-            if (!(part->sum > 0.0 || part->sum != part->sum)) continue;       // nothing in it (a NaN goes on)
-            const double r = part->ref;
-            if (r > ref) { sum = sum == 0.0 ? 0.0 : sum * exp(ref - r); ref = r; }
-            sum += part->sum * exp(r - ref);
+        score = p.scores[row];
+        over = p.finished && p.finished[row];
+        over_s[tid] = over;
+    }
+    // twice the bound of a log-sum-exp's error (log vocab in 32 bits, hence a bit more)
+    if (tid == 0) sel.slack = 2.0 * (3 * 0x1p-22 + 2.5 * 0x1p-24 * ((double)logf((float)p.vocab) + RAISE + 1e-3));
+    __syncthreads();
+    if (tid < p.beams) {
+        const int l0 = tid * slices;
+        float ref = -INFINITY;
+        for (int l = l0; l < l0 + slices; ++l) ref = sums[l] > 0.0 ? fmaxf(ref, refs[l]) : ref;
+        double sum = 0.0;
+        for (int l = l0; l < l0 + slices; ++l) {
+            if (sums[l] != sums[l]) sum = sums[l];
+            else if (sums[l] > 0.0) sum += refs[l] == ref ? sums[l] : sums[l] * exp((double)refs[l] - (double)ref);
         }
         const double lse = ref + log(sum);
         const bool fine = finite(score) && (over || (sum > 0.0 && fabs(lse) < INFINITY));
         sel.score[tid] = fine ? (double)score : -INFINITY;
         sel.lse[tid] = fine && !over ? lse : 0.0;
-        error[tid] = fine && !over ? 0x1p-21 + 2.5 * 0x1p-24 * (log((double)p.vocab) + RAISE) : 0.0;
-        for (int k = 0; k < slices; ++k) counts[tid * slices + k] = !fine ? 0 : over ? k == 0 : part_at(tid * slices + k)->count;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        double e = 0.0;
-        for (int b = 0; b < p.beams; ++b) e = fmax(e, error[b]);
-        sel.slack = 2.0 * e;
+        for (int l = l0; l < l0 + slices; ++l) counts[l] = !fine ? 0 : over ? l == l0 : counts[l];
     }
     __syncthreads();
     auto count_of = [&](int l) { return counts[l]; };
-    auto at = [&](int l, int k) {
-        const long long row = (long long)group * p.beams + l / slices;
-        return p.finished && p.finished[row] ? Cand{0.f, -1} : reinterpret_cast<const Cand*>(part_at(l) + 1)[k];
-    };
+    auto at = [&](int l, int k) { return over_s[l / slices] ? Cand{0.f, -1} : reinterpret_cast<const Cand*>(part_at(l) + 1)[k]; };
     if (pick<MERGE>(sel, p, group, lists, slices, count_of, at)) return;
     const unsigned close = sel.close;
     for (int b = 0; b < p.beams; ++b) {

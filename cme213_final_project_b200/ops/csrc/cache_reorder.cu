@@ -7,7 +7,7 @@
 //
 // What bounds it: the bytes of the last pages of all layers, read and written once; with few beams a launch and the chain parent, length ->
 // page -> rows.  A warp copies the filled slots of one layer, head and tensor at a time.
-#include "common.h"
+#include "paged.h"
 #include "beam_desc.h"
 
 #include <algorithm>
@@ -16,28 +16,34 @@ namespace {
 
 constexpr int WARPS = 4;
 
-template <typename V> __device__ __forceinline__ void copy_rows(const char* src, char* dst, long long stride, int rows, int row_bytes, int lane) {
-    const int pieces = row_bytes / (int)sizeof(V), n = rows * pieces;
+// n pieces of type V, of which `pieces` make up a row; 0: all lie in a row (as the rows of a head do where slots are one behind the other).
+template <typename V> __device__ __forceinline__ void copy_rows(const char* src, char* dst, long long stride, int n, const PagedDiv& pieces, int lane) {
     constexpr int AHEAD = 4;
     for (int i0 = lane; i0 < n; i0 += 32 * AHEAD) {
         V v[AHEAD];
+        long long at[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int i = i0 + u * 32, r = i / pieces;
-            if (i < n) v[u] = *reinterpret_cast<const V*>(src + r * stride + (i - r * pieces) * (int)sizeof(V));
+            const int i = i0 + u * 32;
+            if (pieces.d) {
+                const int r = pieces.div(i);
+                at[u] = r * stride + (i - r * pieces.d) * (int)sizeof(V);
+            } else {
+                at[u] = i * (int)sizeof(V);
+            }
+            if (i < n) v[u] = *reinterpret_cast<const V*>(src + at[u]);
         }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int i = i0 + u * 32, r = i / pieces;
-            if (i < n) *reinterpret_cast<V*>(dst + r * stride + (i - r * pieces) * (int)sizeof(V)) = v[u];
-        }
+        for (int u = 0; u < AHEAD; ++u) if (i0 + u * 32 < n) *reinterpret_cast<V*>(dst + at[u]) = v[u];
     }
 }
 
-__global__ void __launch_bounds__(WARPS * 32) cache_reorder_kernel(const CmeReorder a, int chunks) {
+struct Divisors { PagedDiv sequence, beams, heads[4], pieces[4]; };
+
+__global__ void __launch_bounds__(WARPS * 32) cache_reorder_kernel(const CmeReorder a, const Divisors by, int chunks) {
     pdl_release();
     pdl_wait();
-    const int seq = blockIdx.x / chunks, chunk = blockIdx.x - seq * chunks, group = seq / a.beams, own = seq - group * a.beams;
+    const int seq = by.sequence.div(blockIdx.x), chunk = blockIdx.x - seq * chunks, group = by.beams.div(seq), own = seq - group * a.beams;
     int parent = a.parents[seq];
     const int length = max(0, a.lengths[group]), spare = a.spare[seq];
     if (parent < 0 || parent >= a.beams) parent = own;
@@ -64,12 +70,12 @@ __global__ void __launch_bounds__(WARPS * 32) cache_reorder_kernel(const CmeReor
         const CmePages& t = a.t[k];
         const int n = a.layers * t.heads, rows = (rest + t.per - 1) / t.per;
         for (; item < base + n; item += chunks * WARPS) {
-            const int layer = (item - base) / t.heads, head = (item - base) - layer * t.heads;
+            const int layer = by.heads[k].div(item - base), head = (item - base) - layer * t.heads;
             const char* p = t.base + layer * t.layer + head * t.head;
             char* q = t.base + layer * t.layer + head * t.head + spare * t.page;
             p += src * t.page;
-            if (t.row_bytes & 15) copy_rows<int>(p, q, t.row, rows, t.row_bytes, lane);
-            else copy_rows<uint4>(p, q, t.row, rows, t.row_bytes, lane);
+            if (t.row_bytes & 15) copy_rows<int>(p, q, t.row, rows * t.row_bytes >> 2, by.pieces[k], lane);
+            else copy_rows<uint4>(p, q, t.row, rows * t.row_bytes >> 4, by.pieces[k], lane);
         }
         base += n;
     }
@@ -81,13 +87,17 @@ CME_API int cme_cache_reorder(const CmeReorder* a, void* stream) {
     CME_REQUIRE(a->groups >= 0 && a->beams > 0 && a->width >= 0 && a->slots > 0 && a->layers >= 0 && a->num_pages >= 0 && a->tensors >= 0 &&
                 a->tensors <= 4, CME_ERR_SHAPE, "cache reorder: bad sizes");
     long long items = 0;
+    Divisors by{};
     for (int k = 0; k < a->tensors; ++k) {
         const CmePages& t = a->t[k];
         CME_REQUIRE(t.heads > 0 && t.per > 0 && t.row_bytes > 0, CME_ERR_SHAPE, "cache reorder: bad sizes");
         const int n = t.row_bytes & 15 ? 4 : 16;
         CME_REQUIRE(t.row_bytes % n == 0 && reinterpret_cast<uintptr_t>(t.base) % n == 0 && t.layer % n == 0 && t.page % n == 0 && t.head % n == 0 &&
                     t.row % n == 0, CME_ERR_SHAPE, "cache reorder: the cache has to start, and its strides have to be, at multiples of 16 bytes (scales: 4)");
+        CME_REQUIRE((long long)a->slots * t.row_bytes < (1ll << 31), CME_ERR_LIMIT, "cache reorder: too large pages");
         items += (long long)a->layers * t.heads;
+        by.heads[k] = paged_div(t.heads);
+        if (t.row != t.row_bytes) by.pieces[k] = paged_div(t.row_bytes / n);
     }
     const long long seqs = (long long)a->groups * a->beams;
     if (seqs == 0) return CME_OK;
@@ -97,7 +107,9 @@ CME_API int cme_cache_reorder(const CmeReorder* a, void* stream) {
     if (const int rc = cme_num_sms(&sms)) return rc;
     const long long most = std::max(1ll, (items + WARPS - 1) / WARPS), wanted = (sms * 64ll + seqs - 1) / seqs;
     const int chunks = (int)std::max(1ll, std::min(most, std::min(wanted, ((1ll << 31) - 1) / seqs)));
-    CME_CUDA(cme_launch_dependent(cache_reorder_kernel, dim3((unsigned)(seqs * chunks)), dim3(WARPS * 32), 0, (cudaStream_t)stream, *a, chunks));
+    by.sequence = paged_div(chunks);
+    by.beams = paged_div(a->beams);
+    CME_CUDA(cme_launch_dependent(cache_reorder_kernel, dim3((unsigned)(seqs * chunks)), dim3(WARPS * 32), 0, (cudaStream_t)stream, *a, by, chunks));
     CME_LAUNCH_CHECK();
     return CME_OK;
 }

@@ -140,7 +140,9 @@ int make_plan(const CmePaged* a, bool q8, int backend, int splits, int sms, Page
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
     CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
                 "paged attention: the tcgen05 kernel takes bf16 and up to 128 query heads per key head");
-    auto row_tile = [&](int b) { return b == 1 ? 16 : b == 2 ? 64 : (a->head_dim == 128 ? 2 : 1) * (128 / group * group); };
+    // (8 bits: tiles of 8 rows where the sequences have no more on average)
+    const int few_rows = q8 && rows <= 8ll * a->seqs ? 8 : 16;
+    auto row_tile = [&](int b) { return b == 1 ? few_rows : b == 2 ? 64 : (a->head_dim == 128 ? 2 : 1) * (128 / group * group); };
     auto tiles_of = [&](int b) { return rows / row_tile(b) + std::min(a->seqs, a->rows); };      // at the most: each sequence adds less than one
     auto even_tiles = [&](int b) { return a->seqs ? a->seqs * ((rows + (long long)a->seqs * row_tile(b) - 1) / ((long long)a->seqs * row_tile(b))) : 0; };
     const int longest = (int)std::min((long long)a->max_len, (long long)a->width * a->page);

@@ -42,8 +42,9 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-template <typename T, int D, bool ROWS, bool Q8_> struct Cfg {
+template <typename T, int D, bool ROWS, bool Q8_, int RT_ = 16> struct Cfg {
     static constexpr bool F32 = sizeof(T) == 4, Q8 = Q8_;
+    static constexpr int RT = RT_;                                    // rows of a tile (not ROWS)
     static constexpr int ELEM = Q8 ? 1 : (int)sizeof(T);
     static constexpr int ROW = D * ELEM;                              // bytes of a key
     static constexpr int SLAB = ROW < 128 ? ROW : 128;                // bytes of a key in one swizzled slab
@@ -53,9 +54,9 @@ template <typename T, int D, bool ROWS, bool Q8_> struct Cfg {
     static constexpr int TILE = KEYS * ROW;                           // bytes of its keys (and of its values)
     // (64 KB of the rows' fragments leave room for two stages; of 8-bit tiles as many bytes are on their way as of others)
     static constexpr int STAGES = Q8 ? (ROW == 128 ? (F32 ? 2 : 3) : 6) : ROW == 64 ? 4 : ROWS && ROW == 512 ? 2 : 3;
-    static constexpr int FRAGS = F32 ? D * (Q8 ? 64 : 128) : 0;       // bytes of 16 rows' fragments in shared memory
+    static constexpr int FRAGS = F32 && RT == 16 ? D * (Q8 ? 64 : 128) : 0;       // bytes of 16 rows' fragments in shared memory
     static constexpr int SCALES = Q8 ? STAGES * 128 : 0;              // bytes: [stage] 16 of keys, 16 of values
-    static constexpr int MAXIMA = Q8 && F32 && !ROWS ? 64 : 0;        // bytes: [16] of the rows
+    static constexpr int MAXIMA = Q8 && F32 && !ROWS && RT == 16 ? 64 : 0;        // bytes: [16] of the rows
     // CTAs of an SM, and groups of four warps, which take every other key tile (rows: every other WARP_KEYS keys of each).  Two CTAs' or two groups'
     // chains of products and softmax run at a time; 64 KB tiles, or 64 rows' fragments of fp32, leave room for one CTA.  Rows, fp32, one
     // group / two, us: 16 heads of 64, 512 tokens over 2048 in 4 sequences 469 / 384; 32 heads of 128 on 8, 500 over 2000 in 2 864 / 701;
@@ -623,6 +624,207 @@ __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t
     }
 }
 
+// Up to eight rows over a cache in 8 bits, the other way round: keys, and columns of V, are the 16 rows of a product and the rows its 8 columns, so that no
+// half of the products, exponentials and sums is for nothing (as in tiles of 16 rows).  S^T = K Q^T;  P^T, a product's second operand, is S^T with
+// its 8 x 8 blocks transposed;  O^T = V^T P^T.  A lane's rows are 2 (lane % 4) and the one after it.
+template <typename C, int D> struct WarpStateT {
+    float m[2], l[2], o[D / 16][4];                        // o[c]: columns 16 c + 2 (lane / 4), of both rows, then the next column
+    __device__ __forceinline__ void clear() {
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    }
+    __device__ __forceinline__ void finish() {             // l of the whole row
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+    }
+};
+// The rows as the second operand: lane (row, tq) has columns tq D / 4 + 4 j to + 3 in step j.
+template <typename T, typename C, int D> struct RowsT {
+    static constexpr int KS = D / 16;
+    uint32_t raw[KS][C::F32 ? 4 : 2];                      // as they are, then bf16: the fragments
+    uint32_t hi[C::F32 ? KS : 1][2], lo[C::F32 ? KS : 1][2];
+    float scale[2];                                        // of rows 2 tq and 2 tq + 1
+    __device__ __forceinline__ void load(const T* row, const T*, int) {
+        const int col = (threadIdx.x & 3) * (D / 4);
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            if constexpr (C::F32) {
+                const uint4 a = row ? *reinterpret_cast<const uint4*>(row + col + i * 4) : make_uint4(0, 0, 0, 0);
+                raw[i][0] = a.x; raw[i][1] = a.y; raw[i][2] = a.z; raw[i][3] = a.w;
+            } else {
+                const uint2 a = row ? *reinterpret_cast<const uint2*>(row + col + i * 4) : make_uint2(0, 0);
+                raw[i][0] = a.x; raw[i][1] = a.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void publish(uint8_t*, int, unsigned*) {
+        unsigned m = 0;                                    // largest magnitude of the row, as bits
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int e = 0; e < (C::F32 ? 4 : 2); ++e) {
+                const unsigned w = raw[i][e];
+                if constexpr (C::F32) m = max(m, w & 0x7fffffffu);
+                else m = max(m, max(w & 0x7fff0000u, (w << 16) & 0x7fff0000u));
+            }
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        float inverse;
+        const float f = Rows8<T, C, D, 1>::factor(m >> 23, inverse);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) scale[r] = __shfl_sync(0xffffffffu, inverse, ((threadIdx.x & 3) * 2 + r) * 4);
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if constexpr (C::F32) {
+                    const float x = __uint_as_float(raw[i][2 * e]) * f, y = __uint_as_float(raw[i][2 * e + 1]) * f;
+                    hi[i][e] = f2_to_h2(x, y);
+                    const float2 h = h2_to_f2(hi[i][e]);
+                    lo[i][e] = f2_to_h2(x - h.x, y - h.y);
+                } else {
+                    const float2 x = bf2_to_f2(raw[i][e]);
+                    raw[i][e] = f2_to_h2(x.x * f, x.y * f);
+                }
+            }
+    }
+};
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+template <typename C, int D, typename R>
+__device__ __forceinline__ void attend8(WarpStateT<C, D>& w, const R& q, uint32_t kt, uint32_t vt, uint32_t sc, int key0, int k0, int see0, int see1,
+                                        bool masked, uint32_t there, int box_log, float scale_log2) {
+    constexpr int MT = 2, KS = D / 16;                     // tiles of 16 keys
+    static_assert(C::WARP_KEYS == MT * 16, "a scale for every eight keys, four in a load");
+    const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    float s[MT][4];
+#pragma unroll
+    for (int n = 0; n < MT; ++n) {
+        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        float low[4] = {0.f, 0.f, 0.f, 0.f};               // fp32: the products with a low part
+        uint32_t b[2][KS];                                 // of keys g and g + 8
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = key0 + n * 16 + h * 8 + g;
+            if constexpr (D == 32) {
+                const uint2 v = lds64(kt + chunk_at<C>(row, tq >> 1) + (tq & 1) * 8);
+                b[h][0] = v.x; b[h][1] = v.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    const float4 v = lds128(kt + chunk_at<C>(row, tq * (D / 64) + c));
+                    b[h][c * 4] = __float_as_uint(v.x); b[h][c * 4 + 1] = __float_as_uint(v.y);
+                    b[h][c * 4 + 2] = __float_as_uint(v.z); b[h][c * 4 + 3] = __float_as_uint(v.w);
+                }
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const uint32_t x = b[0][ks] ^ 0x80808080u, y = b[1][ks] ^ 0x80808080u;
+            const uint32_t a[4] = {bytes_to_h2(x, 0x4140), bytes_to_h2(y, 0x4140), bytes_to_h2(x, 0x4342), bytes_to_h2(y, 0x4342)};
+            if constexpr (C::F32) {
+                mma_f16(s[n], a, q.hi[ks][0], q.hi[ks][1]);
+                mma_f16(low, a, q.lo[ks][0], q.lo[ks][1]);
+            } else {
+                mma_f16(s[n], a, q.raw[ks][0], q.raw[ks][1]);
+            }
+        }
+        if constexpr (C::F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] += low[i];
+        }
+    }
+    const float4 sk4 = lds128(sc + (key0 >> 3) * 4), sv4 = lds128(sc + 64 + (key0 >> 3) * 4);
+    const float sk[4] = {sk4.x, sk4.y, sk4.z, sk4.w}, sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
+    const float row_scale[2] = {q.scale[0] * scale_log2, q.scale[1] * scale_log2};
+#pragma unroll
+    for (int n = 0; n < MT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= row_scale[i & 1] * sk[n * 2 + (i >> 1)];
+    if (masked) {
+#pragma unroll
+        for (int n = 0; n < MT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int local = key0 + n * 16 + h * 8 + g, key = k0 + local;
+                const bool in = (there >> (local >> box_log)) & 1;
+                if (!in || key >= see0) s[n][2 * h] = -INFINITY;
+                if (!in || key >= see1) s[n][2 * h + 1] = -INFINITY;
+            }
+    }
+    bool raise = false;
+    float alpha[2], use[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        float mx = fmaxf(fmaxf(s[0][r], s[0][2 + r]), fmaxf(s[1][r], s[1][2 + r]));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        const bool up = mx > w.m[r];
+        raise |= up;
+        alpha[r] = up ? (w.m[r] == -INFINITY ? 0.f : ex2_approx(w.m[r] - mx)) : 1.f;
+        if (up) w.m[r] = mx;
+        use[r] = w.m[r] == -INFINITY ? 0.f : w.m[r];
+    }
+    if (__any_sync(0xffffffffu, raise)) {
+        w.l[0] *= alpha[0];
+        w.l[1] *= alpha[1];
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) { w.o[n][0] *= alpha[0]; w.o[n][1] *= alpha[1]; w.o[n][2] *= alpha[0]; w.o[n][3] *= alpha[1]; }
+    }
+    // (fmaxf passes over a NaN, which is in its own factor all the same)
+    const float most = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+    const float up = most >= PAGED_SMALLEST_SCALE ? 32768.f * rcp_approx(most) : 0.f, down = most * (1.f / 32768.f);
+    uint32_t ph[4], pl[4];                                 // of eight keys each
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const float f = sv[n] * up;
+        const float x = ex2_approx(s[n >> 1][(n & 1) * 2] - use[0]), y = ex2_approx(s[n >> 1][(n & 1) * 2 + 1] - use[1]);
+        w.l[0] += x;
+        w.l[1] += y;
+        const uint32_t p = f2_to_h2(x * f, y * f);
+        ph[n] = transpose8(p);
+        if constexpr (C::F32) {
+            const float2 h = h2_to_f2(p);
+            pl[n] = transpose8(f2_to_h2(fmaf(x, f, -h.x), fmaf(y, f, -h.y)));
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < D / 16; c += 2) {                  // 16 bytes of a value each
+        float acc[2][4], low[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+            low[i][0] = low[i][1] = low[i][2] = low[i][3] = 0.f;
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n += 2) {
+            uint32_t b[4];
+            ldsm4_t(vt + chunk_at<C>(key0 + n * 8 + (((lane >> 3) & 1) << 3) + (lane & 7), c + (lane >> 4)), b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t a[4] = {bytes_to_h2(b[2 * i], 0x4240), bytes_to_h2(b[2 * i], 0x4341), bytes_to_h2(b[2 * i + 1], 0x4240),
+                                       bytes_to_h2(b[2 * i + 1], 0x4341)};
+                mma_f16(acc[i], a, ph[n], ph[n + 1]);
+                if constexpr (C::F32) mma_f16(low[i], a, pl[n], pl[n + 1]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.o[c + i][e] = fmaf(down, C::F32 ? acc[i][e] + low[i][e] : acc[i][e], w.o[c + i][e]);
+    }
+}
+
 // fp32 with R <= 4 rows on the CUDA cores: sixteen rows' worth of tf32 products would take longer than the tile's bytes (a 64 KB tile 2.1 us
 // on the tensor cores for 1.5 us of memory; here 0.3 us a row).  Scores: a lane has a key (and, with 16 keys a warp, half of the columns).
 // Sums: a lane has four columns, and with head sizes below 128 every second or fourth key.
@@ -963,7 +1165,7 @@ struct Walk {
         t.n = hi - lo;
         t.length = paged_length(a, a.lengths[b], t.n);
         t.first = t.rows = 0;
-        tiles = (int)(((long long)t.n * p.group + 15) / 16);
+        tiles = (int)(((long long)t.n * p.group + C::RT - 1) / C::RT);
         keys = max(1, cme_cdiv_dev(min(t.length, a.max_len), C::KEYS)) + ITEM_COST;
     }
     // Takes share `part` of `parts` of the whole; returns how many key tiles a share has.  Whole warps.
@@ -1016,8 +1218,8 @@ struct Walk {
         while (left > 0) {
             const int n = min(left, keys - key), k0 = max(0, key - ITEM_COST), k1 = key + n - ITEM_COST;
             if (k1 > 0) {
-                t.first = tile * 16;
-                t.rows = (int)min(16ll, (long long)t.n * p.group - t.first);
+                t.first = tile * C::RT;
+                t.rows = (int)min((long long)C::RT, (long long)t.n * p.group - t.first);
                 const int limit = tile_sees(p, t);
                 part.t = t;
                 part.head = head;
@@ -1044,11 +1246,12 @@ struct Walk {
     }
 };
 
-template <typename T, int D, bool CLUSTER, bool Q8>
-__global__ void __launch_bounds__(Cfg<T, D, false, Q8>::WARPS * 32 + 32, Cfg<T, D, false, Q8>::CTAS)
+template <typename T, int D, bool CLUSTER, bool Q8, int RT>
+__global__ void __launch_bounds__(Cfg<T, D, false, Q8, RT>::WARPS * 32 + 32, Cfg<T, D, false, Q8, RT>::CTAS)
 paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const MmaParams p) {
-    using C = Cfg<T, D, false, Q8>;
+    using C = Cfg<T, D, false, Q8, RT>;
     constexpr int NT = D / 8;
+    static_assert(RT == 16 || (RT == 8 && Q8), "rows of a tile");
     extern __shared__ __align__(1024) uint8_t smem[];
     Loader<T, C> ld;
     ld.sK = smem;
@@ -1081,7 +1284,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     int share = 0;
     bool some = true;
     if constexpr (CLUSTER) {
-        part.t = paged_find_tile(a, blockIdx.x / p.splits, p.group, 16);
+        part.t = paged_find_tile(a, blockIdx.x / p.splits, p.group, RT);
         part.head = blockIdx.y;
         const int limit = tile_sees(p, part.t);
         const int span = cme_cdiv_dev(cme_cdiv_dev(limit, C::KEYS), p.splits) * C::KEYS;
@@ -1095,9 +1298,9 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             rec[0] = -1;
             if (wk.left > 0 && wk.key > ITEM_COST && wk.key + wk.left >= wk.keys) {
                 rec[0] = (int)(((long long)blockIdx.x * share - wk.key + ITEM_COST) / share);      // the CTA of the item's first key tile
-                rec[1] = (int)min(16ll, (long long)wk.t.n * p.group - wk.tile * 16);
+                rec[1] = (int)min((long long)RT, (long long)wk.t.n * p.group - wk.tile * RT);
                 rec[2] = wk.t.token0;
-                rec[3] = wk.tile * 16;
+                rec[3] = wk.tile * RT;
                 rec[4] = wk.head;
             }
         }
@@ -1117,7 +1320,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
         T* out = static_cast<T*>(a.o);
         int it = 0;
         bool ok = true;
-        using Q = std::conditional_t<Q8, Rows8<T, C, D, C::WARPS>, Rows<T, C, D, C::WARPS>>;
+        using Q = std::conditional_t<RT == 8, RowsT<T, C, D>, std::conditional_t<Q8, Rows8<T, C, D, C::WARPS>, Rows<T, C, D, C::WARPS>>>;
         Q coming;
         if (some) coming.load(row_of_q<T>(p, part.t, part.head, g), row_of_q<T>(p, part.t, part.head, g + 8), warp);
         while (some) {
@@ -1146,7 +1349,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
                 }
                 if (begin >= end && some) coming.load(row_of_q<T>(p, part.t, part.head, g), row_of_q<T>(p, part.t, part.head, g + 8), warp);
             };
-            WarpState<C, D> w;
+            std::conditional_t<RT == 8, WarpStateT<C, D>, WarpState<C, D>> w;
             bool simt = false;
             auto on_cuda_cores = [&](auto rows) {
                 if constexpr (!Q8) {
@@ -1177,7 +1380,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             }
             if constexpr (Q8) {
                 q.publish(sQ, warp, maxima);
-                const int see0 = min(end, row_sees(p, t, g)), see1 = min(end, row_sees(p, t, g + 8));
+                const int see0 = min(end, row_sees(p, t, RT == 8 ? 2 * tq : g)), see1 = min(end, row_sees(p, t, RT == 8 ? 2 * tq + 1 : g + 8));
                 w.clear();
                 tiles([&](int s, int k0, uint32_t there, bool masked) {
                     attend8(w, q, smem_u32(ld.sK) + s * C::TILE, smem_u32(ld.sV) + s * C::TILE, smem_u32(ld.scales + s * 32), key0, k0, see0, see1, masked,
@@ -1198,10 +1401,20 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
             float* own = reinterpret_cast<float*>(smem);   // cluster: [16 rows][D], this CTA's sums (its key tiles are done with)
             float2* own_ml = reinterpret_cast<float2*>(own + 16 * D);
 #pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += JR) {
+            for (int r0 = 0; r0 < RT; r0 += JR) {
                 if (r0 >= t.rows) break;
                 const int r = r0 / 8, own_row = g - r0 % 8;             // this lane has row r0 + own_row, if it is one of them
-                if (!simt && own_row >= 0 && own_row < JR && r0 + own_row < t.rows) {
+                if constexpr (RT == 8) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = 2 * tq + i - r0;
+                        if (row < 0 || row >= JR || r0 + row >= t.rows) continue;
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c)
+                            *reinterpret_cast<float2*>(sums + (warp * JR + row) * D + c * 16 + g * 2) = make_float2(w.o[c][i], w.o[c][2 + i]);
+                        if (g == 0) sML[warp * JR + row] = make_float2(w.m[i], w.l[i]);
+                    }
+                } else if (!simt && own_row >= 0 && own_row < JR && r0 + own_row < t.rows) {
                     if constexpr (Q8) {
                         w.columns4(r, [&](int c, const float4& v) { *reinterpret_cast<float4*>(sums + (warp * JR + own_row) * D + c) = v; });
                     } else {
@@ -1398,15 +1611,15 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const float* __restrict
 // ------------------------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------------------------
-template <typename T, int D, bool ROWS, bool Q8> constexpr int smem_bytes() {
-    using C = Cfg<T, D, ROWS, Q8>;
+template <typename T, int D, bool ROWS, bool Q8, int RT> constexpr int smem_bytes() {
+    using C = Cfg<T, D, ROWS, Q8, RT>;
     return 2 * C::STAGES * C::TILE + (ROWS ? 4 : 1) * C::FRAGS + C::SCALES + C::MAXIMA + C::STAGES * 16 + C::WORDS * 4 + (ROWS ? 0 : 32 * D * 4 + 32 * 8);
 }
 
-template <typename T, int D, bool ROWS, bool Q8, auto Kernel>
+template <typename T, int D, bool ROWS, bool Q8, int RT, auto Kernel>
 int launch(dim3 grid, const CmePaged* a, int cluster, const MmaParams& p, cudaStream_t st) {
-    using C = Cfg<T, D, ROWS, Q8>;
-    constexpr int SMEM = smem_bytes<T, D, ROWS, Q8>();
+    using C = Cfg<T, D, ROWS, Q8, RT>;
+    constexpr int SMEM = smem_bytes<T, D, ROWS, Q8, RT>();
     static_assert(SMEM <= 227 * 1024 && C::CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of a CTA");
     static bool attr[CME_MAX_DEVICES] = {};               // function attributes are per device
     int dev = 0;
@@ -1438,6 +1651,17 @@ int launch(dim3 grid, const CmePaged* a, int cluster, const MmaParams& p, cudaSt
     return CME_OK;
 }
 
+template <typename T, int D, bool Q8, int RT> int launch_single(const CmePaged* a, const PagedPlan& plan, MmaParams& p, cudaStream_t st) {
+    const dim3 grid((unsigned)(plan.tiles * plan.splits), a->kv_heads);
+    if (plan.kernel == PAGED_CLUSTER)
+        return launch<T, D, false, Q8, RT, paged_attn_single_kernel<T, D, true, Q8, RT>>(grid, a, plan.splits, p, st);
+    const int rc = launch<T, D, false, Q8, RT, paged_attn_single_kernel<T, D, false, Q8, RT>>(dim3(plan.splits), a, 1, p, st);
+    if (rc) return rc;
+    CME_CUDA(cme_launch_dependent(paged_stream_join_kernel<T, D>, dim3(plan.splits, 4), dim3(128), 0, st, p));
+    CME_LAUNCH_CHECK();
+    return CME_OK;
+}
+
 template <typename T, int D, bool Q8> int launch_any(const CmePaged* a, const PagedPlan& plan, MmaParams& p, cudaStream_t st) {
     if (plan.kernel == PAGED_ROWS) {
         int sms;
@@ -1446,15 +1670,12 @@ template <typename T, int D, bool Q8> int launch_any(const CmePaged* a, const Pa
         p.by_keys = paged_by_keys(a, p.group) && ctas > (unsigned)sms * Cfg<T, D, true, Q8>::CTAS;
         p.heads = paged_div(a->kv_heads);
         p.parts = paged_div(plan.splits);
-        return launch<T, D, true, Q8, paged_attn_rows_kernel<T, D, Q8>>(dim3(ctas), a, 1, p, st);
+        return launch<T, D, true, Q8, 16, paged_attn_rows_kernel<T, D, Q8>>(dim3(ctas), a, 1, p, st);
     }
-    const dim3 grid((unsigned)(plan.tiles * plan.splits), a->kv_heads);
-    if (plan.kernel == PAGED_CLUSTER) return launch<T, D, false, Q8, paged_attn_single_kernel<T, D, true, Q8>>(grid, a, plan.splits, p, st);
-    const int rc = launch<T, D, false, Q8, paged_attn_single_kernel<T, D, false, Q8>>(dim3(plan.splits), a, 1, p, st);
-    if (rc) return rc;
-    CME_CUDA(cme_launch_dependent(paged_stream_join_kernel<T, D>, dim3(plan.splits, 4), dim3(128), 0, st, p));
-    CME_LAUNCH_CHECK();
-    return CME_OK;
+    if constexpr (Q8) {
+        if (plan.row_tile == 8) return launch_single<T, D, Q8, 8>(a, plan, p, st);
+    }
+    return launch_single<T, D, Q8, 16>(a, plan, p, st);
 }
 
 template <bool Q8> int run(const CmePaged* a, const CmePagedScales* scales, const PagedPlan& plan, cudaStream_t st) {
