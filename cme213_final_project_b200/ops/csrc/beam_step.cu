@@ -9,8 +9,8 @@
 //
 // Two launches: `scan` goes once over the logits, a CTA a slice of a row: sum of exponentials and the `width` largest; `merge`, a CTA a group,
 // joins the slices and picks.  Up to 256 tokens (characters) a row is a warp's, in 64 bits, and one launch does both.
-// In scan a thread keeps the sum and the largest of its elements only, which costs no branch; the width-th largest of the best of those bounds
-// what can be chosen from below, and the few threads that hold something above it look through their elements again.
+// In scan a thread keeps the sum and the largest of each few of its elements only, which costs no branch; the width-th largest of the best of those
+// bounds what can be chosen from below, and the few groups that hold something above it are looked through again, a vector a thread.
 // What bounds it: the bytes of the logits.
 //
 // The bound of a log-sum-exp's error: an exponential's argument x - r is rounded twice and multiplied by a rounded log2 e, 2.5 * 2^-24 of |x - r|, which
@@ -29,9 +29,12 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_WIDTH = 32, MAX_BEAMS = 32;
 constexpr int SCAN = 256;                  // threads of a scan CTA
-constexpr int CAP = 1024;                  // elements above the bound that a scan CTA can hold
-constexpr int MERGE = 512;                 // threads of a merge CTA
+constexpr int AHEAD = 4;                   // vectors of a thread in a step
+constexpr int STEP = SCAN * AHEAD;         // of a CTA
+constexpr int CAP = 1024;                  // elements that reach the bound that a scan CTA can hold
+constexpr int MERGE = 256;                 // threads of a merge CTA
 constexpr int SURVIVORS = MAX_WIDTH * MAX_WIDTH;
+constexpr int NEAR = 1024;                 // candidates that a merge CTA keeps in shared memory
 constexpr int SMALL_VOCAB = 256;
 constexpr float RAISE = 8.f;
 
@@ -49,197 +52,81 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// The largest of the warp; a NaN only if all are.
+__device__ __forceinline__ float warp_most(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.x > b.x || (a.x == b.x && a.token < b.token); }
 
-// The row's elements [v0, v1), four times sixteen bytes of a thread's share at a time: f(values, token of value i, how many); -inf where nothing is
-// (left).  Every call of a thread's walks over the same elements.
+// A row's elements [v0, v1): sixteen bytes at a time from the first 16-byte boundary on, and the few before and behind.
 template <typename T> struct Slice {
     static constexpr int N = 16 / (int)sizeof(T);
     const T* src;
     const unsigned* allowed;
-    int v0, v1, a0, groups;
+    int v0, v1, a0, vectors;
 
     __device__ __forceinline__ Slice(const CmeBeams& p, int row, int from, int to) : v0(from), v1(to) {
         src = static_cast<const T*>(p.logits) + row * p.logits_ld;
         allowed = p.allowed ? reinterpret_cast<const unsigned*>(p.allowed) + row * p.allowed_ld : nullptr;
         const int off = (int)((reinterpret_cast<uintptr_t>(src + v0) / sizeof(T)) % N);
         a0 = min(v1, v0 + (off ? N - off : 0));
-        groups = (v1 - a0) / N;
+        vectors = (v1 - a0) / N;
     }
     __device__ __forceinline__ bool is_allowed(int t) const { return !allowed || (__ldg(allowed + (t >> 5)) >> (t & 31)) & 1; }
     __device__ __forceinline__ float at(int t) const { return is_allowed(t) ? to_f32<T>(src[t]) : -INFINITY; }
-    static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    __device__ __forceinline__ int token(int g) const { return a0 + g * N; }
+    // Vector g; all -inf behind the last one.
+    __device__ __forceinline__ uint4 load(int g) const {
+        constexpr unsigned NONE = N == 8 ? 0xff80ff80u : 0xff800000u;
+        uint4 v = make_uint4(NONE, NONE, NONE, NONE);
+        if (g < vectors) v = *reinterpret_cast<const uint4*>(src + token(g));
+        return v;
+    }
+    // Its elements, those that are not allowed as -inf.
+    __device__ __forceinline__ void unpack(const uint4& v, int g, float* x) const {
         if constexpr (N == 8) unpack8(v, x);
         else { x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w); }
+        if (allowed && g < vectors) {
+            const int t = token(g), w = t >> 5, shift = t & 31;
+            unsigned bits = __ldg(allowed + w) >> shift;
+            if (shift + N > 32) bits |= __ldg(allowed + w + 1) << (32 - shift);      // (the last element's word)
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = bits >> e & 1 ? x[e] : -INFINITY;
+        }
     }
-    template <int THREADS, typename F> __device__ __forceinline__ void each(F&& f) const {
-        constexpr int AHEAD = 4;
-        for (int g0 = threadIdx.x; g0 < groups; g0 += THREADS * AHEAD) {
-            uint4 raw[AHEAD];
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u)
-                if (g0 + u * THREADS < groups) raw[u] = *reinterpret_cast<const uint4*>(src + a0 + (g0 + u * THREADS) * N);
-            float x[AHEAD * N];
-#pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int t = a0 + (g0 + u * THREADS) * N;
-                const bool in = g0 + u * THREADS < groups;
-                unpack(raw[u], x + u * N);
-#pragma unroll
-                for (int e = 0; e < N; ++e) x[u * N + e] = in && (!allowed || is_allowed(t + e)) ? x[u * N + e] : -INFINITY;
-            }
-            f(x, [&](int i) { return a0 + (g0 + i / N * THREADS) * N + i % N; }, std::integral_constant<int, AHEAD * N>{});
-        }
-        // the ends, one by one
-        const int head = a0 - v0, tail = a0 + groups * N, rest = head + v1 - tail;
-        if ((int)threadIdx.x < rest) {
-            const int t = (int)threadIdx.x < head ? v0 + (int)threadIdx.x : tail + (int)threadIdx.x - head;
-            const float x[1] = {at(t)};
-            f(x, [&](int) { return t; }, std::integral_constant<int, 1>{});
-        }
+    // The elements before and behind the vectors, fewer than 2 N: thread i's, or -inf and a token below 0.
+    __device__ __forceinline__ float end(int i, int& t) const {
+        const int head = a0 - v0, tail = token(vectors);
+        t = i < head ? v0 + i : i < head + v1 - tail ? tail + i - head : -1;
+        return t < 0 ? -INFINITY : at(t);
     }
 };
 
 // ------------------------------------------------------------------------------------------------------
 // Scan
 // ------------------------------------------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int slices, int slice) {
+// The best behind the last one, over and over: where more elements than can be held are as large as the bound.
+template <typename T> __device__ __noinline__ int scan_one_by_one(const CmeBeams& p, int row, int v0, int v1, Cand* list) {
     constexpr int WARPS = SCAN / 32;
-    __shared__ float tops[WARPS * 8];
-    __shared__ double sums[WARPS];
-    __shared__ float refs[WARPS], bound_s;
-    __shared__ Cand held[CAP];
-    __shared__ int count;
     __shared__ Cand round_best[WARPS];
-    pdl_wait();
-    const int row = blockIdx.x / slices, part = blockIdx.x - row * slices, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    char* out = static_cast<char*>(p.ws) + (long long)blockIdx.x * (sizeof(Part) + p.width * sizeof(Cand));
-    Part* result = reinterpret_cast<Part*>(out);
-    Cand* list = reinterpret_cast<Cand*>(result + 1);
-    if ((p.finished && p.finished[row]) || !finite(p.scores[row])) {         // nothing of the row counts
-        if (tid == 0) *result = Part{0.0, 0.f, 0, {0, 0, 0, 0}};
-        return;
-    }
-    const int v0 = min((long long)p.vocab, (long long)part * slice), v1 = min((long long)p.vocab, (long long)v0 + slice);
     const Slice<T> s(p, row, v0, v1);
-    // A thread's sum has a reference of its own, the largest of its first elements, and a new one only where that is passed by much.
-    float ref = -INFINITY, top = -INFINITY;
-    double sum = 0.0;
-    s.template each<SCAN>([&](const float* x, auto&&, auto number) {
-        constexpr int n = decltype(number)::value;
-        float m = x[0];
-#pragma unroll
-        for (int e = 1; e < n; ++e) m = fmaxf(m, x[e]);
-        top = fmaxf(top, m);
-        if (m > ref + RAISE || (ref == -INFINITY && m > ref)) {
-            if (ref > -INFINITY) sum *= exp((double)ref - (double)m);         // (else it is 0, or NaN)
-            ref = m;
-        }
-        const float use = ref == -INFINITY ? 0.f : ref;
-        float part = 0.f;
-        if constexpr (n == 1) {
-            part = ex2((x[0] - use) * LOG2E);
-        } else {
-            constexpr int CHAINS = n / 8;                  // of four pairs each: 3 additions, then 1 or 2, and the pair's
-            const F32x2 shift = f2_splat(-use), scale = f2_splat(LOG2E);
-            F32x2 acc[CHAINS];
-#pragma unroll
-            for (int e = 0; e < n; e += 2) {
-                float a, b;
-                f2_unpack(f2_mul(f2_add(f2_pack(x[e], x[e + 1]), shift), scale), a, b);
-                const F32x2 y = f2_pack(ex2(a), ex2(b));
-                acc[e / 2 % CHAINS] = e / 2 < CHAINS ? y : f2_add(acc[e / 2 % CHAINS], y);
-            }
-#pragma unroll
-            for (int step = 1; step < CHAINS; step *= 2)
-#pragma unroll
-                for (int c = 0; c + step < CHAINS; c += 2 * step) acc[c] = f2_add(acc[c], acc[c + step]);
-            float a, b;
-            f2_unpack(acc[0], a, b);
-            part = a + b;
-        }
-        sum += (double)part;
-    });
-    // (a NaN or +inf among the logits makes the sum a NaN, by which the row is left out)
-    float all = ref;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-    if (lane == 0) refs[warp] = all;
-    // each warp's largest 2 ceil(width / warps) of its threads' largest
-    const int per_warp = 2 * ((p.width + WARPS - 1) / WARPS);
-    float left = top;
-    for (int k = 0; k < per_warp; ++k) {
-        float m = left;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        const int who = __ffs(__ballot_sync(0xffffffffu, left == m)) - 1;
-        if (lane == 0) tops[warp * per_warp + k] = m;
-        if (lane == who) left = -INFINITY;
-    }
-    if (tid == 0) { count = 0; bound_s = -INFINITY; }
-    __syncthreads();
-    float block_ref = refs[0];
-#pragma unroll
-    for (int w = 1; w < WARPS; ++w) block_ref = fmaxf(block_ref, refs[w]);
-    if (ref != block_ref && ref > -INFINITY) sum *= exp((double)ref - (double)block_ref);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) sums[warp] = sum;
-    // the width-th largest of what the warps gave: so many elements are as large at least
-    const int given = WARPS * per_warp;
-    if (tid < given) {
-        const float v = tops[tid];
-        int above = 0;
-        for (int k = 0; k < given; ++k) above += tops[k] > v || (tops[k] == v && k < tid);
-        if (above == p.width - 1) bound_s = v;
-    }
-    __syncthreads();
-    const float bound = bound_s;
-    if (tid == 0) {
-        double total = 0.0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) total += sums[w];
-        *result = Part{total, block_ref, 0, {0, 0, 0, 0}};
-    }
-    if (top >= bound && top > -INFINITY) {
-        s.template each<SCAN>([&](const float* x, auto&& token, auto number) {
-            constexpr int n = decltype(number)::value;
-#pragma unroll
-            for (int e = 0; e < n; ++e) {
-                if (x[e] >= bound && x[e] > -INFINITY) {
-                    const int at = atomicAdd(&count, 1);
-                    if (at < CAP) held[at] = Cand{x[e], token(e)};
-                }
-            }
-        });
-    }
-    __syncthreads();
-    const int n = count;
-    if (n <= CAP) {
-        for (int i = tid; i < n; i += SCAN) {
-            const Cand c = held[i];
-            int rank = 0;
-            for (int k = 0; k < n; ++k) rank += before(held[k], c);
-            if (rank < p.width) list[rank] = c;
-        }
-        if (tid == 0) result->count = min(n, p.width);
-        return;
-    }
-    // Too many equals: one after the other, each the best behind the last one.
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Cand last{INFINITY, -1};
     int found = 0;
     for (; found < p.width; ++found) {
         Cand best{-INFINITY, INT_MAX};
-        s.template each<SCAN>([&](const float* x, auto&& token, auto number) {
-            constexpr int n = decltype(number)::value;
-#pragma unroll
-            for (int e = 0; e < n; ++e) {
-                const Cand c{x[e], token(e)};
-                if (before(last, c) && before(c, best)) best = c;
-            }
-        });
+        for (int t = v0 + tid; t < v1; t += SCAN) {
+            const Cand c{s.at(t), t};
+            if (before(last, c) && before(c, best)) best = c;
+        }
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             const Cand c{__shfl_xor_sync(0xffffffffu, best.x, o), __shfl_xor_sync(0xffffffffu, best.token, o)};
@@ -249,13 +136,192 @@ __global__ void __launch_bounds__(SCAN) beam_scan_kernel(const CmeBeams p, int s
         if (lane == 0) round_best[warp] = best;
         __syncthreads();
         best = round_best[0];
-#pragma unroll
         for (int w = 1; w < WARPS; ++w) if (before(round_best[w], best)) best = round_best[w];
         if (!(best.x > -INFINITY)) break;
         if (tid == 0) list[found] = best;
         last = best;
     }
-    if (tid == 0) result->count = found;
+    return found;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SCAN, 4) beam_scan_kernel(const __grid_constant__ CmeBeams p, int slices, int slice) {
+    constexpr int WARPS = SCAN / 32, N = Slice<T>::N, KEPT = 8;
+    __shared__ float group_top[KEPT][SCAN];    // largest of a thread's vectors, `coarse` steps together
+    __shared__ __align__(16) float tops[WARPS * 8];
+    __shared__ float first_refs[WARPS], refs[WARPS];
+    __shared__ double sums[WARPS];
+    __shared__ Cand held[CAP];
+    __shared__ int count;
+    pdl_wait();
+    const int row = blockIdx.x / slices, part = blockIdx.x - row * slices, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    char* out = static_cast<char*>(p.ws) + (long long)blockIdx.x * (sizeof(Part) + p.width * sizeof(Cand));
+    Part* result = reinterpret_cast<Part*>(out);
+    Cand* list = reinterpret_cast<Cand*>(result + 1);
+    const int v0 = (int)min((long long)p.vocab, (long long)part * slice), v1 = (int)min((long long)p.vocab, (long long)v0 + slice);
+    const Slice<T> s(p, row, v0, v1);
+    uint4 raw[AHEAD];                          // the step's vectors; the next one's are on their way while it is reckoned
+    auto fetch = [&](int it) {
+        if ((it + 1) * STEP <= s.vectors) {
+            const uint4* from = reinterpret_cast<const uint4*>(s.src + s.a0) + it * STEP + tid;
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) raw[u] = from[u * SCAN];
+        } else {
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) raw[u] = s.load(it * STEP + u * SCAN + tid);
+        }
+    };
+    fetch(0);
+    int end_token;
+    const float end = s.end(tid, end_token);
+    if ((p.finished && p.finished[row]) || !finite(p.scores[row])) {         // nothing of the row counts
+        if (tid == 0) *result = Part{0.0, 0.f, 0, {0, 0, 0, 0}};
+        return;
+    }
+    // The sums' reference is the largest of the block's first elements; a thread that finds one larger by much takes that.
+    float y[AHEAD][N], top = end;
+    auto step_of = [&](int it) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) s.unpack(raw[u], it * STEP + u * SCAN + tid, y[u]);
+    };
+    step_of(0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int e = 0; e < N; e += 2) top = max3(top, y[u][e], y[u][e + 1]);
+    top = warp_most(top);
+    if (lane == 0) first_refs[warp] = top;
+    if (tid == 0) count = 0;
+    if (tid < WARPS * 8) tops[tid] = -INFINITY;
+    __syncthreads();
+    float ref = first_refs[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) ref = fmaxf(ref, first_refs[w]);
+    double sum = 0.0;
+    top = end;
+    const int steps = (s.vectors + STEP - 1) / STEP, coarse = max(1, (steps + KEPT - 1) / KEPT);
+    float group = -INFINITY;
+    F32x2 shift = f2_splat(ref == -INFINITY ? 0.f : -ref);
+    float limit = ref == -INFINITY ? ref : ref + RAISE;
+    auto raise = [&](float m) {
+        if (ref > -INFINITY) sum *= exp((double)ref - (double)m);             // (else it is 0, or NaN)
+        ref = m;
+        limit = ref + RAISE;
+        shift = f2_splat(-ref);
+    };
+    const F32x2 scale = f2_splat(LOG2E);
+    for (int it = 0, kept = 0, in = 0; it < steps; ++it) {
+        step_of(it);
+        fetch(it + 1);
+        float m[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            m[u] = fmaxf(y[u][0], y[u][1]);
+#pragma unroll
+            for (int e = 2; e < N; e += 2) m[u] = max3(m[u], y[u][e], y[u][e + 1]);
+        }
+        const float most = fmaxf(max3(m[0], m[1], m[2]), m[3]);
+        group = fmaxf(group, most);
+        if (most > limit) raise(most);
+        F32x2 acc[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                float a, b;
+                f2_unpack(f2_mul(f2_add(f2_pack(y[u][e], y[u][e + 1]), shift), scale), a, b);
+                const F32x2 t = f2_pack(ex2(a), ex2(b));
+                acc[u] = e ? f2_add(acc[u], t) : t;
+            }
+        float a, b;
+        f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a, b);
+        sum += (double)(a + b);
+        if (++in == coarse || it + 1 == steps) {
+            group_top[kept++][tid] = group;
+            top = fmaxf(top, group);
+            group = -INFINITY;
+            in = 0;
+        }
+    }
+    if (end_token >= 0) {
+        if (end > limit) raise(end);
+        sum += (double)ex2((end - (ref == -INFINITY ? 0.f : ref)) * LOG2E);
+    }
+    // (a NaN or +inf among the logits makes the sum a NaN, by which the row is left out)
+    // each warp's sum, and the largest 2 ceil(width / warps) of its threads' largest
+    const float warp_ref = warp_most(ref);
+    if (ref != warp_ref && ref > -INFINITY) sum *= exp((double)ref - (double)warp_ref);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) { sums[warp] = sum; refs[warp] = warp_ref; }
+    const int per_warp = 2 * ((p.width + WARPS - 1) / WARPS), given = WARPS * per_warp;
+    float left = top;
+    for (int k = 0; k < per_warp; ++k) {
+        const float m = warp_most(left);
+        const int who = __ffs(__ballot_sync(0xffffffffu, left == m)) - 1;
+        if (lane == 0) tops[warp * per_warp + k] = m;
+        if (lane == who) left = -INFINITY;
+    }
+    __syncthreads();
+    pdl_release();                             // (all but the choice is done: the next kernel's blocks may come)
+    // The width-th largest of what the warps gave, the largest that `width` of them reach: so many elements are as large at least.  Every warp for itself.
+    float bound = -INFINITY;
+    for (int at = lane; at < given; at += 32) {
+        const float v = tops[at];
+        int reach = 0;
+        for (int k = 0; k < given; k += 8) {
+            const float4 a = *reinterpret_cast<const float4*>(tops + k), b = *reinterpret_cast<const float4*>(tops + k + 4);
+            reach += (a.x >= v) + (a.y >= v) + (a.z >= v) + (a.w >= v) + (b.x >= v) + (b.y >= v) + (b.z >= v) + (b.w >= v);
+        }
+        if (reach >= p.width) bound = fmaxf(bound, v);
+    }
+    bound = warp_most(bound);
+    auto offer = [&](float v, int t) {
+        if (v >= bound && v > -INFINITY) {
+            const int at = atomicAdd(&count, 1);
+            if (at < CAP) held[at] = Cand{v, t};
+        }
+    };
+    // The threads' groups that reach it, a thread's next one at a time.
+    unsigned groups = 0;
+    if (top >= bound && top > -INFINITY) {
+        if (end_token >= 0) offer(end, end_token);
+        for (int k = 0; k * coarse < steps; ++k) groups |= (unsigned)(group_top[k][tid] >= bound) << k;
+    }
+    while (groups) {
+        const int k = __ffs(groups) - 1;
+        groups &= groups - 1;
+        for (int it = k * coarse; it < min(steps, (k + 1) * coarse); ++it) {
+            fetch(it);
+            step_of(it);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+                for (int e = 0; e < N; ++e) offer(y[u][e], s.token(it * STEP + u * SCAN + tid) + e);
+        }
+    }
+    __syncthreads();
+    int n = count;
+    if (n > CAP) {
+        n = scan_one_by_one<T>(p, row, v0, v1, list);
+    } else {
+        for (int i = tid; i < n; i += SCAN) {
+            const Cand c = held[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int k = 0; k < n; ++k) rank += before(held[k], c);
+            if (rank < p.width) list[rank] = c;
+        }
+        n = min(n, p.width);
+    }
+    if (tid == 0) {
+        float block_ref = refs[0];
+        for (int w = 1; w < WARPS; ++w) block_ref = fmaxf(block_ref, refs[w]);
+        double total = 0.0;
+        for (int w = 0; w < WARPS; ++w)
+            total += refs[w] == block_ref || refs[w] == -INFINITY ? sums[w] : sums[w] * exp((double)refs[w] - (double)block_ref);
+        *result = Part{total, block_ref, n, {0, 0, 0, 0}};
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -272,14 +338,14 @@ struct Select {
     int last;                              // list of the bound
 };
 
-// Of `lists` lists, best first, list l of beam l / per_beam: count_of(l) candidates at(l, k).  All threads of the block; `width` outputs of the group.
-// False: some order is not certain; sel.close has the beams.
-template <int THREADS, typename Count, typename At>
-__device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, int per_beam, Count&& count_of, At&& at) {
-    const int tid = threadIdx.x;
+// Of `lists` lists, best first, those of lower beams first: list l is beam_of(l)'s, with count_of(l) candidates at(l, k).  All threads of the
+// block; `width` outputs of the group.  False: some order is not certain; sel.close has the beams.
+template <int THREADS, typename Beam, typename Count, typename At>
+__device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, Beam&& beam_of, Count&& count_of, At&& at) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const double slack = sel.slack;
     auto value = [&](int l, int k) {
-        const int b = l / per_beam;
+        const int b = beam_of(l);
         const Cand c = at(l, k);
         return c.token < 0 ? sel.score[b] : sel.score[b] + ((double)c.x - sel.lse[b]);
     };
@@ -293,6 +359,7 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, int p
         for (int l = tid; l < lists; l += THREADS) {
             const double v = sel.heads[l];
             int above = 0;
+#pragma unroll 4
             for (int k = 0; k < lists; ++k) above += sel.heads[k] > v || (sel.heads[k] == v && k < l);
             if (above == p.width - 1) sel.last = l;
         }
@@ -300,13 +367,13 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, int p
     }
     const int bound_list = sel.last < 0 ? lists : sel.last;
     const double bound = sel.last < 0 ? -INFINITY : sel.heads[sel.last] - slack;
-    for (int i = tid; i < lists * p.width; i += THREADS) {
-        const int l = i / p.width, k = i - l * p.width;
+    for (int l = warp; l < lists; l += THREADS / 32) {     // a warp a list
+        const int k = lane;
         if (k >= count_of(l) || sel.heads[l] < bound) continue;
         const double v = value(l, k);
         if (!(v > bound || (v == bound && (slack > 0.0 || l < bound_list || (l == bound_list && k == 0))))) continue;
         const int c = atomicAdd(&sel.counted, 1);
-        if (c < SURVIVORS) { sel.value[c] = v; sel.beam[c] = l / per_beam; sel.token[c] = at(l, k).token; }
+        if (c < SURVIVORS) { sel.value[c] = v; sel.beam[c] = beam_of(l); sel.token[c] = at(l, k).token; }
     }
     __syncthreads();
     const int n = sel.counted;
@@ -316,18 +383,27 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, int p
         return false;
     }
     const int outs = p.width;
-    for (int i = tid; i < n; i += THREADS) {
-        const double v = sel.value[i];
-        const int b = sel.beam[i], t = sel.token[i];
+    constexpr int SHARE = 8;                               // lanes that hold one against the others
+    for (int i0 = 0; i0 < n; i0 += THREADS / SHARE) {      // whole warps
+        const int i = i0 + tid / SHARE;
+        const bool in = i < n;
+        const double v = in ? sel.value[i] : 0.0;
+        const int b = in ? sel.beam[i] : 0, t = in ? sel.token[i] : 0;
         int rank = 0;
         unsigned near = 0;
-        for (int k = 0; k < n; ++k) {
+#pragma unroll 4
+        for (int k = tid % SHARE; k < n; k += SHARE) {
             const double u = sel.value[k];
             const int c = sel.beam[k];
             rank += u > v || (u == v && (c < b || (c == b && sel.token[k] < t)));
             if (c != b && fabs(u - v) <= slack) near |= 1u << c;
         }
-        if (rank < outs) {
+#pragma unroll
+        for (int o = 1; o < SHARE; o <<= 1) {
+            rank += __shfl_xor_sync(0xffffffffu, rank, o);
+            near |= __shfl_xor_sync(0xffffffffu, near, o);
+        }
+        if (in && tid % SHARE == 0 && rank < outs) {
             if (near && slack > 0.0) atomicOr(&sel.close, near | 1u << b);
             const long long o = (long long)group * outs + rank;
             p.parents[o] = b;
@@ -378,20 +454,28 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int
     __shared__ Select sel;
     __shared__ double scratch[MERGE / 32];
     __shared__ int counts[MERGE];
+    __shared__ Cand near_list[NEAR];           // all candidates, if there are no more
     __shared__ double sums[MERGE];
     __shared__ float refs[MERGE];
-    __shared__ unsigned char over_s[MAX_BEAMS];
+    __shared__ unsigned char over_s[MAX_BEAMS], beams_of[MERGE];
     pdl_wait();
     const int group = blockIdx.x, tid = threadIdx.x, lists = p.beams * slices;
     const long long stride = sizeof(Part) + p.width * sizeof(Cand);
     auto part_at = [&](int l) -> const Part* {
         return reinterpret_cast<const Part*>(static_cast<const char*>(p.ws) + ((long long)group * p.beams * slices + l) * stride);
     };
+    const bool close_by = lists * p.width <= NEAR;
+    if (close_by) {
+        for (int l = tid >> 5; l < lists; l += MERGE / 32)
+            if ((tid & 31) < p.width)      // (behind the count there is nothing)
+                near_list[l * p.width + (tid & 31)] = reinterpret_cast<const Cand*>(part_at(l) + 1)[tid & 31];
+    }
     for (int l = tid; l < lists; l += MERGE) {
         const Part part = *part_at(l);
         sums[l] = part.sum;
         refs[l] = part.ref;
         counts[l] = part.count;
+        beams_of[l] = (unsigned char)(l / slices);
     }
     float score = 0.f;
     bool over = false;
@@ -420,9 +504,10 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int
         for (int l = l0; l < l0 + slices; ++l) counts[l] = !fine ? 0 : over ? l == l0 : counts[l];
     }
     __syncthreads();
+    auto beam_of = [&](int l) { return (int)beams_of[l]; };
     auto count_of = [&](int l) { return counts[l]; };
-    auto at = [&](int l, int k) { return over_s[l / slices] ? Cand{0.f, -1} : reinterpret_cast<const Cand*>(part_at(l) + 1)[k]; };
-    if (pick<MERGE>(sel, p, group, lists, slices, count_of, at)) return;
+    auto at = [&](int l, int k) { return over_s[beams_of[l]] ? Cand{0.f, -1} : close_by ? near_list[l * p.width + k] : reinterpret_cast<const Cand*>(part_at(l) + 1)[k]; };
+    if (pick<MERGE>(sel, p, group, lists, beam_of, count_of, at)) return;
     const unsigned close = sel.close;
     for (int b = 0; b < p.beams; ++b) {
         const long long row = (long long)group * p.beams + b;
@@ -433,7 +518,7 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int
     }
     if (tid == 0) sel.slack = 0.0;
     __syncthreads();
-    pick<MERGE>(sel, p, group, lists, slices, count_of, at);
+    pick<MERGE>(sel, p, group, lists, beam_of, count_of, at);
 }
 
 // Few tokens: a warp a row, in 64 bits.
@@ -498,7 +583,7 @@ __global__ void __launch_bounds__(SMALL) beam_small_kernel(const CmeBeams p) {
         }
     }
     __syncthreads();
-    pick<SMALL>(sel, p, group, p.beams, 1, [&](int l) { return counts[l]; }, [&](int l, int k) { return best[l][k]; });
+    pick<SMALL>(sel, p, group, p.beams, [](int l) { return l; }, [&](int l) { return counts[l]; }, [&](int l, int k) { return best[l][k]; });
 }
 
 // ------------------------------------------------------------------------------------------------------
