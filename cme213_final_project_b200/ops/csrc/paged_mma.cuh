@@ -64,6 +64,8 @@ template <typename T, int D, bool ROWS, bool Q8_, int RT_ = 16> struct Cfg {
     static constexpr int CTAS = Q8 ? 2 : ROWS ? (D == 32 ? 2 : 1) : ROW == 512 ? 1 : 2;
     static constexpr int GROUPS = !Q8 && (ROWS ? F32 && D > 32 : ROW == 512) ? 2 : 1, WARPS = 4 * GROUPS;
     static constexpr int JOIN_ROWS = 32 / WARPS;                      // joined at a time (up to 16 rows)
+    static constexpr int LOADERS = Q8 ? 2 : 1;                        // warps that load
+    static constexpr int THREADS = (WARPS + LOADERS) * 32;
     static constexpr int WORDS = 8;                                   // kept for the stages and a flag
     static_assert(STAGES < WORDS, "words kept for the stages");
 };
@@ -79,6 +81,7 @@ struct MmaParams {
     int* status;
     CmePagedScales scales;                 // Q8
     PagedDiv block;                        // Q8: tokens of a scale
+    int copies;                            // Q8: tiles come by copies of 16 bytes instead of boxes
 };
 
 // Address of 16-byte chunk `c` of key `r`, as TMA's swizzle over 128 bytes (64 or 32 for keys of that size) lays it down.
@@ -952,22 +955,83 @@ template <typename T, typename C> struct Loader {
                 for (int c = 0; c < C::SLABS; ++c)
                     tma_load_4d(base + s * C::TILE + c * C::KEYS * 128, map, &full[s], c * (128 / C::ELEM), slot, head, page);
             }
-            if constexpr (C::Q8) load_scales(p, s, head, k0, end, page, slot);
             page = next_page;
             slot = next_slot;
         }
     }
-    // The scales of a tile's groups of eight keys, a lane one; zeros where no key is.  They count as 32 more arrivals at the tile's barrier.
-    __device__ __forceinline__ void load_scales(const MmaParams& p, int s, int head, int k0, int end, int page, int slot) {
-        const int lane = threadIdx.x & 31, at = (lane & 15) * 8, box = (lane & 16) | at >> p.box_log;
-        page = __shfl_sync(0xffffffffu, page, box);
-        slot = __shfl_sync(0xffffffffu, slot, box) + (at & (p.box - 1));
-        const bool in = at < C::KEYS && k0 + at < end && page >= 0 && page < p.a.num_pages;
-        const float* src = lane < 16 ? p.scales.k : p.scales.v;
-        if (in) src += lane < 16 ? page * p.scales.k_page + head * p.scales.k_head : page * p.scales.v_page + head * p.scales.v_head;
-        if (in) src += p.block.div(slot);
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(scales + s * 32 + lane)), "l"(src), "r"(in ? 4 : 0) : "memory");
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+    // Q8.  A lane holds the page of one box (of 32 in a row; as many more are on their way), of which the lanes that load take theirs: one look-up in
+    // memory for several tiles.  With a look-up for each tile, one tile ahead, a tile took as long as a load under way among many.
+    struct Ahead { int now, next; };
+    __device__ __forceinline__ int page_of(const MmaParams& p, int seq, int begin, int end, int box) {
+        const long long key = begin + (long long)box * p.box;
+        if (key >= end) return -1;
+        const int page = p.a.pages[seq * p.a.pages_ld + p.page.div((int)key)];
+        return page < 0 || page >= p.a.num_pages ? p.a.num_pages : page;       // behind the cache: TMA fills the box with zeros
+    }
+    __device__ __forceinline__ Ahead look(const MmaParams& p, int seq, int begin, int end) {
+        const int lane = threadIdx.x & 31;
+        return {page_of(p, seq, begin, end, lane), page_of(p, seq, begin, end, lane + 32)};
+    }
+    // The tiles of keys [begin, end).  `copies`: in copies of 16 bytes, keys by one warp and values by the other one, else in boxes, all by the first one.
+    // between(): once, behind the first tile's loads.
+    template <bool COPIES, typename F>
+    __device__ __forceinline__ void tiles8(const MmaParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV, int seq, int head, int begin, int end,
+                                           bool values, Ahead pages, F&& between) {
+        constexpr int CH = C::ROW / 16;
+        const int lane = threadIdx.x & 31, b = lane & 15, each = C::KEYS >> p.box_log;     // boxes of a tile (they divide 32)
+        if (!COPIES) values = lane >= 16;
+        const char* base = static_cast<const char*>(values ? p.a.v : p.a.k) + head * (values ? p.a.v_head_stride : p.a.k_head_stride);
+        const long long page_stride = values ? p.a.v_page_stride : p.a.k_page_stride, slot_stride = values ? p.a.v_slot_stride : p.a.k_slot_stride;
+        const uint32_t tile = smem_u32(values ? sV : sK);
+        const CUtensorMap* map = values ? tmV : tmK;
+        // the tile's groups of eight keys, of whose scales a lane loads one
+        const int group = b * 8, group_box = group >> p.box_log;
+        const float* scale = values ? p.scales.v + head * p.scales.v_head : p.scales.k + head * p.scales.k_head;
+        const long long scale_page = values ? p.scales.v_page : p.scales.k_page;
+        for (int k0 = begin, box0 = 0; k0 < end && ok; k0 += C::KEYS, ++it, box0 += each) {
+            const int s = it % C::STAGES, first = box0 & 31;
+            if (box0 && first == 0) {
+                pages.now = pages.next;
+                pages.next = page_of(p, seq, begin, end, box0 + 32 + lane);
+            }
+            if (it >= C::STAGES) ok = mbar_wait(&empty[s], (it / C::STAGES - 1) & 1, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int page = __shfl_sync(0xffffffffu, pages.now, first + (b & (each - 1)));
+            const uint32_t mask = __ballot_sync(0xffffffffu, page != p.a.num_pages || b >= each);
+            if (lane == 0 && (!COPIES || !values)) there[s] = mask;
+            if constexpr (COPIES) {
+                const char* from = base + page * page_stride;          // (of lane b: box b's, slot 0)
+                const int at = k0 + b * p.box, slot = at - p.page.div(at) * p.page.d;
+                const bool real = page >= 0 && page < p.a.num_pages;
+                from += slot * slot_stride;
+#pragma unroll
+                for (int i = 0; i < C::KEYS * CH / 32; ++i) {
+                    const int key = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH, box = key >> p.box_log;
+                    const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(real ? from : nullptr), box));
+                    const bool in = src && k0 + key < end;
+                    src = in ? src + (key & (p.box - 1)) * slot_stride + c * 16 : base;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + s * C::TILE + chunk_at<C>(key, c)), "l"(src), "r"(in ? 16 : 0)
+                                 : "memory");
+                }
+            } else {
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(cme_cdiv_dev(min(C::KEYS, end - k0), p.box) * p.box * C::ROW * 2));
+                __syncwarp();
+                if (b < each && page >= 0) {
+                    const int key = k0 + b * p.box;
+                    tma_load_4d(tile + b * p.box * C::SLAB + s * C::TILE, map, &full[s], 0, key - p.page.div(key) * p.page.d, head, page);
+                }
+            }
+            // (zeros where no key is; the lanes' copies count as 32 more arrivals at the tile's barrier)
+            const int key = k0 + group, scaled = __shfl_sync(0xffffffffu, pages.now, first + (group_box & (each - 1)));
+            const bool in = group < C::KEYS && key < end && scaled >= 0 && scaled < p.a.num_pages;
+            const float* src = in ? scale + scaled * scale_page + p.block.div(key - p.page.div(key) * p.page.d) : scale;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(scales + s * 32 + (values ? 16 : 0) + b)), "l"(src), "r"(in ? 4 : 0) : "memory");
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+            if (COPIES && lane == 0 && !values) mbar_arrive(&full[s]);
+            if (k0 == begin) between();
+        }
+        if (begin >= end) between();
     }
     __device__ __forceinline__ void drain() {              // after a wait ran out: copies in flight end before the CTA does
         if (!ok && (threadIdx.x & 31) == 0) for (int i = 0; i < 2000; ++i) __nanosleep(500);
@@ -1001,7 +1065,7 @@ __device__ __forceinline__ int tile_sees(const MmaParams& p, const PagedTile& t)
 // sequences: 351 us, 43 TFLOP/s.  (Two tiles of 16 rows a warp, which split half as often, when it took 378: 344 us there, but 13.0 for 11.4 with
 // 64 tokens over 128 and 36 for 28 with head size 32.)
 template <typename T, int D, bool Q8>
-__global__ void __launch_bounds__(Cfg<T, D, true, Q8>::WARPS * 32 + 32, Cfg<T, D, true, Q8>::CTAS)
+__global__ void __launch_bounds__(Cfg<T, D, true, Q8>::THREADS, Cfg<T, D, true, Q8>::CTAS)
 paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const MmaParams p) {
     using C = Cfg<T, D, true, Q8>;
     constexpr int NT = D / 8;
@@ -1020,7 +1084,7 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     const CmePaged& a = p.a;
     if (threadIdx.x == 0) {
         *ld.abort_flag = 0;
-        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&ld.full[s], Q8 ? 33 : 1); mbar_init(&ld.empty[s], C::WARPS); }
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&ld.full[s], !Q8 ? 1 : p.copies ? 65 : 33); mbar_init(&ld.empty[s], C::WARPS); }
         fence_barrier_init();
         prefetch_tmap(&tmK);
         prefetch_tmap(&tmV);
@@ -1037,8 +1101,13 @@ paged_attn_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_con
     const int limit = tile_sees(p, t);
     const int begin = (int)min((long long)limit, (long long)split * p.split_keys);
     const int end = (int)min((long long)limit, (long long)begin + p.split_keys);
-    if (warp == C::WARPS) {
-        ld.tiles(p, &tmK, &tmV, t.seq, head, begin, end);
+    if (warp >= C::WARPS) {
+        if constexpr (Q8) {
+            if (p.copies) ld.template tiles8<true>(p, &tmK, &tmV, t.seq, head, begin, end, warp > C::WARPS, ld.look(p, t.seq, begin, end), [] {});
+            else if (warp == C::WARPS) ld.template tiles8<false>(p, &tmK, &tmV, t.seq, head, begin, end, false, ld.look(p, t.seq, begin, end), [] {});
+        } else {
+            ld.tiles(p, &tmK, &tmV, t.seq, head, begin, end);
+        }
         ld.drain();
     } else {
         const int of = warp & 3, group = warp >> 2;                    // its 16 rows, and which of the keys it takes
@@ -1247,7 +1316,7 @@ struct Walk {
 };
 
 template <typename T, int D, bool CLUSTER, bool Q8, int RT>
-__global__ void __launch_bounds__(Cfg<T, D, false, Q8, RT>::WARPS * 32 + 32, Cfg<T, D, false, Q8, RT>::CTAS)
+__global__ void __launch_bounds__(Cfg<T, D, false, Q8, RT>::THREADS, Cfg<T, D, false, Q8, RT>::CTAS)
 paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const MmaParams p) {
     using C = Cfg<T, D, false, Q8, RT>;
     constexpr int NT = D / 8;
@@ -1271,7 +1340,7 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     const CmePaged& a = p.a;
     if (threadIdx.x == 0) {
         *ld.abort_flag = 0;
-        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&ld.full[s], Q8 ? 33 : 1); mbar_init(&ld.empty[s], C::WARPS); }
+        for (int s = 0; s < C::STAGES; ++s) { mbar_init(&ld.full[s], !Q8 ? 1 : p.copies ? 65 : 33); mbar_init(&ld.empty[s], C::WARPS); }
         fence_barrier_init();
         prefetch_tmap(&tmK);
         prefetch_tmap(&tmV);
@@ -1309,10 +1378,26 @@ paged_attn_single_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_c
     __syncthreads();
     if (CLUSTER && part.t.rows == 0) return;               // all CTAs of a cluster
 
-    if (warp == C::WARPS) {
-        while (some) {
-            ld.tiles(p, &tmK, &tmV, part.t.seq, part.head, part.begin, part.end);
-            some = !CLUSTER && wk.next<C>(p, part);
+    if (warp >= C::WARPS) {
+        if constexpr (Q8) {
+            if (warp > C::WARPS && !p.copies) some = false;
+            auto pages = some ? ld.look(p, part.t.seq, part.begin, part.end) : typename Loader<T, C>::Ahead{-1, -1};
+            while (some) {
+                const auto now = part;
+                const auto of_now = pages;
+                auto between = [&] {                       // the next part, and the pages of its first tiles
+                    some = !CLUSTER && wk.next<C>(p, part);
+                    if (some) pages = ld.look(p, part.t.seq, part.begin, part.end);
+                };
+                if (p.copies) ld.template tiles8<true>(p, &tmK, &tmV, now.t.seq, now.head, now.begin, now.end, warp > C::WARPS, of_now, between);
+                else ld.template tiles8<false>(p, &tmK, &tmV, now.t.seq, now.head, now.begin, now.end, false, of_now, between);
+                if (!ld.ok) break;
+            }
+        } else {
+            while (some) {
+                ld.tiles(p, &tmK, &tmV, part.t.seq, part.head, part.begin, part.end);
+                some = !CLUSTER && wk.next<C>(p, part);
+            }
         }
         ld.drain();
     } else {
@@ -1635,7 +1720,7 @@ int launch(dim3 grid, const CmePaged* a, int cluster, const MmaParams& p, cudaSt
     if ((rc = paged_make_map(&mv, a, a->v, a->v_page_stride, a->v_head_stride, a->v_slot_stride, C::SLAB / C::ELEM, p.box, swizzle, Q8))) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(C::WARPS * 32 + 32);
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -1689,6 +1774,7 @@ template <bool Q8> int run(const CmePaged* a, const CmePagedScales* scales, cons
     p.box = 1;
     p.box_log = 0;
     while (p.box < tile && a->page % (p.box * 2) == 0) { p.box *= 2; ++p.box_log; }
+    p.copies = Q8 && p.box * a->head_dim < 2048;
     p.splits = plan.splits;
     p.split_keys = plan.split_keys;
     p.tiles = plan.tiles;
