@@ -61,6 +61,19 @@ inline bool paged_by_keys(const CmePaged* a, int group) { return a->seqs <= 32 &
 
 #ifdef __CUDACC__
 
+__device__ __forceinline__ uint32_t f2_to_h2(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+// Two of four signed bytes as fp16.  w: the bytes with their top bits turned over (x + 128); pick: __byte_perm's choice of two of them and two
+// bytes 0x64, which make 1024 + 128 + x.
+__device__ __forceinline__ uint32_t bytes_to_h2(uint32_t w, uint32_t pick) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(w, 0x64646464u, pick)), "r"(0x64806480u));
+    return r;
+}
+
 // What a CTA works on: rows [first, first + rows) of a sequence's tokens x group, for one key head.
 struct PagedTile {
     int seq, first, rows;        // rows == 0: the tile does not exist

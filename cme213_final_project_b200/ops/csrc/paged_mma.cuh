@@ -134,22 +134,10 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t f2_to_h2(float lo, float hi) {
-    uint32_t w;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
-    return w;
-}
 __device__ __forceinline__ float2 h2_to_f2(uint32_t w) {
     float2 f;
     asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.f32.f16 %0, l; cvt.f32.f16 %1, h;}" : "=f"(f.x), "=f"(f.y) : "r"(w));
     return f;
-}
-// Two of four signed bytes as fp16.  w: the bytes with their top bits turned over (x + 128); pick: __byte_perm's choice of two of them and two
-// bytes 0x64, which make 1024 + 128 + x.
-__device__ __forceinline__ uint32_t bytes_to_h2(uint32_t w, uint32_t pick) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(__byte_perm(w, 0x64646464u, pick)), "r"(0x64806480u));
-    return r;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;

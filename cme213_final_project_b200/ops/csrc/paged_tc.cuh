@@ -22,9 +22,14 @@
 // Every mbarrier wait is bounded; on expiry the CTA flags the status word, frees TMEM and returns.
 //
 // Q8: the cache holds 8-bit integers with a scale for each block of tokens and head,  k_t = sk_t k8_t,  v_t = sv_t v8_t.  TMA brings them as they are,
-// four more warps turn them into bf16 (exact up to 128; a byte x of two's complement is (128 + x's lower seven bits) - (x < 0 ? 256 : 128), four
-// instructions for two) in the tiles that the tensor core reads.  Scales come eight keys at a time: sk belongs to the factor of the
-// exponents (the maximum is taken of the groups' maxima times theirs), p is multiplied by sv before it is rounded.
+// four more warps turn them into fp16 (five instructions for four; bf16 has a bit too few and takes eight) in the tiles that the tensor core
+// reads, so that all operands are fp16:
+//   q   times a power of two that takes a row's largest element to 2^14 .. 2^15 (exact for elements down to 2^-32 of that one), which the softmax
+//       warps do to their rows first; its inverse belongs to the factor of the exponents, as sk does, of eight keys at a time (the
+//       maximum is taken of these groups' maxima times theirs);
+//   p   times sv / c 2^7, c the largest sv of the CTA's first tile with one: the logarithm of that factor is added to the exponents, and the reference
+//       maximum is one of x + max(0, log2 sv / c), so that no more than 2^15 comes out.  l is the sum of the groups' sums times its inverse.
+//       Rounded to fp16, 2^-11, and what is below 2^-14 of it to 2^-25: 2^-32 of c, whatever p is.
 #pragma once
 #include "paged.h"
 #include "sm100_ptx.cuh"
@@ -61,6 +66,7 @@ template <> struct Cfg<64, true, true> {
 template <> struct Cfg<128, false, true> {
     static constexpr int HALVES = 2, STAGES = 3, BUFFERS = 2, CTAS = 1, COLS = 512, RAW = 3;
 };
+constexpr int PER_STAGE = 32;              // factors of a tile: 8 of the exponents, 8 added to the maxima, 8 to the exponents, 8 of l
 template <int D, bool FEW, bool Q8_> struct Sizes : Cfg<D, FEW, Q8_> {
     using C = Cfg<D, FEW, Q8_>;
     static constexpr bool Q8 = Q8_;
@@ -72,7 +78,7 @@ template <int D, bool FEW, bool Q8_> struct Sizes : Cfg<D, FEW, Q8_> {
     static constexpr int THREADS = (LOADER + 1 + CONVERTERS) * 32;
     static constexpr int RAW_TILE = KEYS * D;                         // bytes of 8-bit keys, or values
     static constexpr int RAW_BYTES = Q8 ? 2 * RAW_TILE + 64 : 0;      // of a stage: both and their 16 scales
-    static constexpr int FACTORS = Q8 ? C::STAGES * 64 : 0;           // bytes: what the softmax warps make of the scales
+    static constexpr int FACTORS = Q8 ? C::STAGES * PER_STAGE * 4 + 16 : 0;      // bytes: what the scales come to, and c
     static constexpr int SMEM = C::HALVES * Q_BYTES + 2 * C::STAGES * KV_BYTES + C::RAW * RAW_BYTES + FACTORS + 384;
     static constexpr int HALF_COLS = C::COLS / C::HALVES;            // S buffers, then O
     static_assert(C::BUFFERS * KEYS + D <= HALF_COLS && C::CTAS * C::COLS <= 512, "tensor memory");
@@ -103,13 +109,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 __device__ __forceinline__ uint32_t swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
-// Two of four signed bytes as bf16; pick: __byte_perm's choice of two of them, each below a byte 0x43.
-__device__ __forceinline__ uint32_t bytes_to_b2(uint32_t w, uint32_t pick) {
-    const uint32_t t = __byte_perm(w, 0x43434343u, pick);
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t & 0xff7fff7fu), "r"(t & 0xff80ff80u));
-    return r;
-}
 
 template <int D, bool FEW, bool Q8>
 __global__ void __launch_bounds__(Sizes<D, FEW, Q8>::THREADS, Sizes<D, FEW, Q8>::CTAS)
@@ -126,7 +125,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint8_t* sV = sK + C::STAGES * C::KV_BYTES;
     uint8_t* sRaw = sV + C::STAGES * C::KV_BYTES;              // Q8: [stage] keys and values, then [stage] 8 scales of keys, 8 of values
     float* sRawScales = reinterpret_cast<float*>(sRaw + C::RAW * 2 * C::RAW_TILE);
-    float* sFactors = reinterpret_cast<float*>(sRaw + C::RAW * C::RAW_BYTES);    // Q8: [stage of values] 8 of the exponents, 8 of the probabilities
+    float* sFactors = reinterpret_cast<float*>(sRaw + C::RAW * C::RAW_BYTES);    // Q8: [stage of values][PER_STAGE], then c
     uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + C::RAW * C::RAW_BYTES + C::FACTORS);
     uint64_t* q_full = bars;
     uint64_t* k_full = bars + 1;              // [stage]
@@ -142,9 +141,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint64_t* turn = o_done + C::HALVES;      // (two halves only) [softmax warp] it may take its turn at the exponentials
     uint64_t* raw_full = turn + (C::HALVES > 1 ? 8 : 0);      // Q8: [stage] 8-bit tiles and scales are there
     uint64_t* raw_empty = raw_full + C::RAW;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + C::RAW);
+    uint64_t* q_ready = raw_empty + C::RAW;                   // Q8: [half] Q as fp16 (128 arrivals)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + (Q8 ? C::HALVES : 0));
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    static_assert((1 + 4 * C::STAGES + C::HALVES * (2 * C::BUFFERS + 2) + 8 + 2 * C::RAW) * 8 + 8 <= 384, "barriers");
+    static_assert((1 + 4 * C::STAGES + C::HALVES * (2 * C::BUFFERS + 2) + 8 + 2 * C::RAW + C::HALVES) * 8 + 8 <= 384, "barriers");
 
     const CmePaged& a = p.a;
     const int cols = D == 64 ? a.head_dim : D;                         // of the head (32 or 64)
@@ -168,6 +168,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         for (int w = 0; w < (C::HALVES > 1 ? 8 : 0); ++w) mbar_init(&turn[w], 1);
         for (int s = 0; s < C::RAW; ++s) { mbar_init(&raw_full[s], 33); mbar_init(&raw_empty[s], C::CONVERTERS); }
+        for (int h = 0; h < (Q8 ? C::HALVES : 0); ++h) mbar_init(&q_ready[h], 128);
         fence_barrier_init();
         prefetch_tmap(&tmQ);
         prefetch_tmap(&tmK);
@@ -284,8 +285,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t tmem_base = *tmem_slot;
     pdl_release();
 
-    constexpr uint32_t idesc_s = make_idesc(1, false, false, 128, KEYS);      // Q K^T: both K-major
-    constexpr uint32_t idesc_o = make_idesc(1, false, true, 128, D);          // P V: V is MN-major
+    constexpr uint32_t idesc_s = make_idesc(!Q8, false, false, 128, KEYS);    // Q K^T: both K-major
+    constexpr uint32_t idesc_o = make_idesc(!Q8, false, true, 128, D);        // P V: V is MN-major
     const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 0, 1024), k_desc = make_smem_desc(smem_u32(sK), 0, 1024);
     const uint64_t v_desc = make_smem_desc(smem_u32(sV), C::KV_SLAB, 1024);
     auto issue_s = [&](int half, int j, uint32_t tmem_S) {
@@ -307,7 +308,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (warp == C::LOADER) {
             ok = load_tiles(nkv);
         } else if (Q8 && warp > C::LOADER) {
-            // ---------------- 8 bits to bf16 ----------------
+            // ---------------- 8 bits to fp16 ----------------
             constexpr int CH = D / 16, T = C::CONVERTERS * 32;             // 16-byte pieces of a key
             const int tid = threadIdx.x - (C::LOADER + 1) * 32;
             auto convert = [&](const uint8_t* from, uint8_t* to) {
@@ -315,8 +316,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 for (int i = 0; i < KEYS * CH / T; ++i) {
                     const int at = i * T + tid, r = at / CH, c = at % CH;
                     const uint4 v = *reinterpret_cast<const uint4*>(from + at * 16);
-                    const uint4 x = make_uint4(bytes_to_b2(v.x, 0x4140), bytes_to_b2(v.x, 0x4342), bytes_to_b2(v.y, 0x4140), bytes_to_b2(v.y, 0x4342));
-                    const uint4 y = make_uint4(bytes_to_b2(v.z, 0x4140), bytes_to_b2(v.z, 0x4342), bytes_to_b2(v.w, 0x4140), bytes_to_b2(v.w, 0x4342));
+                    const uint32_t a = v.x ^ 0x80808080u, b = v.y ^ 0x80808080u, d = v.z ^ 0x80808080u, e = v.w ^ 0x80808080u;
+                    const uint4 x = make_uint4(bytes_to_h2(a, 0x4140), bytes_to_h2(a, 0x4342), bytes_to_h2(b, 0x4140), bytes_to_h2(b, 0x4342));
+                    const uint4 y = make_uint4(bytes_to_h2(d, 0x4140), bytes_to_h2(d, 0x4342), bytes_to_h2(e, 0x4140), bytes_to_h2(e, 0x4342));
                     // (eight lanes' stores of a row with 128 bytes go to both slabs: the second four begin with their odd piece, in other banks)
                     const bool odd = D == 128 && c >= CH / 2;
                     uint8_t* slab = to + (c >> 2) * C::KV_SLAB;
@@ -327,6 +329,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 fence_proxy_async();
                 __syncwarp();
             };
+            float unit = -1000.f;                                          // log2 c, once there is one (lanes 0-7 of the first warp)
+            if (tid == 0) sFactors[C::STAGES * PER_STAGE] = 0.f;
             for (int j = 0; j < nkv; ++j) {
                 const int s = j % C::STAGES, r = j % C::RAW;
                 const uint32_t parity = (j / C::STAGES - 1) & 1;
@@ -336,16 +340,23 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 if (lane == 0) mbar_arrive(&k_full[s]);
                 ok = j < C::STAGES || mbar_wait(&v_empty[s], parity, abort_flag);
                 if (!ok) break;
-                if (tid < 16) {
-                    float f = sRawScales[r * 16 + tid];
-                    // (of keys: above zero, since a masked -inf is multiplied by it; a NaN stays one)
-                    if (tid < 8) {
-                        f = (f < PAGED_SMALLEST_SCALE ? PAGED_SMALLEST_SCALE : f) * p.scale_log2;
-                        f = f < 1e-37f ? 1e-37f : f;
-                    } else if (f < PAGED_SMALLEST_SCALE) {
-                        f = 0.f;
+                if (tid < 8) {
+                    // (above zero, since a masked -inf is multiplied by it; a NaN stays one)
+                    const float f = sRawScales[r * 16 + tid] * p.scale_log2, v = sRawScales[r * 16 + 8 + tid];
+                    float most = v;
+#pragma unroll
+                    for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffu, most, o));
+                    if (unit == -1000.f && most >= PAGED_SMALLEST_SCALE) {
+                        unit = log2f(most);
+                        if (tid == 0) sFactors[C::STAGES * PER_STAGE] = unit;
                     }
-                    sFactors[s * 16 + tid] = f;
+                    float c = v < PAGED_SMALLEST_SCALE ? -64.f : log2f(v) - unit;
+                    c = c < -64.f ? -64.f : c > 110.f ? 110.f : c;         // (as good as zero, and more than fp32's largest number allows)
+                    float* to = sFactors + s * PER_STAGE + tid;
+                    to[0] = f < 0x1p-60f ? 0x1p-60f : f;
+                    to[8] = fmaxf(c, 0.f);
+                    to[16] = c + 7.f;
+                    to[24] = exp2f(-7.f - c);
                 }
                 convert(sRaw + (r * 2 + 1) * C::RAW_TILE, sV + s * C::KV_BYTES);
                 if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&raw_empty[r]); }
@@ -366,7 +377,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     mma_commit(&k_empty[j % C::STAGES]);
                     return true;
                 };
-                if (nkv > 0) ok = mbar_wait(q_full, 0, abort_flag) && scores(0);
+                if (nkv > 0) ok = mbar_wait(Q8 ? &q_ready[half] : q_full, 0, abort_flag) && scores(0);
                 for (int j = 0; j < nkv && ok; ++j) {
                     if (C::BUFFERS > 1 && j + 1 < nkv && !scores(j + 1)) { ok = false; break; }
                     ok = mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1, abort_flag) &&
@@ -399,9 +410,41 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const int sees = min(end, t.length - t.n + (t.first + row) / p.group + 1);
         const int warp_sees = min(end, t.length - t.n + (t.first + half * p.half_rows + (warp & 3) * 32) / p.group + 1);   // its first row
         float m_ref = -INFINITY, l = 0.f;                 // reference maximum (log2 units) and running row sum
+        float row_scale = 1.f;                            // Q8: what S of the row is multiplied by
+        if constexpr (Q8) {
+            if (nkv > 0 && (ok = mbar_wait(q_full, 0, abort_flag))) {
+                uint4 x[D / 8];
+                uint8_t* base = sQ + half * C::Q_BYTES;
+                unsigned most = 0;                        // largest magnitude, as the bits of an fp32 number
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    x[c] = *reinterpret_cast<const uint4*>(base + (c >> 3) * C::Q_SLAB + swz((warp & 3) * 32 + lane, c & 7));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned w = (&x[c].x)[e];
+                        most = max(most, max(w & 0x7fff0000u, (w << 16) & 0x7fff0000u));
+                    }
+                }
+                // (up to 2^60: its inverse times the smallest factor of the exponents is above zero)
+                const unsigned up = min(268u - (most >> 23), 187u);
+                const float f = __uint_as_float(up << 23);
+                row_scale = __uint_as_float((254u - up) << 23);
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 y = bf2_to_f2((&x[c].x)[e]);
+                        (&x[c].x)[e] = f2_to_h2(y.x * f, y.y * f);
+                    }
+                    *reinterpret_cast<uint4*>(base + (c >> 3) * C::Q_SLAB + swz((warp & 3) * 32 + lane, c & 7)) = x[c];
+                }
+                fence_proxy_async();
+                mbar_arrive(&q_ready[half]);
+            }
+        }
         int page, slot;
         lookup(0, page, slot);
-        for (int j = 0; j < nkv; ++j) {
+        for (int j = 0; j < nkv && ok; ++j) {
             const uint32_t tmem_S = tmem_S0 + (C::BUFFERS > 1 ? (j & 1) * KEYS : 0);
             const uint32_t there = __ballot_sync(0xffffffffu, page != a.num_pages);      // bit b: box b of the tile
             lookup(j + 1, page, slot);
@@ -412,7 +455,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             uint32_t r[64];
             tmem_ld32(tmem_S, r);
             tmem_ld32(tmem_S + 32, r + 32);
-            const float* factors = sFactors + (j % C::STAGES) * 16;
+            const float* factors = sFactors + (j % C::STAGES) * PER_STAGE;
             // (the stage is not filled again before P_j is written)
             if (Q8 && !mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1, abort_flag)) { ok = false; break; }
             tmem_wait_ld();
@@ -426,13 +469,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
                 for (int i = 0; i < 64; ++i) r[i] = (there >> (i >> p.box_log)) & 1 ? r[i] : 0xff800000u;
             }
-            float mx;
+            float mx, by[8];                               // (by: Q8, the groups' factors of the exponents)
             if constexpr (Q8) {
                 float best[8];
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     const float* x = reinterpret_cast<const float*>(r + g * 8);
-                    best[g] = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])) * factors[g];
+                    by[g] = factors[g] * row_scale;
+                    best[g] = fmaf(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])), by[g], factors[8 + g]);
                 }
                 mx = max3(max3(best[0], best[1], best[2]), max3(best[3], best[4], best[5]), fmaxf(best[6], best[7]));
             } else {
@@ -485,18 +529,24 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 float* x = reinterpret_cast<float*>(r + c * 32);
 #pragma unroll
                 for (int i = 0; i < 32; i += 2)
-                    f2_unpack(f2_fma(f2_pack(x[i], x[i + 1]), Q8 ? f2_splat(factors[c * 4 + (i >> 3)]) : sc2, nm2), x[i], x[i + 1]);
+                    f2_unpack(f2_fma(f2_pack(x[i], x[i + 1]), Q8 ? f2_splat(by[c * 4 + (i >> 3)]) : sc2,
+                                     Q8 ? f2_splat(factors[16 + c * 4 + (i >> 3)] - m_use) : nm2), x[i], x[i + 1]);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] = ex2_approx(x[i]);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2_pack(x[i], x[i + 1]));
                 if constexpr (Q8) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) f2_unpack(f2_mul(f2_pack(x[i], x[i + 1]), f2_splat(factors[8 + c * 4 + (i >> 3)])), x[i], x[i + 1]);
+                    for (int g = 0; g < 4; ++g) {
+                        F32x2 t = f2_add(f2_pack(x[g * 8], x[g * 8 + 1]), f2_pack(x[g * 8 + 2], x[g * 8 + 3]));
+                        t = f2_add(t, f2_add(f2_pack(x[g * 8 + 4], x[g * 8 + 5]), f2_pack(x[g * 8 + 6], x[g * 8 + 7])));
+                        sum2[g] = f2_fma(t, f2_splat(factors[24 + c * 4 + g]), sum2[g]);
+                    }
+                } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2_pack(x[i], x[i + 1]));
                 }
                 uint32_t pw[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) pw[i] = f2_to_bf2(x[2 * i], x[2 * i + 1]);
+                for (int i = 0; i < 16; ++i) pw[i] = Q8 ? f2_to_h2(x[2 * i], x[2 * i + 1]) : f2_to_bf2(x[2 * i], x[2 * i + 1]);
                 tmem_st16(tmem_S + c * 16, pw);
             }
             if (C::HALVES > 1 && halves > 1 && lane == 0) mbar_arrive(&turn[warp ^ 4]);
@@ -524,9 +574,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tc_fence_after();
             const int rr = t.first + row, tok = rr / p.group;
             const long long at = (long long)(t.token0 + tok) * a.heads + head * p.group + rr - tok * p.group;
+            const float unit = Q8 && nkv > 0 ? exp2f(sFactors[C::STAGES * PER_STAGE] - 7.f) : 1.f;       // of the sums
             if (p.splits == 1) {
                 // the warp's rows through its part of the Q tile (every product is complete), then whole rows to memory
-                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const float inv = l == 0.f ? 0.f : unit / l;
                 uint8_t* stage = sQ + half * C::Q_BYTES + (warp & 3) * 4096;
 #pragma unroll 1
                 for (int c = 0; c < cols / 32; ++c) {
@@ -561,7 +612,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         if (mine) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
-                                *reinterpret_cast<uint4*>(p.part_o + part * cols + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                                *reinterpret_cast<float4*>(p.part_o + part * cols + c * 32 + i) =
+                                    make_float4(__uint_as_float(o[i]) * unit, __uint_as_float(o[i + 1]) * unit, __uint_as_float(o[i + 2]) * unit,
+                                                __uint_as_float(o[i + 3]) * unit);
                         }
                     }
                 }
