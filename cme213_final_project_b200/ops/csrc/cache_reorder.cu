@@ -105,7 +105,7 @@ CME_API int cme_cache_reorder(const CmeReorder* a, void* stream) {
     // CTAs for four turns of all SMs (sixteen CTAs each), and a warp for each item at the most
     int sms;
     if (const int rc = cme_num_sms(&sms)) return rc;
-    const long long most = std::max(1ll, (items + WARPS - 1) / WARPS), wanted = (sms * 64ll + seqs - 1) / seqs;
+    const long long most = std::max(1ll, (items + WARPS - 1) / WARPS), wanted = (sms * 16ll + seqs - 1) / seqs;
     const int chunks = (int)std::max(1ll, std::min(most, std::min(wanted, ((1ll << 31) - 1) / seqs)));
     by.sequence = paged_div(chunks);
     by.beams = paged_div(a->beams);

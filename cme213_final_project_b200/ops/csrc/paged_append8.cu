@@ -15,7 +15,7 @@
 namespace {
 
 constexpr int WARPS = 4;
-constexpr int KEPT = 8;                    // 16-byte pieces of a lane that stay in registers between the maximum and the rounding
+constexpr int RESIDENT = 12;                // CTAs of an SM
 
 // Rounds 16 bytes' numbers, the bytes in the order of the numbers.  |x inverse| < 2^22: 1.5 * 2^23 more leaves the nearest integer (the even one of two)
 // in the low bits.
@@ -39,12 +39,14 @@ template <typename T> __device__ __forceinline__ unsigned largest(const uint4& v
     return m;
 }
 
-template <typename T, int D>
+// KEPT: 16-byte pieces of a lane that stay in registers between the maximum and the rounding.
+template <typename T, int D, int KEPT>
 __global__ void __launch_bounds__(WARPS * 32) paged_append8_kernel(const CmePaged a, const CmePagedScales s, PagedDiv page_div, PagedDiv block_div) {
     constexpr int LANES = D * (int)sizeof(T) / 16, ROWS = 32 / LANES;      // of a row; rows of a warp at a time
     pdl_release();
     pdl_wait();
-    const int lane = threadIdx.x & 31, item = blockIdx.y * WARPS + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    int item = blockIdx.y * WARPS + (threadIdx.x >> 5);    // head, keys or values; then the next one of this warp's
     if (item >= 2 * a.kv_heads) return;
     // the sequence of unit blockIdx.x, counting the blocks that each sequence's new tokens touch
     int unit = blockIdx.x, seq = -1, row = 0, first = 0, last = 0, blk = 0;
@@ -87,13 +89,13 @@ __global__ void __launch_bounds__(WARPS * 32) paged_append8_kernel(const CmePage
     }
     if (seq < 0 || blk < 0 || first >= last) return;       // (offsets out of order can lead past the sums, not out of the buffers)
     // this warp's rows
-    const int head = item >> 1, of = lane / LANES, piece = lane % LANES;
-    const bool values = item & 1;
-    const T* x = static_cast<const T*>(values ? a.nv : a.q) + row * (values ? a.v_token : a.q_token) + head * (values ? a.v_head : a.q_head) + piece * (16 / (int)sizeof(T));
-    const long long step = values ? a.v_token : a.q_token;
-    const int n = last - first;
+    const int of = lane / LANES, piece = lane % LANES, n = last - first;
     uint4 v[KEPT];
     auto load = [&](int r0) {
+        const bool values = item & 1;
+        const T* x = static_cast<const T*>(values ? a.nv : a.q) + row * (values ? a.v_token : a.q_token) + (item >> 1) * (values ? a.v_head : a.q_head) +
+                     piece * (16 / (int)sizeof(T));
+        const long long step = values ? a.v_token : a.q_token;
 #pragma unroll
         for (int u = 0; u < KEPT; ++u) {
             const int r = r0 + u * ROWS + of;
@@ -104,6 +106,9 @@ __global__ void __launch_bounds__(WARPS * 32) paged_append8_kernel(const CmePage
     const int col = page_div.div(first), slot = first - col * a.page, held = first - blk * s.block;
     const int page = a.pages[seq * a.pages_ld + col];
     if (page < 0 || page >= a.num_pages) return;
+    for (;;) {
+    const int head = item >> 1;
+    const bool values = item & 1;
     char* cache = values ? static_cast<char*>(a.v) + page * a.v_page_stride + head * a.v_head_stride
                          : static_cast<char*>(a.k) + page * a.k_page_stride + head * a.k_head_stride;
     const long long slot_stride = values ? a.v_slot_stride : a.k_slot_stride;
@@ -152,13 +157,27 @@ __global__ void __launch_bounds__(WARPS * 32) paged_append8_kernel(const CmePage
             }
         }
     }
+    item += gridDim.y * WARPS;
+    if (item >= 2 * a.kv_heads) return;
+    load(0);
+    }
 }
 
 template <typename T> int launch(const CmePaged* a, const CmePagedScales* s, cudaStream_t st) {
     // a sequence with n new tokens touches no more than n blocks and no more than n / block + 2
     const long long units = std::min((long long)a->rows, (long long)a->rows / s->block + 2ll * std::min(a->seqs, a->rows));
-    const dim3 grid((unsigned)units, cme_cdiv(2ll * a->kv_heads, WARPS));
-    auto* kernel = a->head_dim == 32 ? paged_append8_kernel<T, 32> : a->head_dim == 64 ? paged_append8_kernel<T, 64> : paged_append8_kernel<T, 128>;
+    // Where there are more warps than run at a time, one has several heads of its block, and looks it up once.
+    int sms;
+    if (const int rc = cme_num_sms(&sms)) return rc;
+    const int most = cme_cdiv(2ll * a->kv_heads, WARPS);
+    int across = most;
+    while (across > 1 && units * across > sms * RESIDENT) across = (across + 1) / 2;
+    const dim3 grid((unsigned)units, across);
+    // (rows of up to 256 bytes in blocks of 16 tokens or fewer: half as many registers, more warps on an SM)
+    const bool small = (long long)s->block * a->head_dim * sizeof(T) <= 4 * 512;
+    auto* kernel = a->head_dim == 32   ? (small ? paged_append8_kernel<T, 32, 4> : paged_append8_kernel<T, 32, 8>)
+                   : a->head_dim == 64 ? (small ? paged_append8_kernel<T, 64, 4> : paged_append8_kernel<T, 64, 8>)
+                                       : (small ? paged_append8_kernel<T, 128, 4> : paged_append8_kernel<T, 128, 8>);
     CME_CUDA(cme_launch_dependent(kernel, grid, dim3(WARPS * 32), 0, st, *a, *s, paged_div(a->page), paged_div(s->block)));
     CME_LAUNCH_CHECK();
     return CME_OK;
