@@ -109,15 +109,16 @@ struct Form {
     int keys;                // of a tile
     int slots;               // CTAs that run at a time
     float tile_us;
+    int start = 0;           // key tiles more in every turn (else two where there are several turns)
 };
 Form form_of(const CmePaged* a, bool q8, int backend, int sms) {
     const bool f32 = a->dtype == CME_F32;
     const int d = a->head_dim;
     if (q8) {
         const int keys = paged_mma_key_tile(a->dtype, d, true);
-        if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 2), d == 128 ? 1.1f : 1.2f};
+        if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 2), d == 128 ? 1.1f : 1.2f, 5};
         if (backend == 1) return {keys, sms * paged_mma_ctas(a->dtype, d, true), d == 128 ? 1.6f : d == 64 ? 1.2f : 1.0f};
-        return {keys, sms * 2, d == 128 ? 5.0f : d == 64 ? 3.2f : 2.4f};
+        return {keys, sms * 2, f32 ? (d == 128 ? 5.0f : d == 64 ? 2.9f : 2.0f) : d == 128 ? 3.6f : d == 64 ? 2.2f : 1.9f};
     }
     if (backend == 3) return {PAGED_TC_KEYS, sms * (d == 128 ? 1 : 3), d == 128 ? 1.0f : 1.15f};
     const int keys = paged_mma_key_tile(a->dtype, d, false);
@@ -128,7 +129,7 @@ float estimate(const CmePaged* a, const Form& f, long long tiles, int key_tiles,
     const long long ctas = tiles * a->kv_heads * parts;
     const double turns = ctas <= f.slots ? 1.0 : (double)ctas / f.slots + 0.5;         // (the shortest last: half a turn at the end)
     const double joined = parts > 1 ? 4.0 + (double)a->rows * a->heads * parts * (a->head_dim + 2) * 8 / 3e6 : 0.0;
-    return (float)(5.0 + turns * (cme_cdiv(key_tiles, parts) + 2 * (turns > 1)) * f.tile_us + joined);
+    return (float)(5.0 + turns * (cme_cdiv(key_tiles, parts) + (f.start ? f.start : 2 * (turns > 1))) * f.tile_us + joined);
 }
 
 // backend: 0 by the rule, 1 up to 16 rows a tile, 2 rows, 3 tc.  splits: 0 by the rule; up to 16 rows: a cluster of so many CTAs (1, 2, 4
@@ -178,9 +179,10 @@ int make_plan(const CmePaged* a, bool q8, int backend, int splits, int sms, Page
             float us;
             best_parts(many, &us);
             // head size 32 wins less on the tensor cores (us, 12 heads, rows / tc: 64 tokens over 256 in 32 sequences 9.5 / 13.6, 512 over 8192
-            // in one 45 / 36, 1100 over 4166 in 5 184 / 141)
+            // in one 45 / 36, 1100 over 4166 in 5 184 / 141), and 8 bits where a tile is half empty or its keys are few (12 heads of 64: 64 over 256 in
+            // 32 19.7 / 25.2, 100 over 1000 in 16 45.9 / 28.7; 32 heads of 128 on 8: 16 over 512 in 64 51 / 67, 64 over 256 in 32 53 / 31.5)
             float rows_us;
-            if (tc && a->head_dim == 32 && (best_parts(2, &rows_us), rows_us < us)) { many = 2; us = rows_us; }
+            if (tc && (q8 || a->head_dim == 32) && (best_parts(2, &rows_us), rows_us < us)) { many = 2; us = rows_us; }
             // (two more tiles an item of the stream, as its kernel reckons)
             const float tiles = turns <= 8 ? (float)((items * c + one.slots - 1) / one.slots) * (float)longest / (float)(one.keys * c)
                                            : (float)((items * (one_keys + 2) + one.slots - 1) / one.slots);
