@@ -377,3 +377,50 @@ def test_refusals():
     with pytest.raises(ops.NativeError):
         ops.cache_append(k, k, k.new_zeros(ck.shape), k.new_zeros(cv.shape), *rest, **scales)
     call()                                                                 # and as it should be
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# Many sequences, streams and graphs
+# ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D,page,block", [(64, 16, 16), (64, 8, 8), (32, 16, 8), (128, 32, 32), (128, 8, 8)])
+@pytest.mark.parametrize("heads,kv_heads,new", [(4, 4, 1), (16, 1, 1), (5, 1, 3), (24, 2, 2)])
+def test_many_sequences(dtype, D, page, block, heads, kv_heads, new):
+    """Items of many lengths in one stream of tiles: pages in boxes and in copies, up to 8 and up to 16 rows a tile, some sequences without new tokens."""
+    pairs = [(new * (b % 7 != 3), max(new, (b * 37) % 300 + 1)) for b in range(90)]
+    args, scales = make(pairs, heads, kv_heads, D, page, block, dtype, seed=9, drop=5)
+    check(args, scales, ops.paged_attention(*args, **scales, backend="single", splits=-1))
+    check(args, scales, ops.paged_attention(*args, **scales))
+
+
+def test_calls_on_two_streams_and_a_captured_append():
+    args, scales = make(SINGLES + CHUNKS, 4, 2, 64, 16, 16, BF16, seed=10)
+    want = ops.paged_attention(*args, **scales)
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s in side:
+            with torch.cuda.stream(s):
+                got.append(ops.paged_attention(*args, **scales))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g[0], want[0]) and torch.equal(g[1], want[1]) for g in got)
+    (ck, ks), (cv, vs) = empty(4, 2, 16, 64, 16), empty(4, 2, 16, 64, 16)
+    (dk, ls), (dv, ws) = empty(4, 2, 16, 64, 16), empty(4, 2, 16, 64, 16)
+    pages, off = torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda(), torch.tensor([0, 1], dtype=torch.int32).cuda()
+    x, length = torch.randn(30, 1, 2, 64).cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    row = x[0].clone()
+    ops.cache_append(row, row, dk, dv, pages, off, length, k_scales=ls, v_scales=ws)      # (length 0: nothing has a place)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        length.add_(1)
+        ops.cache_append(row, row, ck, cv, pages, off, length, k_scales=ks, v_scales=vs)
+    length.zero_()
+    for t in range(30):
+        row.copy_(x[t])
+        graph.replay()
+        ops.cache_append(x[t], x[t], dk, dv, pages, off, torch.tensor([t + 1], dtype=torch.int32).cuda(), k_scales=ls, v_scales=ws)
+    assert torch.equal(values(ck, ks)[[2, 0]].nan_to_num(7.0)[:, :, :14], values(dk, ls)[[2, 0]].nan_to_num(7.0)[:, :, :14])
+    assert torch.equal(values(cv, vs)[2], values(dv, ws)[2])
