@@ -22,7 +22,10 @@
 
 #include <algorithm>
 #include <climits>
+#include <cooperative_groups.h>
 #include <type_traits>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -421,24 +424,20 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, Beam&
     return sel.close == 0;
 }
 
-// The log-sum-exp of a row in 64 bits, whatever its place in memory: the whole block.
-template <int THREADS, typename T> __device__ double exact_lse(const CmeBeams& p, int row, double* scratch) {
-    const Slice<T> s(p, row, 0, p.vocab);
+// Sum of exp(x - top) over tokens [from, to) of a row in 64 bits, in an order that hangs on them only, whatever the row's place in memory: the whole block.
+template <int THREADS, typename T> __device__ double exact_sum(const CmeBeams& p, int row, double top, int from, int to, double* scratch) {
+    const Slice<T> s(p, row, from, to);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float m = -INFINITY;
-    for (int t = tid; t < p.vocab; t += THREADS) m = fmaxf(m, s.at(t));
+    constexpr int CHAINS = 4;
+    double part[CHAINS] = {};
+    for (int t = from + tid; t < to; t += THREADS * CHAINS) {
+        double x[CHAINS];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    __syncthreads();
-    if (lane == 0) scratch[warp] = m;
-    __syncthreads();
-    double top = scratch[0];
-    for (int w = 1; w < THREADS / 32; ++w) top = fmax(top, scratch[w]);
-    double sum = 0.0;
-    for (int t = tid; t < p.vocab; t += THREADS) {
-        const double x = s.at(t);
-        if (x > -INFINITY) sum += exp(x - top);
+        for (int c = 0; c < CHAINS; ++c) x[c] = t + c * THREADS < to ? s.at(t + c * THREADS) : -INFINITY;
+#pragma unroll
+        for (int c = 0; c < CHAINS; ++c) part[c] += exp(x[c] - top);       // (exp(-inf) = 0)
     }
+    double sum = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     __syncthreads();
@@ -446,11 +445,13 @@ template <int THREADS, typename T> __device__ double exact_lse(const CmeBeams& p
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < THREADS / 32; ++w) sum += scratch[w];
-    return top + log(sum);
+    return sum;
 }
 
+// The first CTA of a group's cluster joins and picks; the others are there for the sums in 64 bits, should they be needed (two rows of 50304 take one
+// CTA 20 us; the bound of the error calls for some in one call of two with 64 groups of 16 beams).
 template <typename T>
-__global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int slices) {
+__global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int slices, int size) {
     __shared__ Select sel;
     __shared__ double scratch[MERGE / 32];
     __shared__ int counts[MERGE];
@@ -458,64 +459,90 @@ __global__ void __launch_bounds__(MERGE) beam_merge_kernel(const CmeBeams p, int
     __shared__ double sums[MERGE];
     __shared__ float refs[MERGE];
     __shared__ unsigned char over_s[MAX_BEAMS], beams_of[MERGE];
+    __shared__ double top[MAX_BEAMS], exact[MAX_BEAMS];        // largest x of a row; this CTA's part of its sum in 64 bits
     pdl_wait();
-    const int group = blockIdx.x, tid = threadIdx.x, lists = p.beams * slices;
+    const int group = blockIdx.x / size, rank = blockIdx.x - group * size, tid = threadIdx.x, lists = p.beams * slices;
     const long long stride = sizeof(Part) + p.width * sizeof(Cand);
     auto part_at = [&](int l) -> const Part* {
         return reinterpret_cast<const Part*>(static_cast<const char*>(p.ws) + ((long long)group * p.beams * slices + l) * stride);
     };
     const bool close_by = lists * p.width <= NEAR;
-    if (close_by) {
-        for (int l = tid >> 5; l < lists; l += MERGE / 32)
-            if ((tid & 31) < p.width)      // (behind the count there is nothing)
-                near_list[l * p.width + (tid & 31)] = reinterpret_cast<const Cand*>(part_at(l) + 1)[tid & 31];
-    }
-    for (int l = tid; l < lists; l += MERGE) {
-        const Part part = *part_at(l);
-        sums[l] = part.sum;
-        refs[l] = part.ref;
-        counts[l] = part.count;
-        beams_of[l] = (unsigned char)(l / slices);
-    }
-    float score = 0.f;
-    bool over = false;
-    if (tid < p.beams) {
-        const long long row = (long long)group * p.beams + tid;
-        score = p.scores[row];
-        over = p.finished && p.finished[row];
-        over_s[tid] = over;
-    }
-    // twice the bound of a log-sum-exp's error (log vocab in 32 bits, hence a bit more)
-    if (tid == 0) sel.slack = 2.0 * (3 * 0x1p-22 + 2.5 * 0x1p-24 * ((double)logf((float)p.vocab) + RAISE + 1e-3));
-    __syncthreads();
-    if (tid < p.beams) {
-        const int l0 = tid * slices;
-        float ref = -INFINITY;
-        for (int l = l0; l < l0 + slices; ++l) ref = sums[l] > 0.0 ? fmaxf(ref, refs[l]) : ref;
-        double sum = 0.0;
-        for (int l = l0; l < l0 + slices; ++l) {
-            if (sums[l] != sums[l]) sum = sums[l];
-            else if (sums[l] > 0.0) sum += refs[l] == ref ? sums[l] : sums[l] * exp((double)refs[l] - (double)ref);
-        }
-        const double lse = ref + log(sum);
-        const bool fine = finite(score) && (over || (sum > 0.0 && fabs(lse) < INFINITY));
-        sel.score[tid] = fine ? (double)score : -INFINITY;
-        sel.lse[tid] = fine && !over ? lse : 0.0;
-        for (int l = l0; l < l0 + slices; ++l) counts[l] = !fine ? 0 : over ? l == l0 : counts[l];
-    }
-    __syncthreads();
     auto beam_of = [&](int l) { return (int)beams_of[l]; };
     auto count_of = [&](int l) { return counts[l]; };
-    auto at = [&](int l, int k) { return over_s[beams_of[l]] ? Cand{0.f, -1} : close_by ? near_list[l * p.width + k] : reinterpret_cast<const Cand*>(part_at(l) + 1)[k]; };
-    if (pick<MERGE>(sel, p, group, lists, beam_of, count_of, at)) return;
-    const unsigned close = sel.close;
-    for (int b = 0; b < p.beams; ++b) {
-        const long long row = (long long)group * p.beams + b;
-        if (!(close >> b & 1) || sel.score[b] == -INFINITY || (p.finished && p.finished[row])) continue;
-        const double lse = exact_lse<MERGE, T>(p, (int)row, scratch);
+    auto at = [&](int l, int k) {
+        return over_s[beams_of[l]] ? Cand{0.f, -1} : close_by ? near_list[l * p.width + k] : reinterpret_cast<const Cand*>(part_at(l) + 1)[k];
+    };
+    if (rank == 0) {
+        if (close_by) {
+            for (int l = tid >> 5; l < lists; l += MERGE / 32)
+                if ((tid & 31) < p.width)      // (behind the count there is nothing)
+                    near_list[l * p.width + (tid & 31)] = reinterpret_cast<const Cand*>(part_at(l) + 1)[tid & 31];
+        }
+        for (int l = tid; l < lists; l += MERGE) {
+            const Part part = *part_at(l);
+            sums[l] = part.sum;
+            refs[l] = part.ref;
+            counts[l] = part.count;
+            beams_of[l] = (unsigned char)(l / slices);
+        }
+        float score = 0.f;
+        bool over = false;
+        if (tid < p.beams) {
+            const long long row = (long long)group * p.beams + tid;
+            score = p.scores[row];
+            over = p.finished && p.finished[row];
+            over_s[tid] = over;
+        }
+        // twice the bound of a log-sum-exp's error (log vocab in 32 bits, hence a bit more)
+        if (tid == 0) sel.slack = 2.0 * (3 * 0x1p-22 + 2.5 * 0x1p-24 * ((double)logf((float)p.vocab) + RAISE + 1e-3));
         __syncthreads();
-        if (tid == 0) sel.lse[b] = lse;
+        if (tid < p.beams) {
+            const int l0 = tid * slices;
+            float ref = -INFINITY;
+            for (int l = l0; l < l0 + slices; ++l) ref = sums[l] > 0.0 ? fmaxf(ref, refs[l]) : ref;
+            double sum = 0.0;
+            for (int l = l0; l < l0 + slices; ++l) {
+                if (sums[l] != sums[l]) sum = sums[l];
+                else if (sums[l] > 0.0) sum += refs[l] == ref ? sums[l] : sums[l] * exp((double)refs[l] - (double)ref);
+            }
+            const double lse = ref + log(sum);
+            const bool fine = finite(score) && (over || (sum > 0.0 && fabs(lse) < INFINITY));
+            sel.score[tid] = fine ? (double)score : -INFINITY;
+            sel.lse[tid] = fine && !over ? lse : 0.0;
+            double most = -INFINITY;
+            for (int l = l0; l < l0 + slices; ++l) {
+                if (counts[l]) most = fmax(most, (double)reinterpret_cast<const Cand*>(part_at(l) + 1)->x);
+                counts[l] = !fine ? 0 : over ? l == l0 : counts[l];
+            }
+            top[tid] = most;
+        }
+        __syncthreads();
+        pick<MERGE>(sel, p, group, lists, beam_of, count_of, at);
     }
+    cg::cluster_group cluster = cg::this_cluster();
+    if (size > 1) cluster.sync();
+    const Select& first = *cluster.map_shared_rank(&sel, 0);
+    const unsigned close = first.close;
+    if (close) {
+        const double* tops = cluster.map_shared_rank(top, 0);
+        const int each = (p.vocab + size - 1) / size, from = min((long long)p.vocab, (long long)rank * each), to = min((long long)p.vocab, (long long)from + each);
+        for (int b = 0; b < p.beams; ++b) {
+            const long long row = (long long)group * p.beams + b;
+            if (!(close >> b & 1) || first.score[b] == -INFINITY || (p.finished && p.finished[row])) continue;
+            const double sum = exact_sum<MERGE, T>(p, (int)row, tops[b], from, to, scratch);
+            if (tid == 0) exact[b] = sum;
+        }
+    }
+    if (size > 1) cluster.sync();
+    else __syncthreads();
+    if (close == 0) return;
+    if (rank == 0 && tid < p.beams && close >> tid & 1 && sel.score[tid] != -INFINITY && !over_s[tid]) {
+        double sum = 0.0;
+        for (int r = 0; r < size; ++r) sum += *cluster.map_shared_rank(exact + tid, r);
+        sel.lse[tid] = top[tid] + log(sum);
+    }
+    if (size > 1) cluster.sync();              // (nobody's shared memory goes while it is read)
+    if (rank) return;
     if (tid == 0) sel.slack = 0.0;
     __syncthreads();
     pick<MERGE>(sel, p, group, lists, beam_of, count_of, at);
@@ -612,7 +639,21 @@ template <typename T> int launch(const CmeBeams* a, int sms, cudaStream_t st) {
     const int slices = slices_of(a, sms), slice = cme_cdiv(cme_cdiv(a->vocab, slices), 8) * 8;
     CME_CUDA(cme_launch_dependent(beam_scan_kernel<T>, dim3(a->groups * a->beams * slices), dim3(SCAN), 0, st, *a, slices, slice));
     CME_LAUNCH_CHECK();
-    CME_CUDA(cme_launch_dependent(beam_merge_kernel<T>, dim3(a->groups), dim3(MERGE), 0, st, *a, slices));
+    int size = 8;                                         // of a group's cluster: as many as run at a time
+    while (size > 1 && (long long)a->groups * size > sms * 4ll) size /= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a->groups * size);
+    cfg.blockDim = dim3(MERGE);
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = size;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    CME_CUDA(cudaLaunchKernelEx(&cfg, beam_merge_kernel<T>, *a, slices, size));
     CME_LAUNCH_CHECK();
     return CME_OK;
 }
