@@ -11,7 +11,8 @@
 // joins the slices and picks.  Up to 256 tokens (characters) a row is a warp's, in 64 bits, and one launch does both.
 // In scan a thread keeps the sum and the largest of each few of its elements only, which costs no branch; the width-th largest of the best of those
 // bounds what can be chosen from below, and the few groups that hold something above it are looked through again, a vector a thread.
-// What bounds it: the bytes of the logits.
+// What bounds it: the bytes of the logits; 64 x 16 beams of 50304 in fp32, a fifth of which have ended: 54.8 us, of which the scan 43 at 4 TB/s (a third
+// of a CTA's clocks are its start and its choice) and joining and choosing 9.  16 x 4 beams of 65 tokens 5.8 us.
 //
 // The bound of a log-sum-exp's error: an exponential's argument x - r is rounded twice and multiplied by a rounded log2 e, 2.5 * 2^-24 of |x - r|, which
 // weighted by the softmax comes to 2.5 * 2^-24 (log vocab + RAISE) at the most (a reference r is one of the x, and none above r + RAISE

@@ -7,7 +7,8 @@
 //
 // What bounds it: bytes (new rows read once, a byte a number written); with few tokens the chain offsets -> length -> page -> scale.  One warp has
 // a block and head of keys or of values, so nobody else touches its scale; its rows are on their way before it knows where they go, and with
-// them, once it does, what the block holds.
+// them, once it does, what the block holds.  16 prompts of 500 to 777 tokens, 12 heads of 64, blocks of 16: 11.1 us, 4.3 TB/s (16.1 with a
+// block and head a warp and no more, which looks up its place for two KB); 16 tokens 2.6 us.
 #include "paged.h"
 
 #include <algorithm>
@@ -107,59 +108,59 @@ __global__ void __launch_bounds__(WARPS * 32) paged_append8_kernel(const CmePage
     const int page = a.pages[seq * a.pages_ld + col];
     if (page < 0 || page >= a.num_pages) return;
     for (;;) {
-    const int head = item >> 1;
-    const bool values = item & 1;
-    char* cache = values ? static_cast<char*>(a.v) + page * a.v_page_stride + head * a.v_head_stride
-                         : static_cast<char*>(a.k) + page * a.k_page_stride + head * a.k_head_stride;
-    const long long slot_stride = values ? a.v_slot_stride : a.k_slot_stride;
-    float* scale = (values ? s.v + page * s.v_page + head * s.v_head : s.k + page * s.k_page + head * s.k_head) + block_div.div(slot);
-    const float before = held ? *scale : 0.f;
-    constexpr int PIECES = D / 16;         // of a held row
-    char* const begun = cache + (slot - held) * slot_stride;
-    uint4 h = make_uint4(0, 0, 0, 0);
-    if (lane < held * PIECES) h = *reinterpret_cast<const uint4*>(begun + lane / PIECES * slot_stride + lane % PIECES * 16);
-    unsigned m = 0;
-#pragma unroll
-    for (int u = 0; u < KEPT; ++u) m = max(m, largest<T>(v[u]));
-    for (int r0 = KEPT * ROWS; r0 < n; r0 += KEPT * ROWS) {
-        load(r0);
+        const int head = item >> 1;
+        const bool values = item & 1;
+        char* cache = values ? static_cast<char*>(a.v) + page * a.v_page_stride + head * a.v_head_stride
+                             : static_cast<char*>(a.k) + page * a.k_page_stride + head * a.k_head_stride;
+        const long long slot_stride = values ? a.v_slot_stride : a.k_slot_stride;
+        float* scale = (values ? s.v + page * s.v_page + head * s.v_head : s.k + page * s.k_page + head * s.k_head) + block_div.div(slot);
+        const float before = held ? *scale : 0.f;
+        constexpr int PIECES = D / 16;         // of a held row
+        char* const begun = cache + (slot - held) * slot_stride;
+        uint4 h = make_uint4(0, 0, 0, 0);
+        if (lane < held * PIECES) h = *reinterpret_cast<const uint4*>(begun + lane / PIECES * slot_stride + lane % PIECES * 16);
+        unsigned m = 0;
 #pragma unroll
         for (int u = 0; u < KEPT; ++u) m = max(m, largest<T>(v[u]));
-    }
-    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m)) * (1.f / 127.f);
-    float after = before > top || before != before ? before : top;
-    if (after < PAGED_SMALLEST_SCALE) after = 0.f;
-    if (!(after < INFINITY)) after = __uint_as_float(0x7fffffffu);
-    const float inverse = after > 0.f ? __frcp_rn(after) : 0.f;
-    if (lane == 0) *scale = after;
-    if (held && after != before) {
-        const float f = after > 0.f ? __fdiv_rn(before, after) : 0.f;
-        for (int i = lane; i < held * PIECES; i += 32) {
-            uint4* at = reinterpret_cast<uint4*>(begun + i / PIECES * slot_stride + i % PIECES * 16);
-            if (i != lane) h = *at;
-            *at = make_uint4(again4(h.x, f), again4(h.y, f), again4(h.z, f), again4(h.w, f));
-        }
-    }
-    for (int r0 = 0; r0 < n; r0 += KEPT * ROWS) {
-        if (n > KEPT * ROWS) load(r0);     // (else they are there)
+        for (int r0 = KEPT * ROWS; r0 < n; r0 += KEPT * ROWS) {
+            load(r0);
 #pragma unroll
-        for (int u = 0; u < KEPT; ++u) {
-            const int r = r0 + u * ROWS + of;
-            if (r >= n) continue;
-            char* to = cache + (slot + r) * slot_stride + piece * (16 / (int)sizeof(T));
-            if constexpr (sizeof(T) == 4) {
-                *reinterpret_cast<unsigned*>(to) = round4(__uint_as_float(v[u].x), __uint_as_float(v[u].y), __uint_as_float(v[u].z),
-                                                          __uint_as_float(v[u].w), inverse);
-            } else {
-                float f[8];
-                unpack8(v[u], f);
-                *reinterpret_cast<uint2*>(to) = make_uint2(round4(f[0], f[1], f[2], f[3], inverse), round4(f[4], f[5], f[6], f[7], inverse));
+            for (int u = 0; u < KEPT; ++u) m = max(m, largest<T>(v[u]));
+        }
+        const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, m)) * (1.f / 127.f);
+        float after = before > top || before != before ? before : top;
+        if (after < PAGED_SMALLEST_SCALE) after = 0.f;
+        if (!(after < INFINITY)) after = __uint_as_float(0x7fffffffu);
+        const float inverse = after > 0.f ? __frcp_rn(after) : 0.f;
+        if (lane == 0) *scale = after;
+        if (held && after != before) {
+            const float f = after > 0.f ? __fdiv_rn(before, after) : 0.f;
+            for (int i = lane; i < held * PIECES; i += 32) {
+                uint4* at = reinterpret_cast<uint4*>(begun + i / PIECES * slot_stride + i % PIECES * 16);
+                if (i != lane) h = *at;
+                *at = make_uint4(again4(h.x, f), again4(h.y, f), again4(h.z, f), again4(h.w, f));
             }
         }
-    }
-    item += gridDim.y * WARPS;
-    if (item >= 2 * a.kv_heads) return;
-    load(0);
+        for (int r0 = 0; r0 < n; r0 += KEPT * ROWS) {
+            if (n > KEPT * ROWS) load(r0);     // (else they are there)
+#pragma unroll
+            for (int u = 0; u < KEPT; ++u) {
+                const int r = r0 + u * ROWS + of;
+                if (r >= n) continue;
+                char* to = cache + (slot + r) * slot_stride + piece * (16 / (int)sizeof(T));
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<unsigned*>(to) = round4(__uint_as_float(v[u].x), __uint_as_float(v[u].y), __uint_as_float(v[u].z),
+                                                              __uint_as_float(v[u].w), inverse);
+                } else {
+                    float f[8];
+                    unpack8(v[u], f);
+                    *reinterpret_cast<uint2*>(to) = make_uint2(round4(f[0], f[1], f[2], f[3], inverse), round4(f[4], f[5], f[6], f[7], inverse));
+                }
+            }
+        }
+        item += gridDim.y * WARPS;
+        if (item >= 2 * a.kv_heads) return;
+        load(0);
     }
 }
 
