@@ -125,7 +125,14 @@ class PagedCache:
     def fork(self, beams: int, new: int) -> torch.Tensor:
         """The first sequence of each group of ``beams`` holds a prompt, the others nothing: give all of them room for ``new`` more
         tokens, and a spare page each.  Returns these (int32 ``[seqs]``), as ``ops.cache_reorder`` takes them; that call with all parents 0
-        then lets the others go on from the prompt.  Until :meth:`clear` no sequence grows or is released."""
+        then lets the others go on from the prompt.  Until :meth:`clear` no sequence grows or is released.  Raises :class:`CacheFull` or
+        ``ValueError`` before anything has changed."""
+        if self.shared:
+            raise ValueError("the sequences are beams already: clear()")
+        if beams < 1 or len(self.owned) % beams or new < 0:
+            raise ValueError(f"{len(self.owned)} sequences in groups of {beams}, room for {new} more tokens")
+        if any(o for b, o in enumerate(self.owned) if b % beams):
+            raise ValueError("the first sequence of each group has to be the only one that holds something")
         self.forked([self.lengths[b] for b in range(0, len(self.owned), beams)], beams, new)
         rows, cols, ids, spare = [], [], [], []
         for b in range(len(self.owned)):
@@ -390,7 +397,7 @@ class Generator:
         keep(torch.zeros_like(parents), token)
         graph = None
         for i in range(1, max_new):
-            if end is not None and i % 16 == 0 and bool(finished.all()):
+            if end is not None and i % 16 == 0 and bool((finished | (scores == -torch.inf)).all()):
                 break
             if not cuda_graph or i < 3:                                   # two steps warm everything up
                 step()

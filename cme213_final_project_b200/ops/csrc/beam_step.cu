@@ -623,6 +623,7 @@ int check(const CmeBeams* a) {
     CME_REQUIRE(a->beams > 0 && a->beams <= MAX_BEAMS && a->width > 0 && a->width <= MAX_WIDTH, CME_ERR_LIMIT,
                 "beam step: %d beams and a width of %d (1 to 32 of both)", a->beams, a->width);
     CME_REQUIRE((long long)a->groups * a->beams * 256 < (1ll << 31), CME_ERR_LIMIT, "beam step: too many rows");
+    CME_REQUIRE(a->vocab <= 1 << 30, CME_ERR_LIMIT, "beam step: too many tokens");      // (indexes run up to a few thousand beyond)
     return CME_OK;
 }
 // Slices of a row.

@@ -624,6 +624,7 @@ PyObject* cache_reorder(PyObject*, PyObject* const* a, Py_ssize_t) {
     if (!parents.is_contiguous()) fail(native_error, "parents have to be contiguous");
     if ((a[6] == Py_None) != (a[7] == Py_None)) fail(native_error, "k_scales and v_scales belong together");
     const char* names[4] = {"cache_k", "cache_v", "k_scales", "v_scales"};
+    int cached = 0;
     for (int i = 0; i < 4; ++i) {
         PyObject* o = i < 2 ? a[i] : a[i + 4];
         const at::Tensor t = strided(device, o, names[i], i < 2 ? 5 : 4, i >= 2);
@@ -632,7 +633,8 @@ PyObject* cache_reorder(PyObject*, PyObject* const* a, Py_ssize_t) {
         if (i >= 2) same_type(t, at::kFloat, names[i], "fp32");
         else if (q8) same_type(t, at::kChar, names[i], "int8 (it has scales)");
         else if (t.scalar_type() == at::kChar) fail(native_error, "an int8 cache needs its scales");
-        else dtype(t);
+        else if (const int type = dtype(t); i == 0) cached = type;
+        else if (type != cached) fail(native_error, "cache_k and cache_v have to have one type");
         const long long e = t.element_size();
         if (i == 0) {
             d.layers = int32(t.size(0)); d.num_pages = int32(t.size(1)); d.slots = int32(t.size(3));

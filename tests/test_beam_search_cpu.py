@@ -52,6 +52,25 @@ def test_no_room_for_a_fork():
     assert c.free == free and not c.shared
 
 
+def test_forks_that_are_refused():
+    c = cache()
+    c.grow([9, 0, 2, 9, 0, 0])
+    free, owned = list(c.free), [list(o) for o in c.owned]
+    for beams in (0, 3, 4, 6):                             # none; sequence 2 or 3 holds something; not a divisor of 6
+        with pytest.raises(ValueError):
+            c.fork(beams, 8)
+    with pytest.raises(ValueError):
+        c.fork(1, -1)
+    assert c.free == free and c.owned == owned and not c.shared
+    c.fork(1, 8)
+    with pytest.raises(ValueError):                        # beams already
+        c.fork(1, 8)
+    c.clear()
+    c.grow([9, 0, 0, 9, 0, 0])
+    c.fork(3, 8)
+    assert c.shared
+
+
 def test_scales_of_a_cache():
     assert cache().k_scales is None and cache().scales(0) == {} and cache().scales() == {}
     c = cache(dtype=torch.int8)
@@ -166,6 +185,14 @@ def test_refused_beams(changed):
     d = Beams(**{**dict(groups=2, beams=4, width=4, vocab=100, dtype=1), **changed})
     assert library().cme_beam_step_ws_bytes(ctypes.byref(d), ctypes.byref(LONG())) != 0
     assert library().cme_beam_step(ctypes.byref(d), None) != 0
+
+
+def test_a_vocabulary_near_the_largest_integer_is_refused():
+    for vocab, fine in ((1 << 30, True), ((1 << 30) + 1, False), (2 ** 31 - 1, False)):
+        d = Beams(groups=1, beams=1, width=1, vocab=vocab, dtype=1, ws_bytes=0)
+        library().cme_beam_step_ws_bytes(ctypes.byref(d), ctypes.byref(LONG()))
+        library().cme_last_error.restype = ctypes.c_char_p
+        assert (b"too many tokens" not in library().cme_last_error()) == fine
 
 
 @pytest.mark.parametrize("changed", [dict(beams=0), dict(groups=-1), dict(slots=0), dict(tensors=5), dict(layers=-1), dict(heads=0), dict(row_bytes=0),

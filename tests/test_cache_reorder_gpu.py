@@ -162,3 +162,10 @@ def test_refusals():
         with pytest.raises(ops.NativeError):
             call(**kw)
     call()
+
+
+def test_keys_and_values_of_two_types_are_refused():
+    (k, v, *rest), _ = make([21, 37], 4, 2, 3, 16, 64, BF16)
+    with pytest.raises(ops.NativeError, match="one type"):
+        ops.cache_reorder(k, v[..., :32].float(), *rest)       # (rows of as many bytes)
+    ops.cache_reorder(k, v, *rest)
