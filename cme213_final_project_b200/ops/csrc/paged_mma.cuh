@@ -482,6 +482,20 @@ template <typename T, typename C, int D, int PARTS> struct Rows8 {
     }
 };
 
+// Of a tile that not all rows see: a NaN among the scales of values goes into its group's scores instead, where the mask takes it from the rows that do not
+// see the group (times a probability of zero it would stay).
+template <typename F> __device__ __forceinline__ void without_nan(float (&sv)[4], F&& scores) {
+    const float any = (sv[0] + sv[1]) + (sv[2] + sv[3]);
+    if (any != any) {                                      // (the same in all lanes)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (sv[n] != sv[n]) {
+                sv[n] = 0.f;
+                scores(n);
+            }
+    }
+}
+
 // As attend() for a cache in 8 bits; sc: the tile's scales, of keys and, 16 further, of values.
 template <typename C, int D, typename R>
 __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t kt, uint32_t vt, uint32_t sc, int key0, int k0, int see0, int see1,
@@ -525,7 +539,8 @@ __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t
         }
     }
     const float4 sk4 = lds128(sc + (key0 >> 3) * 4), sv4 = lds128(sc + 64 + (key0 >> 3) * 4);
-    const float sk[NK] = {sk4.x, sk4.y, sk4.z, sk4.w}, sv[NK] = {sv4.x, sv4.y, sv4.z, sv4.w};
+    const float sk[NK] = {sk4.x, sk4.y, sk4.z, sk4.w};
+    float sv[NK] = {sv4.x, sv4.y, sv4.z, sv4.w};
     const float row_scale[2] = {q.scale[0] * scale_log2, q.scale[1] * scale_log2};
 #pragma unroll
     for (int n = 0; n < NK; ++n)
@@ -536,6 +551,7 @@ __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t
             s[n][2 * r + 1] *= f;
         }
     if (masked) {
+        without_nan(sv, [&](int n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = NAN; });
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -736,13 +752,15 @@ __device__ __forceinline__ void attend8(WarpStateT<C, D>& w, const R& q, uint32_
         }
     }
     const float4 sk4 = lds128(sc + (key0 >> 3) * 4), sv4 = lds128(sc + 64 + (key0 >> 3) * 4);
-    const float sk[4] = {sk4.x, sk4.y, sk4.z, sk4.w}, sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
+    const float sk[4] = {sk4.x, sk4.y, sk4.z, sk4.w};
+    float sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
     const float row_scale[2] = {q.scale[0] * scale_log2, q.scale[1] * scale_log2};
 #pragma unroll
     for (int n = 0; n < MT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[n][i] *= row_scale[i & 1] * sk[n * 2 + (i >> 1)];
     if (masked) {
+        without_nan(sv, [&](int n) { s[n >> 1][(n & 1) * 2] = s[n >> 1][(n & 1) * 2 + 1] = NAN; });
 #pragma unroll
         for (int n = 0; n < MT; ++n)
 #pragma unroll

@@ -31,7 +31,7 @@
 //       maximum is one of x + max(0, log2 sv / c), so that no more than 2^15 comes out.  l is the sum of the groups' sums times its inverse.
 //       Rounded to fp16, 2^-11, and what is below 2^-14 of it to 2^-25: 2^-32 of c, whatever p is.
 // Results are as near to 64 bits as 32-bit sums give (0.0017 of their size; with bf16 operands 0.0023).  Head size 64 has two CTAs an SM: ten warps' registers
-// leave no room for three.  16 chunks of GPT-2 small 35 us; two of 1500 to 2048 over 8192, 32 heads of 128 on 8, 410 us, 0.85 PFLOP/s: shared memory,
+// leave no room for three.  16 chunks of GPT-2 small 36 us; two of 1500 to 2048 over 8192, 32 heads of 128 on 8, 414 us, 0.84 PFLOP/s: shared memory,
 // which the products' operands take for 1000 of a step's 1400 clocks and the tiles' arrival, reading and writing as fp16 for 400 (without those 361 us).
 #pragma once
 #include "paged.h"
@@ -344,7 +344,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 ok = j < C::STAGES || mbar_wait(&v_empty[s], parity, abort_flag);
                 if (!ok) break;
                 if (tid < 8) {
-                    // (above zero, since a masked -inf is multiplied by it; a NaN stays one)
+                    // The exponents' factor is above zero, since a masked -inf is multiplied by it.  Where either scale is a NaN, what is added makes infinite
+                    // probabilities, of which infinite sums become NaN in the end: a NaN would stay where the mask takes the group from a row.
                     const float f = sRawScales[r * 16 + tid] * p.scale_log2, v = sRawScales[r * 16 + 8 + tid];
                     float most = v;
 #pragma unroll
@@ -353,12 +354,12 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         unit = log2f(most);
                         if (tid == 0) sFactors[C::STAGES * PER_STAGE] = unit;
                     }
-                    float c = v < PAGED_SMALLEST_SCALE ? -64.f : log2f(v) - unit;
+                    float c = v >= PAGED_SMALLEST_SCALE ? log2f(v) - unit : -64.f;
                     c = c < -64.f ? -64.f : c > 110.f ? 110.f : c;         // (as good as zero, and more than fp32's largest number allows)
                     float* to = sFactors + s * PER_STAGE + tid;
-                    to[0] = f < 0x1p-60f ? 0x1p-60f : f;
+                    to[0] = f >= 0x1p-60f ? f : 0x1p-60f;
                     to[8] = fmaxf(c, 0.f);
-                    to[16] = c + 7.f;
+                    to[16] = f != f || v != v ? 0x1p127f : c + 7.f;
                     to[24] = exp2f(-7.f - c);
                 }
                 convert(sRaw + (r * 2 + 1) * C::RAW_TILE, sV + s * C::KV_BYTES);
@@ -573,6 +574,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         // (a barrier of its own: the parity of pv_done does not tell the last phase from the one before the one before)
         if (ok && nkv > 0) ok = mbar_wait(&o_done[half], 0, abort_flag);
+        if (Q8) l += l - l;                               // (infinite: NaN)
         if (ok) {
             tc_fence_after();
             const int rr = t.first + row, tok = rr / p.group;

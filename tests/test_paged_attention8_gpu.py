@@ -191,6 +191,28 @@ def test_a_length_at_the_most(dtype, pairs, max_len):
         assert not bool(out.any()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("dtype,backend", [(BF16, "auto"), (BF16, "single"), (BF16, "rows"), (BF16, "tc"), (F32, "auto"), (F32, "single"), (F32, "rows")])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("which", ["k_scales", "v_scales"])
+@pytest.mark.parametrize("splits", [0, 2])
+def test_what_is_no_number_behind_a_row(dtype, backend, D, which, splits):
+    """A block of new tokens is NaN: rows that see some of it are, those before it, which share its tiles, are as they were."""
+    pairs = [(2, 9), (16, 24), (64, 64), (130, 300), (40, 201), (3, 17)]
+    args, scales = make(pairs, 4, 2, D, 16, 8, dtype, seed=11)
+    clean = ops.paged_attention(*args, **scales, backend=backend, splits=splits)
+    table, bad, rows = args[3].cpu(), dict(scales), []
+    bad[which] = bad[which].clone()
+    for b, (n, length) in enumerate(pairs):
+        at = (length - 1 - (n // 3 if n > 16 else 0)) // 8 * 8
+        bad[which][int(table[b, at // 16]), :, at % 16 // 8] = math.nan
+        rows += [length - n + i >= at for i in range(n)]
+    sees = torch.tensor(rows).cuda()
+    assert bool(sees.any()) and not bool(sees.all())
+    out, lse = ops.paged_attention(*args, **bad, backend=backend, splits=splits)
+    assert bool(out[sees].isnan().all()) and bool(out[~sees].isfinite().all())
+    check(args, scales, (torch.where(sees[:, None, None], clean[0], out), torch.where(sees[:, None], clean[1], lse)))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_other_strides_and_scales_of_them(dtype):
     args, scales = make(SINGLES + CHUNKS, 4, 2, 64, 32, 16, dtype, seed=7, token_major=True)
