@@ -11,7 +11,7 @@
 // joins the slices and picks.  Up to 256 tokens (characters) a row is a warp's, in 64 bits, and one launch does both.
 // In scan a thread keeps the sum and the largest of each few of its elements only, which costs no branch; the width-th largest of the best of those
 // bounds what can be chosen from below, and the few groups that hold something above it are looked through again, a vector a thread.
-// What bounds it: the bytes of the logits; 64 x 16 beams of 50304 in fp32, a fifth of which have ended: 54.8 us, of which the scan 43 at 4 TB/s (a third
+// What bounds it: the bytes of the logits; 64 x 16 beams of 50304 in fp32, a fifth of which have ended: 53.9 us, of which the scan 42 at 4 TB/s (a third
 // of a CTA's clocks are its start and its choice) and joining and choosing 9.  16 x 4 beams of 65 tokens 5.8 us.
 //
 // The bound of a log-sum-exp's error: an exponential's argument x - r is rounded twice and multiplied by a rounded log2 e, 2.5 * 2^-24 of |x - r|, which
@@ -34,6 +34,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_WIDTH = 32, MAX_BEAMS = 32;
 constexpr int SCAN = 256;                  // threads of a scan CTA
 constexpr int AHEAD = 4;                   // vectors of a thread in a step
+constexpr int SCANS = 4;                   // CTAs of an SM (six of two vectors ahead: the same time)
 constexpr int STEP = SCAN * AHEAD;         // of a CTA
 constexpr int CAP = 1024;                  // elements that reach the bound that a scan CTA can hold
 constexpr int MERGE = 256;                 // threads of a merge CTA
@@ -149,7 +150,7 @@ template <typename T> __device__ __noinline__ int scan_one_by_one(const CmeBeams
 }
 
 template <typename T>
-__global__ void __launch_bounds__(SCAN, 4) beam_scan_kernel(const __grid_constant__ CmeBeams p, int slices, int slice) {
+__global__ void __launch_bounds__(SCAN, SCANS) beam_scan_kernel(const __grid_constant__ CmeBeams p, int slices, int slice, int resident) {
     constexpr int WARPS = SCAN / 32, N = Slice<T>::N, KEPT = 8;
     __shared__ float group_top[KEPT][SCAN];    // largest of a thread's vectors, `coarse` steps together
     __shared__ __align__(16) float tops[WARPS * 8];
@@ -250,6 +251,17 @@ __global__ void __launch_bounds__(SCAN, 4) beam_scan_kernel(const __grid_constan
     if (end_token >= 0) {
         if (end > limit) raise(end);
         sum += (double)ex2((end - (ref == -INFINITY ? 0.f : ref)) * LOG2E);
+    }
+    // The first two steps of the slice whose CTA comes when this one has gone are on their way to L2 while this one chooses (54.8 us without, 61 with
+    // the whole slice from the start on).
+    if (tid == 0 && blockIdx.x + resident < gridDim.x) {
+        const int other = blockIdx.x + resident, other_row = other / slices, other_part = other - other_row * slices;
+        if (!p.finished || !p.finished[other_row]) {
+            const int from = (int)min((long long)p.vocab, (long long)other_part * slice);
+            const Slice<T> o(p, other_row, from, (int)min((long long)p.vocab, (long long)from + slice));
+            if (o.vectors > 0)
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(o.src + o.a0), "r"(min(o.vectors, 2 * STEP) * 16) : "memory");
+        }
     }
     // (a NaN or +inf among the logits makes the sum a NaN, by which the row is left out)
     // each warp's sum, and the largest 2 ceil(width / warps) of its threads' largest
@@ -639,7 +651,7 @@ template <typename T> int launch(const CmeBeams* a, int sms, cudaStream_t st) {
         return CME_OK;
     }
     const int slices = slices_of(a, sms), slice = cme_cdiv(cme_cdiv(a->vocab, slices), 8) * 8;
-    CME_CUDA(cme_launch_dependent(beam_scan_kernel<T>, dim3(a->groups * a->beams * slices), dim3(SCAN), 0, st, *a, slices, slice));
+    CME_CUDA(cme_launch_dependent(beam_scan_kernel<T>, dim3(a->groups * a->beams * slices), dim3(SCAN), 0, st, *a, slices, slice, sms * SCANS));
     CME_LAUNCH_CHECK();
     int size = 8;                                         // of a group's cluster: as many as run at a time
     while (size > 1 && (long long)a->groups * size > sms * 4ll) size /= 2;
