@@ -27,9 +27,12 @@
 //   q   times a power of two that takes a row's largest element to 2^14 .. 2^15 (exact for elements down to 2^-32 of that one), which the softmax
 //       warps do to their rows first; its inverse belongs to the factor of the exponents, as sk does, of eight keys at a time (the
 //       maximum is taken of these groups' maxima times theirs);
-//   p   times sv / c 2^7, c the largest sv of the CTA's first tile with one: the logarithm of that factor is added to the exponents, and the reference
-//       maximum is one of x + max(0, log2 sv / c), so that no more than 2^15 comes out.  l is the sum of the groups' sums times its inverse.
-//       Rounded to fp16, 2^-11, and what is below 2^-14 of it to 2^-25: 2^-32 of c, whatever p is.
+//   p   times sv 2^7: log2 sv is added to the exponents x, and the reference maximum M is a row's own one of x + log2 sv, so that no more than 2^15 comes
+//       out, whatever scales the keys have that a row does not see.  Rounded to fp16, 2^-11, and what is below 2^-14 to 2^-25: 2^-32 of the
+//       row's largest p sv.  l is the sum of the groups' sums times 2^-8 / (2^7 sv) (2^-8: with sv = 2^-100 the sum of 2^27 keys has room).  A part
+//       of the keys leaves sums that are divided by l, and M + log2 l: 2^M, sv with it, would go out of range in the join.
+//       Values whose sv is below 2^-100, or 2^-100 of a larger one of their tile or before, count as zeros: their p stays in l, which takes no
+//       wider range of log2 sv.
 // Results are as near to 64 bits as 32-bit sums give (0.0017 of their size; with bf16 operands 0.0023).  Head size 64 has two CTAs an SM: ten warps' registers
 // leave no room for three.  16 chunks of GPT-2 small 36 us; two of 1500 to 2048 over 8192, 32 heads of 128 on 8, 414 us, 0.84 PFLOP/s: shared memory,
 // which the products' operands take for 1000 of a step's 1400 clocks and the tiles' arrival, reading and writing as fp16 for 400 (without those 361 us).
@@ -69,7 +72,7 @@ template <> struct Cfg<64, true, true> {
 template <> struct Cfg<128, false, true> {
     static constexpr int HALVES = 2, STAGES = 3, BUFFERS = 2, CTAS = 1, COLS = 512, RAW = 3;
 };
-constexpr int PER_STAGE = 32;              // factors of a tile: 8 of the exponents, 8 added to the maxima, 8 to the exponents, 8 of l
+constexpr int PER_STAGE = 32;              // of a tile: 8 factors of the exponents, 8 log2 sv, 8 that are added to the exponents, 8 factors of l
 template <int D, bool FEW, bool Q8_> struct Sizes : Cfg<D, FEW, Q8_> {
     using C = Cfg<D, FEW, Q8_>;
     static constexpr bool Q8 = Q8_;
@@ -81,7 +84,7 @@ template <int D, bool FEW, bool Q8_> struct Sizes : Cfg<D, FEW, Q8_> {
     static constexpr int THREADS = (LOADER + 1 + CONVERTERS) * 32;
     static constexpr int RAW_TILE = KEYS * D;                         // bytes of 8-bit keys, or values
     static constexpr int RAW_BYTES = Q8 ? 2 * RAW_TILE + 64 : 0;      // of a stage: both and their 16 scales
-    static constexpr int FACTORS = Q8 ? C::STAGES * PER_STAGE * 4 + 16 : 0;      // bytes: what the scales come to, and c
+    static constexpr int FACTORS = Q8 ? C::STAGES * PER_STAGE * 4 : 0;           // bytes: what the scales come to
     static constexpr int SMEM = C::HALVES * Q_BYTES + 2 * C::STAGES * KV_BYTES + C::RAW * RAW_BYTES + FACTORS + 384;
     static constexpr int HALF_COLS = C::COLS / C::HALVES;            // S buffers, then O
     static_assert(C::BUFFERS * KEYS + D <= HALF_COLS && C::CTAS * C::COLS <= 512, "tensor memory");
@@ -128,7 +131,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint8_t* sV = sK + C::STAGES * C::KV_BYTES;
     uint8_t* sRaw = sV + C::STAGES * C::KV_BYTES;              // Q8: [stage] keys and values, then [stage] 8 scales of keys, 8 of values
     float* sRawScales = reinterpret_cast<float*>(sRaw + C::RAW * 2 * C::RAW_TILE);
-    float* sFactors = reinterpret_cast<float*>(sRaw + C::RAW * C::RAW_BYTES);    // Q8: [stage of values][PER_STAGE], then c
+    float* sFactors = reinterpret_cast<float*>(sRaw + C::RAW * C::RAW_BYTES);    // Q8: [stage of values][PER_STAGE]
     uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + C::RAW * C::RAW_BYTES + C::FACTORS);
     uint64_t* q_full = bars;
     uint64_t* k_full = bars + 1;              // [stage]
@@ -314,12 +317,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             // ---------------- 8 bits to fp16 ----------------
             constexpr int CH = D / 16, T = C::CONVERTERS * 32;             // 16-byte pieces of a key
             const int tid = threadIdx.x - (C::LOADER + 1) * 32;
-            auto convert = [&](const uint8_t* from, uint8_t* to) {
+            auto convert = [&](const uint8_t* from, uint8_t* to, auto&& kept) {      // kept(row): all ones, or 0 for zeros in its place
 #pragma unroll
                 for (int i = 0; i < KEYS * CH / T; ++i) {
                     const int at = i * T + tid, r = at / CH, c = at % CH;
                     const uint4 v = *reinterpret_cast<const uint4*>(from + at * 16);
-                    const uint32_t a = v.x ^ 0x80808080u, b = v.y ^ 0x80808080u, d = v.z ^ 0x80808080u, e = v.w ^ 0x80808080u;
+                    const uint32_t k = kept(r);
+                    const uint32_t a = (v.x & k) ^ 0x80808080u, b = (v.y & k) ^ 0x80808080u, d = (v.z & k) ^ 0x80808080u, e = (v.w & k) ^ 0x80808080u;
                     const uint4 x = make_uint4(bytes_to_h2(a, 0x4140), bytes_to_h2(a, 0x4342), bytes_to_h2(b, 0x4140), bytes_to_h2(b, 0x4342));
                     const uint4 y = make_uint4(bytes_to_h2(d, 0x4140), bytes_to_h2(d, 0x4342), bytes_to_h2(e, 0x4140), bytes_to_h2(e, 0x4342));
                     // (eight lanes' stores of a row with 128 bytes go to both slabs: the second four begin with their odd piece, in other banks)
@@ -332,37 +336,31 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 fence_proxy_async();
                 __syncwarp();
             };
-            float unit = -1000.f;                                          // log2 c, once there is one (lanes 0-7 of the first warp)
-            if (tid == 0) sFactors[C::STAGES * PER_STAGE] = 0.f;
+            float largest = 1.f;                                           // scale of values so far, 1 at least
             for (int j = 0; j < nkv; ++j) {
                 const int s = j % C::STAGES, r = j % C::RAW;
                 const uint32_t parity = (j / C::STAGES - 1) & 1;
                 ok = mbar_wait(&raw_full[r], (j / C::RAW) & 1, abort_flag) && (j < C::STAGES || mbar_wait(&k_empty[s], parity, abort_flag));
                 if (!ok) break;
-                convert(sRaw + r * 2 * C::RAW_TILE, sK + s * C::KV_BYTES);
+                convert(sRaw + r * 2 * C::RAW_TILE, sK + s * C::KV_BYTES, [](int) { return 0xffffffffu; });
                 if (lane == 0) mbar_arrive(&k_full[s]);
                 ok = j < C::STAGES || mbar_wait(&v_empty[s], parity, abort_flag);
                 if (!ok) break;
-                if (tid < 8) {
-                    // The exponents' factor is above zero, since a masked -inf is multiplied by it.  Where either scale is a NaN, what is added makes infinite
-                    // probabilities, of which infinite sums become NaN in the end: a NaN would stay where the mask takes the group from a row.
-                    const float f = sRawScales[r * 16 + tid] * p.scale_log2, v = sRawScales[r * 16 + 8 + tid];
-                    float most = v;
+                const float* sv = sRawScales + r * 16 + 8;
 #pragma unroll
-                    for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffu, most, o));
-                    if (unit == -1000.f && most >= PAGED_SMALLEST_SCALE) {
-                        unit = log2f(most);
-                        if (tid == 0) sFactors[C::STAGES * PER_STAGE] = unit;
-                    }
-                    float c = v >= PAGED_SMALLEST_SCALE ? log2f(v) - unit : -64.f;
-                    c = c < -64.f ? -64.f : c > 110.f ? 110.f : c;         // (as good as zero, and more than fp32's largest number allows)
+                for (int g = 0; g < 8; ++g) largest = sv[g] < INFINITY ? fmaxf(largest, sv[g]) : largest;
+                const float least = largest * PAGED_SMALLEST_SCALE;
+                if (tid < 8) {
+                    // Where the scale of values is not finite or that of keys a NaN, what is added makes infinite probabilities, of which infinite sums
+                    // become NaN in the end: a NaN would stay where the mask takes the group from a row.
+                    const float f = sv[tid - 8] * p.scale_log2, v = sv[tid], c = log2f(v >= least && v < INFINITY ? v : least);
                     float* to = sFactors + s * PER_STAGE + tid;
-                    to[0] = f >= 0x1p-60f ? f : 0x1p-60f;
-                    to[8] = fmaxf(c, 0.f);
-                    to[16] = f != f || v != v ? 0x1p127f : c + 7.f;
-                    to[24] = exp2f(-7.f - c);
+                    to[0] = f >= 0x1p-60f ? f : 0x1p-60f;                  // (above zero: a masked -inf is multiplied by it)
+                    to[8] = c;
+                    to[16] = f != f || !(v < INFINITY) ? 0x1p127f : c + 7.f;
+                    to[24] = exp2f(-15.f - c);
                 }
-                convert(sRaw + (r * 2 + 1) * C::RAW_TILE, sV + s * C::KV_BYTES);
+                convert(sRaw + (r * 2 + 1) * C::RAW_TILE, sV + s * C::KV_BYTES, [&](int row) { return sv[row >> 3] >= least ? 0xffffffffu : 0u; });
                 if (lane == 0) { mbar_arrive(&v_full[s]); mbar_arrive(&raw_empty[r]); }
             }
         } else if (elect_one()) {
@@ -499,9 +497,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 mx *= p.scale_log2;                            // scale > 0, so the maximum commutes with it
             }
             const bool raise = j == 0 || mx > m_ref + (j == 1 ? 0.f : RESCALE_THRESHOLD);
-            float alpha = 1.f;
+            float alpha = 1.f, root = 1.f;                     // (root: Q8, of alpha, which can be 0 where l times it is not)
             if (raise) {
-                alpha = (m_ref == -INFINITY) ? 0.f : ex2_approx(m_ref - mx);
+                if (Q8) {
+                    root = (m_ref == -INFINITY) ? 0.f : ex2_approx(0.5f * (m_ref - mx));
+                    alpha = root * root;
+                } else {
+                    alpha = (m_ref == -INFINITY) ? 0.f : ex2_approx(m_ref - mx);
+                }
                 m_ref = mx;
             }
             if (j > 0 && __any_sync(0xffffffffu, raise)) {
@@ -517,7 +520,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
                     tmem_st16(tmem_O + c * 16, o);
                 }
-                l *= alpha;
+                l = Q8 ? l * root * root : l * alpha;
             }
             const float m_use = (m_ref == -INFINITY) ? 0.f : m_ref;
             // The two halves' warps of a scheduler take turns at the exponentials; left alone they fall into step, both wait for the tensor
@@ -579,10 +582,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tc_fence_after();
             const int rr = t.first + row, tok = rr / p.group;
             const long long at = (long long)(t.token0 + tok) * a.heads + head * p.group + rr - tok * p.group;
-            const float unit = Q8 && nkv > 0 ? exp2f(sFactors[C::STAGES * PER_STAGE] - 7.f) : 1.f;       // of the sums
+            constexpr float UNIT = Q8 ? 0x1p-15f : 1.f, RAISED = Q8 ? 8.f : 0.f;       // of the sums over l; log2 of l's own
             if (p.splits == 1) {
                 // the warp's rows through its part of the Q tile (every product is complete), then whole rows to memory
-                const float inv = l == 0.f ? 0.f : unit / l;
+                const float inv = l == 0.f ? 0.f : UNIT / l;
                 uint8_t* stage = sQ + half * C::Q_BYTES + (warp & 3) * 4096;
 #pragma unroll 1
                 for (int c = 0; c < cols / 32; ++c) {
@@ -605,9 +608,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         *reinterpret_cast<uint4*>(out + to * cols + c * 8) =
                             *reinterpret_cast<const uint4*>(stage + (c >> 3) * C::Q_SLAB + swz(r, c & 7));
                 }
-                if (mine) a.lse[at] = l == 0.f ? -INFINITY : m_ref == -INFINITY ? l : (m_ref + log2f(l)) / LOG2E;
+                if (mine) a.lse[at] = l == 0.f ? -INFINITY : m_ref == -INFINITY ? l : (m_ref + (log2f(l) + RAISED)) / LOG2E;
             } else {
                 const long long part = at * p.splits + split;
+                const float inv = Q8 ? (l == 0.f ? 0.f : UNIT / l) : 1.f;
                 if (nkv > 0) {
 #pragma unroll 1
                     for (int c = 0; c < cols / 32; ++c) {
@@ -618,12 +622,12 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
                                 *reinterpret_cast<float4*>(p.part_o + part * cols + c * 32 + i) =
-                                    make_float4(__uint_as_float(o[i]) * unit, __uint_as_float(o[i + 1]) * unit, __uint_as_float(o[i + 2]) * unit,
-                                                __uint_as_float(o[i + 3]) * unit);
+                                    make_float4(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv, __uint_as_float(o[i + 2]) * inv,
+                                                __uint_as_float(o[i + 3]) * inv);
                         }
                     }
                 }
-                if (mine) p.part_ml[part] = make_float2(m_ref, l);
+                if (mine) p.part_ml[part] = !Q8 ? make_float2(m_ref, l) : l == 0.f ? make_float2(-INFINITY, 0.f) : make_float2(m_ref + (log2f(l) + RAISED), 1.f);
             }
         }
     }
