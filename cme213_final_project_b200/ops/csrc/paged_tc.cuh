@@ -355,7 +355,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                     // become NaN in the end: a NaN would stay where the mask takes the group from a row.
                     const float f = sv[tid - 8] * p.scale_log2, v = sv[tid], c = log2f(v >= least && v < INFINITY ? v : least);
                     float* to = sFactors + s * PER_STAGE + tid;
-                    to[0] = f >= 0x1p-60f ? f : 0x1p-60f;                  // (above zero: a masked -inf is multiplied by it)
+                    to[0] = f == f ? f : 0.f;
                     to[8] = c;
                     to[16] = f != f || !(v < INFINITY) ? 0x1p127f : c + 7.f;
                     to[24] = exp2f(-15.f - c);
@@ -427,8 +427,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                         most = max(most, max(w & 0x7fff0000u, (w << 16) & 0x7fff0000u));
                     }
                 }
-                // (up to 2^60: its inverse times the smallest factor of the exponents is above zero)
-                const unsigned up = min(268u - (most >> 23), 187u);
+                const unsigned up = min(268u - (most >> 23), 253u);        // (as far as its inverse is not denormal)
                 const float f = __uint_as_float(up << 23);
                 row_scale = __uint_as_float((254u - up) << 23);
 #pragma unroll
@@ -477,7 +476,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     const float* x = reinterpret_cast<const float*>(r + g * 8);
-                    by[g] = factors[g] * row_scale;
+                    by[g] = fmaxf(factors[g] * row_scale, 0x1p-126f);      // (above zero: a masked -inf is multiplied by it)
                     best[g] = fmaf(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7])), by[g], factors[8 + g]);
                 }
                 mx = max3(max3(best[0], best[1], best[2]), max3(best[3], best[4], best[5]), fmaxf(best[6], best[7]));

@@ -96,3 +96,12 @@ def test_blocks_of_no_values(backend, splits, D, value):
     for sv in ([value] * blocks, [value] * 20 + [3.0] * 10, [value] * 3 + [2.0 ** 40] + [value] * 26, [2.0 ** 40] + [value] * 29):
         args, scales = case(200, 240, D, [0.01] * blocks, sv, seed=2)
         check(args, scales, ops.paged_attention(*args, **scales, backend=backend, splits=splits), D ** -0.5, beyond=True)
+
+
+@pytest.mark.parametrize("backend,splits", FORMS)
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("power", [-90, -60, 60, 90])
+def test_large_queries_and_small_keys(backend, splits, D, power):
+    """Queries times 2^-power, keys times 2^power: the scores are what they were."""
+    args, scales = case(100, 240, D, [0.01 * 2.0 ** power] * 30, [0.02] * 30, q_scale=2.0 ** -power, seed=3)
+    check(args, scales, ops.paged_attention(*args, **scales, backend=backend, splits=splits), D ** -0.5)
