@@ -454,8 +454,8 @@ def paged_attention(q, cache_k, cache_v, pages, offsets, lengths, *, scale: Opti
     through scratch memory in any case.
 
     ``k_scales``, ``v_scales``: of an int8 cache, as :func:`cache_append` makes it; ``q`` and the result are bf16 or fp32 all the same.  Scales
-    of values below ``2 ** -100`` count as 0, and those below that of a larger one of the sequence may; those of blocks that no sequence has reached may be anything.  Where one is a NaN, rows that see some
-    of its block are NaN, and no others."""
+    (not below 0) of values below ``2 ** -100`` count as 0, and those below that of a larger one of the sequence may.  Scales of blocks that a row does not
+    see may be anything, as those that no sequence has reached; where one is a NaN, rows that see some of its block are NaN, and no others."""
     if k_scales is not None or v_scales is not None:
         return _native().paged_attention8(q, cache_k, cache_v, pages, offsets, lengths, scale, max_len, _PAGED_BACKENDS[backend], splits,
                                           k_scales, v_scales)

@@ -19,8 +19,8 @@
 // a bit too few and takes four), so the products run on fp16 operands:
 //   scores   q times a power of two that takes a row's largest element to 2^14 .. 2^15 (exact for bf16 elements down to 2^-32 of that one;
 //            fp32 in two fp16 parts, 22 bits), S times its inverse and sk afterwards;
-//   sums     p times 2^15 sv / (the largest sv of 32 keys), so that a key with p = 2^-29 still has all 11 bits, for bf16 queries rounded to fp16 (2^-12),
-//            for fp32 in two parts; the 32 keys' sum times (the largest sv) 2^-15 is added in 32 bits.
+//   sums     p times 2^15 sv / (the largest sv of 32 keys, of those that the row sees), so that a key with p = 2^-29 still has all 11 bits, for bf16 queries
+//            rounded to fp16 (2^-11), for fp32 in two parts; the 32 keys' sum times (the largest sv) 2^-15 is added in 32 bits.
 // A lane reads K in pieces of 16 bytes along its row (which column stands at which place of a product's step does not matter, as long as q's stand
 // there too); V comes through ldmatrix as pairs of bytes, of which the low ones are one column tile and the high ones another.
 // The scales of a tile travel with it, four bytes each, one for every eight keys.
@@ -482,18 +482,20 @@ template <typename T, typename C, int D, int PARTS> struct Rows8 {
     }
 };
 
-// Of a tile that not all rows see: a NaN among the scales of values goes into its group's scores instead, where the mask takes it from the rows that do not
-// see the group (times a probability of zero it would stay).
-template <typename F> __device__ __forceinline__ void without_nan(float (&sv)[4], F&& scores) {
-    const float any = (sv[0] + sv[1]) + (sv[2] + sv[3]);
-    if (any != any) {                                      // (the same in all lanes)
+// What the probabilities of four groups of eight keys are multiplied by for one row, and (returned) what their products with the integers are: 2^15 sv / (the
+// largest sv that the row sees) and its inverse times sv.  A group that the row does not see has 0, so that neither its scale's size nor a NaN or an
+// infinity there touches the row (times a probability of zero these would stay); where it sees one, its factors are NaN.
+template <typename F> __device__ __forceinline__ float value_factors(const float (&sv)[4], float (&f)[4], F&& seen) {
+    float most = 0.f;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-            if (sv[n] != sv[n]) {
-                sv[n] = 0.f;
-                scores(n);
-            }
+    for (int n = 0; n < 4; ++n) {
+        f[n] = seen(n) ? sv[n] : 0.f;
+        most = fmaxf(most, f[n]);                          // (passes over a NaN, which is in its own factor all the same)
     }
+    const float up = most >= PAGED_SMALLEST_SCALE ? 32768.f * rcp_approx(most) : 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) f[n] *= up;
+    return most * (1.f / 32768.f);
 }
 
 // As attend() for a cache in 8 bits; sc: the tile's scales, of keys and, 16 further, of values.
@@ -540,7 +542,7 @@ __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t
     }
     const float4 sk4 = lds128(sc + (key0 >> 3) * 4), sv4 = lds128(sc + 64 + (key0 >> 3) * 4);
     const float sk[NK] = {sk4.x, sk4.y, sk4.z, sk4.w};
-    float sv[NK] = {sv4.x, sv4.y, sv4.z, sv4.w};
+    const float sv[NK] = {sv4.x, sv4.y, sv4.z, sv4.w};
     const float row_scale[2] = {q.scale[0] * scale_log2, q.scale[1] * scale_log2};
 #pragma unroll
     for (int n = 0; n < NK; ++n)
@@ -551,7 +553,6 @@ __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t
             s[n][2 * r + 1] *= f;
         }
     if (masked) {
-        without_nan(sv, [&](int n) { s[n][0] = s[n][1] = s[n][2] = s[n][3] = NAN; });
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -583,54 +584,63 @@ __device__ __forceinline__ void attend8(WarpState<C, D>& w, const R& q, uint32_t
 #pragma unroll
         for (int n = 0; n < NT; ++n) { w.o[n][0] *= alpha[0]; w.o[n][1] *= alpha[0]; w.o[n][2] *= alpha[1]; w.o[n][3] *= alpha[1]; }
     }
-    // (fmaxf passes over a NaN, which is in its own factor all the same)
-    const float most = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-    const float up = most >= PAGED_SMALLEST_SCALE ? 32768.f * rcp_approx(most) : 0.f, down = most * (1.f / 32768.f);
-    uint32_t ph[NK][2], pl[NK][2];
+    // (A tile that all rows see, as most are, has one set of factors for both: with two sets in every tile 64 single tokens of up to 1024, 16 heads of 64, take
+    // 34.9 us for 31.6.)
+    auto add_values = [&](auto each) {
+        constexpr int EACH = decltype(each)::value;            // sets of factors
+        float f[EACH][4], down[EACH];
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-        const float f = sv[n] * up;
+        for (int r = 0; r < EACH; ++r)
+            down[r] = value_factors(sv, f[r], [&](int n) {
+                return EACH == 1 || ((there >> ((key0 + n * 8) >> box_log)) & 1 && k0 + key0 + n * 8 < (r ? see1 : see0));
+            });
+        uint32_t ph[NK][2], pl[NK][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float x = ex2_approx(s[n][2 * r] - use[r]), y = ex2_approx(s[n][2 * r + 1] - use[r]);
-            w.l[r] += x + y;
-            ph[n][r] = f2_to_h2(x * f, y * f);
-            if constexpr (C::F32) {
-                const float2 h = h2_to_f2(ph[n][r]);
-                pl[n][r] = f2_to_h2(fmaf(x, f, -h.x), fmaf(y, f, -h.y));
-            }
-        }
-    }
+        for (int n = 0; n < NK; ++n) {
 #pragma unroll
-    for (int c = 0; c < D / 16; c += 2) {                  // 16 bytes of a value each
-        float acc[4][4], low[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-            low[i][0] = low[i][1] = low[i][2] = low[i][3] = 0.f;
-        }
-#pragma unroll
-        for (int n = 0; n < NK; n += 2) {
-            const uint32_t pa[4] = {ph[n][0], ph[n][1], ph[n + 1][0], ph[n + 1][1]};
-            uint32_t b[4];
-            ldsm4_t(vt + chunk_at<C>(key0 + n * 8 + (((lane >> 3) & 1) << 3) + (lane & 7), c + (lane >> 4)), b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {                  // tile i: even (odd) columns of chunk c + i / 2
-                const uint32_t pick = i & 1 ? 0x4341 : 0x4240, b0 = bytes_to_h2(b[i & 2], pick), b1 = bytes_to_h2(b[(i & 2) + 1], pick);
-                mma_f16(acc[i], pa, b0, b1);
+            for (int r = 0; r < 2; ++r) {
+                const float x = ex2_approx(s[n][2 * r] - use[r]), y = ex2_approx(s[n][2 * r + 1] - use[r]);
+                w.l[r] += x + y;
+                ph[n][r] = f2_to_h2(x * f[EACH > 1 ? r : 0][n], y * f[EACH > 1 ? r : 0][n]);
                 if constexpr (C::F32) {
-                    const uint32_t pb[4] = {pl[n][0], pl[n][1], pl[n + 1][0], pl[n + 1][1]};
-                    mma_f16(low[i], pb, b0, b1);
+                    const float2 h = h2_to_f2(ph[n][r]);
+                    pl[n][r] = f2_to_h2(fmaf(x, f[EACH > 1 ? r : 0][n], -h.x), fmaf(y, f[EACH > 1 ? r : 0][n], -h.y));
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int c = 0; c < D / 16; c += 2) {                  // 16 bytes of a value each
+            float acc[4][4], low[4][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[c * 2 + i][e] = fmaf(down, C::F32 ? acc[i][e] + low[i][e] : acc[i][e], w.o[c * 2 + i][e]);
-    }
+            for (int i = 0; i < 4; ++i) {
+                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+                low[i][0] = low[i][1] = low[i][2] = low[i][3] = 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < NK; n += 2) {
+                const uint32_t pa[4] = {ph[n][0], ph[n][1], ph[n + 1][0], ph[n + 1][1]};
+                uint32_t b[4];
+                ldsm4_t(vt + chunk_at<C>(key0 + n * 8 + (((lane >> 3) & 1) << 3) + (lane & 7), c + (lane >> 4)), b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {                  // tile i: even (odd) columns of chunk c + i / 2
+                    const uint32_t pick = i & 1 ? 0x4341 : 0x4240, b0 = bytes_to_h2(b[i & 2], pick), b1 = bytes_to_h2(b[(i & 2) + 1], pick);
+                    mma_f16(acc[i], pa, b0, b1);
+                    if constexpr (C::F32) {
+                        const uint32_t pb[4] = {pl[n][0], pl[n][1], pl[n + 1][0], pl[n + 1][1]};
+                        mma_f16(low[i], pb, b0, b1);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[c * 2 + i][e] = fmaf(down[EACH > 1 ? e >> 1 : 0], C::F32 ? acc[i][e] + low[i][e] : acc[i][e], w.o[c * 2 + i][e]);
+        }
+    };
+    if (masked) add_values(std::integral_constant<int, 2>{});
+    else add_values(std::integral_constant<int, 1>{});
 }
 
 // Up to eight rows over a cache in 8 bits, the other way round: keys, and columns of V, are the 16 rows of a product and the rows its 8 columns, so that no
@@ -753,14 +763,13 @@ __device__ __forceinline__ void attend8(WarpStateT<C, D>& w, const R& q, uint32_
     }
     const float4 sk4 = lds128(sc + (key0 >> 3) * 4), sv4 = lds128(sc + 64 + (key0 >> 3) * 4);
     const float sk[4] = {sk4.x, sk4.y, sk4.z, sk4.w};
-    float sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
+    const float sv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
     const float row_scale[2] = {q.scale[0] * scale_log2, q.scale[1] * scale_log2};
 #pragma unroll
     for (int n = 0; n < MT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[n][i] *= row_scale[i & 1] * sk[n * 2 + (i >> 1)];
     if (masked) {
-        without_nan(sv, [&](int n) { s[n >> 1][(n & 1) * 2] = s[n >> 1][(n & 1) * 2 + 1] = NAN; });
 #pragma unroll
         for (int n = 0; n < MT; ++n)
 #pragma unroll
@@ -790,50 +799,59 @@ __device__ __forceinline__ void attend8(WarpStateT<C, D>& w, const R& q, uint32_
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) { w.o[n][0] *= alpha[0]; w.o[n][1] *= alpha[1]; w.o[n][2] *= alpha[0]; w.o[n][3] *= alpha[1]; }
     }
-    // (fmaxf passes over a NaN, which is in its own factor all the same)
-    const float most = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-    const float up = most >= PAGED_SMALLEST_SCALE ? 32768.f * rcp_approx(most) : 0.f, down = most * (1.f / 32768.f);
-    uint32_t ph[4], pl[4];                                 // of eight keys each
+    // (A tile that all rows see, as most are, has one set of factors for both: with two sets in every tile 64 single tokens of up to 1024, 16 heads of 64, take
+    // 34.9 us for 31.6.)
+    auto add_values = [&](auto each) {
+        constexpr int EACH = decltype(each)::value;            // sets of factors
+        float f[EACH][4], down[EACH];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const float f = sv[n] * up;
-        const float x = ex2_approx(s[n >> 1][(n & 1) * 2] - use[0]), y = ex2_approx(s[n >> 1][(n & 1) * 2 + 1] - use[1]);
-        w.l[0] += x;
-        w.l[1] += y;
-        const uint32_t p = f2_to_h2(x * f, y * f);
-        ph[n] = transpose8(p);
-        if constexpr (C::F32) {
-            const float2 h = h2_to_f2(p);
-            pl[n] = transpose8(f2_to_h2(fmaf(x, f, -h.x), fmaf(y, f, -h.y)));
-        }
-    }
+        for (int r = 0; r < EACH; ++r)
+            down[r] = value_factors(sv, f[r], [&](int n) {
+                return EACH == 1 || ((there >> ((key0 + n * 8) >> box_log)) & 1 && k0 + key0 + n * 8 < (r ? see1 : see0));
+            });
+        uint32_t ph[4], pl[4];                                 // of eight keys each
 #pragma unroll
-    for (int c = 0; c < D / 16; c += 2) {                  // 16 bytes of a value each
-        float acc[2][4], low[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-            low[i][0] = low[i][1] = low[i][2] = low[i][3] = 0.f;
-        }
-#pragma unroll
-        for (int n = 0; n < 4; n += 2) {
-            uint32_t b[4];
-            ldsm4_t(vt + chunk_at<C>(key0 + n * 8 + (((lane >> 3) & 1) << 3) + (lane & 7), c + (lane >> 4)), b);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t a[4] = {bytes_to_h2(b[2 * i], 0x4240), bytes_to_h2(b[2 * i], 0x4341), bytes_to_h2(b[2 * i + 1], 0x4240),
-                                       bytes_to_h2(b[2 * i + 1], 0x4341)};
-                mma_f16(acc[i], a, ph[n], ph[n + 1]);
-                if constexpr (C::F32) mma_f16(low[i], a, pl[n], pl[n + 1]);
+        for (int n = 0; n < 4; ++n) {
+            const float x = ex2_approx(s[n >> 1][(n & 1) * 2] - use[0]), y = ex2_approx(s[n >> 1][(n & 1) * 2 + 1] - use[1]);
+            w.l[0] += x;
+            w.l[1] += y;
+            const uint32_t p = f2_to_h2(x * f[0][n], y * f[EACH - 1][n]);
+            ph[n] = transpose8(p);
+            if constexpr (C::F32) {
+                const float2 h = h2_to_f2(p);
+                pl[n] = transpose8(f2_to_h2(fmaf(x, f[0][n], -h.x), fmaf(y, f[EACH - 1][n], -h.y)));
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int c = 0; c < D / 16; c += 2) {                  // 16 bytes of a value each
+            float acc[2][4], low[2][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[c + i][e] = fmaf(down, C::F32 ? acc[i][e] + low[i][e] : acc[i][e], w.o[c + i][e]);
-    }
+            for (int i = 0; i < 2; ++i) {
+                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+                low[i][0] = low[i][1] = low[i][2] = low[i][3] = 0.f;
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n += 2) {
+                uint32_t b[4];
+                ldsm4_t(vt + chunk_at<C>(key0 + n * 8 + (((lane >> 3) & 1) << 3) + (lane & 7), c + (lane >> 4)), b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) b[i] ^= 0x80808080u;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t a[4] = {bytes_to_h2(b[2 * i], 0x4240), bytes_to_h2(b[2 * i], 0x4341), bytes_to_h2(b[2 * i + 1], 0x4240),
+                                           bytes_to_h2(b[2 * i + 1], 0x4341)};
+                    mma_f16(acc[i], a, ph[n], ph[n + 1]);
+                    if constexpr (C::F32) mma_f16(low[i], a, pl[n], pl[n + 1]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[c + i][e] = fmaf(down[EACH > 1 ? e & 1 : 0], C::F32 ? acc[i][e] + low[i][e] : acc[i][e], w.o[c + i][e]);
+        }
+    };
+    if (masked) add_values(std::integral_constant<int, 2>{});
+    else add_values(std::integral_constant<int, 1>{});
 }
 
 // fp32 with R <= 4 rows on the CUDA cores: sixteen rows' worth of tf32 products would take longer than the tile's bytes (a 64 KB tile 2.1 us

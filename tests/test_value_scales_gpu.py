@@ -105,3 +105,36 @@ def test_large_queries_and_small_keys(backend, splits, D, power):
     """Queries times 2^-power, keys times 2^power: the scores are what they were."""
     args, scales = case(100, 240, D, [0.01 * 2.0 ** power] * 30, [0.02] * 30, q_scale=2.0 ** -power, seed=3)
     check(args, scales, ops.paged_attention(*args, **scales, backend=backend, splits=splits), D ** -0.5)
+
+
+@pytest.mark.parametrize("backend,splits", [f for f in FORMS if f[0] != "tc"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("small", [-20, -40, -60])
+def test_rows_that_see_small_blocks_only_by_warps(backend, splits, D, small):
+    test_rows_that_see_small_blocks_only(backend, splits, D, small)
+
+
+@pytest.mark.parametrize("dtype,backend,splits", [(BF16, *f) for f in FORMS] + [(F32, *f) for f in FORMS if f[0] != "tc"])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("n,length", [(8, 20), (100, 140)])
+@pytest.mark.parametrize("behind", [0.0, 2.0 ** -60, 2.0 ** 60, math.inf, math.nan])
+def test_bits_hang_on_what_a_row_sees(dtype, backend, splits, D, n, length, behind):
+    """The scales of blocks that a row does not see, of keys or of values, may be anything."""
+    blocks = -(-length // BLOCK)
+    args, scales = case(n, length, D, [0.01] * blocks, [0.02] * blocks, seed=4)
+    args[0] = args[0].to(dtype)
+    clean = ops.paged_attention(*args, **scales, backend=backend, splits=splits)
+    at = length - n // 2
+    first = -(-at // BLOCK)                                  # of the changed blocks
+    rows = first * BLOCK - (length - n)                      # those before it
+    assert 0 < rows < n
+    for which in scales:
+        other = {name: s.clone() for name, s in scales.items()}
+        for b in range(first, blocks):
+            other[which][b // 2, :, b % 2] = behind
+        got = ops.paged_attention(*args, **other, backend=backend, splits=splits)
+        for x, y in zip(clean, got):
+            assert torch.equal(x[:rows], y[:rows])
+        if behind == math.nan or behind == math.inf and which == "v_scales":
+            assert bool(got[0][rows:].isnan().any())
+    assert ops.attention_check_status() == 0
