@@ -487,7 +487,8 @@ def beam_step(logits, scores, width: Optional[int] = None, *, finished=None, all
     ``logits``: bf16 or fp32 ``[groups * beams, vocab]``, after each beam's last token; ``scores``: fp32 ``[groups, beams]``.  Token t
     after beam b is worth ``scores[b] + logits[b, t] - logsumexp(logits[b])``, over the tokens whose bit of ``allowed`` (as
     :func:`next_token` takes it) is set.  A beam of ``finished`` (bool ``[groups, beams]``) has one continuation: itself, with token -1
-    and its score.  Ordered by these values as real numbers (not by their rounded ones); equals by beam, then by token.  A beam
+    and its score.  Ordered by these values as real numbers (not by their rounded ones; those of
+    different beams as far as 64 bits tell them apart); equals by beam, then by token.  A beam
     whose score is not finite, and one without a finite log-sum-exp (no token allowed, a NaN or ``inf`` among its logits), has none.
     Where a group has fewer than ``width``, the others are ``(place % beams, -1, -inf)``."""
     return _native().beam_step(logits, scores, width, finished, allowed)

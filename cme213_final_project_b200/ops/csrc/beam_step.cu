@@ -2,9 +2,10 @@
 //
 //     value(beam, token) = score[beam] + x[token] - log sum exp x;      a finished beam has one continuation, itself, with its score
 //
-// The order is that of the values as real numbers; equal ones: lower beam, lower token.  Within a beam that is the order of x.  Between beams
+// The order is that of the values as real numbers; equal ones: lower beam, lower token.  Within a beam that is the order of x, also where the values'
+// 64 bits are the same.  Between beams
 // it hangs on the log-sum-exps, whose 32-bit sums are off by some 2^-20; so every pair of different beams that decides something is held
-// against a bound of that error, and where one is closer, the log-sum-exps of its beams are made anew in 64 bits.  Equal rows have equal
+// against a bound of that error, and where one is closer, the log-sum-exps of its beams are made anew in 64 bits, which decide.  Equal rows have equal
 // ones then, too.
 //
 // Two launches: `scan` goes once over the logits, a CTA a slice of a row: sum of exponentials and the `width` largest; `merge`, a CTA a group,
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(SCAN, SCANS) beam_scan_kernel(const __grid_con
 // ------------------------------------------------------------------------------------------------------
 struct Select {
     double value[SURVIVORS];
-    int beam[SURVIVORS], token[SURVIVORS];
+    int from[SURVIVORS], token[SURVIVORS]; // from: beam, list << 8, place in it << 16
     double lse[MAX_BEAMS], score[MAX_BEAMS];
     double slack;                          // twice the largest error of a log-sum-exp
     int counted;
@@ -365,8 +366,12 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, Beam&
         const Cand c = at(l, k);
         return c.token < 0 ? sel.score[b] : sel.score[b] + ((double)c.x - sel.lse[b]);
     };
-    // The width-th best of the lists' first ones bounds the choice from below.  Of equal values those of the list before come first: a list
-    // of a lower beam, or of lower tokens.  With slack 0 no more than `width` lists are that good, so all that is chosen from fits.
+    // Whether (v, b, x, t) comes before (u, c, y, s): value, beam, logit, token.
+    auto ahead = [](double v, int b, float x, int t, double u, int c, float y, int s) {
+        return v > u || (v == u && (b < c || (b == c && (x > y || (x == y && t < s)))));
+    };
+    // The width-th best of the lists' first ones bounds the choice from below (of a beam's lists those before have the lower tokens).  With slack 0 no
+    // more than `width` lists are that good, so all that is chosen from fits.
     __syncthreads();
     if (tid == 0) { sel.counted = 0; sel.close = 0; sel.last = -1; }
     for (int l = tid; l < lists; l += THREADS) sel.heads[l] = count_of(l) ? value(l, 0) : -INFINITY;
@@ -374,22 +379,26 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, Beam&
     if (lists > p.width) {
         for (int l = tid; l < lists; l += THREADS) {
             const double v = sel.heads[l];
-            int above = 0;
+            if (v == -INFINITY) continue;
+            int above = 0, equal = 0;                      // (itself among them)
 #pragma unroll 4
-            for (int k = 0; k < lists; ++k) above += sel.heads[k] > v || (sel.heads[k] == v && k < l);
+            for (int k = 0; k < lists; ++k) { above += sel.heads[k] > v; equal += sel.heads[k] == v; }
+            for (int k = 0; equal > 1 && k < lists; ++k) above += sel.heads[k] == v && ahead(v, beam_of(k), at(k, 0).x, k, v, beam_of(l), at(l, 0).x, l);
             if (above == p.width - 1) sel.last = l;
         }
         __syncthreads();
     }
-    const int bound_list = sel.last < 0 ? lists : sel.last;
-    const double bound = sel.last < 0 ? -INFINITY : sel.heads[sel.last] - slack;
+    const int last = sel.last, last_beam = last < 0 ? 0 : beam_of(last);
+    const double bound = last < 0 ? -INFINITY : sel.heads[last] - slack;
+    const Cand last_head = last < 0 || sel.heads[last] == -INFINITY ? Cand{0.f, 0} : at(last, 0);
     for (int l = warp; l < lists; l += THREADS / 32) {     // a warp a list
         const int k = lane;
         if (k >= count_of(l) || sel.heads[l] < bound) continue;
         const double v = value(l, k);
-        if (!(v > bound || (v == bound && (slack > 0.0 || l < bound_list || (l == bound_list && k == 0))))) continue;
+        const Cand own = at(l, k);
+        if (v < bound || (v == bound && slack == 0.0 && ahead(v, last_beam, last_head.x, last_head.token, v, beam_of(l), own.x, own.token))) continue;
         const int c = atomicAdd(&sel.counted, 1);
-        if (c < SURVIVORS) { sel.value[c] = v; sel.beam[c] = beam_of(l); sel.token[c] = at(l, k).token; }
+        if (c < SURVIVORS) { sel.value[c] = v; sel.from[c] = beam_of(l) | l << 8 | k << 16; sel.token[c] = own.token; }
     }
     __syncthreads();
     const int n = sel.counted;
@@ -404,16 +413,20 @@ __device__ bool pick(Select& sel, const CmeBeams& p, int group, int lists, Beam&
         const int i = i0 + tid / SHARE;
         const bool in = i < n;
         const double v = in ? sel.value[i] : 0.0;
-        const int b = in ? sel.beam[i] : 0, t = in ? sel.token[i] : 0;
-        int rank = 0;
+        const int from = in ? sel.from[i] : 0, b = from & 255, t = in ? sel.token[i] : 0;
+        int rank = 0, equal = 0;
         unsigned near = 0;
 #pragma unroll 4
         for (int k = tid % SHARE; k < n; k += SHARE) {
             const double u = sel.value[k];
-            const int c = sel.beam[k];
-            rank += u > v || (u == v && (c < b || (c == b && sel.token[k] < t)));
+            const int c = sel.from[k] & 255;
+            rank += u > v || (u == v && c < b);
+            equal += u == v && c == b && k != i;
             if (c != b && fabs(u - v) <= slack) near |= 1u << c;
         }
+        for (int k = tid % SHARE; equal && k < n; k += SHARE)
+            if (sel.value[k] == v && (sel.from[k] & 255) == b)
+                rank += ahead(v, b, at(sel.from[k] >> 8 & 255, sel.from[k] >> 16).x, sel.token[k], v, b, at(from >> 8 & 255, from >> 16).x, t);
 #pragma unroll
         for (int o = 1; o < SHARE; o <<= 1) {
             rank += __shfl_xor_sync(0xffffffffu, rank, o);
