@@ -380,6 +380,7 @@ class Generator:
             of = parents.long()
             history.copy_(history[(first_row + of).view(-1)])
             history.index_copy_(1, newest.view(1), token.view(-1, 1))
+            history.masked_fill_((scores == -torch.inf).view(-1, 1), -1)      # (no continuation: none of a past one either)
             over = finished.gather(1, of)
             finished.copy_(over if end is None else over | (token == end))
 
