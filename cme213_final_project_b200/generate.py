@@ -117,16 +117,16 @@ class PagedCache:
             if n + new > self.max_len:
                 raise ValueError(f"sequence {g}: {n + new} tokens, {self.max_len} at the most")
             full = n // self.page
-            need += full + beams * (-(-(n + new) // self.page) - full + 1)
+            need += full + beams * (-(-(n + new) // self.page) - full + (beams > 1))
         if need > pages:
             raise CacheFull(f"{need} pages are needed, the cache has {pages}")
         return need
 
     def fork(self, beams: int, new: int) -> torch.Tensor:
         """The first sequence of each group of ``beams`` holds a prompt, the others nothing: give all of them room for ``new`` more
-        tokens, and a spare page each.  Returns these (int32 ``[seqs]``), as ``ops.cache_reorder`` takes them; that call with all parents 0
-        then lets the others go on from the prompt.  Until :meth:`clear` no sequence grows or is released.  Raises :class:`CacheFull` or
-        ``ValueError`` before anything has changed."""
+        tokens, and a spare page each (-1: a beam alone, which goes on from none but itself, needs none).  Returns these (int32 ``[seqs]``), as
+        ``ops.cache_reorder`` takes them; that call with all parents 0 then lets the others go on from the prompt.  Until :meth:`clear` no
+        sequence grows or is released.  Raises :class:`CacheFull` or ``ValueError`` before anything has changed."""
         if self.shared:
             raise ValueError("the sequences are beams already: clear()")
         if beams < 1 or len(self.owned) % beams or new < 0:
@@ -142,8 +142,9 @@ class PagedCache:
                 cols.append(col)
                 ids.append(self.free.pop())
                 self.owned[b].append(ids[-1])
-            spare.append(self.free.pop())
-            self.owned[b].append(spare[-1])
+            spare.append(self.free.pop() if beams > 1 else -1)
+            if beams > 1:
+                self.owned[b].append(spare[-1])
         self.shared = True
         device = self.table.device
         if ids:
@@ -503,7 +504,7 @@ def main(argv: Optional[Sequence[str]] = None) -> int:
         else:
             sampling = Sampling(0.8 if a.temperature is None else a.temperature, a.repetition, a.presence, a.frequency, None, allowed)
             tokens, logprobs = gen.generate(prompts, a.max_new, sampling, a.seed, a.chunk, not a.no_cuda_graph)
-    except ValueError as e:
+    except (ValueError, CacheFull) as e:
         print(f"Error: {e}", file=sys.stderr)
         return 1
     from . import ops

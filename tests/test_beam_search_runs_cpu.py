@@ -103,3 +103,33 @@ def test_few_tokens_at_first():
     assert bool((scores[:, :2] > -math.inf).all()) and bool((scores[:, 2:] == -math.inf).all()) and bool((tokens[:, 2:] == -1).all())
     tokens, scores = g.beam_search(PROMPTS, 3, allowed=[3, 7], cuda_graph=False)
     assert bool((scores > -math.inf).all()) and set(tokens.unique().tolist()) == {3, 7}
+
+
+@pytest.mark.parametrize("beams", [1, 2, 4])
+def test_up_to_the_last_position_with_the_pages_of_the_default(beams):
+    g = generator(beams)
+    tokens, _ = g.beam_search([PROMPTS[0], [1] * 5], 48 - 5 + 1, cuda_graph=False)
+    assert tokens.shape == (2, beams, 44) and bool((tokens >= 0).all())
+    g.beam_search([PROMPTS[0], [1] * 48], 1, cuda_graph=False)                   # a prompt that fills it
+
+
+def test_one_beam_is_a_run():
+    """Of one beam the best continuation goes on, as in a run without sampling; it needs no spare page."""
+    g = generator(1)
+    tokens, scores = g.beam_search(PROMPTS, 9, cuda_graph=False)
+    for row, p in zip(tokens[:, 0].tolist(), PROMPTS):
+        one = generator(1)
+        for t in row:
+            assert int(one.prefill([p, [0]])[0].argmax()) == t
+            p = p + [t]
+
+
+def test_books_of_one_beam():
+    g = generator(1)
+    c = g.cache
+    c.grow([9, 17])
+    free = len(c.free)
+    spare = c.fork(1, 8)
+    assert spare.tolist() == [-1, -1] and len(c.free) == free - 2 and [len(o) for o in c.owned] == [3, 4]
+    c.clear()
+    assert c.forked([9, 17], 1, 8) == 7 and sorted(c.free) == list(range(c.k.shape[1]))
