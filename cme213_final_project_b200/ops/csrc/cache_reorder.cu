@@ -7,8 +7,8 @@
 //
 // What bounds it: the bytes of the last pages of all layers, read and written once; with few beams a launch and the chain parent, length ->
 // page -> rows.  A warp copies the filled slots of one layer, head and tensor at a time.  8 groups of 8 beams, 24 layers, 16 heads of 64, pages of
-// 16: 11.2 us for 57 MB, 5 TB/s, 20.5 where nothing of it is in L2 (20.8 and more with a division for each piece's row and a CTA for four
-// items; two items of a warp at a time 12.3 and 22.5); 4 beams of 12 layers 2.8 us.
+// 16, 57 MB: 16.4 us on inputs that are not in L2, 3.5 TB/s, 20.5 with L2 cleared before each call, 11.2 replayed on one input (20.8 and more then with
+// a division for each piece's row and a CTA for four items; two items of a warp at a time 12.3, cleared 22.5); 4 beams of 12 layers 2.8 us.
 #include "paged.h"
 #include "beam_desc.h"
 

@@ -7,8 +7,9 @@
 //
 // What bounds it: bytes (new rows read once, a byte a number written); with few tokens the chain offsets -> length -> page -> scale.  One warp has
 // a block and head of keys or of values, so nobody else touches its scale; its rows are on their way before it knows where they go, and with
-// them, once it does, what the block holds.  16 prompts of 500 to 777 tokens, 12 heads of 64, blocks of 16: 11.1 us, 4.3 TB/s (16.1 with a
-// block and head a warp and no more, which looks up its place for two KB); 16 tokens 2.6 us.
+// them, once it does, what the block holds.  16 prompts of 500 to 777 tokens, 12 heads of 64, blocks of 16, 47 MB: 14.4 us where the new rows are
+// not in L2, 3.3 TB/s (fp32, 78 MB: 17.4), 11.1 replayed on one input, of which L2 holds all (16.1 then with a block and head a warp and no
+// more, which looks up its place for two KB); 16 tokens 2.6 us.
 #include "paged.h"
 
 #include <algorithm>

@@ -105,6 +105,11 @@ constexpr int MAX_SPLITS = 128;
 // and a launch).  The host does not know the sequences: they are taken to be as long as the longest, and to share the new tokens evenly.
 // Measured / estimated: 12 heads of 64, 128 tokens over 4096 in 4 sequences: tc in 1, 4, 8 parts 72 / 79, 32 / 32, 31 / 27, stream 62 / 72;
 // 4 heads of 128 in fp32, 256 over 512 in 8: rows 56 / 53, stream 97 / 107; 12 heads of 64 in fp32, 256 over 512 in 8: rows 72 / 98, stream 109 / 113.
+// 8 bits: measured with two CTAs (head size 128 on tcgen05: one) on every SM and keys in L2, us a tile, head sizes 32 / 64 / 128: up to 8 rows of
+// bf16 0.75 / 1.1 / 1.8, of fp32 0.86 / 1.3 / 2.2, 64 rows 2.6 / 3.7 / 5.8 and 3.2 / 5.0 / 8.7, tcgen05 1.3 / 1.3 / 1.2.  The times below are fitted to
+// whole calls, 72 shapes of both types (12, 32 on 8 and 4 heads of 64, 128 and 32, 1 to 64 sequences, 4 to 1024 tokens over 256 to 16384).  The form
+// that the estimates pick is within 8 % of the fastest in 69 of them; the others are bf16 16 over 2048 in 4, 32 heads of 128 on 8 (27.2 us, rows 24.0), fp32 128 over 4096 in 4, the same heads (281, 8 rows 247), and bf16 64
+// over 256 in 32, 4 heads of 32 (10.4, rows 8.8).
 struct Form {
     int keys;                // of a tile
     int slots;               // CTAs that run at a time
@@ -141,7 +146,8 @@ int make_plan(const CmePaged* a, bool q8, int backend, int splits, int sms, Page
     CME_REQUIRE(backend >= 0 && backend <= 3, CME_ERR_UNSUPPORTED, "paged attention: unknown backend");
     CME_REQUIRE(backend != 3 || tc, CME_ERR_UNSUPPORTED,
                 "paged attention: the tcgen05 kernel takes bf16 and up to 128 query heads per key head");
-    // (8 bits: tiles of 8 rows where the sequences have no more on average)
+    // (8 bits: tiles of 8 rows where the sequences have no more on average.  The host knows no more of them: one chunk among many single tokens has such
+    // tiles too.  12 heads of 64 over 1024 keys, 127 single tokens and a chunk of 512: 89 us, apart 62 and 20; of 800: 105, apart 62 and 29; tcgen05 163.)
     const int few_rows = q8 && rows <= 8ll * a->seqs ? 8 : 16;
     auto row_tile = [&](int b) { return b == 1 ? few_rows : b == 2 ? 64 : (a->head_dim == 128 ? 2 : 1) * (128 / group * group); };
     auto tiles_of = [&](int b) { return rows / row_tile(b) + std::min(a->seqs, a->rows); };      // at the most: each sequence adds less than one

@@ -24,8 +24,8 @@
 // A lane reads K in pieces of 16 bytes along its row (which column stands at which place of a product's step does not matter, as long as q's stand
 // there too); V comes through ldmatrix as pairs of bytes, of which the low ones are one column tile and the high ones another.
 // The scales of a tile travel with it, four bytes each, one for every eight keys.
-// Single tokens, calls one after the other: one sequence of 701, 12 heads of 64 5.4 us; 64 of up to 1024, 16 heads of 64 29.8 us; 16 of 2000 to 32768, 32 heads of
-// 128 on 8 94 to 101 us on inputs that are not in L2, 5 to 5.4 TB/s.
+// Single tokens, calls one after the other: one sequence of 701, 12 heads of 64 5.5 us; 64 of up to 1024, 16 heads of 64 31.6 us; 16 of 2000 to 32768, 32 heads of
+// 128 on 8 88 to 102 us on inputs that are not in L2, 5 to 5.8 TB/s.
 #pragma once
 #include "paged.h"
 #include "sm100_ptx.cuh"
